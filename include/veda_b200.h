@@ -496,6 +496,63 @@ int veda_compensate(const void* o_kept, int64_t ok_stride_n,
                     float softmax_scale, void* workspace,
                     int64_t workspace_bytes, void* stream);
 
+/* ---- the paged key-value cache ------------------------------------------- */
+/* No counterpart in the reference (it attends over one clip at a time).
+ *
+ * Pages are [n_pages, kv_heads, page_size, head_dim], contiguous, of bf16
+ * (storage 0), int8 (1) or e4m3 (2) codes; the last two with one fp32 scale
+ * per row, [n_pages, kv_heads, page_size] (NULL for bf16). head_dim is 64 or
+ * 128, page_size 16, 32, 64, 128 or 256. Row j of sequence b lies in row
+ * j % page_size of page table[b * table_ld + j / page_size]; a table row has
+ * max_pages entries. Tables, offsets, starts and lengths are read on the
+ * device. A place outside the table or a page outside the cache is not
+ * touched and sets VEDA_ERR_INVALID in the device status word. */
+
+/* Stores packed rows k, v [n_tokens, kv_heads, head_dim] bf16: row
+ * offsets[b] + i (i < offsets[b + 1] - offsets[b]) becomes row starts[b] + i
+ * of sequence b. int8: scale max|x| / 127; e4m3: scale 2^e, e the smallest
+ * integer >= -120 with max|x| <= 448 * 2^e; codes rounded to nearest, ties to
+ * even; a row with a non-finite value gets the scale NaN. */
+int veda_cache_write(void* k_pages, void* v_pages, float* k_scale,
+                     float* v_scale, int64_t n_pages, int32_t page_size,
+                     int32_t kv_heads, int32_t head_dim, int32_t storage,
+                     const int32_t* table, int64_t table_ld,
+                     int64_t max_pages, int64_t n_seqs, const void* k,
+                     int64_t k_stride_t, int64_t k_stride_h, const void* v,
+                     int64_t v_stride_t, int64_t v_stride_h, int64_t n_tokens,
+                     const int32_t* offsets, const int32_t* starts,
+                     void* stream);
+
+/* Reads contexts back as packed bf16 rows [n_tokens, kv_heads, head_dim]:
+ * row offsets[b] + j receives row j of sequence b (code * scale, rounded
+ * once; zeros for a place that does not exist). */
+int veda_cache_read(const void* k_pages, const void* v_pages,
+                    const float* k_scale, const float* v_scale,
+                    int64_t n_pages, int32_t page_size, int32_t kv_heads,
+                    int32_t head_dim, int32_t storage, const int32_t* table,
+                    int64_t table_ld, int64_t max_pages, int64_t n_seqs,
+                    const int32_t* offsets, int64_t n_tokens, void* k,
+                    void* v, void* stream);
+
+/* Bytes of workspace veda_decode needs on the current device; -1 for a
+ * head_dim that is not 64 or 128. */
+int64_t veda_decode_workspace(int32_t head_dim);
+
+/* Attention of one query per sequence, q [n_seqs, n_heads, head_dim] bf16,
+ * over rows 0 .. lengths[b] - 1 of its context; head h reads kv head
+ * h / (n_heads / kv_heads). out [n_seqs, n_heads, head_dim] bf16 contiguous,
+ * lse [n_seqs, n_heads] fp32 or NULL; 0 and -inf without rows. A length
+ * outside [0, max_pages * page_size] is held inside it and sets
+ * VEDA_ERR_INVALID in the device status word. */
+int veda_decode(const void* k_pages, const void* v_pages,
+                const float* k_scale, const float* v_scale, int64_t n_pages,
+                int32_t page_size, int32_t kv_heads, int32_t head_dim,
+                int32_t storage, const int32_t* table, int64_t table_ld,
+                int64_t max_pages, int64_t n_seqs, const int32_t* lengths,
+                const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                int32_t n_heads, void* out, float* lse, float softmax_scale,
+                void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- diagnostics --------------------------------------------------------- */
 
 /* One 128x128x128 bf16 tcgen05 MMA per mode, for checking operand and

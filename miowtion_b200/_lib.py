@@ -43,6 +43,10 @@ class ColumnBlockC(ctypes.Structure):
                 ('keeps_all', c_i32), ('pad_', c_i32)]
 
 
+# The arguments that describe a paged cache and its table.
+_CACHE = [c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i32, c_i32, c_i32, c_i32,
+          c_ptr, c_i64, c_i64, c_i64]
+
 # name -> (restype, argtypes), in the order of include/veda_b200.h
 SIGNATURES = {
     'veda_last_error': (c_i32, [ctypes.c_char_p, ctypes.c_size_t]),
@@ -124,6 +128,12 @@ SIGNATURES = {
                                 c_i64, c_i32, c_i64, c_i64, c_ptr, c_ptr,
                                 c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_i64,
                                 c_i64, c_f32, c_ptr, c_i64, c_ptr]),
+    'veda_cache_write': (c_i32, _CACHE + [c_ptr, c_i64, c_i64, c_ptr, c_i64,
+                                          c_i64, c_i64, c_ptr, c_ptr, c_ptr]),
+    'veda_cache_read': (c_i32, _CACHE + [c_ptr, c_i64, c_ptr, c_ptr, c_ptr]),
+    'veda_decode_workspace': (c_i64, [c_i32]),
+    'veda_decode': (c_i32, _CACHE + [c_ptr, c_ptr, c_i64, c_i64, c_i32, c_ptr,
+                                     c_ptr, c_f32, c_ptr, c_i64, c_ptr]),
     'veda_probe_umma': (c_i32, [c_ptr, c_ptr, c_ptr, c_i32, c_ptr]),
     'veda_expire_wait': (c_i32, [c_i64, c_ptr, c_ptr]),
 }

@@ -1,0 +1,891 @@
+// Attention of one new token per sequence over the paged key-value cache,
+// split over the cache's length and joined.
+//
+// For head h of a sequence with cached rows j < length, kv head h / group:
+//     s_j = scale q_h . k_j,  out_h = sum_j softmax(s)_j v_j,
+//     lse_h = log sum_j exp(s_j);  no rows: out 0, lse -inf.
+//
+// The cache is read once and each of its bytes meets all heads of a group,
+// so the kernel is bound by memory. The heads of a group are the rows of
+// m16n8k16 tensor-core products (a group of 16 or fewer is one tile, larger
+// ones take several and find the rows in L2): tcgen05's 128 rows would leave
+// seven eighths or more of them empty, and at the cache's rate the legacy
+// products take a fraction of the time of its loads.
+//
+// The contexts of a call are cut into chunks of 16 keys of one kv head
+// (a page holds a multiple of 16 rows, so a chunk is one contiguous piece),
+// numbered sequence by sequence and head by head, and CTA i of G takes the
+// i-th of G equal runs of the numbers, whatever the lengths: the split needs
+// the lengths on the device only. A warp takes every kWarps-th chunk of the
+// CTA's piece of a (sequence, head) and streams it through a ring of its
+// own with cp.async (rows past the length are filled with zeros, not read),
+// with its own running maximum, sum and accumulator; the warps join in shared
+// memory at the piece's end while the ring already loads the next piece. A
+// piece that is a whole (sequence, head) is written out; others leave
+// maximum, sum and accumulator in the workspace, which decode_join_kernel
+// adds up in the order of the keys. No atomics: repeats are bit-identical.
+//
+// int8 and e4m3 codes become fp16 exactly, in registers. A key's scale
+// multiplies its scores; a value row's scale multiplies its weights, relative
+// to the largest scale met so far so that they stay inside fp16. q is brought
+// to [1, 2) per head by a power of two, so it loses nothing in fp16 but
+// elements 2^-14 below the head's largest. Scores, maxima, sums and
+// accumulators are fp32; weights are rounded to the 16-bit type of the
+// products (bf16 pages: bf16), as everywhere in this library.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <math.h>
+
+#include "kvcache.cuh"
+
+namespace veda {
+
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kChunk = 16;  // keys
+constexpr int kRows = 16;   // heads of a tile
+constexpr int kJoinThreads = 128;
+constexpr float kWeight = 64.f;  // factor of the fp16 weights
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.69314718055994531f;
+
+struct DecodeParams {
+  CacheView c;
+  const __nv_bfloat16* q;
+  int64_t q_sb, q_sh;
+  const int32_t* lengths;
+  int group;   // query heads of a kv head
+  int tiles;   // tiles of kRows heads in a group
+  __nv_bfloat16* out;  // [n_seqs, heads, D]
+  float* lse;          // [n_seqs, heads] or null
+  float* partial;      // [G][2][kRows][D + 2]
+  int n_ctas;
+  float scale_log2;
+  unsigned int* status;
+};
+
+// Rows of sequence b: its length, held inside what its table row addresses.
+__device__ __forceinline__ int context(const DecodeParams& p, int b) {
+  const int n = p.lengths[b];
+  const int cap = p.c.max_pages << p.c.page_shift;
+  return n < 0 ? 0 : (n > cap ? cap : n);
+}
+
+__device__ __forceinline__ int chunks_of(int length) {
+  return (length + kChunk - 1) / kChunk;
+}
+
+// CTAs that take part: with more of them than chunks, one for each chunk, so
+// that no run is empty.
+__device__ __forceinline__ int active_ctas(const DecodeParams& p,
+                                           int64_t total) {
+  return total < p.n_ctas ? static_cast<int>(total) : p.n_ctas;
+}
+
+// First chunk number of CTA i: [0, total) in n equal runs.
+__device__ __forceinline__ int64_t run_begin(int64_t total, int i, int n) {
+  return total * i / n;
+}
+
+// Block-wide sums over the sequences: *total = chunks of all of them, and
+// the sequence that chunk number `at` lies in with the chunks before it
+// (where kFind; -1 if at >= total). Chunks are per tile and kv head, so a
+// sequence has chunks_of(length) * heads of them.
+template <int kBlock>
+struct Prefix {
+  int64_t warp_sum[kBlock / 32];
+  int64_t base;
+  int found;
+  int64_t before;
+};
+
+template <int kBlock>
+__device__ __forceinline__ int64_t block_scan(Prefix<kBlock>* s, int64_t x,
+                                              int64_t* sum) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int64_t inc = x;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += y;
+  }
+  __syncthreads();
+  if (lane == 31) s->warp_sum[warp] = inc;
+  __syncthreads();
+  int64_t pre = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kBlock / 32; ++w) {
+    const int64_t y = s->warp_sum[w];
+    if (w < warp) pre += y;
+    all += y;
+  }
+  *sum = all;
+  return pre + inc - x;  // exclusive
+}
+
+// Chunks of all sequences, per (kv head, tile).
+template <int kBlock>
+__device__ __forceinline__ int64_t total_chunks(Prefix<kBlock>* s,
+                                                const DecodeParams& p) {
+  int64_t mine = 0;
+  for (int b = threadIdx.x; b < p.c.n_seqs; b += kBlock)
+    mine += chunks_of(context(p, b));
+  int64_t sum;
+  block_scan<kBlock>(s, mine, &sum);
+  return sum;
+}
+
+// The sequence of chunk `at` (numbers of one head: chunks before sequence b
+// sum to before <= at < before + its own); all threads return it.
+template <int kBlock>
+__device__ __forceinline__ void find_chunk(Prefix<kBlock>* s,
+                                           const DecodeParams& p, int64_t at,
+                                           int64_t heads, int* seq,
+                                           int64_t* before) {
+  int64_t base = 0;
+  if (threadIdx.x == 0) s->found = -1;
+  for (int b0 = 0; b0 < p.c.n_seqs; b0 += kBlock) {
+    const int b = b0 + threadIdx.x;
+    const int64_t n =
+        b < p.c.n_seqs ? chunks_of(context(p, b)) * heads : int64_t(0);
+    int64_t sum;
+    const int64_t pre = base + block_scan<kBlock>(s, n, &sum);
+    if (n > 0 && pre <= at && at < pre + n) {
+      s->found = b;
+      s->before = pre;
+    }
+    base += sum;
+    __syncthreads();
+    if (s->found >= 0 || at < base) break;
+  }
+  *seq = s->found;
+  *before = s->before;
+}
+
+// The pieces of a CTA's run: sequence, head tile, chunks [c0, c1).
+struct Pieces {
+  int b, vh, c0, c1, n;  // n: chunks of the whole (sequence, head)
+  int length;
+  int64_t left;  // chunks of the run from c0 on
+  int heads;     // kv heads x tiles
+  __device__ void bound() {
+    const int64_t room = n - c0;
+    c1 = c0 + static_cast<int>(left < room ? left : room);
+  }
+  __device__ bool valid() const { return left > 0; }
+  __device__ void next(const DecodeParams& p) {
+    left -= c1 - c0;
+    c0 = 0;
+    if (left <= 0) return;
+    if (++vh == heads) {
+      vh = 0;
+      length = 0;
+      while (length == 0 && ++b < p.c.n_seqs) length = context(p, b);
+      n = chunks_of(length);
+      if (n == 0) {  // not reached while the lengths stay as they are
+        left = 0;
+        return;
+      }
+    }
+    bound();
+  }
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src,
+                                           bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
+               "l"(src), "r"(take ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src,
+                                          bool take) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst),
+               "l"(src), "r"(take ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int kLeft>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+      : "r"(addr)
+      : "memory");
+}
+
+// c[4] += A (16 x 16) . B (16 x 8), bf16 or fp16 in, fp32 accumulate.
+template <bool kHalf>
+__device__ __forceinline__ void mma16816(float* c, const uint32_t* a,
+                                         uint32_t b0, uint32_t b1) {
+  if constexpr (kHalf)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+        "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, "
+        "%3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Four codes (bytes 0 .. 3) as two fp16 pairs, exactly.
+template <int kStore>
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t* lo,
+                                              uint32_t* hi) {
+  if constexpr (kStore == kStoreInt8) {
+    // 0x6400 | u is the fp16 number 1024 + u; u = code + 128.
+    w ^= 0x80808080u;
+    const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+    uint32_t a = __byte_perm(w, 0x64646464u, 0x4140);
+    uint32_t b = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), bias);
+    const __half2 y = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
+    *lo = *reinterpret_cast<const uint32_t*>(&x);
+    *hi = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2(
+        static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
+    const __half2_raw y = __nv_cvt_fp8x2_to_halfraw2(
+        static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
+    *lo = static_cast<uint32_t>(x.x) | (static_cast<uint32_t>(x.y) << 16);
+    *hi = static_cast<uint32_t>(y.x) | (static_cast<uint32_t>(y.y) << 16);
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <int kD, int kStore>
+struct Shape {
+  static constexpr bool kHalf = kStore != kStoreBf16;
+  static constexpr int kRowBytes = kHalf ? kD : 2 * kD;
+  static constexpr int kTileBytes = kChunk * kRowBytes;  // k or v of a chunk
+  // k, v, and (8-bit) 16 k scales and 16 v scales.
+  static constexpr int kStageBytes = 2 * kTileBytes + (kHalf ? 128 : 0);
+  static constexpr int kPieces = kRowBytes / 16;  // 16-byte pieces of a row
+  static constexpr int kJoinFloats = kD + 4;      // a row of the join buffer
+};
+
+// Byte offset of 16-byte piece `c` of row `r` of a k or v tile: the pieces
+// are permuted within groups of eight rows so that ldmatrix, which reads the
+// same piece of eight rows, meets all banks.
+template <int kPieces>
+__device__ __forceinline__ uint32_t piece_at(int r, int c) {
+  if constexpr (kPieces >= 8)
+    return (r * kPieces + (c ^ (r & 7))) * 16;
+  else  // 64-byte rows: two rows make up 128 bytes
+    return (r * kPieces + (c ^ ((r >> 1) & 3))) * 16;
+}
+
+template <int kD, int kStore, int kStages>
+__global__ void __launch_bounds__(kThreads, 1)
+    decode_kernel(const __grid_constant__ DecodeParams p) {
+  using S = Shape<kD, kStore>;
+  constexpr bool kHalf = S::kHalf;
+  constexpr int kSteps = kD / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ Prefix<kThreads> prefix;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int quad = lane % 4, row_lo = lane / 4;  // fragment coordinates
+
+  uint8_t* ring = smem + warp * (kStages * S::kStageBytes);
+  float* join =
+      reinterpret_cast<float*>(smem + kWarps * kStages * S::kStageBytes);
+
+  const int heads = p.c.kv_heads * p.tiles;
+  const int64_t total = total_chunks<kThreads>(&prefix, p) * heads;
+  if (blockIdx.x == 0) {
+    // A length that its table row cannot hold is reported.
+    const int64_t cap = static_cast<int64_t>(p.c.max_pages)
+                        << p.c.page_shift;
+    for (int b = threadIdx.x; b < p.c.n_seqs; b += kThreads)
+      if (p.lengths[b] < 0 || p.lengths[b] > cap)
+        raise_status(p.status, VEDA_ERR_INVALID);
+  }
+  const int n_ctas = active_ctas(p, total);
+  if (static_cast<int>(blockIdx.x) >= n_ctas) return;
+  const int64_t lo = run_begin(total, blockIdx.x, n_ctas);
+  const int64_t hi = run_begin(total, blockIdx.x + 1, n_ctas);
+  Pieces seg;
+  int64_t before;
+  find_chunk<kThreads>(&prefix, p, lo, heads, &seg.b, &before);
+  if (seg.b < 0) return;
+  seg.length = context(p, seg.b);
+  seg.n = chunks_of(seg.length);
+  seg.heads = heads;
+  seg.vh = static_cast<int>((lo - before) / seg.n);
+  seg.c0 = static_cast<int>((lo - before) % seg.n);
+  seg.left = hi - lo;
+  seg.bound();
+  const bool starts_inside = seg.c0 > 0;
+
+  // ---- loads: this warp's chunks, piece after piece ----
+  Pieces ld = seg;
+  int ld_chunk = ld.c0 + warp;
+  auto settle = [&]() {
+    while (ld.valid() && ld_chunk >= ld.c1) {
+      ld.next(p);
+      ld_chunk = ld.c0 + warp;
+    }
+  };
+  // The page of the next chunk is looked up one load ahead of its use.
+  int next_page = -1;
+  auto look_up = [&]() {
+    settle();
+    if (ld.valid())
+      next_page = p.c.table[ld.b * p.c.table_ld +
+                            ((ld_chunk * kChunk) >> p.c.page_shift)];
+  };
+  look_up();
+  int ld_stage = 0;
+  auto load_next = [&]() {
+    if (ld.valid()) {
+      const int key0 = ld_chunk * kChunk;
+      const bool ok = next_page >= 0 && next_page < p.c.n_pages;
+      if (!ok && lane == 0) raise_status(p.status, VEDA_ERR_INVALID);
+      // Keys of the chunk that exist; those of a bad page count as absent.
+      const int live = ok ? ld.length - key0 : 0;
+      const int64_t row0 =
+          ok ? (((static_cast<int64_t>(next_page) * p.c.kv_heads +
+                  ld.vh / p.tiles)
+                 << p.c.page_shift) +
+                (key0 & ((1 << p.c.page_shift) - 1)))
+             : 0;
+      const uint32_t dst = smem_u32(ring + ld_stage * S::kStageBytes);
+      const uint8_t* ksrc = p.c.k + row0 * S::kRowBytes;
+      const uint8_t* vsrc = p.c.v + row0 * S::kRowBytes;
+#pragma unroll
+      for (int i = 0; i < kChunk * S::kPieces / 32; ++i) {
+        const int piece = i * 32 + lane;
+        const int r = piece / S::kPieces, c = piece % S::kPieces;
+        const uint32_t off = piece_at<S::kPieces>(r, c);
+        cp_async16(dst + off, ksrc + piece * 16, r < live);
+        cp_async16(dst + S::kTileBytes + off, vsrc + piece * 16, r < live);
+      }
+      if constexpr (kHalf) {
+        const int r = lane % 16;
+        const float* src = (lane < 16 ? p.c.k_scale : p.c.v_scale) + row0 + r;
+        cp_async4(dst + 2 * S::kTileBytes + lane * 4, src, r < live);
+      }
+      ld_chunk += kWarps;
+      look_up();
+    }
+    cp_async_commit();
+    ld_stage = ld_stage + 1 == kStages ? 0 : ld_stage + 1;
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) load_next();
+
+  int stage = 0;
+  for (; seg.valid(); seg.next(p)) {
+    const int kvh = seg.vh / p.tiles, tile = seg.vh % p.tiles;
+    const int n_rows = min(kRows, p.group - tile * kRows);
+    const int head0 = kvh * p.group + tile * kRows;
+    // ---- q fragments of the piece's heads ----
+    uint32_t qf[kSteps][4];
+    float row_scale[2] = {p.scale_log2, p.scale_log2};
+    if (seg.c0 + warp < seg.c1) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int r = row_lo + 8 * half;
+        const __nv_bfloat16* src =
+            p.q + seg.b * p.q_sb + (head0 + (r < n_rows ? r : 0)) * p.q_sh;
+        if constexpr (!kHalf) {
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            qf[s][half] =
+                *reinterpret_cast<const uint32_t*>(src + s * 16 + quad * 2);
+            qf[s][half + 2] =
+                *reinterpret_cast<const uint32_t*>(src + s * 16 + 8 + quad * 2);
+          }
+        } else {
+          // The products' depth index runs over d in the order that a
+          // thread's four consecutive code bytes give.
+          float x[kSteps][4];
+          float top = 0.f;
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            const uint2 w =
+                *reinterpret_cast<const uint2*>(src + s * 16 + quad * 4);
+            x[s][0] = __uint_as_float(w.x << 16);
+            x[s][1] = __uint_as_float(w.x & 0xFFFF0000u);
+            x[s][2] = __uint_as_float(w.y << 16);
+            x[s][3] = __uint_as_float(w.y & 0xFFFF0000u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[s][i]));
+          }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          // 2^e <= top < 2^(e+1), e held to [-126, 126] so that its inverse
+          // exists.
+          int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+          e = max(-126, min(126, e));
+          const float inv =
+              __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+          row_scale[half] =
+              p.scale_log2 *
+              __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            qf[s][half] = pack_half(x[s][0] * inv, x[s][1] * inv);
+            qf[s][half + 2] = pack_half(x[s][2] * inv, x[s][3] * inv);
+          }
+        }
+      }
+    }
+
+    // ---- the piece's chunks of this warp ----
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float v_ref = 0.f;
+    float o[kD / 8][4];
+#pragma unroll
+    for (int i = 0; i < kD / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    for (int chunk = seg.c0 + warp; chunk < seg.c1; chunk += kWarps) {
+      // This chunk has landed, and the stage of the one before has been read
+      // by the whole warp: it takes the next load.
+      cp_async_wait<kStages - 2>();
+      __syncwarp();
+      load_next();
+      const uint8_t* st = ring + stage * S::kStageBytes;
+      const uint32_t k_addr = smem_u32(st);
+      const uint32_t v_addr = k_addr + S::kTileBytes;
+      const float* scales =
+          reinterpret_cast<const float*>(st + 2 * S::kTileBytes);
+
+      // Scores: [16 heads] x [2 x 8 keys].
+      float s[2][4] = {};
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const int key = nt * 8 + (lane & 7);
+        if constexpr (!kHalf) {
+#pragma unroll
+          for (int st2 = 0; st2 < kSteps; st2 += 2) {
+            uint32_t b[4];
+            ldsm4(k_addr + piece_at<S::kPieces>(key, st2 * 2 + lane / 8), b);
+            mma16816<false>(s[nt], qf[st2], b[0], b[1]);
+            mma16816<false>(s[nt], qf[st2 + 1], b[2], b[3]);
+          }
+        } else {
+#pragma unroll
+          for (int st4 = 0; st4 < kSteps; st4 += 4) {
+            uint32_t b[4];
+            ldsm4(k_addr + piece_at<S::kPieces>(key, st4 + lane / 8), b);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t b0, b1;
+              codes_to_half<kStore>(b[i], &b0, &b1);
+              mma16816<true>(s[nt], qf[st4 + i], b0, b1);
+            }
+          }
+        }
+      }
+      // Columns of this thread: keys 2 quad + {0, 1} of each half.
+      const int live = seg.length - chunk * kChunk;
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const int key = nt * 8 + quad * 2;
+        float k0 = 1.f, k1 = 1.f;
+        if constexpr (kHalf) {
+          const float2 ks = *reinterpret_cast<const float2*>(scales + key);
+          k0 = ks.x;
+          k1 = ks.y;
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float& a = s[nt][2 * half];
+          float& b = s[nt][2 * half + 1];
+          a *= row_scale[half] * k0;
+          b *= row_scale[half] * k1;
+          if (key >= live) a = -INFINITY;
+          if (key + 1 >= live) b = -INFINITY;
+          top[half] = fmaxf(top[half], fmaxf(a, b));
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        top[half] =
+            fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
+        top[half] =
+            fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
+      }
+      // The references move only when they must: a maximum by more than 2^8,
+      // the values' scale by more than 2. fp16 weights carry a factor 2^6
+      // (kWeight) and stay below 2^15; those down to 2^-20 of the references
+      // keep all of fp16's bits.
+      float v_top = 0.f;
+      float2 vs[2];
+      if constexpr (kHalf) {
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          vs[nt] = *reinterpret_cast<const float2*>(scales + 16 + nt * 8 +
+                                                    quad * 2);
+          v_top = fmaxf(v_top, fmaxf(vs[nt].x, vs[nt].y));
+        }
+        v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, 1));
+        v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, 2));
+      }
+      const bool grow = top[0] > m[0] + 8.f || top[1] > m[1] + 8.f ||
+                        (kHalf && v_top > 2.f * v_ref);
+      if (__any_sync(0xffffffffu, grow)) {
+        float f[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float next = fmaxf(m[half], top[half]);
+          f[half] = m[half] == -INFINITY ? 0.f : ex2_approx(m[half] - next);
+          m[half] = next;
+          l[half] *= f[half];
+        }
+        if constexpr (kHalf) {
+          // (Held above 2^-100: its inverse exists.)
+          const float next =
+              v_top > 0.f ? fmaxf(fmaxf(v_ref, v_top), 0x1p-100f) : v_ref;
+          const float g = v_ref > 0.f ? v_ref / next : 0.f;
+          v_ref = next;
+          f[0] *= g;
+          f[1] *= g;
+        }
+#pragma unroll
+        for (int i = 0; i < kD / 8; ++i) {
+          o[i][0] *= f[0];
+          o[i][1] *= f[0];
+          o[i][2] *= f[1];
+          o[i][3] *= f[1];
+        }
+      }
+      // Weights, as the A operand of the second product.
+      uint32_t a[4];
+      const float v_inv = kHalf && v_ref > 0.f ? kWeight / v_ref : 0.f;
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          // m is -inf where no key of the row has existed so far.
+          const float ref = m[half] == -INFINITY ? 0.f : m[half];
+          const float p0 = ex2_approx(s[nt][2 * half] - ref);
+          const float p1 = ex2_approx(s[nt][2 * half + 1] - ref);
+          l[half] += p0 + p1;
+          if constexpr (kHalf)
+            a[nt * 2 + half] = pack_half(p0 * (vs[nt].x * v_inv),
+                                         p1 * (vs[nt].y * v_inv));
+          else
+            a[nt * 2 + half] = pack_bf16(p0, p1);
+        }
+      // O += P V.
+      const int vkey = (lane & 7) + ((lane >> 3) & 1) * 8;
+      if constexpr (!kHalf) {
+#pragma unroll
+        for (int dt = 0; dt < kD / 8; dt += 2) {
+          uint32_t b[4];
+          ldsm4_trans(v_addr + piece_at<S::kPieces>(vkey, dt + lane / 16), b);
+          mma16816<false>(o[dt], a, b[0], b[1]);
+          mma16816<false>(o[dt + 1], a, b[2], b[3]);
+        }
+      } else {
+        // A 16-byte piece of a row is 16 d: column n of the even tile is
+        // d = 2 n, of the odd tile 2 n + 1.
+#pragma unroll
+        for (int dt = 0; dt < kD / 8; dt += 4) {
+          uint32_t b[4];
+          ldsm4_trans(
+              v_addr + piece_at<S::kPieces>(vkey, dt / 2 + lane / 16), b);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t lo0, hi0, lo1, hi1;
+            codes_to_half<kStore>(__byte_perm(b[2 * i], 0, 0x3120), &lo0,
+                                  &hi0);
+            codes_to_half<kStore>(__byte_perm(b[2 * i + 1], 0, 0x3120), &lo1,
+                                  &hi1);
+            mma16816<true>(o[dt + 2 * i], a, lo0, lo1);
+            mma16816<true>(o[dt + 2 * i + 1], a, hi0, hi1);
+          }
+        }
+      }
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+
+    // ---- join the warps ----
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+    }
+    const float unit = kHalf ? v_ref * (1.f / kWeight) : 1.f;
+    const int pitch = min(p.group, kRows);
+    __syncthreads();  // the previous piece's join has been read
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = row_lo + 8 * half;
+      if (r >= n_rows) continue;
+      float* dst = join + (warp * pitch + r) * S::kJoinFloats;
+      if (quad == 0) {
+        dst[kD] = m[half];
+        dst[kD + 1] = l[half];
+      }
+#pragma unroll
+      for (int dt = 0; dt < kD / 8; dt += 2) {
+        const float a0 = o[dt][2 * half] * unit;
+        const float a1 = o[dt][2 * half + 1] * unit;
+        const float b0 = o[dt + 1][2 * half] * unit;
+        const float b1 = o[dt + 1][2 * half + 1] * unit;
+        if constexpr (!kHalf) {
+          *reinterpret_cast<float2*>(dst + dt * 8 + quad * 2) =
+              make_float2(a0, a1);
+          *reinterpret_cast<float2*>(dst + dt * 8 + 8 + quad * 2) =
+              make_float2(b0, b1);
+        } else {
+          *reinterpret_cast<float4*>(dst + dt * 8 + quad * 4) =
+              make_float4(a0, b0, a1, b1);
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = seg.c0 == 0 && seg.c1 == seg.n;
+    // The CTA's first piece if it does not begin its (sequence, head), else
+    // its last: at most these two are parts.
+    const int slot =
+        starts_inside && seg.left == hi - lo ? 0 : 1;
+    float* part =
+        p.partial + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * kRows *
+                        (kD + 2);
+    for (int i = threadIdx.x; i < n_rows * (kD / 2); i += kThreads) {
+      const int r = i / (kD / 2), d = (i % (kD / 2)) * 2;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w)
+        top = fmaxf(top, join[(w * pitch + r) * S::kJoinFloats + kD]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float x = 0.f, y = 0.f, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float* src = join + (w * pitch + r) * S::kJoinFloats;
+        const float f = ex2_approx(src[kD] - ref);
+        const float2 ow = *reinterpret_cast<const float2*>(src + d);
+        x = fmaf(f, ow.x, x);
+        y = fmaf(f, ow.y, y);
+        sum = fmaf(f, src[kD + 1], sum);
+      }
+      if (whole) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int64_t at = static_cast<int64_t>(seg.b) *
+                               (p.c.kv_heads * p.group) +
+                           head0 + r;
+        *reinterpret_cast<uint32_t*>(p.out + at * kD + d) =
+            pack_bf16(x * inv, y * inv);
+        if (d == 0 && p.lse != nullptr)
+          p.lse[at] = (top + log2f(sum)) * kLn2;
+      } else {
+        float* dst = part + r * (kD + 2);
+        *reinterpret_cast<float2*>(dst + d) = make_float2(x, y);
+        if (d == 0) {
+          dst[kD] = top;
+          dst[kD + 1] = sum;
+        }
+      }
+    }
+  }
+}
+
+// Adds up the pieces of the (sequence, head tile)s that several CTAs share,
+// in the order of their keys; writes the rows of empty sequences. One block
+// per (sequence, head tile).
+template <int kD>
+__global__ void __launch_bounds__(kJoinThreads)
+    decode_join_kernel(const __grid_constant__ DecodeParams p) {
+  __shared__ Prefix<kJoinThreads> prefix;
+  const int heads = p.c.kv_heads * p.tiles;
+  const int b = blockIdx.x / heads, vh = blockIdx.x % heads;
+  int64_t before = 0, all = 0;
+  for (int i = threadIdx.x; i < p.c.n_seqs; i += kJoinThreads) {
+    const int n = chunks_of(context(p, i));
+    all += n;
+    if (i < b) before += n;
+  }
+  int64_t total, sum_before;
+  block_scan<kJoinThreads>(&prefix, all, &total);
+  block_scan<kJoinThreads>(&prefix, before, &sum_before);
+  total *= heads;
+  const int n_ctas = active_ctas(p, total);
+  const int n = chunks_of(context(p, b));
+  const int64_t first = sum_before * heads + static_cast<int64_t>(vh) * n;
+  const int64_t last = first + n - 1;
+  const int kvh = vh / p.tiles, tile = vh % p.tiles;
+  const int n_rows = min(kRows, p.group - tile * kRows);
+  const int64_t at0 = static_cast<int64_t>(b) * (p.c.kv_heads * p.group) +
+                      kvh * p.group + tile * kRows;
+  // The CTA of chunk c: the largest i with run_begin(i) <= c.
+  auto cta_of = [&](int64_t c) {
+    int i = static_cast<int>((c * n_ctas) / total);
+    while (i + 1 < n_ctas && run_begin(total, i + 1, n_ctas) <= c) ++i;
+    while (i > 0 && run_begin(total, i, n_ctas) > c) --i;
+    return i;
+  };
+  int c0 = 0, c1 = -1;
+  if (n > 0) {
+    c0 = cta_of(first);
+    c1 = cta_of(last);
+    if (c0 == c1) return;  // one CTA had all of it
+  }
+  for (int i = threadIdx.x; i < n_rows * (kD / 2); i += kJoinThreads) {
+    const int r = i / (kD / 2), d = (i % (kD / 2)) * 2;
+    float top = -INFINITY, sum = 0.f, x = 0.f, y = 0.f;
+    for (int c = c0; c <= c1; ++c) {
+      // Slot 0 holds a CTA's first piece if it starts inside its head.
+      const int slot = run_begin(total, c, n_ctas) > first ? 0 : 1;
+      const float* src =
+          p.partial +
+          ((static_cast<int64_t>(c) * 2 + slot) * kRows + r) * (kD + 2);
+      const float m = src[kD];
+      const float2 ow = *reinterpret_cast<const float2*>(src + d);
+      const float next = fmaxf(top, m);
+      const float ref = next == -INFINITY ? 0.f : next;
+      const float f = ex2_approx(top - ref), g = ex2_approx(m - ref);
+      x = fmaf(x, f, ow.x * g);
+      y = fmaf(y, f, ow.y * g);
+      sum = fmaf(sum, f, src[kD + 1] * g);
+      top = next;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<uint32_t*>(p.out + (at0 + r) * kD + d) =
+        pack_bf16(x * inv, y * inv);
+    if (d == 0 && p.lse != nullptr)
+      p.lse[at0 + r] = (top + log2f(sum)) * kLn2;
+  }
+}
+
+int sm_count(int* sms) {
+  int dev = 0;
+  VEDA_CUDA(cudaGetDevice(&dev));
+  VEDA_CUDA(
+      cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+  return VEDA_OK;
+}
+
+template <int kD, int kStore, int kStages>
+int launch(const DecodeParams& p, cudaStream_t stream) {
+  using S = Shape<kD, kStore>;
+  const int pitch = p.group < kRows ? p.group : kRows;
+  const int smem = kWarps * kStages * S::kStageBytes +
+                   kWarps * pitch * S::kJoinFloats * 4;
+  VEDA_CUDA(cudaFuncSetAttribute(decode_kernel<kD, kStore, kStages>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 smem));
+  decode_kernel<kD, kStore, kStages>
+      <<<p.n_ctas, kThreads, smem, stream>>>(p);
+  int rc = check_launch("decode_kernel");
+  if (rc != VEDA_OK) return rc;
+  const int64_t blocks =
+      static_cast<int64_t>(p.c.n_seqs) * p.c.kv_heads * p.tiles;
+  decode_join_kernel<kD>
+      <<<static_cast<unsigned>(blocks), kJoinThreads, 0, stream>>>(p);
+  return check_launch("decode_join_kernel");
+}
+
+// The ring is as deep as shared memory allows beside the join buffer, whose
+// rows are the group's heads (16 at most).
+template <int kD, int kStore>
+int launch_stages(const DecodeParams& p, cudaStream_t stream) {
+  if constexpr (kD == 64) {
+    return launch<kD, kStore, kStore == kStoreBf16 ? 5 : 8>(p, stream);
+  } else if constexpr (kStore == kStoreBf16) {
+    return p.group <= 8 ? launch<kD, kStore, 3>(p, stream)
+                        : launch<kD, kStore, 2>(p, stream);
+  } else {
+    return p.group <= 8 ? launch<kD, kStore, 5>(p, stream)
+                        : launch<kD, kStore, 4>(p, stream);
+  }
+}
+
+}  // namespace
+
+}  // namespace veda
+
+using namespace veda;
+
+extern "C" int64_t veda_decode_workspace(int32_t head_dim) {
+  if (head_dim != 64 && head_dim != 128) return -1;
+  int sms = 0;
+  if (sm_count(&sms) != VEDA_OK) return -1;
+  return static_cast<int64_t>(sms) * 2 * kRows * (head_dim + 2) *
+         static_cast<int64_t>(sizeof(float));
+}
+
+extern "C" int veda_decode(
+    const void* k_pages, const void* v_pages, const float* k_scale,
+    const float* v_scale, int64_t n_pages, int32_t page_size, int32_t kv_heads,
+    int32_t head_dim, int32_t storage, const int32_t* table, int64_t table_ld,
+    int64_t max_pages, int64_t n_seqs, const int32_t* lengths, const void* q,
+    int64_t q_stride_b, int64_t q_stride_h, int32_t n_heads, void* out,
+    float* lse, float softmax_scale, void* workspace, int64_t workspace_bytes,
+    void* stream) {
+  int rc = require_sm100("veda_decode");
+  if (rc != VEDA_OK) return rc;
+  DecodeParams p{};
+  rc = make_cache_view(&p.c, const_cast<void*>(k_pages),
+                       const_cast<void*>(v_pages),
+                       const_cast<float*>(k_scale),
+                       const_cast<float*>(v_scale), n_pages, page_size,
+                       kv_heads, head_dim, storage, table, table_ld, max_pages,
+                       n_seqs);
+  if (rc != VEDA_OK) return rc;
+  VEDA_REQUIRE(lengths && q && out && workspace,
+               "lengths, q, out and workspace are required");
+  VEDA_REQUIRE(n_heads >= 1 && n_heads % kv_heads == 0,
+               "n_heads must be a multiple of kv_heads");
+  VEDA_REQUIRE(n_seqs * n_heads < (int64_t(1) << 31), "too many rows");
+  VEDA_REQUIRE(softmax_scale > 0.f && isfinite(softmax_scale),
+               "softmax_scale must be positive and finite");
+  VEDA_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
+                   q_stride_b % 8 == 0 && q_stride_h % 8 == 0 &&
+                   reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+               "q, out and workspace must be 16-byte aligned, q's strides "
+               "multiples of 8");
+  const int64_t need = veda_decode_workspace(head_dim);
+  VEDA_REQUIRE(need > 0 && workspace_bytes >= need,
+               "workspace too small (veda_decode_workspace)");
+  rc = sm_count(&p.n_ctas);
+  if (rc != VEDA_OK) return rc;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_sb = q_stride_b;
+  p.q_sh = q_stride_h;
+  p.lengths = lengths;
+  p.group = n_heads / kv_heads;
+  p.tiles = (p.group + kRows - 1) / kRows;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.lse = lse;
+  p.partial = static_cast<float*>(workspace);
+  p.scale_log2 = softmax_scale * kLog2e;
+  p.status = device_status_ptr();
+  cudaStream_t s = as_stream(stream);
+  if (head_dim == 128) {
+    if (storage == kStoreBf16) return launch_stages<128, kStoreBf16>(p, s);
+    if (storage == kStoreInt8) return launch_stages<128, kStoreInt8>(p, s);
+    return launch_stages<128, kStoreE4m3>(p, s);
+  }
+  if (storage == kStoreBf16) return launch_stages<64, kStoreBf16>(p, s);
+  if (storage == kStoreInt8) return launch_stages<64, kStoreInt8>(p, s);
+  return launch_stages<64, kStoreE4m3>(p, s);
+}

@@ -1,0 +1,386 @@
+// The paged key-value cache: rows quantised as they are written, contexts
+// read back as packed bf16 rows.
+//
+// A row x (one token, one head) is stored as codes and one scale:
+//     int8   scale = max|x| / 127, code = round(127 x / max|x|)
+//     e4m3   scale = 2^e with the smallest integer e >= -120 for which
+//            max|x| <= 448 2^e; code = x / scale rounded to e4m3
+//     bf16   the row itself, no scale
+// rounding to nearest, ties to even. A power-of-two scale costs a
+// floating-point code nothing (but at its subnormals) and makes both the
+// division before the rounding and the product on reading exact, so the one
+// rounding is that to e4m3. For int8 the quotient is taken as the correctly
+// rounded fp32 quotient of 127 x (exact: 8 + 7 bits) and max|x|: an exact
+// half is representable and stays one, and a quotient that is not a half
+// differs from it by more than the quotient's rounding error (bf16 operands),
+// so the codes are those of real arithmetic. A row with a value that is not
+// finite gets the scale NaN, and reads back as NaN throughout; an all-zero
+// row has scale 0.
+//
+// Both kernels are bound by memory: a group of D / 8 lanes holds a row of k
+// and the row of v at the same place, 16 bytes of bf16 a lane each, and the
+// maximum crosses the group with shuffles, so a row is read once and written
+// once.
+#include "kvcache.cuh"
+
+#include <cuda_fp8.h>
+
+namespace veda {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// The sequence that packed row t belongs to: offsets[b] <= t < offsets[b+1].
+__device__ __forceinline__ int find_sequence(const int32_t* offsets, int n,
+                                             int64_t t) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (offsets[mid] <= t)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void unpack8(const uint4& w, float* x) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(u[i] << 16);
+    x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+  }
+}
+
+// Codes of a lane's 8 values of a row and the row's scale. kGroup lanes hold
+// the row.
+template <int kStore, int kGroup>
+__device__ __forceinline__ uint2 encode8(const uint4& w, float* scale) {
+  float x[8];
+  unpack8(w, x);
+  float top = 0.f;
+  // NaN must not vanish in the maximum: it is carried as infinity.
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    top = fmaxf(top, x[i] == x[i] ? fabsf(x[i]) : INFINITY);
+#pragma unroll
+  for (int s = kGroup / 2; s > 0; s >>= 1)
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+  uint32_t word[2] = {0u, 0u};
+  if (top == INFINITY) {
+    *scale = __int_as_float(0x7fffffff);
+    return make_uint2(0u, 0u);
+  }
+  if (top == 0.f) {
+    *scale = 0.f;
+    return make_uint2(0u, 0u);
+  }
+  if constexpr (kStore == kStoreInt8) {
+    *scale = __fdiv_rn(top, 127.f);
+    // Large rows are brought down by a power of two: 127 x stays finite.
+    const float pre = top > 1.f ? 0x1p-8f : 1.f;
+    const float den = top * pre, num = 127.f * pre;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = __float2int_rn(__fdiv_rn(x[i] * num, den));
+      word[i >> 2] |= (static_cast<uint32_t>(c) & 0xffu) << (8 * (i & 3));
+    }
+  } else {
+    // top = 1.f 2^x: 448 = 1.75 2^8. Subnormal tops end at the clamp.
+    const uint32_t bits = __float_as_uint(top);
+    int e = static_cast<int>(bits >> 23) - 127 - 8 +
+            ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    if (e < -120) e = -120;
+    *scale = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+    const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_fp8x2_storage_t c = __nv_cvt_float2_to_fp8x2(
+          make_float2(x[2 * i] * inv, x[2 * i + 1] * inv), __NV_SATFINITE,
+          __NV_E4M3);
+      word[i >> 1] |= static_cast<uint32_t>(c) << (16 * (i & 1));
+    }
+  }
+  return make_uint2(word[0], word[1]);
+}
+
+// Eight codes times their scale, rounded once to bf16.
+template <int kStore>
+__device__ __forceinline__ uint4 decode8(const uint2& w, float scale) {
+  float x[8];
+  const uint32_t u[2] = {w.x, w.y};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t pair = (u[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+    if constexpr (kStore == kStoreInt8) {
+      x[2 * i] = static_cast<float>(static_cast<int8_t>(pair & 0xffu));
+      x[2 * i + 1] = static_cast<float>(static_cast<int8_t>(pair >> 8));
+    } else {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
+          static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3);
+      const float2 f = __half22float2(__half2(h));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+  return make_uint4(pack_bf16(x[0] * scale, x[1] * scale),
+                    pack_bf16(x[2] * scale, x[3] * scale),
+                    pack_bf16(x[4] * scale, x[5] * scale),
+                    pack_bf16(x[6] * scale, x[7] * scale));
+}
+
+template <int kStore, int kD>
+__global__ void __launch_bounds__(kThreads)
+    cache_write_kernel(CacheView c, const __nv_bfloat16* k, int64_t k_st,
+                       int64_t k_sh, const __nv_bfloat16* v, int64_t v_st,
+                       int64_t v_sh, const int32_t* offsets,
+                       const int32_t* starts, int64_t n_rows,
+                       unsigned int* status) {
+  constexpr int kGroup = kD / 8;
+  const int64_t row =
+      (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kGroup;
+  const int lane = threadIdx.x % kGroup;
+  // A group past the end repeats the last row's work without storing it: the
+  // shuffles need whole warps.
+  const bool live = row < n_rows;
+  const int64_t r = live ? row : n_rows - 1;
+  const int64_t t = r / c.kv_heads;
+  const int h = static_cast<int>(r % c.kv_heads);
+  const uint4 kw = *reinterpret_cast<const uint4*>(k + t * k_st + h * k_sh +
+                                                   lane * 8);
+  const uint4 vw = *reinterpret_cast<const uint4*>(v + t * v_st + h * v_sh +
+                                                   lane * 8);
+  const int b = find_sequence(offsets, c.n_seqs, t);
+  const int64_t pos = static_cast<int64_t>(starts[b]) + (t - offsets[b]);
+  const int64_t at = cache_row(c, b, h, pos);
+  if (at < 0) {
+    if (live && lane == 0) raise_status(status, VEDA_ERR_INVALID);
+  }
+  const bool store = live && at >= 0;
+  if constexpr (kStore == kStoreBf16) {
+    if (store) {
+      reinterpret_cast<uint4*>(c.k)[at * kGroup + lane] = kw;
+      reinterpret_cast<uint4*>(c.v)[at * kGroup + lane] = vw;
+    }
+  } else {
+    float ks, vs;
+    const uint2 kc = encode8<kStore, kGroup>(kw, &ks);
+    const uint2 vc = encode8<kStore, kGroup>(vw, &vs);
+    if (store) {
+      reinterpret_cast<uint2*>(c.k)[at * kGroup + lane] = kc;
+      reinterpret_cast<uint2*>(c.v)[at * kGroup + lane] = vc;
+      if (lane == 0) {
+        c.k_scale[at] = ks;
+        c.v_scale[at] = vs;
+      }
+    }
+  }
+}
+
+template <int kStore, int kD>
+__global__ void __launch_bounds__(kThreads)
+    cache_read_kernel(CacheView c, const int32_t* offsets, int64_t n_rows,
+                      __nv_bfloat16* k, __nv_bfloat16* v,
+                      unsigned int* status) {
+  constexpr int kGroup = kD / 8;
+  const int64_t row =
+      (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kGroup;
+  const int lane = threadIdx.x % kGroup;
+  if (row >= n_rows) return;
+  const int64_t t = row / c.kv_heads;
+  const int h = static_cast<int>(row % c.kv_heads);
+  const int b = find_sequence(offsets, c.n_seqs, t);
+  const int64_t at = cache_row(c, b, h, t - offsets[b]);
+  uint4 kw = make_uint4(0, 0, 0, 0), vw = kw;
+  if (at < 0) {
+    if (lane == 0) raise_status(status, VEDA_ERR_INVALID);
+  } else if constexpr (kStore == kStoreBf16) {
+    kw = reinterpret_cast<const uint4*>(c.k)[at * kGroup + lane];
+    vw = reinterpret_cast<const uint4*>(c.v)[at * kGroup + lane];
+  } else {
+    const uint2 kc = reinterpret_cast<const uint2*>(c.k)[at * kGroup + lane];
+    const uint2 vc = reinterpret_cast<const uint2*>(c.v)[at * kGroup + lane];
+    kw = decode8<kStore>(kc, c.k_scale[at]);
+    vw = decode8<kStore>(vc, c.v_scale[at]);
+  }
+  // Packed outputs [rows, kv_heads, D]: row-major in (token, head).
+  reinterpret_cast<uint4*>(k)[row * kGroup + lane] = kw;
+  reinterpret_cast<uint4*>(v)[row * kGroup + lane] = vw;
+}
+
+// Calls fn.template operator()<kStore, kD>() for the runtime pair.
+template <typename Fn>
+int dispatch(int storage, int head_dim, Fn fn) {
+  if (head_dim == 128) {
+    if (storage == kStoreBf16) return fn.template operator()<kStoreBf16, 128>();
+    if (storage == kStoreInt8) return fn.template operator()<kStoreInt8, 128>();
+    return fn.template operator()<kStoreE4m3, 128>();
+  }
+  if (storage == kStoreBf16) return fn.template operator()<kStoreBf16, 64>();
+  if (storage == kStoreInt8) return fn.template operator()<kStoreInt8, 64>();
+  return fn.template operator()<kStoreE4m3, 64>();
+}
+
+struct WriteLaunch {
+  CacheView c;
+  const __nv_bfloat16 *k, *v;
+  int64_t k_st, k_sh, v_st, v_sh;
+  const int32_t *offsets, *starts;
+  int64_t rows;
+  unsigned int* status;
+  cudaStream_t stream;
+  template <int kStore, int kD>
+  int operator()() const {
+    const int64_t blocks = (rows * (kD / 8) + kThreads - 1) / kThreads;
+    cache_write_kernel<kStore, kD>
+        <<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
+            c, k, k_st, k_sh, v, v_st, v_sh, offsets, starts, rows, status);
+    return check_launch("cache_write_kernel");
+  }
+};
+
+struct ReadLaunch {
+  CacheView c;
+  const int32_t* offsets;
+  int64_t rows;
+  __nv_bfloat16 *k, *v;
+  unsigned int* status;
+  cudaStream_t stream;
+  template <int kStore, int kD>
+  int operator()() const {
+    const int64_t blocks = (rows * (kD / 8) + kThreads - 1) / kThreads;
+    cache_read_kernel<kStore, kD>
+        <<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
+            c, offsets, rows, k, v, status);
+    return check_launch("cache_read_kernel");
+  }
+};
+
+}  // namespace
+
+int make_cache_view(CacheView* view, void* k, void* v, float* k_scale,
+                    float* v_scale, int64_t n_pages, int32_t page_size,
+                    int32_t kv_heads, int32_t head_dim, int32_t storage,
+                    const int32_t* table, int64_t table_ld, int64_t max_pages,
+                    int64_t n_seqs) {
+  VEDA_REQUIRE(storage == kStoreBf16 || storage == kStoreInt8 ||
+                   storage == kStoreE4m3,
+               "storage must be 0 (bf16), 1 (int8) or 2 (e4m3)");
+  VEDA_REQUIRE(head_dim == 64 || head_dim == 128,
+               "head_dim must be 64 or 128");
+  int shift = 0;
+  while (shift < 9 && (1 << shift) < page_size) ++shift;
+  VEDA_REQUIRE(page_size >= 16 && page_size <= 256 &&
+                   (1 << shift) == page_size,
+               "page_size must be 16, 32, 64, 128 or 256");
+  VEDA_REQUIRE(kv_heads >= 1 && kv_heads <= 65535, "bad kv_heads");
+  VEDA_REQUIRE(n_pages >= 1 && n_pages < (int64_t(1) << 31), "bad n_pages");
+  VEDA_REQUIRE(n_seqs >= 1 && n_seqs < (int64_t(1) << 24), "bad n_seqs");
+  VEDA_REQUIRE(max_pages >= 1 && max_pages * page_size < (int64_t(1) << 31) &&
+                   table_ld >= max_pages,
+               "a table row must hold 1 page or more and address fewer than "
+               "2^31 rows");
+  VEDA_REQUIRE(k && v && table, "k, v and table are required");
+  VEDA_REQUIRE(reinterpret_cast<uintptr_t>(k) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(v) % 16 == 0,
+               "the pages must be 16-byte aligned");
+  VEDA_REQUIRE(storage == kStoreBf16 ? (!k_scale && !v_scale)
+                                     : (k_scale && v_scale),
+               "int8 and e4m3 pages have scales, bf16 pages have none");
+  VEDA_REQUIRE(storage == kStoreBf16 ||
+                   (reinterpret_cast<uintptr_t>(k_scale) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(v_scale) % 16 == 0),
+               "the scales must be 16-byte aligned");
+  view->k = static_cast<uint8_t*>(k);
+  view->v = static_cast<uint8_t*>(v);
+  view->k_scale = k_scale;
+  view->v_scale = v_scale;
+  view->n_pages = static_cast<int>(n_pages);
+  view->page_shift = shift;
+  view->kv_heads = kv_heads;
+  view->table = table;
+  view->table_ld = table_ld;
+  view->max_pages = static_cast<int>(max_pages);
+  view->n_seqs = static_cast<int>(n_seqs);
+  return VEDA_OK;
+}
+
+}  // namespace veda
+
+using namespace veda;
+
+extern "C" int veda_cache_write(
+    void* k_pages, void* v_pages, float* k_scale, float* v_scale,
+    int64_t n_pages, int32_t page_size, int32_t kv_heads, int32_t head_dim,
+    int32_t storage, const int32_t* table, int64_t table_ld, int64_t max_pages,
+    int64_t n_seqs, const void* k, int64_t k_stride_t, int64_t k_stride_h,
+    const void* v, int64_t v_stride_t, int64_t v_stride_h, int64_t n_tokens,
+    const int32_t* offsets, const int32_t* starts, void* stream) {
+  int rc = require_sm100("veda_cache_write");
+  if (rc != VEDA_OK) return rc;
+  CacheView c;
+  rc = make_cache_view(&c, k_pages, v_pages, k_scale, v_scale, n_pages,
+                       page_size, kv_heads, head_dim, storage, table, table_ld,
+                       max_pages, n_seqs);
+  if (rc != VEDA_OK) return rc;
+  VEDA_REQUIRE(n_tokens >= 0 && n_tokens * kv_heads < (int64_t(1) << 31),
+               "n_tokens * kv_heads must lie in [0, 2^31)");
+  VEDA_REQUIRE(offsets && starts, "offsets and starts are required");
+  if (n_tokens == 0) return VEDA_OK;
+  VEDA_REQUIRE(k && v, "k and v are required");
+  auto aligned = [](const void* p, int64_t st, int64_t sh) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && st % 8 == 0 &&
+           sh % 8 == 0;
+  };
+  VEDA_REQUIRE(aligned(k, k_stride_t, k_stride_h) &&
+                   aligned(v, v_stride_t, v_stride_h),
+               "k and v must be 16-byte aligned with strides multiple of 8");
+  WriteLaunch launch{c,
+                     static_cast<const __nv_bfloat16*>(k),
+                     static_cast<const __nv_bfloat16*>(v),
+                     k_stride_t,
+                     k_stride_h,
+                     v_stride_t,
+                     v_stride_h,
+                     offsets,
+                     starts,
+                     n_tokens * kv_heads,
+                     device_status_ptr(),
+                     as_stream(stream)};
+  return dispatch(storage, head_dim, launch);
+}
+
+extern "C" int veda_cache_read(
+    const void* k_pages, const void* v_pages, const float* k_scale,
+    const float* v_scale, int64_t n_pages, int32_t page_size, int32_t kv_heads,
+    int32_t head_dim, int32_t storage, const int32_t* table, int64_t table_ld,
+    int64_t max_pages, int64_t n_seqs, const int32_t* offsets,
+    int64_t n_tokens, void* k, void* v, void* stream) {
+  int rc = require_sm100("veda_cache_read");
+  if (rc != VEDA_OK) return rc;
+  CacheView c;
+  rc = make_cache_view(&c, const_cast<void*>(k_pages),
+                       const_cast<void*>(v_pages),
+                       const_cast<float*>(k_scale),
+                       const_cast<float*>(v_scale), n_pages, page_size,
+                       kv_heads, head_dim, storage, table, table_ld, max_pages,
+                       n_seqs);
+  if (rc != VEDA_OK) return rc;
+  VEDA_REQUIRE(n_tokens >= 0 && n_tokens * kv_heads < (int64_t(1) << 31),
+               "n_tokens * kv_heads must lie in [0, 2^31)");
+  VEDA_REQUIRE(offsets != nullptr, "offsets are required");
+  if (n_tokens == 0) return VEDA_OK;
+  VEDA_REQUIRE(k && v && reinterpret_cast<uintptr_t>(k) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(v) % 16 == 0,
+               "k and v are required, 16-byte aligned");
+  ReadLaunch launch{c,
+                    offsets,
+                    n_tokens * kv_heads,
+                    static_cast<__nv_bfloat16*>(k),
+                    static_cast<__nv_bfloat16*>(v),
+                    device_status_ptr(),
+                    as_stream(stream)};
+  return dispatch(storage, head_dim, launch);
+}

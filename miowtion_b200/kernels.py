@@ -132,6 +132,34 @@ def _require(q: torch.Tensor, op: str) -> None:
             'to dense attention')
 
 
+def softmax_scale(scale: float | None, dim: int) -> float:
+    """The softmax scale of a call: `scale`, or dim ** -0.5 for None."""
+    if scale is None:
+        return dim ** -0.5
+    scale = float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f'scale must be positive and finite: {scale}')
+    return scale
+
+
+def aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """t [rows, heads, D] as the kernels read it (16-byte pieces of a row):
+    itself, or a contiguous copy where its address or strides do not allow
+    that."""
+    if t.data_ptr() % 16 == 0 and t.stride(2) == 1 and all(
+            s >= 0 and s % 8 == 0 for s in t.stride()[:2]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def on_stream(t: torch.Tensor) -> torch.Tensor:
+    """t, kept alive for the work of the current stream: a pack's tensors
+    may be dropped by their owner while another stream still reads them."""
+    if not torch.cuda.is_current_stream_capturing():
+        t.record_stream(torch.cuda.current_stream(t.device))
+    return t
+
+
 def block_sparse_attention_lists(q: torch.Tensor, k: torch.Tensor,
                                  v: torch.Tensor,
                                  lists: veda_mask.BlockLists,

@@ -1,0 +1,178 @@
+"""Sequences of different lengths packed into one run of rows.
+
+    pack = SequencePack(q_lengths, k_lengths)      # once per batch
+    out = kernels.causal_attention(q, k, v, pack)  # every layer
+
+The counterpart, for packed sequences, of the tile layout of a clip: the row
+offsets on the device and, per number of query heads that share a key head,
+the work tables that the attention kernels walk. All of it comes from the
+lengths on the host, so a pack that exists is consistent, and no call that
+uses it reads the device.
+"""
+
+from __future__ import annotations
+
+import dataclasses
+from typing import Sequence
+
+import numpy as np
+import torch
+
+# Rows of a query tile and keys of a key tile of the attention kernels.
+TILE = 128
+# Fields of a work item (one int32 each; csrc/causal.cuh).
+ITEM_FIELDS = 8
+
+
+@dataclasses.dataclass(frozen=True)
+class WorkTables:
+    """Work items of one group size: forward (pairs of query tiles), query
+    gradient (query tiles) and key gradient (key tiles), each [n, 8] int32 on
+    the device, longest first; `n_tiles` query tiles in all."""
+
+    group: int
+    forward: torch.Tensor
+    query: torch.Tensor
+    key: torch.Tensor
+    n_tiles: int
+
+
+class SequencePack:
+    """Row ranges of packed sequences.
+
+    Sequence b owns `q_lengths[b]` consecutive query rows and `k_lengths[b]`
+    consecutive key rows (the same rows by default). Its queries are the last
+    tokens of its keys: query i sees keys j <= i + k_length - q_length. With
+    fewer keys than queries the first rows see none. Any length may be zero.
+
+    Args:
+        q_lengths: Query rows of each sequence (host integers).
+        k_lengths: Key rows of each sequence; None for q_lengths.
+        device: CUDA device of the offsets and tables.
+    """
+
+    def __init__(self, q_lengths: Sequence[int],
+                 k_lengths: Sequence[int] | None = None,
+                 device: torch.device | str = 'cuda'):
+        self.q_lengths = _lengths(q_lengths, 'q_lengths')
+        self.k_lengths = (self.q_lengths if k_lengths is None
+                          else _lengths(k_lengths, 'k_lengths'))
+        if self.q_lengths.size != self.k_lengths.size:
+            raise ValueError('q_lengths and k_lengths must name the same '
+                             f'sequences: {self.q_lengths.size} and '
+                             f'{self.k_lengths.size}')
+        self.device = torch.device(device)
+        if self.device.type == 'cuda' and self.device.index is None:
+            self.device = torch.device('cuda', torch.cuda.current_device())
+        self.total_q = int(self.q_lengths.sum())
+        self.total_k = int(self.k_lengths.sum())
+        if max(self.total_q, self.total_k) >= 2 ** 31 - 2 * TILE:
+            raise ValueError('a pack holds fewer than 2^31 - 256 rows')
+        self._q0 = np.concatenate([[0], np.cumsum(self.q_lengths)])
+        self._k0 = np.concatenate([[0], np.cumsum(self.k_lengths)])
+        both = _to_device(np.stack([self._q0, self._k0]), self.device)
+        self.q_offsets, self.k_offsets = both[0], both[1]
+        self._tables: dict[int, WorkTables] = {}
+
+    @property
+    def n_sequences(self) -> int:
+        return self.q_lengths.size
+
+    @property
+    def single_tokens(self) -> bool:
+        """Every sequence has exactly one query."""
+        return bool((self.q_lengths == 1).all())
+
+    @property
+    def whole(self) -> bool:
+        """No sequence has keys before (or without) its queries."""
+        return bool((self.q_lengths == self.k_lengths).all())
+
+    def tables(self, group: int) -> WorkTables:
+        """The work tables for `group` query heads per key head, built (and
+        copied to the device) on first use; build them before capturing a
+        CUDA graph."""
+        if group not in self._tables:
+            if (self.device.type == 'cuda'
+                    and torch.cuda.is_current_stream_capturing()):
+                raise RuntimeError(
+                    'the work tables of this pack do not exist yet: call '
+                    f'tables({group}) or run once before the capture')
+            forward, query, key, n = work_items(
+                self.q_lengths, self.k_lengths, group)
+            flat = _to_device(np.concatenate([forward, query, key]),
+                              self.device)
+            a, b = len(forward), len(forward) + len(query)
+            self._tables[group] = WorkTables(group, flat[:a], flat[a:b],
+                                             flat[b:], n)
+        return self._tables[group]
+
+
+def _lengths(values: Sequence[int], name: str) -> np.ndarray:
+    if isinstance(values, torch.Tensor):
+        if values.is_cuda:
+            raise ValueError(f'{name} must be host integers (a CUDA tensor '
+                             'would have to be read back)')
+        values = values.numpy()
+    out = np.asarray(values)
+    if out.ndim != 1 or out.size == 0 or out.dtype.kind not in 'iu':
+        raise ValueError(f'{name} must be a non-empty list of integers')
+    out = out.astype(np.int64)
+    if (out < 0).any():
+        raise ValueError(f'{name} must not be negative')
+    if (out >= 2 ** 31).any():
+        raise ValueError(f'{name} must be below 2^31')
+    return out
+
+
+def _to_device(values: np.ndarray, device: torch.device) -> torch.Tensor:
+    host = torch.from_numpy(np.ascontiguousarray(values, dtype=np.int32))
+    return host.to(device)
+
+
+def _expand(counts: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+    """(sequence, index inside it) of each of counts.sum() elements."""
+    seq = np.repeat(np.arange(counts.size), counts)
+    first = np.cumsum(counts) - counts
+    return seq, np.arange(seq.size) - first[seq]
+
+
+def work_items(q_lengths: np.ndarray, k_lengths: np.ndarray, group: int
+               ) -> tuple[np.ndarray, np.ndarray, np.ndarray, int]:
+    """Work items of the attention kernels (int64 [n, 8] arrays; see
+    csrc/causal.cuh for the fields), longest first, and the number of query
+    tiles. A query tile is `128 // group` tokens of one sequence with the
+    `group` heads of one key head."""
+    if not 1 <= group <= TILE:
+        raise ValueError('1 to 128 query heads may share a key head: '
+                         f'{group}')
+    tokens = TILE // group
+    q0 = np.cumsum(q_lengths) - q_lengths
+    k0 = np.cumsum(k_lengths) - k_lengths
+    before = k_lengths - q_lengths  # keys before the first query
+    tiles = -(-q_lengths // tokens)
+    tile_base = np.cumsum(tiles) - tiles
+
+    def query_items(per_item: int) -> np.ndarray:
+        span = per_item * tokens
+        seq, i = _expand(-(-q_lengths // span))
+        t0 = i * span
+        n = np.minimum(span, q_lengths[seq] - t0)
+        kpos = before[seq] + t0
+        blocks = -(-np.clip(kpos + n, 0, k_lengths[seq]) // TILE)
+        items = np.stack([q0[seq] + t0, n, k0[seq], kpos, k_lengths[seq],
+                          blocks, tile_base[seq] + i * per_item,
+                          np.zeros_like(n)], axis=1)
+        return items[np.argsort(-blocks, kind='stable')]
+
+    seq, i = _expand(-(-k_lengths // TILE))
+    j0 = i * TILE
+    # Token t of the sequence sees key j0 + r if t >= shift + r.
+    shift = j0 - before[seq]
+    first = np.maximum(shift, 0) // tokens
+    blocks = np.maximum(tiles[seq] - first, 0)
+    key = np.stack([k0[seq] + j0, np.minimum(TILE, k_lengths[seq] - j0),
+                    q0[seq], q_lengths[seq], shift, first, blocks,
+                    tile_base[seq]], axis=1)
+    key = key[np.argsort(-blocks, kind='stable')]
+    return query_items(2), query_items(1), key, int(tiles.sum())

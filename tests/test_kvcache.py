@@ -1,0 +1,155 @@
+"""The paged cache and packed sequences on the host: refusals, and the work
+tables against a walk over every (query, key) pair. No GPU needed."""
+
+import numpy as np
+import pytest
+import torch
+
+from miowtion_b200 import kvcache
+from miowtion_b200 import sequences
+
+
+def pack(q, k=None):
+    return sequences.SequencePack(q, k, 'cpu')
+
+
+def cache(storage='int8', pages=4, size=16, heads=2, dim=64):
+    return kvcache.PagedCache.empty(pages, size, heads, dim, storage, 'cpu')
+
+
+@pytest.mark.parametrize('lengths, match', [
+    ([], 'non-empty'), ([1.5], 'integers'), ([3, -1], 'negative'),
+    ([[1, 2]], 'non-empty'), ([2 ** 31], 'below'),
+    ([2 ** 30, 2 ** 30], 'fewer than')])
+def test_pack_refuses(lengths, match):
+    with pytest.raises(ValueError, match=match):
+        pack(lengths)
+
+
+def test_pack_refuses_other_sequence_counts():
+    with pytest.raises(ValueError, match='same'):
+        pack([1, 2], [1, 2, 3])
+
+
+def test_pack_properties():
+    p = pack([3, 0, 5], [4, 7, 5])
+    assert (p.total_q, p.total_k, p.n_sequences) == (8, 16, 3)
+    assert p.q_offsets.tolist() == [0, 3, 3, 8]
+    assert p.k_offsets.tolist() == [0, 4, 11, 16]
+    assert not p.whole and not p.single_tokens
+    assert pack([1, 1], [5, 1]).single_tokens and pack([2, 0]).whole
+
+
+@pytest.mark.parametrize('group', [1, 3, 8, 128])
+@pytest.mark.parametrize('q, k', [
+    ([1], [1]), ([129, 0, 1], [129, 0, 1]), ([5, 300], [400, 301]),
+    ([200, 7], [90, 0]), ([0, 0], [3, 0]), ([130], [513])])
+def test_work_items_cover_every_visible_pair_once(group, q, k):
+    forward, query, key, n_tiles = sequences.work_items(
+        np.array(q), np.array(k), group)
+    tokens = 128 // group
+    p = pack(q, k)
+    want = np.zeros((p.total_q, p.total_k), bool)
+    q0, k0 = np.cumsum([0] + q), np.cumsum([0] + k)
+    for b in range(len(q)):
+        for i in range(q[b]):
+            want[q0[b] + i, k0[b]:k0[b] + max(0, i + 1 + k[b] - q[b])] = True
+    for items, per_item in ((forward, 2), (query, 1)):
+        got = np.zeros_like(want)
+        rows = np.zeros(p.total_q, int)
+        for row, n, kr, kpos, c, blocks, tile, _ in items:
+            assert 1 <= n <= per_item * tokens and 0 <= tile < n_tiles
+            rows[row:row + n] += 1
+            for t in range(n):
+                seen = min(c, max(0, kpos + t + 1))
+                assert seen <= 128 * blocks
+                got[row + t, kr:kr + seen] = True
+        assert (rows == 1).all() and np.array_equal(got, want)
+        assert (np.diff(items[:, 5]) <= 0).all()
+    got = np.zeros_like(want)
+    keys = np.zeros(p.total_k, int)
+    tiles = set()
+    for row, n, qr, nq, shift, first, blocks, base in key:
+        assert 1 <= n <= 128
+        keys[row:row + n] += 1
+        for blk in range(blocks):
+            t0 = (first + blk) * tokens
+            assert t0 < nq
+            tiles.add(base + first + blk)
+            for t in range(t0, min(nq, t0 + tokens)):
+                seen = min(n, max(0, t - shift + 1))
+                got[qr + t, row:row + seen] = True
+    assert (keys == 1).all() and np.array_equal(got, want)
+    assert tiles <= set(range(n_tiles))
+
+
+def test_group_is_bounded():
+    for group in (0, 129):
+        with pytest.raises(ValueError, match='share'):
+            sequences.work_items(np.array([4]), np.array([4]), group)
+
+
+def test_cache_refuses_wrong_pages():
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.int8)
+    s = torch.zeros(4, 2, 16)
+    good = dict(k=k, v=k, k_scale=s, v_scale=s)
+    kvcache.PagedCache(**good)
+    for change, match in [
+            (dict(v=k[:3]), 'one shape'), (dict(k_scale=None), 'scales'),
+            (dict(v_scale=s.double()), 'scales'),
+            (dict(k_scale=s[:, :, :8]), 'scales'),
+            (dict(k=k.float(), v=k.float()), 'pages are'),
+            (dict(k=k.bfloat16(), v=k.bfloat16()), 'no scales'),
+            (dict(k=k.transpose(0, 1), v=k.transpose(0, 1),
+                  k_scale=s.transpose(0, 1), v_scale=s.transpose(0, 1)),
+             'contiguous')]:
+        with pytest.raises(ValueError, match=match):
+            kvcache.PagedCache(**{**good, **change})
+    for size, dim, match in [(8, 64, 'page_size'), (24, 64, 'page_size'),
+                             (512, 64, 'page_size'), (16, 96, 'head dim')]:
+        with pytest.raises(ValueError, match=match):
+            cache(size=size, dim=dim)
+    with pytest.raises(ValueError, match='storage'):
+        cache('fp4')
+
+
+def test_cache_calls_refuse_wrong_arguments():
+    c = cache()
+    p = pack([3, 2])
+    k = torch.zeros(5, 2, 64, dtype=torch.bfloat16)
+    table = torch.zeros(2, 1, dtype=torch.int32)
+    starts = torch.zeros(2, dtype=torch.int32)
+    for args, match in [
+            ((k[:4], k, table, starts, p), 'k must be'),
+            ((k, k.float(), table, starts, p), 'v must be'),
+            ((k, k, table.long(), starts, p), 'table must be'),
+            ((k, k, table[:1], starts, p), 'table must be'),
+            ((k, k, table[:, :0], starts, p), 'one page'),
+            ((k, k, table, starts[:1], p), 'starts must be')]:
+        with pytest.raises(ValueError, match=match):
+            c.write(*args)
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    for args, match in [
+            ((q[:, :3], table, starts), 'multiple'),
+            ((q[:, :, :32], table, starts), 'q must be'),
+            ((q.float(), table, starts), 'q must be'),
+            ((q, table, starts.float()), 'lengths must be'),
+            ((q, table, starts, 0.0), 'scale'),
+            ((q, table, starts, float('nan')), 'scale'),
+            ((q.clone().requires_grad_(), table, starts), 'no gradient')]:
+        with pytest.raises(ValueError, match=match):
+            c.attend(*args)
+    with pytest.raises(ValueError, match='table must be'):
+        c.read(table[:1], p)
+
+
+def test_cache_calls_refuse_to_fall_back():
+    c = cache('bf16')
+    p = pack([1])
+    k = torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    table = torch.zeros(1, 1, dtype=torch.int32)
+    one = torch.zeros(1, dtype=torch.int32)
+    for call in (lambda: c.write(k, k, table, one, p),
+                 lambda: c.read(table, p), lambda: c.attend(k, table, one)):
+        with pytest.raises(NotImplementedError, match='unavailable'):
+            call()
