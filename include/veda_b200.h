@@ -496,6 +496,29 @@ int veda_compensate(const void* o_kept, int64_t ok_stride_n,
                     float softmax_scale, void* workspace,
                     int64_t workspace_bytes, void* stream);
 
+/* ---- causal attention of packed sequences -------------------------------- */
+/* No counterpart in the reference (its attention is bidirectional over one
+ * clip, with as many key heads as query heads).
+ *
+ * q [total_q, n_heads, head_dim], k and v [total_k, kv_heads, head_dim] bf16,
+ * head_dim 64 or 128, n_heads a multiple (up to 128) of kv_heads; query head
+ * h reads key head h / (n_heads / kv_heads). Sequences own consecutive rows;
+ * token i of a sequence of n queries and c keys sees keys j <= i + c - n. The
+ * work items describe the sequences (miowtion_b200/sequences.py builds them;
+ * csrc/causal.cuh gives the fields) and must agree with the sizes. */
+
+/* out [total_q, n_heads, head_dim] bf16, lse (fp32, or NULL): the
+ * log-sum-exp of the scaled scores; 0 and -inf for a token without keys.
+ * items: n_items forward work items. */
+int veda_causal_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                    const void* k, int64_t k_stride_t, int64_t k_stride_h,
+                    const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                    int64_t total_q, int64_t total_k, int32_t n_heads,
+                    int32_t kv_heads, int32_t head_dim, const int32_t* items,
+                    int64_t n_items, void* out, int64_t out_stride_t,
+                    int64_t out_stride_h, float* lse, int64_t lse_stride_t,
+                    int64_t lse_stride_h, float softmax_scale, void* stream);
+
 /* ---- the paged key-value cache ------------------------------------------- */
 /* No counterpart in the reference (it attends over one clip at a time).
  *

@@ -128,6 +128,10 @@ SIGNATURES = {
                                 c_i64, c_i32, c_i64, c_i64, c_ptr, c_ptr,
                                 c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_i64,
                                 c_i64, c_f32, c_ptr, c_i64, c_ptr]),
+    'veda_causal_fwd': (c_i32, [c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64,
+                                c_ptr, c_i64, c_i64, c_i64, c_i64, c_i32,
+                                c_i32, c_i32, c_ptr, c_i64, c_ptr, c_i64,
+                                c_i64, c_ptr, c_i64, c_i64, c_f32, c_ptr]),
     'veda_cache_write': (c_i32, _CACHE + [c_ptr, c_i64, c_i64, c_ptr, c_i64,
                                           c_i64, c_i64, c_ptr, c_ptr, c_ptr]),
     'veda_cache_read': (c_i32, _CACHE + [c_ptr, c_i64, c_ptr, c_ptr, c_ptr]),

@@ -7,6 +7,7 @@
 #include <mutex>
 #include <string>
 
+#include "causal.cuh"
 #include "common.cuh"
 
 namespace veda {
@@ -179,6 +180,52 @@ int make_box_map(CUtensorMap* map, const void* base, const int grid[3],
   }
   return VEDA_OK;
 }
+
+namespace causal {
+
+int make_rows_map(CUtensorMap* map, const void* base, int64_t rows,
+                  int64_t heads, int head_dim, int64_t stride_row,
+                  int64_t stride_head, int heads_box, int rows_box,
+                  const char* name) {
+  auto fn = encode_fn();
+  if (fn == nullptr)
+    return set_error(VEDA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  // Strides of dimensions of one element are not used, but must be valid.
+  if (heads == 1) stride_head = head_dim;
+  if (rows == 1) stride_row = heads * static_cast<int64_t>(head_dim);
+  if (reinterpret_cast<uintptr_t>(base) % 16 != 0 || stride_row % 8 != 0 ||
+      stride_head % 8 != 0 || stride_row < 0 || stride_head < 0)
+    return set_error(VEDA_ERR_INVALID,
+                     std::string(name) +
+                         ": base address and row/head strides must be "
+                         "16-byte aligned for TMA");
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim),
+                        static_cast<cuuint64_t>(heads),
+                        static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride_head * 2),
+                           static_cast<cuuint64_t>(stride_row * 2)};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(heads_box),
+                       static_cast<cuuint32_t>(rows_box)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                  const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    char buf[200];
+    snprintf(buf, sizeof(buf),
+             "%s: cuTensorMapEncodeTiled failed (%d) for rows=%lld "
+             "heads=%lld strides=(%lld,%lld)",
+             name, static_cast<int>(r), static_cast<long long>(rows),
+             static_cast<long long>(heads), static_cast<long long>(stride_row),
+             static_cast<long long>(stride_head));
+    return set_error(VEDA_ERR_INVALID, buf);
+  }
+  return VEDA_OK;
+}
+
+}  // namespace causal
 
 // ---------------------------------------------------------------------------
 // UMMA layout probe: one 128x128x128 MMA, operands as the attention kernels

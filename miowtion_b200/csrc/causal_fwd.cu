@@ -1,0 +1,623 @@
+// Causal attention of packed sequences with grouped heads, forward.
+//
+// Token i of a sequence with n queries and c keys sees keys j <= i + c - n:
+//     out_i = sum_j softmax_j(scale q_i . k_j) v_j,
+//     lse_i = log sum_j exp(scale q_i . k_j);  no keys: out 0, lse -inf.
+//
+// A persistent kernel, one CTA per SM, on tcgen05. A CTA holds two query
+// tiles A and B of one key head (causal.cuh: 128 rows of tokens x heads) and
+// streams the key and value tiles of 128 keys once for both. Tensor memory:
+//     S_A [0,128)  S_B [128,256)  O_A [256,384)  O_B [384,512) columns
+//   warps 0-7   softmax and epilogue: warps 4g .. 4g + 3 own tile g, a query
+//               row a thread over all 128 keys, with the running maximum and
+//               sum of an online softmax (the maximum moves only when it
+//               grows by more than 2^8, then O is rescaled). P goes back over
+//               S as bf16, in two halves of 64 keys.
+//   warp 8      TMA producer: the two Q tiles of an item, then its K and V
+//               tiles through one ring, V one tile behind K.
+//   warp 9      S = Q K^T of both tiles (owner of the tensor memory).
+//   warp 10     O += P V of both tiles.
+//   warp 11     idle; it completes the third warpgroup, whose registers go to
+//               the softmax warps (setmaxnreg).
+// While one tile's softmax runs the tensor core has the other tile's
+// products. Rows past a sequence's end belong to the next sequence (or to
+// nothing): their scores are set to -inf by selection and the value rows are
+// cleared in shared memory, so what stands there, NaN included, reaches no
+// row of this sequence.
+//
+// All waits are bounded (common.cuh).
+#include "causal.cuh"
+
+namespace veda {
+namespace causal {
+
+namespace {
+
+constexpr int kWarps = 12;
+constexpr int kProducer = 8, kQk = 9, kPv = 10;
+constexpr uint32_t kTmemCols = 512;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.69314718055994531f;
+
+template <int kD>
+struct Fwd {
+  static constexpr uint32_t kTileBytes = kTile * kD * 2;
+  static constexpr int kRing = kD == 128 ? 5 : 8;
+  static constexpr int kSmem = (2 + kRing) * kTileBytes + 512 + 1024;
+  static constexpr int kSteps = kD / 16;  // K-steps of Q K^T
+};
+
+enum Bar {
+  kQFull = 0,   // Q of the item landed
+  kQEmpty,      // the item's last S products finished
+  kSFull,       // [2] S of the tile's block finished
+  kPHalfA = kSFull + 2,   // [2] P of keys 0-63 written (4 warps)
+  kPHalfB = kPHalfA + 2,  // [2] P of keys 64-127 written (4 warps)
+  kPvDone = kPHalfB + 2,  // [2] O += P V of the tile's block finished
+  kODone = kPvDone + 2,   // the item's last products finished
+  kOFree,                 // the epilogue has read O (8 warps)
+  kDrainQk,
+  kDrainPv,
+  kFull,                  // [kRing]
+  kEmpty = kFull + 8,     // [kRing]
+  kNumBars = kEmpty + 8
+};
+
+struct FwdParams {
+  const int32_t* table;
+  int entries;
+  int kv_heads;
+  int group;
+  int tokens;    // of a query tile: 128 / group
+  __nv_bfloat16* out;
+  int64_t out_st, out_sh;
+  float* lse;    // or null
+  int64_t lse_st, lse_sh;
+  float scale_log2;
+  unsigned int* status;
+};
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+__device__ __forceinline__ float row_max32(const float* s) {
+  float m[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m[i] = max3(s[i], s[8 + i], s[16 + i]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m[i] = fmaxf(m[i], s[24 + i]);
+  return max3(max3(m[0], m[1], m[2]), max3(m[3], m[4], m[5]),
+              fmaxf(m[6], m[7]));
+}
+
+// exp2(s * scale - m) of 32 scores, as bf16 pairs into r; returns their sum.
+__device__ __forceinline__ float2 weights32(uint32_t* r, const float* s,
+                                            float2 scale2, float2 neg_m2) {
+  float2 sum_a = make_float2(0.f, 0.f), sum_b = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int c = 0; c < 32; c += 4) {
+    const float2 x0 = __ffma2_rn(make_float2(s[c], s[c + 1]), scale2, neg_m2);
+    const float2 x1 =
+        __ffma2_rn(make_float2(s[c + 2], s[c + 3]), scale2, neg_m2);
+    const float2 e0 = make_float2(ex2_approx(x0.x), ex2_approx(x0.y));
+    const float2 e1 = make_float2(ex2_approx(x1.x), ex2_approx(x1.y));
+    sum_a = __fadd2_rn(sum_a, e0);
+    sum_b = __fadd2_rn(sum_b, e1);
+    r[c / 2] = pack_bf16(e0.x, e0.y);
+    r[c / 2 + 1] = pack_bf16(e1.x, e1.y);
+  }
+  return __fadd2_rn(sum_a, sum_b);
+}
+
+__device__ __forceinline__ void rescale16(uint32_t t_row, float alpha) {
+  uint32_t o[16];
+  tmem_ld16(t_row, o);
+  tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+  tmem_st16(t_row, o);
+  tmem_wait_st();
+}
+
+// Position in the ring's sequence of the K and V tiles of block j of an item
+// of n blocks: K0, K1, V0, K2, V1, ..., K(n-1), V(n-2), V(n-1).
+__device__ __forceinline__ int k_place(int j) { return j == 0 ? 0 : 2 * j - 1; }
+__device__ __forceinline__ int v_place(int j, int n) {
+  return j == n - 1 ? 2 * n - 1 : 2 * j + 2;
+}
+
+template <int kD>
+__global__ void __launch_bounds__(32 * kWarps, 1)
+    causal_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
+                      const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v,
+                      const __grid_constant__ FwdParams p) {
+  using C = Fwd<kD>;
+  constexpr int kRing = C::kRing;
+  constexpr uint32_t kTileBytes = C::kTileBytes;
+  constexpr uint32_t kTileUnits = kTileBytes >> 4;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* s_q = smem;                     // [2] tiles
+  uint8_t* s_ring = smem + 2 * kTileBytes;  // [kRing] tiles
+  uint64_t* bars =
+      reinterpret_cast<uint64_t*>(smem + (2 + kRing) * kTileBytes);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int tid = threadIdx.x;
+  const int warp = tid / 32;
+  const int lane = tid % 32;
+  const int64_t n_items = static_cast<int64_t>(p.entries) * p.kv_heads;
+
+  if (tid == 0) {
+    for (int b = 0; b < kNumBars; ++b) {
+      uint32_t count = 1;
+      if (b >= kPHalfA && b < kPvDone) count = 4;
+      if (b == kOFree) count = 8;
+      mbar_init(&bars[b], count);
+    }
+    *abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == kQk) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= kProducer) {
+    // 3 warpgroups x 128 threads x 168 registers = 2 x 128 x 216 + 128 x 72.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == kProducer) {
+      // ---------------- TMA producer ----------------
+      if (lane == 0) {
+        prefetch_tensor_map(&map_q);
+        prefetch_tensor_map(&map_k);
+        prefetch_tensor_map(&map_v);
+      }
+      const uint32_t q_bytes = 2u * p.group * p.tokens * kD * 2;
+      int n_ring = 0, q_loads = 0;
+      bool run = true;
+      // One K or V tile (rows k_row ..) into the ring's next place.
+      auto load = [&](const CUtensorMap* map, int h, int row) -> bool {
+        const int slot = n_ring % kRing;
+        if (n_ring >= kRing && !wait_all(&bars[kEmpty + slot],
+                                         ((n_ring / kRing) - 1) & 1, abort,
+                                         p.status))
+          return false;
+        if (lane == 0) {
+          uint8_t* dst = s_ring + slot * kTileBytes;
+          mbar_arrive_expect_tx(&bars[kFull + slot], kTileBytes);
+#pragma unroll
+          for (int c = 0; c < kD / 64; ++c)
+            tma_load_3d(dst + c * 16384, map, &bars[kFull + slot], c * 64, h,
+                        row);
+        }
+        __syncwarp();
+        ++n_ring;
+        return true;
+      };
+      for (int t = 0; run; ++t) {
+        const int64_t i = turn(t);
+        if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
+        if (i >= n_items) continue;
+        const int h = static_cast<int>(i % p.kv_heads);
+        const QueryItem it =
+            load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads));
+        if (it.blocks == 0) continue;
+        if (q_loads > 0 && !wait_all(&bars[kQEmpty], (q_loads - 1) & 1, abort,
+                                     p.status))
+          break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars[kQFull], q_bytes);
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int c = 0; c < kD / 64; ++c)
+              tma_load_3d(s_q + g * kTileBytes + c * 16384, &map_q,
+                          &bars[kQFull], c * 64, h * p.group,
+                          it.row + g * p.tokens);
+        }
+        __syncwarp();
+        ++q_loads;
+        for (int j = 0; run && j < it.blocks; ++j) {
+          run = load(&map_k, h, it.k_row + j * kTile);
+          if (run && j >= 1)
+            run = load(&map_v, h, it.k_row + (j - 1) * kTile);
+        }
+        if (run) run = load(&map_v, h, it.k_row + (it.blocks - 1) * kTile);
+      }
+      if (lane == 0 && *abort) {
+        // Let the copies in flight land before the CTA retires.
+        volatile int never = 0;
+        if (q_loads > 0)
+          mbar_wait(&bars[kQFull], (q_loads - 1) & 1, &never, nullptr);
+        for (int k = n_ring - kRing; k < n_ring; ++k)
+          if (k >= 0)
+            mbar_wait(&bars[kFull + k % kRing], (k / kRing) & 1, &never,
+                      nullptr);
+      }
+    } else if (warp == kQk) {
+      // ---------------- S = Q K^T ----------------
+      constexpr uint32_t idesc = idesc_bf16(128, 128, false, false);
+      const uint32_t q_lo = sw128_desc_lo(smem_u32(s_q), 16);
+      const uint32_t r_lo = sw128_desc_lo(smem_u32(s_ring), 16);
+      uint32_t b = 0;
+      int base = 0, items = 0;
+      bool ok = true;
+      for (int t = 0; ok; ++t) {
+        const int64_t i = turn(t);
+        if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
+        if (i >= n_items) continue;
+        const int n =
+            load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads))
+                .blocks;
+        if (n == 0) continue;
+        for (int j = 0; j < n; ++j, ++b) {
+          const int place = base + k_place(j);
+          const int slot = place % kRing;
+          if (!wait_all(&bars[kFull + slot], (place / kRing) & 1, abort,
+                        p.status) ||
+              (j == 0 &&
+               !wait_all(&bars[kQFull], items & 1, abort, p.status))) {
+            ok = false;
+            break;
+          }
+          for (int g = 0; g < 2; ++g) {
+            // S held the P of the tile's previous block until its product.
+            if (b >= 1 && !wait_all(&bars[kPvDone + g], (b - 1) & 1, abort,
+                                    p.status)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a = q_lo + g * kTileUnits;
+            const uint32_t bk = r_lo + slot * kTileUnits;
+#pragma unroll
+            for (int kk = 0; kk < C::kSteps; ++kk) {
+              const uint32_t off = (kk >> 2) * (16384 >> 4) + (kk & 3) * 2;
+              umma_ss_warp(tmem + g * 128, a + off, bk + off, idesc,
+                           kk > 0 ? 1u : 0u);
+            }
+            umma_commit_warp(&bars[kSFull + g]);
+          }
+          if (!ok) break;
+          umma_commit_warp(&bars[kEmpty + slot]);
+          if (j == n - 1) umma_commit_warp(&bars[kQEmpty]);
+        }
+        base += 2 * n;
+        ++items;
+      }
+      if (*abort) {
+        volatile int never = 0;
+        umma_commit_warp(&bars[kDrainQk]);
+        mbar_wait(&bars[kDrainQk], 0, &never, nullptr);
+      }
+    } else if (warp == kPv) {
+      // ---------------- O += P V ----------------
+      constexpr uint32_t idesc = idesc_bf16(128, kD, false, true);
+      const uint32_t v_lo = sw128_desc_lo(smem_u32(s_ring), 16384);
+      uint32_t b = 0;
+      int base = 0, items = 0;
+      bool ok = true;
+      for (int t = 0; ok; ++t) {
+        const int64_t i = turn(t);
+        if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
+        if (i >= n_items) continue;
+        const QueryItem it =
+            load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads));
+        const int n = it.blocks;
+        if (n == 0) continue;
+        for (int j = 0; j < n; ++j, ++b) {
+          const int place = base + v_place(j, n);
+          const int slot = place % kRing;
+          if (!wait_all(&bars[kFull + slot], (place / kRing) & 1, abort,
+                        p.status))
+            ok = false;
+          if (ok && j == 0 && items >= 1 &&
+              !wait_all(&bars[kOFree], (items - 1) & 1, abort, p.status))
+            ok = false;
+          if (!ok) break;
+          // Rows behind the sequence's last key take no part: a weight of 0
+          // would not keep a NaN out.
+          const int rows = it.keys - j * kTile;
+          if (rows < kTile)
+            clear_rows<kD>(s_ring + slot * kTileBytes, rows, lane);
+          const uint32_t bv = v_lo + slot * kTileUnits;
+          for (int g = 0; g < 2; ++g) {
+            if (!wait_all(&bars[kPHalfA + g], b & 1, abort, p.status)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_ts_warp(tmem + 256 + g * 128, tmem + g * 128 + kk * 8,
+                           bv + kk * 128, idesc, (kk > 0 || j > 0) ? 1u : 0u);
+            if (!wait_all(&bars[kPHalfB + g], b & 1, abort, p.status)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 4; kk < 8; ++kk)
+              umma_ts_warp(tmem + 256 + g * 128, tmem + g * 128 + kk * 8,
+                           bv + kk * 128, idesc, 1u);
+            umma_commit_warp(&bars[kPvDone + g]);
+          }
+          if (!ok) break;
+          umma_commit_warp(&bars[kEmpty + slot]);
+          if (j == n - 1) umma_commit_warp(&bars[kODone]);
+        }
+        base += 2 * n;
+        ++items;
+      }
+      if (*abort) {
+        volatile int never = 0;
+        umma_commit_warp(&bars[kDrainPv]);
+        mbar_wait(&bars[kDrainPv], 0, &never, nullptr);
+      }
+    }
+  } else {
+    // ---------------- softmax and epilogue (warps 0-7) ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int grp = warp / 4;
+    const int quarter = warp % 4;
+    const int row = quarter * 32 + lane;
+    const int token = grp * p.tokens + row / p.group;  // of the item
+    const int head = row % p.group;
+    const bool row_used = row < p.tokens * p.group;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t t_s = tmem + grp * 128 + lane_base;
+    const uint32_t t_o = tmem + 256 + grp * 128 + lane_base;
+    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+    uint32_t b = 0;
+    int items = 0;
+    bool ok = true;
+    for (int t = 0; ok; ++t) {
+      const int64_t i = turn(t);
+      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
+      if (i >= n_items) continue;
+      const int h = static_cast<int>(i % p.kv_heads);
+      const QueryItem it =
+          load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads));
+      const int n = it.blocks;
+      // Keys of this row.
+      const int seen = max(0, min(it.keys, it.kpos + token + 1));
+      float m_ref = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j, ++b) {
+        const int visible = seen - j * kTile;
+        const bool masked = __any_sync(0xffffffffu, visible < kTile);
+        if (!wait_all(&bars[kSFull + grp], b & 1, abort, p.status)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t x[4][32];
+#pragma unroll
+        for (int q32 = 0; q32 < 4; ++q32) tmem_ld32(t_s + q32 * 32, x[q32]);
+        tmem_wait_ld();
+        if (masked) {
+#pragma unroll
+          for (int q32 = 0; q32 < 4; ++q32) {
+            const int k = visible - q32 * 32;
+            const uint32_t word =
+                k >= 32 ? ~0u : (k <= 0 ? 0u : (1u << k) - 1u);
+            float* f = reinterpret_cast<float*>(x[q32]);
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (!((word >> c) & 1u)) f[c] = -INFINITY;
+          }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int q32 = 0; q32 < 4; ++q32)
+          mx = fmaxf(mx, row_max32(reinterpret_cast<float*>(x[q32])));
+        const float mb = mx * p.scale_log2;
+        const bool grow = mb > m_ref + 8.0f;
+        if (j == 0) {
+          m_ref = mb;
+        } else if (__any_sync(0xffffffffu, grow)) {
+          const float m_new = grow ? mb : m_ref;
+          // A row without a key so far has an O of zeros.
+          const float alpha =
+              m_ref == -INFINITY ? 0.f : ex2_approx(m_ref - m_new);
+          m_ref = m_new;
+          // O holds the previous blocks once their product finished; it is
+          // rescaled before this block's P is released.
+          if (!wait_all(&bars[kPvDone + grp], (b - 1) & 1, abort, p.status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll 1
+          for (int q16 = 0; q16 < kD / 16; ++q16)
+            rescale16(t_o + q16 * 16, alpha);
+          l *= alpha;
+        }
+        const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
+        const float2 negm2 = make_float2(neg, neg);
+        float2 sums[4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int q32 = half * 2 + q;
+            sums[q32] = weights32(x[q32], reinterpret_cast<float*>(x[q32]),
+                                  scale2, negm2);
+            tmem_st16(t_s + q32 * 16, x[q32]);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive(&bars[(half == 0 ? kPHalfA : kPHalfB) + grp]);
+        }
+        l += ((sums[0].x + sums[0].y) + (sums[1].x + sums[1].y)) +
+             ((sums[2].x + sums[2].y) + (sums[3].x + sums[3].y));
+      }
+      if (!ok) break;
+      // ---------------- epilogue ----------------
+      const bool write = row_used && token < it.tokens;
+      const int64_t out_row = static_cast<int64_t>(it.row) + token;
+      const int64_t out_head = static_cast<int64_t>(h) * p.group + head;
+      __nv_bfloat16* dst = p.out + out_row * p.out_st + out_head * p.out_sh;
+      const float inv_l = l == 0.f ? 0.f : 1.0f / l;
+      if (n > 0) {
+        if (!wait_all(&bars[kODone], items & 1, abort, p.status)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+      }
+#pragma unroll 1
+      for (int c = 0; c < kD / 32; ++c) {
+        uint32_t o[32];
+        if (n > 0) {
+          tmem_ld32(t_o + c * 32, o);
+          tmem_wait_ld();
+        }
+        if (l == 0.f) {  // no key
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        if (write) {
+          uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            d4[e] = make_uint4(
+                pack_bf16(__uint_as_float(o[8 * e]) * inv_l,
+                          __uint_as_float(o[8 * e + 1]) * inv_l),
+                pack_bf16(__uint_as_float(o[8 * e + 2]) * inv_l,
+                          __uint_as_float(o[8 * e + 3]) * inv_l),
+                pack_bf16(__uint_as_float(o[8 * e + 4]) * inv_l,
+                          __uint_as_float(o[8 * e + 5]) * inv_l),
+                pack_bf16(__uint_as_float(o[8 * e + 6]) * inv_l,
+                          __uint_as_float(o[8 * e + 7]) * inv_l));
+        }
+      }
+      if (n > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[kOFree]);
+        ++items;
+      }
+      if (write && p.lse != nullptr)
+        p.lse[out_row * p.lse_st + out_head * p.lse_sh] =
+            l == 0.f ? -INFINITY : (m_ref + log2f(l)) * kLn2;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kQk) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <int kD>
+int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+           const FwdParams& p, cudaStream_t stream) {
+  int sms = 0;
+  int rc = device_sms(&sms);
+  if (rc != VEDA_OK) return rc;
+  VEDA_CUDA(cudaFuncSetAttribute(causal_fwd_kernel<kD>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 Fwd<kD>::kSmem));
+  const int cap = sms - sm_reserve() > 0 ? sms - sm_reserve() : 1;
+  const int64_t items = static_cast<int64_t>(p.entries) * p.kv_heads;
+  const int grid = static_cast<int>(items < cap ? items : cap);
+  causal_fwd_kernel<kD><<<grid, 32 * kWarps, Fwd<kD>::kSmem, stream>>>(
+      mq, mk, mv, p);
+  return check_launch("causal_fwd_kernel");
+}
+
+}  // namespace
+
+int device_sms(int* sms) {
+  int dev = 0;
+  VEDA_CUDA(cudaGetDevice(&dev));
+  VEDA_CUDA(
+      cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+  return VEDA_OK;
+}
+
+}  // namespace causal
+}  // namespace veda
+
+using namespace veda;
+
+extern "C" int veda_causal_fwd(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+    int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+    int64_t v_stride_h, int64_t total_q, int64_t total_k, int32_t n_heads,
+    int32_t kv_heads, int32_t head_dim, const int32_t* items, int64_t n_items,
+    void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse,
+    int64_t lse_stride_t, int64_t lse_stride_h, float softmax_scale,
+    void* stream) {
+  int rc = require_sm100("veda_causal_fwd");
+  if (rc != VEDA_OK) return rc;
+  VEDA_REQUIRE(head_dim == 64 || head_dim == 128,
+               "head_dim must be 64 or 128");
+  VEDA_REQUIRE(kv_heads >= 1 && n_heads >= 1 && n_heads % kv_heads == 0 &&
+                   n_heads / kv_heads <= kTile,
+               "n_heads must be 1 to 128 times kv_heads");
+  VEDA_REQUIRE(total_q >= 0 && total_k >= 0 && total_q < (int64_t(1) << 31) &&
+                   total_k < (int64_t(1) << 31) && n_items >= 0 &&
+                   n_items * kv_heads < (int64_t(1) << 40) &&
+                   n_items < (int64_t(1) << 31),
+               "bad sizes");
+  VEDA_REQUIRE(softmax_scale > 0.f && isfinite(softmax_scale),
+               "softmax_scale must be positive and finite");
+  if (total_q == 0 || n_items == 0) return VEDA_OK;
+  VEDA_REQUIRE(q && out && items, "q, out and items are required");
+  VEDA_REQUIRE(reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
+                   out_stride_t % 8 == 0 && out_stride_h % 8 == 0 &&
+                   reinterpret_cast<uintptr_t>(items) % 16 == 0,
+               "out must be 16-byte aligned with strides multiple of 8, items "
+               "16-byte aligned");
+  const int group = n_heads / kv_heads;
+  const int tokens = kTile / group;
+  CUtensorMap mq, mk, mv;
+  rc = causal::make_rows_map(&mq, q, total_q, n_heads, head_dim, q_stride_t,
+                             q_stride_h, group, tokens, "q");
+  // Without keys no item loads any; the maps then only have to exist.
+  if (total_k == 0) {
+    mk = mv = mq;
+  } else {
+    VEDA_REQUIRE(k && v, "k and v are required");
+    if (rc == VEDA_OK)
+      rc = causal::make_rows_map(&mk, k, total_k, kv_heads, head_dim,
+                                 k_stride_t, k_stride_h, 1, kTile, "k");
+    if (rc == VEDA_OK)
+      rc = causal::make_rows_map(&mv, v, total_k, kv_heads, head_dim,
+                                 v_stride_t, v_stride_h, 1, kTile, "v");
+  }
+  if (rc != VEDA_OK) return rc;
+  causal::FwdParams p{};
+  p.table = items;
+  p.entries = static_cast<int>(n_items);
+  p.kv_heads = kv_heads;
+  p.group = group;
+  p.tokens = tokens;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.out_st = out_stride_t;
+  p.out_sh = out_stride_h;
+  p.lse = lse;
+  p.lse_st = lse_stride_t;
+  p.lse_sh = lse_stride_h;
+  p.scale_log2 = softmax_scale * causal::kLog2e;
+  p.status = device_status_ptr();
+  cudaStream_t s = as_stream(stream);
+  return head_dim == 128 ? causal::launch<128>(mq, mk, mv, p, s)
+                         : causal::launch<64>(mq, mk, mv, p, s);
+}

@@ -21,6 +21,7 @@ import torch
 
 from miowtion_b200 import _lib
 from miowtion_b200 import mask as veda_mask
+from miowtion_b200 import sequences
 from miowtion_b200 import tiling
 
 _TILE = tiling.TILE_SIZE
@@ -469,3 +470,82 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             return (out, lse) if return_lse else out
         return block_sparse_attention_lists(q, k, v, lists, layout,
                                             return_lse)
+
+
+def _causal_checks(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                   pack: sequences.SequencePack) -> int:
+    """Argument checks of the causal attention; returns the heads per key
+    head."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
+        raise ValueError('q, k and v must be [rows, heads, D], k and v of '
+                         'one shape')
+    if q.shape[2] not in (64, 128) or k.shape[2] != q.shape[2]:
+        raise ValueError('q, k and v need one head dim, 64 or 128: '
+                         f'{q.shape[2]} and {k.shape[2]}')
+    heads, kv_heads = q.shape[1], k.shape[1]
+    if (kv_heads < 1 or heads % kv_heads
+            or not 1 <= heads // kv_heads <= sequences.TILE):
+        raise ValueError('the query heads must be 1 to 128 times the key '
+                         f'heads: {heads} and {kv_heads}')
+    if q.shape[0] != pack.total_q or k.shape[0] != pack.total_k:
+        raise ValueError(f'the pack has {pack.total_q} query and '
+                         f'{pack.total_k} key rows, not {q.shape[0]} and '
+                         f'{k.shape[0]}')
+    if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
+        raise ValueError('q, k and v must be bf16: '
+                         f'{q.dtype}, {k.dtype}, {v.dtype}')
+    if any(t.device != pack.device for t in (q, k, v)):
+        raise ValueError(f'q, k and v must be on {pack.device}, as the pack')
+    return heads // kv_heads
+
+
+def causal_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                         pack: sequences.SequencePack, scale: float,
+                         return_lse: bool = True):
+    """(out [rows, heads, D] bf16, lse [rows, heads] fp32 or None) of
+    `causal_attention`, without gradients."""
+    group = _causal_checks(q, k, v, pack)
+    _require(q, 'causal_attention')
+    q, k, v = aligned_rows(q), aligned_rows(k), aligned_rows(v)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = (torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+           if return_lse else None)
+    with torch.cuda.device(q.device):
+        items = on_stream(pack.tables(group).forward)
+        _lib.call('veda_causal_fwd', q.data_ptr(), q.stride(0), q.stride(1),
+                  k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                  v.stride(0), v.stride(1), q.shape[0], k.shape[0],
+                  q.shape[1], k.shape[1], q.shape[2], items.data_ptr(),
+                  items.shape[0], out.data_ptr(), out.stride(0),
+                  out.stride(1), _lib.ptr(lse),
+                  lse.stride(0) if lse is not None else 0,
+                  lse.stride(1) if lse is not None else 0, scale,
+                  _lib.stream_ptr(q.device))
+    return out, lse
+
+
+def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                     pack: sequences.SequencePack,
+                     scale: float | None = None, return_lse: bool = False):
+    """Causal attention of packed sequences with grouped heads.
+
+    Args:
+        q: [pack.total_q, heads, D] bf16, D 64 or 128.
+        k, v: [pack.total_k, kv_heads, D] bf16; heads a multiple (up to 128)
+            of kv_heads, query head h reading key head h // (heads //
+            kv_heads).
+        pack: The sequences. Query i of a sequence sees its keys
+            j <= i + k_length - q_length.
+        scale: Softmax scale; None for D ** -0.5.
+        return_lse: Also return the [total_q, heads] fp32 log-sum-exp of the
+            scaled scores (no gradient flows through it).
+
+    Returns:
+        out [total_q, heads, D] bf16 (and lse); 0 and -inf for rows without
+        keys. Rows of one sequence never reach another, whatever they hold;
+        inside a sequence a value row that is not finite may reach queries
+        before it that share its key tile.
+    """
+    scale = softmax_scale(scale, q.shape[-1])
+    out, lse = causal_attention_fwd(q, k, v, pack, scale, return_lse)
+    return (out, lse) if return_lse else out

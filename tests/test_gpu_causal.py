@@ -1,0 +1,173 @@
+"""Causal attention of packed sequences against its definition in 64 bits.
+
+Bounds count the roundings of the forward: weights to bf16 (half a step,
+2^-8, relative), the output to bf16 (2^-8) and what the fp32 scores are off,
+    |out - want| <= (2^-8 + 2 s + 2^-14) sum_j p_j |v_j| + 2^-8 |want|
+with s = (D + 8) 2^-24 A for scores of total size A = scale max_j sum_d
+|q_d k_jd| (a relative error of a weight, and again of the weights' sum).
+"""
+
+import math
+
+import pytest
+import torch
+
+from miowtion_b200 import _lib
+from miowtion_b200 import kernels
+from miowtion_b200 import sequences
+
+pytestmark = pytest.mark.gpu
+
+DEV = 'cuda'
+
+
+@pytest.fixture(autouse=True)
+def _status_clean():
+    _lib.device_status(reset=True)
+    yield
+    assert _lib.device_status(reset=True) == 0, 'the status word was set'
+
+
+def rows(n, heads, dim, seed, scale=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, heads, dim, generator=gen) * scale
+    return x.to(torch.bfloat16).to(DEV)
+
+
+def problem(q_lengths, k_lengths, heads, kv_heads, dim, seed=3, scale=1.0):
+    pack = sequences.SequencePack(q_lengths, k_lengths, DEV)
+    q = rows(pack.total_q, heads, dim, seed, scale)
+    k, v = (rows(pack.total_k, kv_heads, dim, seed + i) for i in (1, 2))
+    return pack, q, k, v
+
+
+def each_head(pack, q, k):
+    """(query rows, key rows, query head, key head, mask) of every pair."""
+    group = q.shape[1] // k.shape[1]
+    i0 = j0 = 0
+    for n, c in zip(pack.q_lengths.tolist(), pack.k_lengths.tolist()):
+        i = torch.arange(n, device=DEV)[:, None]
+        j = torch.arange(c, device=DEV)[None, :]
+        for h in range(q.shape[1]):
+            yield (slice(i0, i0 + n), slice(j0, j0 + c), h, h // group,
+                   j <= i + c - n)
+        i0, j0 = i0 + n, j0 + c
+
+
+def softmax64(q, k, sees, scale):
+    s = (scale * q @ k.T).masked_fill(~sees, -math.inf)
+    lse = torch.logsumexp(s, -1) if s.shape[1] else torch.full(
+        s.shape[:1], -math.inf, device=DEV, dtype=torch.float64)
+    p = torch.exp(s - lse[:, None]).masked_fill(~sees, 0.0)
+    return p, lse
+
+
+def check_forward(pack, q, k, v, out, lse, scale=None):
+    dim = q.shape[2]
+    scale = dim ** -0.5 if scale is None else scale
+    assert out.isfinite().all()
+    for at, keys, h, hk, sees in each_head(pack, q, k):
+        qb, kb, vb = q[at, h].double(), k[keys, hk].double(), v[
+            keys, hk].double()
+        p, want_lse = softmax64(qb, kb, sees, scale)
+        want = p @ vb
+        if kb.shape[0] == 0 or qb.shape[0] == 0:
+            assert (out[at, h] == 0).all()
+            continue
+        size = ((qb.abs() @ kb.abs().T) * sees).amax(-1) * scale
+        off = 2.0 ** -24 * (dim + 8) * size
+        bound = ((2.0 ** -8 + 2.0 ** -14 + 2 * off)[:, None] * (
+            p @ vb.abs()) + 2.0 ** -8 * want.abs() + 1e-30)
+        err = (out[at, h].double() - want).abs()
+        assert (err <= bound).all(), (h, float((err / bound).max()))
+        empty = want_lse == -math.inf
+        assert torch.equal(lse[at, h] == -math.inf, empty)
+        err = (lse[at, h].double() - want_lse).abs()[~empty]
+        bound = (off + 2.0 ** -20 * (1 + want_lse.abs()))[~empty]
+        assert (err <= bound).all(), (h, float((err / bound).max()))
+
+
+SHAPES = [
+    # q lengths, k lengths, heads, key heads
+    ([1], None, 1, 1),
+    ([128], None, 2, 2),
+    ([129, 1, 127], None, 3, 3),
+    ([300, 0, 17, 64], None, 4, 1),
+    ([5, 260], [400, 261], 6, 2),        # groups of 3: 126 rows of a tile
+    ([200, 7, 30], [90, 0, 300], 8, 1),  # rows without a key
+    ([1, 1, 1], [513, 1, 77], 14, 2),    # single tokens, groups of 7
+    ([37, 90], None, 128, 1),            # a token fills a tile
+    ([40], [170], 100, 1),
+    ([700, 650], None, 16, 2),
+]
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('q_lengths, k_lengths, heads, kv_heads', SHAPES)
+def test_forward_matches_the_definition(q_lengths, k_lengths, heads, kv_heads,
+                                        dim):
+    pack, q, k, v = problem(q_lengths, k_lengths, heads, kv_heads, dim)
+    out, lse = kernels.causal_attention(q, k, v, pack, return_lse=True)
+    check_forward(pack, q, k, v, out, lse)
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+def test_forward_of_more_items_than_processors(dim):
+    lengths = [(37 * i) % 211 for i in range(90)]
+    pack, q, k, v = problem(lengths, None, 8, 4, dim)
+    out, lse = kernels.causal_attention(q, k, v, pack, return_lse=True)
+    check_forward(pack, q, k, v, out, lse)
+
+
+def test_forward_of_scores_that_grow_along_the_keys():
+    # Maxima rise from tile to tile, so the accumulator is rescaled, and a
+    # scale of its own.
+    pack, q, k, v = problem([1000], None, 4, 2, 128)
+    ramp = torch.linspace(0.05, 6.0, 1000, device=DEV)[:, None, None]
+    k = (k.abs() * ramp).to(torch.bfloat16)
+    q = q.abs()
+    out, lse = kernels.causal_attention(q, k, v, pack, 0.05, return_lse=True)
+    check_forward(pack, q, k, v, out, lse, 0.05)
+
+
+def test_forward_of_strided_and_broadcast_inputs():
+    pack, _, _, _ = problem([200, 90], None, 4, 2, 64)
+    fused = rows(290, 8, 64, 5)
+    q, k, v = fused[:, :4], fused[:, 4:6], fused[:, 6:]
+    out, lse = kernels.causal_attention(q, k, v, pack, return_lse=True)
+    check_forward(pack, q, k, v, out, lse)
+    k = rows(290, 1, 64, 6).expand(290, 2, 64)
+    v = rows(290, 2, 65, 7)[:, :, 1:]
+    out, lse = kernels.causal_attention(q, k, v, pack, return_lse=True)
+    check_forward(pack, q, k, v, out, lse)
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+def test_sequences_do_not_reach_one_another(dim):
+    pack, q, k, v = problem([150, 70, 33], [150, 200, 33], 6, 2, dim)
+    want, want_lse = kernels.causal_attention(q, k, v, pack, return_lse=True)
+    q[150:220] = math.nan
+    k[150:350] = math.inf
+    v[150:350] = math.nan
+    out, lse = kernels.causal_attention(q, k, v, pack, return_lse=True)
+    for got, ref in ((out, want), (lse, want_lse)):
+        assert torch.equal(got[:150], ref[:150])
+        assert torch.equal(got[220:], ref[220:])
+    assert out[150:220].isnan().all()
+
+
+def test_forward_repeats_and_replays():
+    pack, q, k, v = problem([500, 120], None, 8, 2, 128)
+    want = kernels.causal_attention(q, k, v, pack)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(g, stream=side):
+        out = kernels.causal_attention(q, k, v, pack)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    fresh = sequences.SequencePack([500, 120], device=DEV)
+    with pytest.raises(RuntimeError, match='before the capture'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            kernels.causal_attention(q, k, v, fresh)
