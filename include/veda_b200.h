@@ -519,6 +519,30 @@ int veda_causal_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                     int64_t out_stride_h, float* lse, int64_t lse_stride_t,
                     int64_t lse_stride_h, float softmax_scale, void* stream);
 
+/* Bytes of workspace veda_causal_bwd needs; -1 for sizes out of range. */
+int64_t veda_causal_bwd_workspace(int32_t kv_heads, int64_t n_tiles);
+
+/* Gradients of sum(out * dout): dq of q's shape, dk and dv of k's, bf16. dq
+ * may be NULL, dk and dv together too. out and lse are the forward's;
+ * q_items and k_items the query tile and key tile work items, n_tiles the
+ * query tiles of the pack. Deterministic. */
+int veda_causal_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                    const void* k, int64_t k_stride_t, int64_t k_stride_h,
+                    const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                    const void* out, int64_t out_stride_t,
+                    int64_t out_stride_h, const void* dout,
+                    int64_t dout_stride_t, int64_t dout_stride_h,
+                    const float* lse, int64_t lse_stride_t,
+                    int64_t lse_stride_h, int64_t total_q, int64_t total_k,
+                    int32_t n_heads, int32_t kv_heads, int32_t head_dim,
+                    const int32_t* q_items, int64_t n_q_items,
+                    const int32_t* k_items, int64_t n_k_items,
+                    int64_t n_tiles, void* dq, int64_t dq_stride_t,
+                    int64_t dq_stride_h, void* dk, int64_t dk_stride_t,
+                    int64_t dk_stride_h, void* dv, int64_t dv_stride_t,
+                    int64_t dv_stride_h, float softmax_scale, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+
 /* ---- the paged key-value cache ------------------------------------------- */
 /* No counterpart in the reference (it attends over one clip at a time).
  *

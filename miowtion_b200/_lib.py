@@ -132,6 +132,12 @@ SIGNATURES = {
                                 c_ptr, c_i64, c_i64, c_i64, c_i64, c_i32,
                                 c_i32, c_i32, c_ptr, c_i64, c_ptr, c_i64,
                                 c_i64, c_ptr, c_i64, c_i64, c_f32, c_ptr]),
+    'veda_causal_bwd_workspace': (c_i64, [c_i32, c_i64]),
+    'veda_causal_bwd': (c_i32, [c_ptr, c_i64, c_i64] * 5 +
+                        [c_ptr, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32,
+                         c_i32, c_ptr, c_i64, c_ptr, c_i64, c_i64] +
+                        [c_ptr, c_i64, c_i64] * 3 +
+                        [c_f32, c_ptr, c_i64, c_ptr]),
     'veda_cache_write': (c_i32, _CACHE + [c_ptr, c_i64, c_i64, c_ptr, c_i64,
                                           c_i64, c_i64, c_ptr, c_ptr, c_ptr]),
     'veda_cache_read': (c_i32, _CACHE + [c_ptr, c_i64, c_ptr, c_ptr, c_ptr]),

@@ -1,0 +1,1035 @@
+// Causal attention of packed sequences with grouped heads, backward.
+//
+// With the forward's log-sum-exp L and D_i = rowsum(dO_i * O_i):
+//     P  = exp(S * scale - L)  (S = Q K^T; 0 where the mask hides a pair),
+//     dP = dO V^T,  dS = P * (dP - D),
+//     dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO,
+// dK and dV summed over the query heads of a key head. Query tiles hold all
+// heads of a group (causal.cuh), so that sum is one more stretch of the
+// product's depth: no atomics, no second pass, and repeats are bit-identical.
+//
+// Three launches:
+//   prep    D and L * log2(e) of each query row into the workspace, in tile
+//           order [kv_heads][tiles][128], a row without keys or token as
+//           L = inf, D = 0;
+//   dq      a query tile an item, its key tiles one after the other: S and dP
+//           (SS products), dS written back over S in tensor memory as bf16,
+//           dQ += dS K (TS product);
+//   dkdv    a key tile an item, the query tiles that see it: S^T = K Q^T and
+//           dP^T = V dO^T, P^T and dS^T written back over them, dV += P^T dO
+//           and dK += dS^T Q.
+// Each block's 128 columns run as two halves of 64, so that the tensor core
+// has one half's products while the compute warps work on the other. One CTA
+// per SM, 8 compute warps (warp w: TMEM lanes 32(w%4).., 32 of a half's
+// columns), a TMA producer warp and a converged MMA warp.
+//
+// Rows behind a sequence's end are cleared in shared memory where they are
+// the depth of a product (keys in dq, queries in dkdv); elsewhere they are
+// other rows of the result and are not stored, or masked by selection. So
+// nothing that stands there, NaN included, reaches this sequence.
+//
+// The dS of the two kernels is computed twice (7 products a block instead of
+// 5) in place of a reduction of dQ over CTAs. All waits are bounded
+// (common.cuh).
+#include "causal.cuh"
+
+namespace veda {
+namespace causal {
+
+namespace {
+
+constexpr int kThreads = 320;
+constexpr int kProducer = 8;
+constexpr int kMma = 9;
+constexpr uint32_t kTmemCols = 512;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int kD>
+struct Bwd {
+  static constexpr uint32_t kTileBytes = kTile * kD * 2;
+  static constexpr uint32_t kTileUnits = kTileBytes >> 4;
+  static constexpr int kSteps = kD / 16;
+  static constexpr int kStages = kD == 128 ? 2 : 4;  // pairs of tiles
+  static constexpr int kSmem = (2 + 2 * kStages) * kTileBytes +
+                               kStages * 1024 + 512 + 1024;
+};
+
+struct BwdParams {
+  const int32_t* table;
+  int entries;
+  int kv_heads;
+  int group;
+  int tokens;           // of a query tile
+  int n_tiles;          // query tiles of the pack
+  const float* lse2;    // [kv_heads][n_tiles][128]
+  const float* delta;   // [kv_heads][n_tiles][128]
+  __nv_bfloat16* grad;  // dq or dk
+  int64_t grad_st, grad_sh;
+  __nv_bfloat16* grad2;  // dv
+  int64_t grad2_st, grad2_sh;
+  float scale;
+  float scale_log2;
+  unsigned int* status;
+};
+
+__device__ __forceinline__ void arrive_warp(uint64_t* bar) {
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// One box (64-column pieces) of rows row .. of heads h .. into a tile.
+template <int kD>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map,
+                                          uint64_t* bar, int h, int row) {
+#pragma unroll
+  for (int c = 0; c < kD / 64; ++c)
+    tma_load_3d(dst + c * 16384, map, bar, c * 64, h, row);
+}
+
+// Writes kN bf16 columns of a row (kN / 2 words).
+template <int kN>
+__device__ __forceinline__ void store_row(__nv_bfloat16* dst,
+                                          const uint32_t* w) {
+  uint4* d4 = reinterpret_cast<uint4*>(dst);
+#pragma unroll
+  for (int i = 0; i < kN / 8; ++i)
+    d4[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+}
+
+// Reads kN fp32 TMEM columns of this thread's lane, scales them and packs
+// them to bf16 pairs.
+template <int kN>
+__device__ __forceinline__ void tmem_row_bf16(uint32_t taddr, float scale,
+                                              uint32_t* w) {
+  uint32_t o[32];
+#pragma unroll
+  for (int c = 0; c < kN / 32; ++c) {
+    tmem_ld32(taddr + c * 32, o);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      w[c * 16 + i] = pack_bf16(__uint_as_float(o[2 * i]) * scale,
+                                __uint_as_float(o[2 * i + 1]) * scale);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// prep: one warp per (query tile row, key head).
+// ---------------------------------------------------------------------------
+template <int kD>
+__global__ void causal_bwd_prep_kernel(
+    const int32_t* table, int entries, int kv_heads, int group, int tokens,
+    const __nv_bfloat16* out, int64_t o_st, int64_t o_sh,
+    const __nv_bfloat16* dout, int64_t d_st, int64_t d_sh, const float* lse,
+    int64_t l_st, int64_t l_sh, float* lse2, float* delta, int n_tiles) {
+  constexpr int kPer = kD / 32;  // elements a lane
+  const int64_t w =
+      (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
+  const int lane = threadIdx.x % 32;
+  const int r = static_cast<int>(w % kTile);
+  const int64_t u = w / kTile;
+  if (u >= static_cast<int64_t>(entries) * kv_heads) return;
+  const int h = static_cast<int>(u % kv_heads);
+  const QueryItem it =
+      load_item<QueryItem>(table, static_cast<int>(u / kv_heads));
+  const int token = r / group, head = r % group;
+  const int64_t at =
+      (static_cast<int64_t>(h) * n_tiles + it.tile) * kTile + r;
+  if (token >= it.tokens || token >= tokens) {
+    if (lane == 0) {
+      delta[at] = 0.f;
+      lse2[at] = INFINITY;
+    }
+    return;
+  }
+  const int64_t row = static_cast<int64_t>(it.row) + token;
+  const int64_t hq = static_cast<int64_t>(h) * group + head;
+  const __nv_bfloat162* a = reinterpret_cast<const __nv_bfloat162*>(
+      out + row * o_st + hq * o_sh + lane * kPer);
+  const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(
+      dout + row * d_st + hq * d_sh + lane * kPer);
+  float acc = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer / 2; ++i) {
+    const float2 x = __bfloat1622float2(a[i]);
+    const float2 y = __bfloat1622float2(b[i]);
+    acc = fmaf(x.x, y.x, fmaf(x.y, y.y, acc));
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, s);
+  if (lane == 0) {
+    const float l = lse[row * l_st + hq * l_sh];
+    const bool none = l == -INFINITY;
+    delta[at] = none ? 0.f : acc;
+    lse2[at] = none ? INFINITY : l * kLog2e;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dq. TMEM, per half h: S [128h, 128h+64) (dS over its columns 0-15 and
+// 32-47), dP [128h+64, 128h+128); dQ [256, 256 + kD).
+// ---------------------------------------------------------------------------
+enum DqBar {
+  kQFull = 0,                 // Q and dO of the item landed
+  kQEmpty,                    // the item's last S and dP finished
+  kSdFull,                    // [2 halves] S and dP of the block's half
+  kDsFull = kSdFull + 2,      // [2 halves] dS written (8 warps)
+  kDqDone = kDsFull + 2,      // the item's last dQ product finished
+  kDqFree,                    // the epilogue has read dQ (8 warps)
+  kDqDrain,
+  kKvFull,                    // [kStages] K and V of the block landed
+  kKvEmpty = kKvFull + 4,     // [kStages] the block's products finished
+  kDqNumBars = kKvEmpty + 4
+};
+
+template <int kD>
+__global__ void __launch_bounds__(kThreads, 1)
+    causal_dq_kernel(const __grid_constant__ CUtensorMap map_q,
+                     const __grid_constant__ CUtensorMap map_do,
+                     const __grid_constant__ CUtensorMap map_k,
+                     const __grid_constant__ CUtensorMap map_v,
+                     const __grid_constant__ BwdParams p) {
+  using C = Bwd<kD>;
+  constexpr int kStages = C::kStages;
+  constexpr uint32_t kTileBytes = C::kTileBytes;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* s_q = smem;
+  uint8_t* s_do = smem + kTileBytes;
+  uint8_t* s_kv = smem + 2 * kTileBytes;  // [kStages] x (K, V)
+  uint64_t* bars =
+      reinterpret_cast<uint64_t*>(smem + (2 + 2 * kStages) * kTileBytes);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kDqNumBars);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int tid = threadIdx.x;
+  const int warp = tid / 32;
+  const int lane = tid % 32;
+  const int64_t n_items = static_cast<int64_t>(p.entries) * p.kv_heads;
+  if (tid == 0) {
+    for (int b = 0; b < kDqNumBars; ++b)
+      mbar_init(&bars[b],
+                (b == kDsFull || b == kDsFull + 1 || b == kDqFree) ? 8 : 1);
+    *abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMma) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == kProducer) {
+    if (lane == 0) {
+      prefetch_tensor_map(&map_q);
+      prefetch_tensor_map(&map_do);
+      prefetch_tensor_map(&map_k);
+      prefetch_tensor_map(&map_v);
+    }
+    const uint32_t q_bytes = 2u * p.group * p.tokens * kD * 2;
+    int q_loads = 0, kv_loads = 0;
+    bool run = true;
+    for (int t = 0; run; ++t) {
+      const int64_t i = turn(t);
+      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
+      if (i >= n_items) continue;
+      const int h = static_cast<int>(i % p.kv_heads);
+      const QueryItem it =
+          load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads));
+      if (it.blocks == 0) continue;
+      if (q_loads > 0 &&
+          !wait_all(&bars[kQEmpty], (q_loads - 1) & 1, abort, p.status))
+        break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bars[kQFull], q_bytes);
+        load_tile<kD>(s_q, &map_q, &bars[kQFull], h * p.group, it.row);
+        load_tile<kD>(s_do, &map_do, &bars[kQFull], h * p.group, it.row);
+      }
+      __syncwarp();
+      ++q_loads;
+      for (int j = 0; j < it.blocks; ++j) {
+        const int stage = kv_loads % kStages;
+        if (kv_loads >= kStages &&
+            !wait_all(&bars[kKvEmpty + stage],
+                      ((kv_loads / kStages) - 1) & 1, abort, p.status)) {
+          run = false;
+          break;
+        }
+        if (lane == 0) {
+          uint8_t* dst = s_kv + stage * 2 * kTileBytes;
+          mbar_arrive_expect_tx(&bars[kKvFull + stage], 2 * kTileBytes);
+          load_tile<kD>(dst, &map_k, &bars[kKvFull + stage], h,
+                        it.k_row + j * kTile);
+          load_tile<kD>(dst + kTileBytes, &map_v, &bars[kKvFull + stage], h,
+                        it.k_row + j * kTile);
+        }
+        __syncwarp();
+        ++kv_loads;
+      }
+    }
+    if (lane == 0 && *abort) {
+      volatile int never = 0;
+      if (q_loads > 0)
+        mbar_wait(&bars[kQFull], (q_loads - 1) & 1, &never, nullptr);
+      for (int b = kv_loads - kStages; b < kv_loads; ++b)
+        if (b >= 0)
+          mbar_wait(&bars[kKvFull + b % kStages], (b / kStages) & 1, &never,
+                    nullptr);
+    }
+  } else if (warp == kMma) {
+    // Per block j, halves a (keys 0-63) and b (64-127):
+    //   S_a, dP_a, S_b, dP_b of block 0 of the item, then for each j
+    //   dQ += half a of j; S_a, dP_a of j + 1;
+    //   dQ += half b of j; S_b, dP_b of j + 1.
+    constexpr uint32_t idesc_sd = idesc_bf16(128, 64, false, false);
+    constexpr uint32_t idesc_acc = idesc_bf16(128, kD, false, true);
+    const uint32_t q_lo = sw128_desc_lo(smem_u32(s_q), 16);
+    const uint32_t do_lo = sw128_desc_lo(smem_u32(s_do), 16);
+    const uint32_t kv_lo = sw128_desc_lo(smem_u32(s_kv), 16);
+    const uint32_t kvmn_lo = sw128_desc_lo(smem_u32(s_kv), 16384);
+    const uint32_t t_dq = tmem + 256;
+    auto issue_sd = [&](int stage, int h) {
+      const uint32_t k_lo =
+          kv_lo + stage * 2 * C::kTileUnits + h * (8192 >> 4);
+      const uint32_t v_lo = k_lo + C::kTileUnits;
+      const uint32_t t_s = tmem + h * 128, t_dp = t_s + 64;
+#pragma unroll
+      for (int kk = 0; kk < C::kSteps; ++kk) {
+        const uint32_t off = (kk >> 2) * (16384 >> 4) + (kk & 3) * 2;
+        umma_ss_warp(t_s, q_lo + off, k_lo + off, idesc_sd, kk > 0);
+      }
+#pragma unroll
+      for (int kk = 0; kk < C::kSteps; ++kk) {
+        const uint32_t off = (kk >> 2) * (16384 >> 4) + (kk & 3) * 2;
+        umma_ss_warp(t_dp, do_lo + off, v_lo + off, idesc_sd, kk > 0);
+      }
+      umma_commit_warp(&bars[kSdFull + h]);
+    };
+    // dQ += dS K over half h's 64 keys (dS of keys 16kk' .. lies in columns
+    // 32(kk'/2) + 8(kk'%2) of the half's S).
+    auto issue_dq = [&](int stage, int h, bool first) {
+      const uint32_t kmn = kvmn_lo + stage * 2 * C::kTileUnits;
+      const uint32_t t_a = tmem + h * 128;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        umma_ts_warp(t_dq, t_a + (kk >> 1) * 32 + (kk & 1) * 8,
+                     kmn + (4 * h + kk) * 128, idesc_acc,
+                     (kk > 0 || h > 0 || !first) ? 1u : 0u);
+    };
+    int blk = 0, items = 0;
+    bool run = true;
+    for (int t = 0; run; ++t) {
+      const int64_t i = turn(t);
+      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
+      if (i >= n_items) continue;
+      const QueryItem it =
+          load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads));
+      const int n = it.blocks;
+      if (n == 0) continue;
+      // K and V of block j of the item have landed, and the key rows behind
+      // the sequence are clear (they are the depth of dQ's product).
+      auto block_ready = [&](int j) -> bool {
+        const int b = blk + j;
+        if (!wait_all(&bars[kKvFull + b % kStages], (b / kStages) & 1, abort,
+                      p.status))
+          return false;
+        if (it.keys - j * kTile < kTile)
+          clear_rows<kD>(s_kv + (b % kStages) * 2 * kTileBytes,
+                         it.keys - j * kTile, lane);
+        tc_fence_after();
+        return true;
+      };
+      if (!wait_all(&bars[kQFull], items & 1, abort, p.status) ||
+          !block_ready(0))
+        break;
+      issue_sd(blk % kStages, 0);
+      issue_sd(blk % kStages, 1);
+      if (n == 1) umma_commit_warp(&bars[kQEmpty]);
+      for (int j = 0; j < n; ++j) {
+        const int b = blk + j;
+        const int stage = b % kStages;
+        const int next = (b + 1) % kStages;
+        const bool first = j == 0, last = j == n - 1;
+        // The item's first dQ overwrites dQ: the epilogue must have read it.
+        if (first && items > 0 &&
+            !wait_all(&bars[kDqFree], (items - 1) & 1, abort, p.status)) {
+          run = false;
+          break;
+        }
+        if (!wait_all(&bars[kDsFull + 0], b & 1, abort, p.status)) {
+          run = false;
+          break;
+        }
+        tc_fence_after();
+        issue_dq(stage, 0, first);
+        if (!last) {
+          if (!block_ready(j + 1)) {
+            run = false;
+            break;
+          }
+          issue_sd(next, 0);
+        }
+        if (!wait_all(&bars[kDsFull + 1], b & 1, abort, p.status)) {
+          run = false;
+          break;
+        }
+        tc_fence_after();
+        issue_dq(stage, 1, first);
+        umma_commit_warp(&bars[kKvEmpty + stage]);
+        if (!last) {
+          issue_sd(next, 1);
+          if (j + 1 == n - 1) umma_commit_warp(&bars[kQEmpty]);
+        } else {
+          umma_commit_warp(&bars[kDqDone]);
+        }
+      }
+      blk += n;
+      ++items;
+    }
+    if (*abort) {
+      volatile int never = 0;
+      umma_commit_warp(&bars[kDqDrain]);
+      mbar_wait(&bars[kDqDrain], 0, &never, nullptr);
+    }
+  } else {
+    // ---------------- compute warps 0-7 ----------------
+    const int wq = warp / 4;  // keys 32 wq .. 32 wq + 31 of each half
+    const int quarter = warp % 4;
+    const int row = quarter * 32 + lane;
+    const int token = row / p.group;
+    const int head = row % p.group;
+    const bool row_used = row < p.tokens * p.group;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    int blk = 0, items = 0;
+    bool ok = true;
+    for (int t = 0; ok; ++t) {
+      const int64_t i = turn(t);
+      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
+      if (i >= n_items) continue;
+      const int h = static_cast<int>(i % p.kv_heads);
+      const QueryItem it =
+          load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads));
+      const int n = it.blocks;
+      const bool write = row_used && token < it.tokens;
+      __nv_bfloat16* dst =
+          p.grad + (static_cast<int64_t>(it.row) + token) * p.grad_st +
+          (static_cast<int64_t>(h) * p.group + head) * p.grad_sh +
+          wq * (kD / 2);
+      if (n == 0) {
+        uint32_t z[kD / 4] = {0};
+        if (write) store_row<kD / 2>(dst, z);
+        continue;
+      }
+      const int64_t at =
+          (static_cast<int64_t>(h) * p.n_tiles + it.tile) * kTile + row;
+      const float l2 = p.lse2[at];
+      const float dlt = p.delta[at];
+      const int seen = max(0, min(it.keys, it.kpos + token + 1));
+      for (int j = 0; j < n && ok; ++j, ++blk) {
+        const int visible = seen - j * kTile;
+        const bool masked = __any_sync(0xffffffffu, visible < kTile);
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          if (!wait_all(&bars[kSdFull + hh], blk & 1, abort, p.status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const int key0 = hh * 64 + wq * 32;  // key column of the block
+          const uint32_t t_s = tmem + hh * 128 + wq * 32 + lane_base;
+          uint32_t s[32], dp[32];
+          tmem_ld32(t_s, s);
+          tmem_ld32(t_s + 64, dp);
+          tmem_wait_ld();
+          uint32_t w[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            float d2[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int cc = 2 * c + e;
+              const float pr = ex2_approx(
+                  fmaf(__uint_as_float(s[cc]), p.scale_log2, -l2));
+              d2[e] = pr * (__uint_as_float(dp[cc]) - dlt);
+              if (masked && key0 + cc >= visible) d2[e] = 0.f;
+            }
+            w[c] = pack_bf16(d2[0], d2[1]);
+          }
+          // dS of these 32 keys over the first 16 of this warp's own 32
+          // columns of S.
+          tmem_st16(t_s, w);
+          tmem_wait_st();
+          arrive_warp(&bars[kDsFull + hh]);
+        }
+      }
+      if (!ok) break;
+      if (!wait_all(&bars[kDqDone], items & 1, abort, p.status)) break;
+      ++items;
+      tc_fence_after();
+      uint32_t w[kD / 4];
+      tmem_row_bf16<kD / 2>(tmem + 256 + wq * (kD / 2) + lane_base, p.scale,
+                            w);
+      arrive_warp(&bars[kDqFree]);
+      if (write) store_row<kD / 2>(dst, w);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dkdv. TMEM, per half h: S^T [128h, 128h+64) (P^T over its columns 0-15 and
+// 32-47), dP^T [128h+64, 128h+128) (dS^T likewise); dV [256, 256 + kD), dK
+// [384, 384 + kD).
+// ---------------------------------------------------------------------------
+enum KvBar {
+  kKtFull = 0,                // K and V of the key tile landed
+  kKtEmpty,                   // the item's last S^T and dP^T finished
+  kStFull,                    // [2 halves] S^T and dP^T of the block's half
+  kPdsFull = kStFull + 2,     // [2 halves] P^T and dS^T written (8 warps)
+  kKvDone = kPdsFull + 2,     // the item's last dV and dK products finished
+  kKvFree,                    // the epilogue has read dV and dK (8 warps)
+  kKvDrain,
+  kQdFull,                    // [kStages] Q, dO, L and D of the block landed
+  kQdEmpty = kQdFull + 4,     // [kStages] the block's products finished
+  kKvNumBars = kQdEmpty + 4
+};
+
+template <int kD>
+__global__ void __launch_bounds__(kThreads, 1)
+    causal_dkdv_kernel(const __grid_constant__ CUtensorMap map_q,
+                       const __grid_constant__ CUtensorMap map_do,
+                       const __grid_constant__ CUtensorMap map_k,
+                       const __grid_constant__ CUtensorMap map_v,
+                       const __grid_constant__ BwdParams p) {
+  using C = Bwd<kD>;
+  constexpr int kStages = C::kStages;
+  constexpr uint32_t kTileBytes = C::kTileBytes;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* s_k = smem;
+  uint8_t* s_v = smem + kTileBytes;
+  uint8_t* s_qd = smem + 2 * kTileBytes;  // [kStages] x (Q, dO)
+  float* s_vec = reinterpret_cast<float*>(
+      smem + (2 + 2 * kStages) * kTileBytes);  // [kStages] x (L, D)
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_vec + kStages * 256);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kKvNumBars);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int tid = threadIdx.x;
+  const int warp = tid / 32;
+  const int lane = tid % 32;
+  const int64_t n_items = static_cast<int64_t>(p.entries) * p.kv_heads;
+  const int tile_rows = p.tokens * p.group;
+  if (tid == 0) {
+    for (int b = 0; b < kKvNumBars; ++b)
+      mbar_init(&bars[b],
+                (b == kPdsFull || b == kPdsFull + 1 || b == kKvFree) ? 8 : 1);
+    *abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMma) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  // Rows that no box fills (a group that does not divide 128) are the depth
+  // of the products: they stay zero.
+  if (tile_rows < kTile) {
+    for (int i = tid; i < 2 * kStages * static_cast<int>(C::kTileUnits);
+         i += kThreads)
+      reinterpret_cast<uint4*>(s_qd)[i] = make_uint4(0, 0, 0, 0);
+    fence_async_shared();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == kProducer) {
+    if (lane == 0) {
+      prefetch_tensor_map(&map_q);
+      prefetch_tensor_map(&map_do);
+      prefetch_tensor_map(&map_k);
+      prefetch_tensor_map(&map_v);
+    }
+    const uint32_t qd_bytes = 2u * tile_rows * kD * 2 + 1024;
+    int kt_loads = 0, qd_loads = 0;
+    bool run = true;
+    for (int t = 0; run; ++t) {
+      const int64_t i = turn(t);
+      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
+      if (i >= n_items) continue;
+      const int h = static_cast<int>(i % p.kv_heads);
+      const KeyItem it =
+          load_item<KeyItem>(p.table, static_cast<int>(i / p.kv_heads));
+      if (it.blocks == 0) continue;
+      if (kt_loads > 0 &&
+          !wait_all(&bars[kKtEmpty], (kt_loads - 1) & 1, abort, p.status))
+        break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bars[kKtFull], 2 * kTileBytes);
+        load_tile<kD>(s_k, &map_k, &bars[kKtFull], h, it.row);
+        load_tile<kD>(s_v, &map_v, &bars[kKtFull], h, it.row);
+      }
+      __syncwarp();
+      ++kt_loads;
+      for (int j = 0; j < it.blocks; ++j) {
+        const int stage = qd_loads % kStages;
+        if (qd_loads >= kStages &&
+            !wait_all(&bars[kQdEmpty + stage],
+                      ((qd_loads / kStages) - 1) & 1, abort, p.status)) {
+          run = false;
+          break;
+        }
+        if (lane == 0) {
+          uint8_t* dst = s_qd + stage * 2 * kTileBytes;
+          const int64_t base = (static_cast<int64_t>(h) * p.n_tiles +
+                                it.tile0 + it.first + j) *
+                               kTile;
+          const int q_row = it.q_row + (it.first + j) * p.tokens;
+          uint64_t* bar = &bars[kQdFull + stage];
+          mbar_arrive_expect_tx(bar, qd_bytes);
+          load_tile<kD>(dst, &map_q, bar, h * p.group, q_row);
+          load_tile<kD>(dst + kTileBytes, &map_do, bar, h * p.group, q_row);
+          bulk_load(s_vec + stage * 256, p.lse2 + base, 512, bar);
+          bulk_load(s_vec + stage * 256 + 128, p.delta + base, 512, bar);
+        }
+        __syncwarp();
+        ++qd_loads;
+      }
+    }
+    if (lane == 0 && *abort) {
+      volatile int never = 0;
+      if (kt_loads > 0)
+        mbar_wait(&bars[kKtFull], (kt_loads - 1) & 1, &never, nullptr);
+      for (int b = qd_loads - kStages; b < qd_loads; ++b)
+        if (b >= 0)
+          mbar_wait(&bars[kQdFull + b % kStages], (b / kStages) & 1, &never,
+                    nullptr);
+    }
+  } else if (warp == kMma) {
+    // Per block j, halves a (query rows 0-63) and b (64-127):
+    //   S^T_a, dP^T_a, S^T_b, dP^T_b of block 0 of the item, then for each j
+    //   dV, dK += half a of j; S^T_a, dP^T_a of j + 1;
+    //   dV, dK += half b of j; S^T_b, dP^T_b of j + 1.
+    constexpr uint32_t idesc_st = idesc_bf16(128, 64, false, false);
+    constexpr uint32_t idesc_acc = idesc_bf16(128, kD, false, true);
+    const uint32_t k_lo = sw128_desc_lo(smem_u32(s_k), 16);
+    const uint32_t v_lo = sw128_desc_lo(smem_u32(s_v), 16);
+    const uint32_t qd_lo = sw128_desc_lo(smem_u32(s_qd), 16);
+    const uint32_t qdmn_lo = sw128_desc_lo(smem_u32(s_qd), 16384);
+    const uint32_t t_dv = tmem + 256, t_dk = tmem + 384;
+    auto issue_st = [&](int stage, int h) {
+      const uint32_t q_lo =
+          qd_lo + stage * 2 * C::kTileUnits + h * (8192 >> 4);
+      const uint32_t do_lo = q_lo + C::kTileUnits;
+      const uint32_t t_s = tmem + h * 128, t_dp = t_s + 64;
+#pragma unroll
+      for (int kk = 0; kk < C::kSteps; ++kk) {
+        const uint32_t off = (kk >> 2) * (16384 >> 4) + (kk & 3) * 2;
+        umma_ss_warp(t_s, k_lo + off, q_lo + off, idesc_st, kk > 0);
+      }
+#pragma unroll
+      for (int kk = 0; kk < C::kSteps; ++kk) {
+        const uint32_t off = (kk >> 2) * (16384 >> 4) + (kk & 3) * 2;
+        umma_ss_warp(t_dp, v_lo + off, do_lo + off, idesc_st, kk > 0);
+      }
+      umma_commit_warp(&bars[kStFull + h]);
+    };
+    // dV += P^T dO and dK += dS^T Q over half h's 64 query rows.
+    auto issue_acc = [&](int stage, int h, bool first) {
+      const uint32_t qmn = qdmn_lo + stage * 2 * C::kTileUnits;
+      const uint32_t domn = qmn + C::kTileUnits;
+      const uint32_t t_p = tmem + h * 128, t_ds = t_p + 64;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        umma_ts_warp(t_dv, t_p + (kk >> 1) * 32 + (kk & 1) * 8,
+                     domn + (4 * h + kk) * 128, idesc_acc,
+                     (kk > 0 || h > 0 || !first) ? 1u : 0u);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        umma_ts_warp(t_dk, t_ds + (kk >> 1) * 32 + (kk & 1) * 8,
+                     qmn + (4 * h + kk) * 128, idesc_acc,
+                     (kk > 0 || h > 0 || !first) ? 1u : 0u);
+    };
+    int blk = 0, items = 0;
+    bool run = true;
+    for (int t = 0; run; ++t) {
+      const int64_t i = turn(t);
+      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
+      if (i >= n_items) continue;
+      const KeyItem it =
+          load_item<KeyItem>(p.table, static_cast<int>(i / p.kv_heads));
+      const int n = it.blocks;
+      if (n == 0) continue;
+      // Q and dO of block j have landed, and the query rows behind the
+      // sequence are clear.
+      auto block_ready = [&](int j) -> bool {
+        const int b = blk + j;
+        if (!wait_all(&bars[kQdFull + b % kStages], (b / kStages) & 1, abort,
+                      p.status))
+          return false;
+        const int left =
+            (it.tokens - (it.first + j) * p.tokens) * p.group;
+        if (left < tile_rows) {
+          uint8_t* dst = s_qd + (b % kStages) * 2 * kTileBytes;
+          clear_rows<kD>(dst, left, lane);
+          clear_rows<kD>(dst + kTileBytes, left, lane);
+        }
+        tc_fence_after();
+        return true;
+      };
+      if (!wait_all(&bars[kKtFull], items & 1, abort, p.status) ||
+          !block_ready(0))
+        break;
+      issue_st(blk % kStages, 0);
+      issue_st(blk % kStages, 1);
+      if (n == 1) umma_commit_warp(&bars[kKtEmpty]);
+      for (int j = 0; j < n; ++j) {
+        const int b = blk + j;
+        const int stage = b % kStages;
+        const int next = (b + 1) % kStages;
+        const bool first = j == 0, last = j == n - 1;
+        // The item's first dV and dK overwrite the accumulators, which the
+        // epilogue must have read.
+        if (first && items > 0 &&
+            !wait_all(&bars[kKvFree], (items - 1) & 1, abort, p.status)) {
+          run = false;
+          break;
+        }
+        if (!wait_all(&bars[kPdsFull + 0], b & 1, abort, p.status)) {
+          run = false;
+          break;
+        }
+        tc_fence_after();
+        issue_acc(stage, 0, first);
+        if (!last) {
+          if (!block_ready(j + 1)) {
+            run = false;
+            break;
+          }
+          issue_st(next, 0);
+        }
+        if (!wait_all(&bars[kPdsFull + 1], b & 1, abort, p.status)) {
+          run = false;
+          break;
+        }
+        tc_fence_after();
+        issue_acc(stage, 1, first);
+        umma_commit_warp(&bars[kQdEmpty + stage]);
+        if (!last) {
+          issue_st(next, 1);
+          if (j + 1 == n - 1) umma_commit_warp(&bars[kKtEmpty]);
+        } else {
+          umma_commit_warp(&bars[kKvDone]);
+        }
+      }
+      blk += n;
+      ++items;
+    }
+    if (*abort) {
+      volatile int never = 0;
+      umma_commit_warp(&bars[kKvDrain]);
+      mbar_wait(&bars[kKvDrain], 0, &never, nullptr);
+    }
+  } else {
+    // ---------------- compute warps 0-7 ----------------
+    const int wq = warp / 4;  // query rows 32 wq .. of each half
+    const int quarter = warp % 4;
+    const int row = quarter * 32 + lane;  // key row of the tile
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    int blk = 0, items = 0;
+    bool ok = true;
+    for (int t = 0; ok; ++t) {
+      const int64_t i = turn(t);
+      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
+      if (i >= n_items) continue;
+      const int h = static_cast<int>(i % p.kv_heads);
+      const KeyItem it =
+          load_item<KeyItem>(p.table, static_cast<int>(i / p.kv_heads));
+      const int n = it.blocks;
+      const bool write = row < it.keys;
+      const int64_t k_row = static_cast<int64_t>(it.row) + row;
+      __nv_bfloat16* dk_dst =
+          p.grad + k_row * p.grad_st + h * p.grad_sh + wq * (kD / 2);
+      __nv_bfloat16* dv_dst =
+          p.grad2 + k_row * p.grad2_st + h * p.grad2_sh + wq * (kD / 2);
+      if (n == 0) {
+        uint32_t z[kD / 4] = {0};
+        if (write) {
+          store_row<kD / 2>(dk_dst, z);
+          store_row<kD / 2>(dv_dst, z);
+        }
+        continue;
+      }
+      for (int j = 0; j < n && ok; ++j, ++blk) {
+        const float* vl = s_vec + (blk % kStages) * 256;  // L log2(e), then D
+        // First query row of the block that sees this key.
+        const int64_t from =
+            (static_cast<int64_t>(it.shift) + row -
+             static_cast<int64_t>(it.first + j) * p.tokens) *
+            p.group;
+        const bool masked = __any_sync(0xffffffffu, from > 0);
+        const int cmin = static_cast<int>(from < 0 ? 0 : min(from, (int64_t)kTile));
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          if (!wait_all(&bars[kStFull + hh], blk & 1, abort, p.status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const int q0 = hh * 64 + wq * 32;  // query column of the block
+          const uint32_t t_s = tmem + hh * 128 + wq * 32 + lane_base;
+          const uint32_t t_dp = t_s + 64;
+          uint32_t s[32], dp[32];
+          tmem_ld32(t_s, s);
+          tmem_ld32(t_dp, dp);
+          tmem_wait_ld();
+          uint32_t wp[16], wd[16];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const float4 l4 = *reinterpret_cast<const float4*>(vl + q0 + 4 * c);
+            const float4 d4 =
+                *reinterpret_cast<const float4*>(vl + 128 + q0 + 4 * c);
+            const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+            const float dv[4] = {d4.x, d4.y, d4.z, d4.w};
+            float pr[4], ds[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int cc = 4 * c + e;
+              pr[e] = ex2_approx(
+                  fmaf(__uint_as_float(s[cc]), p.scale_log2, -lv[e]));
+              ds[e] = pr[e] * (__uint_as_float(dp[cc]) - dv[e]);
+              if (masked && q0 + cc < cmin) {
+                pr[e] = 0.f;
+                ds[e] = 0.f;
+              }
+            }
+            wp[2 * c] = pack_bf16(pr[0], pr[1]);
+            wp[2 * c + 1] = pack_bf16(pr[2], pr[3]);
+            wd[2 * c] = pack_bf16(ds[0], ds[1]);
+            wd[2 * c + 1] = pack_bf16(ds[2], ds[3]);
+          }
+          // P^T and dS^T of these 32 queries over the first 16 of this
+          // warp's own 32 columns of S^T and dP^T.
+          tmem_st16(t_s, wp);
+          tmem_st16(t_dp, wd);
+          tmem_wait_st();
+          arrive_warp(&bars[kPdsFull + hh]);
+        }
+      }
+      if (!ok) break;
+      if (!wait_all(&bars[kKvDone], items & 1, abort, p.status)) break;
+      ++items;
+      tc_fence_after();
+      uint32_t wv[kD / 4], wk[kD / 4];
+      tmem_row_bf16<kD / 2>(tmem + 256 + wq * (kD / 2) + lane_base, 1.0f, wv);
+      tmem_row_bf16<kD / 2>(tmem + 384 + wq * (kD / 2) + lane_base, p.scale,
+                            wk);
+      arrive_warp(&bars[kKvFree]);
+      if (write) {
+        store_row<kD / 2>(dv_dst, wv);
+        store_row<kD / 2>(dk_dst, wk);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+struct Maps {
+  CUtensorMap q, dout, k, v;
+};
+
+struct PrepArgs {
+  const void* out;
+  int64_t o_st, o_sh;
+  const void* dout;
+  int64_t d_st, d_sh;
+  const float* lse;
+  int64_t l_st, l_sh;
+  float *lse2, *delta;
+};
+
+template <int kD>
+int launch(const Maps& m, const BwdParams& pq, const BwdParams& pk,
+           const PrepArgs& a, bool want_q, bool want_k, cudaStream_t stream) {
+  using C = Bwd<kD>;
+  int sms = 0;
+  int rc = device_sms(&sms);
+  if (rc != VEDA_OK) return rc;
+  if (pq.entries > 0) {
+    const int64_t warps =
+        static_cast<int64_t>(pq.entries) * pq.kv_heads * kTile;
+    causal_bwd_prep_kernel<kD>
+        <<<static_cast<unsigned>((warps * 32 + 255) / 256), 256, 0, stream>>>(
+            pq.table, pq.entries, pq.kv_heads, pq.group, pq.tokens,
+            static_cast<const __nv_bfloat16*>(a.out), a.o_st, a.o_sh,
+            static_cast<const __nv_bfloat16*>(a.dout), a.d_st, a.d_sh, a.lse,
+            a.l_st, a.l_sh, a.lse2, a.delta, pq.n_tiles);
+    rc = check_launch("causal_bwd_prep_kernel");
+    if (rc != VEDA_OK) return rc;
+  }
+  const int64_t q_items = static_cast<int64_t>(pq.entries) * pq.kv_heads;
+  if (want_q && q_items > 0) {
+    VEDA_CUDA(cudaFuncSetAttribute(
+        causal_dq_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        C::kSmem));
+    const int grid = static_cast<int>(q_items < sms ? q_items : sms);
+    causal_dq_kernel<kD><<<grid, kThreads, C::kSmem, stream>>>(
+        m.q, m.dout, m.k, m.v, pq);
+    rc = check_launch("causal_dq_kernel");
+    if (rc != VEDA_OK) return rc;
+  }
+  const int64_t k_items = static_cast<int64_t>(pk.entries) * pk.kv_heads;
+  if (want_k && k_items > 0) {
+    VEDA_CUDA(cudaFuncSetAttribute(
+        causal_dkdv_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        C::kSmem));
+    const int grid = static_cast<int>(k_items < sms ? k_items : sms);
+    causal_dkdv_kernel<kD><<<grid, kThreads, C::kSmem, stream>>>(
+        m.q, m.dout, m.k, m.v, pk);
+    return check_launch("causal_dkdv_kernel");
+  }
+  return VEDA_OK;
+}
+
+}  // namespace
+
+}  // namespace causal
+}  // namespace veda
+
+using namespace veda;
+
+extern "C" int64_t veda_causal_bwd_workspace(int32_t kv_heads,
+                                             int64_t n_tiles) {
+  if (kv_heads < 1 || n_tiles < 0 || n_tiles >= (int64_t(1) << 31)) return -1;
+  // L log2(e) and D of each row of each query tile.
+  return 2 * static_cast<int64_t>(kv_heads) * n_tiles * kTile *
+         static_cast<int64_t>(sizeof(float));
+}
+
+extern "C" int veda_causal_bwd(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+    int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+    int64_t v_stride_h, const void* out, int64_t out_stride_t,
+    int64_t out_stride_h, const void* dout, int64_t dout_stride_t,
+    int64_t dout_stride_h, const float* lse, int64_t lse_stride_t,
+    int64_t lse_stride_h, int64_t total_q, int64_t total_k, int32_t n_heads,
+    int32_t kv_heads, int32_t head_dim, const int32_t* q_items,
+    int64_t n_q_items, const int32_t* k_items, int64_t n_k_items,
+    int64_t n_tiles, void* dq, int64_t dq_stride_t, int64_t dq_stride_h,
+    void* dk, int64_t dk_stride_t, int64_t dk_stride_h, void* dv,
+    int64_t dv_stride_t, int64_t dv_stride_h, float softmax_scale,
+    void* workspace, int64_t workspace_bytes, void* stream) {
+  int rc = require_sm100("veda_causal_bwd");
+  if (rc != VEDA_OK) return rc;
+  VEDA_REQUIRE(head_dim == 64 || head_dim == 128,
+               "head_dim must be 64 or 128");
+  VEDA_REQUIRE(kv_heads >= 1 && n_heads >= 1 && n_heads % kv_heads == 0 &&
+                   n_heads / kv_heads <= kTile,
+               "n_heads must be 1 to 128 times kv_heads");
+  VEDA_REQUIRE(total_q >= 0 && total_k >= 0 && total_q < (int64_t(1) << 31) &&
+                   total_k < (int64_t(1) << 31) && n_q_items >= 0 &&
+                   n_k_items >= 0 && n_tiles >= n_q_items &&
+                   n_tiles * kv_heads < (int64_t(1) << 24) &&
+                   n_k_items < (int64_t(1) << 31),
+               "bad sizes (at most 2^24 query tiles times key heads)");
+  VEDA_REQUIRE(softmax_scale > 0.f && isfinite(softmax_scale),
+               "softmax_scale must be positive and finite");
+  VEDA_REQUIRE((dk == nullptr) == (dv == nullptr),
+               "dk and dv are computed together");
+  const int64_t need = veda_causal_bwd_workspace(kv_heads, n_tiles);
+  VEDA_REQUIRE(need >= 0 && workspace_bytes >= need &&
+                   (need == 0 || workspace != nullptr) &&
+                   reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+               "workspace too small or not 16-byte aligned "
+               "(veda_causal_bwd_workspace)");
+  auto aligned = [](const void* ptr, int64_t st, int64_t sh) {
+    return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && st % 8 == 0 &&
+           sh % 8 == 0;
+  };
+  VEDA_REQUIRE(aligned(out, out_stride_t, out_stride_h) &&
+                   aligned(dout, dout_stride_t, dout_stride_h) &&
+                   aligned(dq, dq_stride_t, dq_stride_h) &&
+                   aligned(dk, dk_stride_t, dk_stride_h) &&
+                   aligned(dv, dv_stride_t, dv_stride_h),
+               "out, dout, dq, dk, dv must be 16-byte aligned with strides "
+               "multiple of 8");
+  cudaStream_t s = as_stream(stream);
+  const int group = n_heads / kv_heads;
+  const int tokens = kTile / group;
+  VEDA_REQUIRE(n_q_items == 0 || (q && out && dout && lse && q_items),
+               "q, out, dout, lse and q_items are required");
+  VEDA_REQUIRE(n_k_items == 0 || (k && v && k_items),
+               "k, v and k_items are required");
+  causal::Maps m;
+  if (total_q > 0) {
+    rc = causal::make_rows_map(&m.q, q, total_q, n_heads, head_dim,
+                               q_stride_t, q_stride_h, group, tokens, "q");
+    if (rc == VEDA_OK)
+      rc = causal::make_rows_map(&m.dout, dout, total_q, n_heads, head_dim,
+                                 dout_stride_t, dout_stride_h, group, tokens,
+                                 "dout");
+  }
+  if (rc == VEDA_OK && total_k > 0) {
+    rc = causal::make_rows_map(&m.k, k, total_k, kv_heads, head_dim,
+                               k_stride_t, k_stride_h, 1, kTile, "k");
+    if (rc == VEDA_OK)
+      rc = causal::make_rows_map(&m.v, v, total_k, kv_heads, head_dim,
+                                 v_stride_t, v_stride_h, 1, kTile, "v");
+  }
+  if (rc != VEDA_OK) return rc;
+  // With no rows on one side every item of the other is empty and loads
+  // nothing; its maps only have to exist.
+  if (total_q == 0) m.q = m.dout = m.k;
+  if (total_k == 0) m.k = m.v = m.q;
+  causal::BwdParams p{};
+  p.kv_heads = kv_heads;
+  p.group = group;
+  p.tokens = tokens;
+  p.n_tiles = static_cast<int>(n_tiles);
+  float* lse2 = static_cast<float*>(workspace);
+  float* delta = lse2 + static_cast<int64_t>(kv_heads) * n_tiles * kTile;
+  p.lse2 = lse2;
+  p.delta = delta;
+  p.scale = softmax_scale;
+  p.scale_log2 = softmax_scale * causal::kLog2e;
+  p.status = device_status_ptr();
+  causal::BwdParams pq = p, pk = p;
+  pq.table = q_items;
+  pq.entries = static_cast<int>(n_q_items);
+  pq.grad = static_cast<__nv_bfloat16*>(dq);
+  pq.grad_st = dq_stride_t;
+  pq.grad_sh = dq_stride_h;
+  pk.table = k_items;
+  pk.entries = static_cast<int>(n_k_items);
+  pk.grad = static_cast<__nv_bfloat16*>(dk);
+  pk.grad_st = dk_stride_t;
+  pk.grad_sh = dk_stride_h;
+  pk.grad2 = static_cast<__nv_bfloat16*>(dv);
+  pk.grad2_st = dv_stride_t;
+  pk.grad2_sh = dv_stride_h;
+  const causal::PrepArgs a{out,           out_stride_t, out_stride_h, dout,
+                           dout_stride_t, dout_stride_h, lse,
+                           lse_stride_t,  lse_stride_h,  lse2, delta};
+  return head_dim == 128
+             ? causal::launch<128>(m, pq, pk, a, dq != nullptr, dk != nullptr,
+                                   s)
+             : causal::launch<64>(m, pq, pk, a, dq != nullptr, dk != nullptr,
+                                  s);
+}

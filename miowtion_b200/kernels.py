@@ -524,6 +524,67 @@ def causal_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     return out, lse
 
 
+def causal_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                         out: torch.Tensor, dout: torch.Tensor,
+                         lse: torch.Tensor, pack: sequences.SequencePack,
+                         scale: float, want_q: bool = True,
+                         want_kv: bool = True):
+    """(dq, dk, dv) of `causal_attention` (None where not wanted); out and lse
+    as the forward returned them."""
+    group = _causal_checks(q, k, v, pack)
+    _require(q, 'causal_attention backward')
+    q, k, v, out, dout = (aligned_rows(t) for t in (q, k, v, out, dout))
+
+    def empty(t, wanted):
+        return (torch.empty(t.shape, dtype=t.dtype, device=t.device)
+                if wanted else None)
+
+    dq, dk, dv = empty(q, want_q), empty(k, want_kv), empty(v, want_kv)
+    grads = []
+    for g in (dq, dk, dv):
+        grads += ([g.data_ptr(), g.stride(0), g.stride(1)] if g is not None
+                  else [None, 0, 0])
+    with torch.cuda.device(q.device):
+        tables = pack.tables(group)
+        need = _lib.load().veda_causal_bwd_workspace(k.shape[1],
+                                                     tables.n_tiles)
+        ws = torch.empty(max(need, 16) // 4, dtype=torch.float32,
+                         device=q.device)
+        q_items, k_items = on_stream(tables.query), on_stream(tables.key)
+        _lib.call('veda_causal_bwd', q.data_ptr(), q.stride(0), q.stride(1),
+                  k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                  v.stride(0), v.stride(1), out.data_ptr(), out.stride(0),
+                  out.stride(1), dout.data_ptr(), dout.stride(0),
+                  dout.stride(1), lse.data_ptr(), lse.stride(0),
+                  lse.stride(1), q.shape[0], k.shape[0], q.shape[1],
+                  k.shape[1], q.shape[2], q_items.data_ptr(),
+                  q_items.shape[0], k_items.data_ptr(), k_items.shape[0],
+                  tables.n_tiles, *grads, scale, ws.data_ptr(),
+                  ws.numel() * 4, _lib.stream_ptr(q.device))
+    return dq, dk, dv
+
+
+class _CausalAttention(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, q, k, v, pack, scale):
+        out, lse = causal_attention_fwd(q, k, v, pack, scale)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.pack, ctx.scale = pack, scale
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _dlse):
+        q, k, v, out, lse = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dq, dk, dv = causal_attention_bwd(q, k, v, out, dout, lse, ctx.pack,
+                                          ctx.scale, need[0],
+                                          need[1] or need[2])
+        return dq, dk, dv, None, None
+
+
 def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                      pack: sequences.SequencePack,
                      scale: float | None = None, return_lse: bool = False):
@@ -540,6 +601,9 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         return_lse: Also return the [total_q, heads] fp32 log-sum-exp of the
             scaled scores (no gradient flows through it).
 
+    q, k and v receive gradients (once differentiable), those of a key head
+    summed over its query heads; repeats are bit-identical.
+
     Returns:
         out [total_q, heads, D] bf16 (and lse); 0 and -inf for rows without
         keys. Rows of one sequence never reach another, whatever they hold;
@@ -547,5 +611,8 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         before it that share its key tile.
     """
     scale = softmax_scale(scale, q.shape[-1])
-    out, lse = causal_attention_fwd(q, k, v, pack, scale, return_lse)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+        out, lse = _CausalAttention.apply(q, k, v, pack, scale)
+    else:
+        out, lse = causal_attention_fwd(q, k, v, pack, scale, return_lse)
     return (out, lse) if return_lse else out

@@ -5,6 +5,14 @@ Bounds count the roundings of the forward: weights to bf16 (half a step,
     |out - want| <= (2^-8 + 2 s + 2^-14) sum_j p_j |v_j| + 2^-8 |want|
 with s = (D + 8) 2^-24 A for scores of total size A = scale max_j sum_d
 |q_d k_jd| (a relative error of a weight, and again of the weights' sum).
+
+Gradients: with half steps u = 2^-8 of P, dS and the stored gradient, of the
+stored out in D = rowsum(dO O), and e = 2 s + 2^-14 relative in P,
+    |dv_j - want| <= (u + e) sum_i p_ij |do_i| + u |want|,
+    |ds_ij - want| <= (u + e) |ds_ij| + p_ij u sum_d |do_id out_id|
+                      + p_ij 2^-16 sum_d |do_id| (|v_jd| + |out_id|),
+and dq, dk bounded by scale times the sums of these against |k| and |q|, plus
+u |want|.
 """
 
 import math
@@ -154,6 +162,150 @@ def test_sequences_do_not_reach_one_another(dim):
         assert torch.equal(got[:150], ref[:150])
         assert torch.equal(got[220:], ref[220:])
     assert out[150:220].isnan().all()
+
+
+def gradients(pack, q, k, v, dout, scale=None):
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+    out = kernels.causal_attention(*leaves, pack, scale)
+    return torch.autograd.grad(out, leaves, dout)
+
+
+def check_gradients(pack, q, k, v, dout, grads, scale=None):
+    dim = q.shape[2]
+    scale = dim ** -0.5 if scale is None else scale
+    want = [torch.zeros(t.shape, dtype=torch.float64, device=DEV)
+            for t in (q, k, v)]
+    bound = [torch.zeros_like(t) for t in want]
+    u = 2.0 ** -8
+    for at, keys, h, hk, sees in each_head(pack, q, k):
+        qb, kb, vb = q[at, h].double(), k[keys, hk].double(), v[
+            keys, hk].double()
+        if 0 in (qb.shape[0], kb.shape[0]):
+            continue
+        g = dout[at, h].double()
+        p, _ = softmax64(qb, kb, sees, scale)
+        out = p @ vb
+        size = ((qb.abs() @ kb.abs().T) * sees).amax(-1) * scale
+        e = 2 * 2.0 ** -24 * (dim + 8) * size[:, None] + 2.0 ** -14
+        ds = p * (g @ vb.T - (g * out).sum(-1, keepdim=True))
+        off = ((u + e) * ds.abs() +
+               p * u * (g * out).abs().sum(-1, keepdim=True) +
+               p * 2.0 ** -16 * (g.abs() @ vb.abs().T +
+                                 (g * out).abs().sum(-1, keepdim=True)))
+        want[0][at, h] += scale * ds @ kb
+        want[1][keys, hk] += scale * ds.T @ qb
+        want[2][keys, hk] += p.T @ g
+        bound[0][at, h] += scale * off @ kb.abs()
+        bound[1][keys, hk] += scale * off.T @ qb.abs()
+        bound[2][keys, hk] += ((u + e) * p).T @ g.abs()
+    for name, got, ref, off in zip(('dq', 'dk', 'dv'), grads, want, bound):
+        assert got.isfinite().all(), name
+        err = (got.double() - ref).abs()
+        off = off + u * ref.abs() + 1e-30
+        assert (err <= off).all(), (name, float((err / off).max()))
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('q_lengths, k_lengths, heads, kv_heads', SHAPES)
+def test_gradients_match_the_definition(q_lengths, k_lengths, heads, kv_heads,
+                                        dim):
+    pack, q, k, v = problem(q_lengths, k_lengths, heads, kv_heads, dim)
+    dout = rows(pack.total_q, heads, dim, 9)
+    grads = gradients(pack, q, k, v, dout)
+    check_gradients(pack, q, k, v, dout, grads)
+    again = gradients(pack, q, k, v, dout)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+def test_gradients_of_more_items_than_processors(dim):
+    lengths = [(37 * i) % 211 for i in range(90)]
+    pack, q, k, v = problem(lengths, None, 8, 4, dim)
+    dout = rows(pack.total_q, 8, dim, 9)
+    check_gradients(pack, q, k, v, dout, gradients(pack, q, k, v, dout))
+
+
+def test_gradients_agree_with_differences():
+    pack, q, k, v = problem([60, 150], [90, 150], 4, 2, 64)
+    dout = rows(pack.total_q, 4, 64, 9)
+    grads = gradients(pack, q, k, v, dout)
+
+    def loss(*args):
+        total = 0.0
+        for at, keys, h, hk, sees in each_head(pack, args[0], args[1]):
+            p, _ = softmax64(args[0][at, h], args[1][keys, hk], sees, 0.125)
+            total = total + (p @ args[2][keys, hk] *
+                             dout[at, h].double()).sum()
+        return float(total)
+
+    base = [t.double() for t in (q, k, v)]
+    for n, grad in enumerate(grads):
+        way = rows(*base[n].shape, 40 + n).double()
+        step = 1e-4
+        plus, minus = ([t + s * way if m == n else t
+                        for m, t in enumerate(base)] for s in (step, -step))
+        slope = (loss(*plus) - loss(*minus)) / (2 * step)
+        # Each gradient is off by at most a few 2^-8 of its size, with
+        # independent signs along the direction: far below the sum of sizes.
+        size = float((grad.double() * way).abs().sum())
+        got = float((grad.double() * way).sum())
+        assert abs(got - slope) <= 2.0 ** -8 * size, (n, got, slope)
+
+
+def test_gradients_of_shared_broadcast_and_single_inputs():
+    pack, q, _, _ = problem([90, 40], None, 4, 2, 64)
+    dout = rows(130, 4, 64, 9)
+    k1, v = rows(130, 1, 64, 4), rows(130, 2, 64, 5)
+    full = gradients(pack, q, k1.expand(130, 2, 64), v, dout)
+    leaf = k1.clone().requires_grad_(True)
+    out = kernels.causal_attention(q, leaf.expand(130, 2, 64), v, pack)
+    (got,) = torch.autograd.grad(out, leaf, dout)
+    assert torch.equal(got, full[1].sum(1, keepdim=True))
+    leaf = v.clone().requires_grad_(True)
+    out = kernels.causal_attention(q, k1.expand(130, 2, 64), leaf, pack)
+    out.backward(dout)
+    assert torch.equal(leaf.grad, full[2])
+    # A gradient without strides of its own (that of a sum).
+    leaves = [t.clone().requires_grad_(True) for t in (q, v, v)]
+    ones = torch.ones_like(dout)
+    got = torch.autograd.grad(kernels.causal_attention(*leaves, pack).sum(),
+                              leaves)
+    want = gradients(pack, q, v, v, ones)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('heads', [6, 8])
+def test_gradients_of_sequences_do_not_reach_one_another(heads, dim):
+    pack, q, k, v = problem([150, 70, 33], [150, 200, 33], heads, 2, dim)
+    dout = rows(253, heads, dim, 9)
+    want = gradients(pack, q, k, v, dout)
+    for t in (q, dout):
+        t[150:220] = math.nan
+    for t in (k, v):
+        t[150:350] = math.inf
+    got = gradients(pack, q, k, v, dout)
+    for a, b, mid in zip(got, want, (220, 350, 350)):
+        assert torch.equal(a[:150], b[:150])
+        assert torch.equal(a[mid:], b[mid:])
+
+
+def test_backward_replays_in_a_graph():
+    pack, q, k, v = problem([300, 77], None, 4, 2, 128)
+    dout = rows(377, 4, 128, 9)
+    want = gradients(pack, q, k, v, dout)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(g, stream=side):
+            out = kernels.causal_attention(*leaves, pack)
+            got = torch.autograd.grad(out, leaves, dout)
+    for _ in range(2):
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_forward_repeats_and_replays():
