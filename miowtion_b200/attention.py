@@ -23,9 +23,11 @@ import torch
 from miowtion_b200 import compensation
 from miowtion_b200 import heatmap
 from miowtion_b200 import kernels
+from miowtion_b200 import kvcache
 from miowtion_b200 import mask as veda_mask
 from miowtion_b200 import plan as veda_plan
 from miowtion_b200 import predictor as veda_predictor
+from miowtion_b200 import sequences
 from miowtion_b200 import tiling
 
 # Default VedaConfig.collect_bytes (attention.py:30-34): bound on one
@@ -694,6 +696,75 @@ class DenseAttention:
     def __call__(self, q, k, v, layer_index):
         del layer_index
         return dense_attention(q, k, v, self.used, backend=self.backend)[0]
+
+
+class CausalAttention:
+    """Causal AttentionFn over packed sequences, differentiable: q
+    [total_q, heads, D], k and v [total_k, kv_heads, D] of `pack`'s rows (see
+    `kernels.causal_attention`)."""
+
+    def __init__(self, pack: sequences.SequencePack,
+                 scale: float | None = None):
+        self.pack = pack
+        self.scale = scale
+
+    def __call__(self, q, k, v, layer_index):
+        del layer_index
+        return kernels.causal_attention(q, k, v, self.pack, self.scale)
+
+
+class CachedAttention:
+    """Causal AttentionFn that keeps the keys and values: every call stores
+    the rows of k and v in the layer's cache and attends over the contexts.
+
+    A step's rows are `pack`: q_lengths new rows per sequence, k_lengths rows
+    in all once they are stored. A prompt (no earlier rows) attends to k and v
+    as they came; a chunk behind earlier rows to its contexts as the cache
+    holds them; single tokens straight over the pages. With int8 or e4m3
+    pages the first therefore sees unquantised rows, the others quantised
+    ones.
+
+    Args:
+        caches: One `kvcache.PagedCache` per layer.
+        table: [n_sequences, max_pages] int32 page numbers (all layers').
+        pack: The rows of this step.
+        scale: Softmax scale; None for D ** -0.5.
+    """
+
+    def __init__(self, caches: list[kvcache.PagedCache], table: torch.Tensor,
+                 pack: sequences.SequencePack, scale: float | None = None):
+        self.caches = caches
+        self.table = table
+        self.pack = pack
+        self.scale = scale
+        # Rows of each context with and without this step's.
+        self.lengths = pack.k_offsets.diff()
+        self.starts = self.lengths - pack.q_offsets.diff()
+        if (pack.k_lengths < pack.q_lengths).any():
+            raise ValueError('a context holds its new rows: k_lengths must '
+                             'not be below q_lengths')
+
+    def advance(self) -> None:
+        """Moves a step of single tokens on by one row per sequence, on the
+        device (a captured step followed by this replays as a decoding
+        loop)."""
+        if not self.pack.single_tokens:
+            raise ValueError('only a step of single tokens advances')
+        self.lengths.add_(1)
+        self.starts.add_(1)
+
+    def __call__(self, q, k, v, layer_index):
+        if torch.is_grad_enabled() and any(t.requires_grad
+                                           for t in (q, k, v)):
+            raise ValueError('attention over the cache has no gradient; use '
+                             'CausalAttention')
+        cache = self.caches[layer_index]
+        cache.write(k, v, self.table, self.starts, self.pack)
+        if self.pack.single_tokens:
+            return cache.attend(q, self.table, self.lengths, self.scale)
+        if not self.pack.whole:
+            k, v = cache.read(self.table, self.pack)
+        return kernels.causal_attention(q, k, v, self.pack, self.scale)
 
 
 ORACLE_TARGETS = ('mass', 'max', 'mean')
