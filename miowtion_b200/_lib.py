@@ -217,5 +217,17 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def call_on(index: int, name: str, *args) -> None:
+    """`call` with the current stream of CUDA device `index` as the last
+    argument, on that device. (A launch costs the host a few microseconds:
+    the stream's number is read without building a Stream, and the device is
+    switched only where it is another.)"""
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()

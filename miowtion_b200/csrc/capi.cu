@@ -55,6 +55,24 @@ unsigned int* device_status_ptr() {
   return cache[dev];
 }
 
+int device_sms(int* sms) {
+  int dev = 0;
+  VEDA_CUDA(cudaGetDevice(&dev));
+  VEDA_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+  return VEDA_OK;
+}
+
+int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>* done) {
+  int dev = 0;
+  VEDA_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done->load(std::memory_order_relaxed) & bit) return VEDA_OK;
+  VEDA_CUDA(cudaFuncSetAttribute(
+      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done->fetch_or(bit, std::memory_order_relaxed);
+  return VEDA_OK;
+}
+
 namespace {
 std::atomic<int> g_sm_reserve{0};
 }  // namespace
@@ -207,11 +225,22 @@ int make_rows_map(CUtensorMap* map, const void* base, int64_t rows,
   cuuint32_t box[3] = {64, static_cast<cuuint32_t>(heads_box),
                        static_cast<cuuint32_t>(rows_box)};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-                  const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&]() {
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+              const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // A thread that has made no runtime call yet (an autograd worker) has no
+    // context; the runtime binds the device's.
+    int dev = 0;
+    VEDA_CUDA(cudaGetDevice(&dev));
+    VEDA_CUDA(cudaSetDevice(dev));
+    r = encode();
+  }
   if (r != CUDA_SUCCESS) {
     char buf[200];
     snprintf(buf, sizeof(buf),

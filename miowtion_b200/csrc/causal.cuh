@@ -99,8 +99,5 @@ int make_rows_map(CUtensorMap* map, const void* base, int64_t rows,
                   int64_t stride_head, int heads_box, int rows_box,
                   const char* name);
 
-// Kernel launches depend on the device: its SMs.
-int device_sms(int* sms);
-
 }  // namespace causal
 }  // namespace veda

@@ -886,9 +886,10 @@ int launch(const Maps& m, const BwdParams& pq, const BwdParams& pk,
   }
   const int64_t q_items = static_cast<int64_t>(pq.entries) * pq.kv_heads;
   if (want_q && q_items > 0) {
-    VEDA_CUDA(cudaFuncSetAttribute(
-        causal_dq_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-        C::kSmem));
+    static std::atomic<uint64_t> allowed{0};
+    rc = allow_smem(reinterpret_cast<const void*>(causal_dq_kernel<kD>),
+                    C::kSmem, &allowed);
+    if (rc != VEDA_OK) return rc;
     const int grid = static_cast<int>(q_items < sms ? q_items : sms);
     causal_dq_kernel<kD><<<grid, kThreads, C::kSmem, stream>>>(
         m.q, m.dout, m.k, m.v, pq);
@@ -897,9 +898,10 @@ int launch(const Maps& m, const BwdParams& pq, const BwdParams& pk,
   }
   const int64_t k_items = static_cast<int64_t>(pk.entries) * pk.kv_heads;
   if (want_k && k_items > 0) {
-    VEDA_CUDA(cudaFuncSetAttribute(
-        causal_dkdv_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-        C::kSmem));
+    static std::atomic<uint64_t> allowed{0};
+    rc = allow_smem(reinterpret_cast<const void*>(causal_dkdv_kernel<kD>),
+                    C::kSmem, &allowed);
+    if (rc != VEDA_OK) return rc;
     const int grid = static_cast<int>(k_items < sms ? k_items : sms);
     causal_dkdv_kernel<kD><<<grid, kThreads, C::kSmem, stream>>>(
         m.q, m.dout, m.k, m.v, pk);

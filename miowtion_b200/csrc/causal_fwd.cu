@@ -530,9 +530,10 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
   int sms = 0;
   int rc = device_sms(&sms);
   if (rc != VEDA_OK) return rc;
-  VEDA_CUDA(cudaFuncSetAttribute(causal_fwd_kernel<kD>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 Fwd<kD>::kSmem));
+  static std::atomic<uint64_t> allowed{0};
+  rc = allow_smem(reinterpret_cast<const void*>(causal_fwd_kernel<kD>),
+                  Fwd<kD>::kSmem, &allowed);
+  if (rc != VEDA_OK) return rc;
   const int cap = sms - sm_reserve() > 0 ? sms - sm_reserve() : 1;
   const int64_t items = static_cast<int64_t>(p.entries) * p.kv_heads;
   const int grid = static_cast<int>(items < cap ? items : cap);
@@ -542,14 +543,6 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
 }
 
 }  // namespace
-
-int device_sms(int* sms) {
-  int dev = 0;
-  VEDA_CUDA(cudaGetDevice(&dev));
-  VEDA_CUDA(
-      cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
-  return VEDA_OK;
-}
 
 }  // namespace causal
 }  // namespace veda

@@ -8,6 +8,7 @@
 #include <cudaTypedefs.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 #include "veda_b200.h"
@@ -43,6 +44,13 @@ unsigned int* device_status_ptr();
 
 // SMs the persistent attention forward leaves free (veda_set_sm_reserve).
 int sm_reserve();
+
+// SMs of the current device.
+int device_sms(int* sms);
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device;
+// `done` (one static word per kernel) remembers the devices that allow it.
+int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>* done);
 
 // 3D bf16 tensor map over a [rows, heads, 128] tensor with a (64, 1, 128)
 // box and 128-byte swizzle: coordinates are (d0 in {0, 64}, head, row0).

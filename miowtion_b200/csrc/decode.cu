@@ -14,16 +14,17 @@
 //
 // The contexts of a call are cut into chunks of 16 keys of one kv head
 // (a page holds a multiple of 16 rows, so a chunk is one contiguous piece),
-// numbered sequence by sequence and head by head, and CTA i of G takes the
-// i-th of G equal runs of the numbers, whatever the lengths: the split needs
-// the lengths on the device only. A warp takes every kWarps-th chunk of the
-// CTA's piece of a (sequence, head) and streams it through a ring of its
-// own with cp.async (rows past the length are filled with zeros, not read),
-// with its own running maximum, sum and accumulator; the warps join in shared
-// memory at the piece's end while the ring already loads the next piece. A
-// piece that is a whole (sequence, head) is written out; others leave
-// maximum, sum and accumulator in the workspace, which decode_join_kernel
-// adds up in the order of the keys. No atomics: repeats are bit-identical.
+// numbered sequence by sequence and head by head, and warp i of all W warps
+// of the grid takes the i-th of W equal runs of the numbers, whatever the
+// lengths: the split needs the lengths on the device only. A warp streams its
+// run through a ring of its own with cp.async (rows past the length are
+// filled with zeros, not read), two chunks a step, with its own running
+// maximum, sum and accumulator, and never waits for another warp. A
+// (sequence, head) that lies inside the run is written out; the run's first
+// and last may be parts, which the CTA adds up in shared memory at its end and,
+// where they go on in another CTA, leaves in the workspace for
+// decode_join_kernel. Parts are added in the order of the keys, with no
+// atomics: repeats are bit-identical.
 //
 // int8 and e4m3 codes become fp16 exactly, in registers. A key's scale
 // multiplies its scores; a value row's scale multiplies its weights, relative
@@ -36,6 +37,8 @@
 #include <cuda_fp8.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "kvcache.cuh"
 
 namespace veda {
@@ -46,7 +49,7 @@ constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kChunk = 16;  // keys
 constexpr int kRows = 16;   // heads of a tile
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 512;
 constexpr float kWeight = 64.f;  // factor of the fp16 weights
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
@@ -60,7 +63,7 @@ struct DecodeParams {
   int tiles;   // tiles of kRows heads in a group
   __nv_bfloat16* out;  // [n_seqs, heads, D]
   float* lse;          // [n_seqs, heads] or null
-  float* partial;      // [G][2][kRows][D + 2]
+  float* partial;      // [n_ctas][2][kRows][D + 2]
   int n_ctas;
   float scale_log2;
   unsigned int* status;
@@ -77,32 +80,41 @@ __device__ __forceinline__ int chunks_of(int length) {
   return (length + kChunk - 1) / kChunk;
 }
 
-// CTAs that take part: with more of them than chunks, one for each chunk, so
-// that no run is empty.
-__device__ __forceinline__ int active_ctas(const DecodeParams& p,
-                                           int64_t total) {
-  return total < p.n_ctas ? static_cast<int>(total) : p.n_ctas;
+// a / b for b >= 1, by the 32-bit quotient where that does (a 64-bit one is
+// a few hundred cycles, and these are on the way to the first load).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 31) == 0)
+    return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
 }
 
-// First chunk number of CTA i: [0, total) in n equal runs.
-__device__ __forceinline__ int64_t run_begin(int64_t total, int i, int n) {
-  return total * i / n;
-}
-
-// Block-wide sums over the sequences: *total = chunks of all of them, and
-// the sequence that chunk number `at` lies in with the chunks before it
-// (where kFind; -1 if at >= total). Chunks are per tile and kv head, so a
-// sequence has chunks_of(length) * heads of them.
-template <int kBlock>
-struct Prefix {
-  int64_t warp_sum[kBlock / 32];
-  int64_t base;
-  int found;
-  int64_t before;
+// [0, total) chunks in runs for the grid's warps: the first `extra` warps
+// take size + 1, the others size. With more warps than chunks one for each
+// chunk takes part, so that no run is empty.
+struct Split {
+  int64_t size;
+  int extra;
+  int warps;
+  __device__ __forceinline__ Split(const DecodeParams& p, int64_t total) {
+    const int all = p.n_ctas * kWarps;
+    warps = total < all ? static_cast<int>(total) : all;
+    size = warps > 0 ? quotient(total, warps) : 0;
+    extra = static_cast<int>(total - size * warps);
+  }
+  __device__ __forceinline__ int64_t begin(int warp) const {
+    return size * warp + min(warp, extra);
+  }
+  __device__ __forceinline__ int warp_of(int64_t chunk) const {
+    const int64_t big = (size + 1) * extra;
+    return static_cast<int>(chunk < big
+                                ? quotient(chunk, size + 1)
+                                : extra + quotient(chunk - big, size));
+  }
 };
 
+// Exclusive prefix of x over the block's threads; *sum receives the total.
 template <int kBlock>
-__device__ __forceinline__ int64_t block_scan(Prefix<kBlock>* s, int64_t x,
+__device__ __forceinline__ int64_t block_scan(int64_t* warp_sum, int64_t x,
                                               int64_t* sum) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   int64_t inc = x;
@@ -112,59 +124,70 @@ __device__ __forceinline__ int64_t block_scan(Prefix<kBlock>* s, int64_t x,
     if (lane >= d) inc += y;
   }
   __syncthreads();
-  if (lane == 31) s->warp_sum[warp] = inc;
+  if (lane == 31) warp_sum[warp] = inc;
   __syncthreads();
   int64_t pre = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kBlock / 32; ++w) {
-    const int64_t y = s->warp_sum[w];
+    const int64_t y = warp_sum[w];
     if (w < warp) pre += y;
     all += y;
   }
   *sum = all;
-  return pre + inc - x;  // exclusive
+  return pre + inc - x;
 }
 
-// Chunks of all sequences, per (kv head, tile).
-template <int kBlock>
-__device__ __forceinline__ int64_t total_chunks(Prefix<kBlock>* s,
-                                                const DecodeParams& p) {
+// Where this warp's run begins: chunk numbers [*lo, *hi), the sequence of the
+// first and the chunks before that sequence. `ends` holds kThreads numbers.
+// Returns false for a warp without a run. All threads of the block call it.
+__device__ __forceinline__ bool find_run(const DecodeParams& p, int heads,
+                                         int64_t* warp_sum, int64_t* ends,
+                                         int64_t* lo, int64_t* hi, int* seq,
+                                         int64_t* before) {
+  const int n = p.c.n_seqs;
+  const int tid = threadIdx.x, lane = tid % 32;
+  const bool one_pass = n <= kThreads;
   int64_t mine = 0;
-  for (int b = threadIdx.x; b < p.c.n_seqs; b += kBlock)
-    mine += chunks_of(context(p, b));
+  for (int b = tid; b < n; b += kThreads) mine += chunks_of(context(p, b));
+  mine *= heads;
   int64_t sum;
-  block_scan<kBlock>(s, mine, &sum);
-  return sum;
-}
-
-// The sequence of chunk `at` (numbers of one head: chunks before sequence b
-// sum to before <= at < before + its own); all threads return it.
-template <int kBlock>
-__device__ __forceinline__ void find_chunk(Prefix<kBlock>* s,
-                                           const DecodeParams& p, int64_t at,
-                                           int64_t heads, int* seq,
-                                           int64_t* before) {
+  int64_t pre = block_scan<kThreads>(warp_sum, mine, &sum);
+  const Split split(p, sum);
+  const int w = blockIdx.x * kWarps + tid / 32;
+  const bool run = w < split.warps;
+  *lo = run ? split.begin(w) : 0;
+  *hi = run ? split.begin(w + 1) : 0;
+  *seq = -1;
   int64_t base = 0;
-  if (threadIdx.x == 0) s->found = -1;
-  for (int b0 = 0; b0 < p.c.n_seqs; b0 += kBlock) {
-    const int b = b0 + threadIdx.x;
-    const int64_t n =
-        b < p.c.n_seqs ? chunks_of(context(p, b)) * heads : int64_t(0);
-    int64_t sum;
-    const int64_t pre = base + block_scan<kBlock>(s, n, &sum);
-    if (n > 0 && pre <= at && at < pre + n) {
-      s->found = b;
-      s->before = pre;
+  for (int b0 = 0; b0 < n; b0 += kThreads) {
+    if (!one_pass) {
+      const int b = b0 + tid;
+      mine = b < n ? chunks_of(context(p, b)) * static_cast<int64_t>(heads)
+                   : int64_t(0);
+      pre = base + block_scan<kThreads>(warp_sum, mine, &sum);
+    }
+    __syncthreads();
+    ends[tid] = pre + mine;
+    __syncthreads();
+    if (run && *seq < 0 && *lo < ends[kThreads - 1]) {
+      // The first sequence of the block that ends behind lo.
+      for (int i = 0; i < kThreads; i += 32) {
+        const unsigned hit =
+            __ballot_sync(0xffffffffu, ends[i + lane] > *lo);
+        if (hit != 0) {
+          const int at = i + __ffs(hit) - 1;
+          *seq = b0 + at;
+          *before = at > 0 ? ends[at - 1] : base;
+          break;
+        }
+      }
     }
     base += sum;
-    __syncthreads();
-    if (s->found >= 0 || at < base) break;
   }
-  *seq = s->found;
-  *before = s->before;
+  return run && *seq >= 0;
 }
 
-// The pieces of a CTA's run: sequence, head tile, chunks [c0, c1).
+// The pieces of a warp's run: sequence, head tile, chunks [c0, c1).
 struct Pieces {
   int b, vh, c0, c1, n;  // n: chunks of the whole (sequence, head)
   int length;
@@ -283,6 +306,8 @@ struct Shape {
   // k, v, and (8-bit) 16 k scales and 16 v scales.
   static constexpr int kStageBytes = 2 * kTileBytes + (kHalf ? 128 : 0);
   static constexpr int kPieces = kRowBytes / 16;  // 16-byte pieces of a row
+  // Chunks a step: two share the maxima and the loop's overhead.
+  static constexpr int kPair = kHalf ? 2 : 1;
   static constexpr int kJoinFloats = kD + 4;      // a row of the join buffer
 };
 
@@ -297,23 +322,47 @@ __device__ __forceinline__ uint32_t piece_at(int r, int c) {
     return (r * kPieces + (c ^ ((r >> 1) & 3))) * 16;
 }
 
+// A part of a (sequence, head tile) that a warp leaves for its CTA.
+struct Part {
+  int b, vh;    // -1: none
+  int starts;   // it holds the first chunk
+  int ends;     // it holds the last chunk
+};
+
+// Shared memory behind the rings: every warp's first part (a last part lies
+// in the warp's own ring, which is free by then).
+template <int kD, int kStore>
+__host__ __device__ constexpr int part_floats(int pitch) {
+  return pitch * Shape<kD, kStore>::kJoinFloats;
+}
+
 template <int kD, int kStore, int kStages>
 __global__ void __launch_bounds__(kThreads, 1)
     decode_kernel(const __grid_constant__ DecodeParams p) {
   using S = Shape<kD, kStore>;
   constexpr bool kHalf = S::kHalf;
   constexpr int kSteps = kD / 16;
+  constexpr int kRingBytes = kStages * S::kStageBytes;
+  static_assert(kRingBytes >= kRows * S::kJoinFloats * 4,
+                "a last part fits the ring");
+  static_assert(kWarps * kRingBytes >= kThreads * 8, "find_run's numbers fit");
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ Prefix<kThreads> prefix;
+  __shared__ int64_t s_sums[kWarps];
+  __shared__ Part s_parts[kWarps][2];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int quad = lane % 4, row_lo = lane / 4;  // fragment coordinates
+  const int pitch = min(p.group, kRows);
 
-  uint8_t* ring = smem + warp * (kStages * S::kStageBytes);
-  float* join =
-      reinterpret_cast<float*>(smem + kWarps * kStages * S::kStageBytes);
+  uint8_t* ring = smem + warp * kRingBytes;
+  float* firsts = reinterpret_cast<float*>(smem + kWarps * kRingBytes);
+  auto part_at = [&](int w, int slot) -> float* {
+    return slot == 0 ? firsts + w * part_floats<kD, kStore>(pitch)
+                     : reinterpret_cast<float*>(smem + w * kRingBytes);
+  };
 
+  // The join kernel may start; it waits for this grid's end before it reads.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int heads = p.c.kv_heads * p.tiles;
-  const int64_t total = total_chunks<kThreads>(&prefix, p) * heads;
   if (blockIdx.x == 0) {
     // A length that its table row cannot hold is reported.
     const int64_t cap = static_cast<int64_t>(p.c.max_pages)
@@ -322,41 +371,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (p.lengths[b] < 0 || p.lengths[b] > cap)
         raise_status(p.status, VEDA_ERR_INVALID);
   }
-  const int n_ctas = active_ctas(p, total);
-  if (static_cast<int>(blockIdx.x) >= n_ctas) return;
-  const int64_t lo = run_begin(total, blockIdx.x, n_ctas);
-  const int64_t hi = run_begin(total, blockIdx.x + 1, n_ctas);
+  if (lane < 2) s_parts[warp][lane].b = -1;
+  int64_t lo, hi, before = 0;
   Pieces seg;
-  int64_t before;
-  find_chunk<kThreads>(&prefix, p, lo, heads, &seg.b, &before);
-  if (seg.b < 0) return;
-  seg.length = context(p, seg.b);
-  seg.n = chunks_of(seg.length);
-  seg.heads = heads;
-  seg.vh = static_cast<int>((lo - before) / seg.n);
-  seg.c0 = static_cast<int>((lo - before) % seg.n);
-  seg.left = hi - lo;
-  seg.bound();
-  const bool starts_inside = seg.c0 > 0;
-
-  // ---- loads: this warp's chunks, piece after piece ----
-  Pieces ld = seg;
-  int ld_chunk = ld.c0 + warp;
-  auto settle = [&]() {
-    while (ld.valid() && ld_chunk >= ld.c1) {
-      ld.next(p);
-      ld_chunk = ld.c0 + warp;
+  seg.left = 0;
+  if (find_run(p, heads, s_sums, reinterpret_cast<int64_t*>(smem), &lo, &hi,
+               &seg.b, &before)) {
+    seg.length = context(p, seg.b);
+    seg.n = chunks_of(seg.length);
+    seg.heads = heads;
+    if (seg.n > 0) {
+      seg.vh = static_cast<int>(quotient(lo - before, seg.n));
+      seg.c0 = static_cast<int>(lo - before -
+                                static_cast<int64_t>(seg.vh) * seg.n);
+      seg.left = hi - lo;
+      seg.bound();
     }
-  };
+  }
+  __syncthreads();  // find_run's numbers lie in the rings
+
+  // ---- loads: the run's chunks, piece after piece ----
+  Pieces ld = seg;
+  int ld_chunk = ld.c0;
   // The page of the next chunk is looked up one load ahead of its use.
   int next_page = -1;
   auto look_up = [&]() {
-    settle();
+    if (ld.valid() && ld_chunk >= ld.c1) {
+      ld.next(p);
+      ld_chunk = ld.c0;
+    }
     if (ld.valid())
       next_page = p.c.table[ld.b * p.c.table_ld +
                             ((ld_chunk * kChunk) >> p.c.page_shift)];
   };
-  look_up();
+  if (ld.valid()) look_up();
   int ld_stage = 0;
   auto load_next = [&]() {
     if (ld.valid()) {
@@ -372,22 +420,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                 (key0 & ((1 << p.c.page_shift) - 1)))
              : 0;
       const uint32_t dst = smem_u32(ring + ld_stage * S::kStageBytes);
-      const uint8_t* ksrc = p.c.k + row0 * S::kRowBytes;
-      const uint8_t* vsrc = p.c.v + row0 * S::kRowBytes;
+      const uint8_t* ksrc = p.c.k + row0 * S::kRowBytes + lane * 16;
+      const uint8_t* vsrc = p.c.v + row0 * S::kRowBytes + lane * 16;
 #pragma unroll
       for (int i = 0; i < kChunk * S::kPieces / 32; ++i) {
         const int piece = i * 32 + lane;
         const int r = piece / S::kPieces, c = piece % S::kPieces;
         const uint32_t off = piece_at<S::kPieces>(r, c);
-        cp_async16(dst + off, ksrc + piece * 16, r < live);
-        cp_async16(dst + S::kTileBytes + off, vsrc + piece * 16, r < live);
+        cp_async16(dst + off, ksrc + i * 512, r < live);
+        cp_async16(dst + S::kTileBytes + off, vsrc + i * 512, r < live);
       }
       if constexpr (kHalf) {
         const int r = lane % 16;
         const float* src = (lane < 16 ? p.c.k_scale : p.c.v_scale) + row0 + r;
         cp_async4(dst + 2 * S::kTileBytes + lane * 4, src, r < live);
       }
-      ld_chunk += kWarps;
+      ++ld_chunk;
       look_up();
     }
     cp_async_commit();
@@ -404,57 +452,55 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- q fragments of the piece's heads ----
     uint32_t qf[kSteps][4];
     float row_scale[2] = {p.scale_log2, p.scale_log2};
-    if (seg.c0 + warp < seg.c1) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = row_lo + 8 * half;
-        const __nv_bfloat16* src =
-            p.q + seg.b * p.q_sb + (head0 + (r < n_rows ? r : 0)) * p.q_sh;
-        if constexpr (!kHalf) {
+    for (int half = 0; half < 2; ++half) {
+      const int r = row_lo + 8 * half;
+      const __nv_bfloat16* src =
+          p.q + seg.b * p.q_sb + (head0 + (r < n_rows ? r : 0)) * p.q_sh;
+      if constexpr (!kHalf) {
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s) {
-            qf[s][half] =
-                *reinterpret_cast<const uint32_t*>(src + s * 16 + quad * 2);
-            qf[s][half + 2] =
-                *reinterpret_cast<const uint32_t*>(src + s * 16 + 8 + quad * 2);
-          }
-        } else {
-          // The products' depth index runs over d in the order that a
-          // thread's four consecutive code bytes give.
-          float x[kSteps][4];
-          float top = 0.f;
+        for (int s = 0; s < kSteps; ++s) {
+          qf[s][half] =
+              *reinterpret_cast<const uint32_t*>(src + s * 16 + quad * 2);
+          qf[s][half + 2] =
+              *reinterpret_cast<const uint32_t*>(src + s * 16 + 8 + quad * 2);
+        }
+      } else {
+        // The products' depth index runs over d in the order that a thread's
+        // four consecutive code bytes give.
+        float x[kSteps][4];
+        float top = 0.f;
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s) {
-            const uint2 w =
-                *reinterpret_cast<const uint2*>(src + s * 16 + quad * 4);
-            x[s][0] = __uint_as_float(w.x << 16);
-            x[s][1] = __uint_as_float(w.x & 0xFFFF0000u);
-            x[s][2] = __uint_as_float(w.y << 16);
-            x[s][3] = __uint_as_float(w.y & 0xFFFF0000u);
+        for (int s = 0; s < kSteps; ++s) {
+          const uint2 w =
+              *reinterpret_cast<const uint2*>(src + s * 16 + quad * 4);
+          x[s][0] = __uint_as_float(w.x << 16);
+          x[s][1] = __uint_as_float(w.x & 0xFFFF0000u);
+          x[s][2] = __uint_as_float(w.y << 16);
+          x[s][3] = __uint_as_float(w.y & 0xFFFF0000u);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[s][i]));
-          }
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          // 2^e <= top < 2^(e+1), e held to [-126, 126] so that its inverse
-          // exists.
-          int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-          e = max(-126, min(126, e));
-          const float inv =
-              __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-          row_scale[half] =
-              p.scale_log2 *
-              __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[s][i]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^e <= top < 2^(e+1), e held to [-126, 126] so that its inverse
+        // exists.
+        int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+        e = max(-126, min(126, e));
+        const float inv =
+            __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        row_scale[half] =
+            p.scale_log2 *
+            __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s) {
-            qf[s][half] = pack_half(x[s][0] * inv, x[s][1] * inv);
-            qf[s][half + 2] = pack_half(x[s][2] * inv, x[s][3] * inv);
-          }
+        for (int s = 0; s < kSteps; ++s) {
+          qf[s][half] = pack_half(x[s][0] * inv, x[s][1] * inv);
+          qf[s][half + 2] = pack_half(x[s][2] * inv, x[s][3] * inv);
         }
       }
     }
 
-    // ---- the piece's chunks of this warp ----
+    // ---- the piece's chunks, kPair a step ----
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     float v_ref = 0.f;
     float o[kD / 8][4];
@@ -462,28 +508,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < kD / 8; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-    for (int chunk = seg.c0 + warp; chunk < seg.c1; chunk += kWarps) {
-      // This chunk has landed, and the stage of the one before has been read
-      // by the whole warp: it takes the next load.
-      cp_async_wait<kStages - 2>();
+    // kN chunks (1 or kPair) from `chunk` on.
+    auto step = [&](auto count, int chunk) {
+      constexpr int kN = decltype(count)::value;
+      cp_async_wait<kStages - 1 - kN>();
       __syncwarp();
-      load_next();
-      const uint8_t* st = ring + stage * S::kStageBytes;
-      const uint32_t k_addr = smem_u32(st);
-      const uint32_t v_addr = k_addr + S::kTileBytes;
-      const float* scales =
-          reinterpret_cast<const float*>(st + 2 * S::kTileBytes);
-
-      // Scores: [16 heads] x [2 x 8 keys].
-      float s[2][4] = {};
+      uint32_t k_addr[kN], v_addr[kN];
+      const float* scales[kN];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        const int key = nt * 8 + (lane & 7);
+      for (int u = 0; u < kN; ++u) {
+        const uint8_t* st = ring + stage * S::kStageBytes;
+        k_addr[u] = smem_u32(st);
+        v_addr[u] = k_addr[u] + S::kTileBytes;
+        scales[u] = reinterpret_cast<const float*>(st + 2 * S::kTileBytes);
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+      }
+      // The chunks have landed, and the whole warp has read the stages before
+      // them: the first of those takes the next load.
+      load_next();
+
+      // Scores: [16 heads] x [2 kN x 8 keys].
+      float s[2 * kN][4] = {};
+#pragma unroll
+      for (int nt = 0; nt < 2 * kN; ++nt) {
+        const int key = (nt & 1) * 8 + (lane & 7);
         if constexpr (!kHalf) {
 #pragma unroll
           for (int st2 = 0; st2 < kSteps; st2 += 2) {
             uint32_t b[4];
-            ldsm4(k_addr + piece_at<S::kPieces>(key, st2 * 2 + lane / 8), b);
+            ldsm4(k_addr[nt / 2] +
+                      piece_at<S::kPieces>(key, st2 * 2 + lane / 8),
+                  b);
             mma16816<false>(s[nt], qf[st2], b[0], b[1]);
             mma16816<false>(s[nt], qf[st2 + 1], b[2], b[3]);
           }
@@ -491,7 +546,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int st4 = 0; st4 < kSteps; st4 += 4) {
             uint32_t b[4];
-            ldsm4(k_addr + piece_at<S::kPieces>(key, st4 + lane / 8), b);
+            ldsm4(k_addr[nt / 2] + piece_at<S::kPieces>(key, st4 + lane / 8),
+                  b);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint32_t b0, b1;
@@ -501,28 +557,35 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      // Columns of this thread: keys 2 quad + {0, 1} of each half.
+      // Columns of this thread: keys 2 quad + {0, 1} of each tile of 8.
       const int live = seg.length - chunk * kChunk;
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        const int key = nt * 8 + quad * 2;
+      for (int nt = 0; nt < 2 * kN; ++nt) {
         float k0 = 1.f, k1 = 1.f;
         if constexpr (kHalf) {
-          const float2 ks = *reinterpret_cast<const float2*>(scales + key);
+          const float2 ks = *reinterpret_cast<const float2*>(
+              scales[nt / 2] + (nt & 1) * 8 + quad * 2);
           k0 = ks.x;
           k1 = ks.y;
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          float& a = s[nt][2 * half];
-          float& b = s[nt][2 * half + 1];
-          a *= row_scale[half] * k0;
-          b *= row_scale[half] * k1;
-          if (key >= live) a = -INFINITY;
-          if (key + 1 >= live) b = -INFINITY;
-          top[half] = fmaxf(top[half], fmaxf(a, b));
+          s[nt][2 * half] *= row_scale[half] * k0;
+          s[nt][2 * half + 1] *= row_scale[half] * k1;
         }
+        if (live < kN * kChunk) {
+          const int key = nt * 8 + quad * 2;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (key >= live) s[nt][2 * half] = -INFINITY;
+            if (key + 1 >= live) s[nt][2 * half + 1] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          top[half] = fmaxf(top[half],
+                            fmaxf(s[nt][2 * half], s[nt][2 * half + 1]));
       }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -536,12 +599,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       // (kWeight) and stay below 2^15; those down to 2^-20 of the references
       // keep all of fp16's bits.
       float v_top = 0.f;
-      float2 vs[2];
+      [[maybe_unused]] float2 vs[2 * kN];
       if constexpr (kHalf) {
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          vs[nt] = *reinterpret_cast<const float2*>(scales + 16 + nt * 8 +
-                                                    quad * 2);
+        for (int nt = 0; nt < 2 * kN; ++nt) {
+          vs[nt] = *reinterpret_cast<const float2*>(
+              scales[nt / 2] + 16 + (nt & 1) * 8 + quad * 2);
           v_top = fmaxf(v_top, fmaxf(vs[nt].x, vs[nt].y));
         }
         v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, 1));
@@ -576,10 +639,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // Weights, as the A operand of the second product.
-      uint32_t a[4];
-      const float v_inv = kHalf && v_ref > 0.f ? kWeight / v_ref : 0.f;
+      uint32_t a[kN][4];
+      [[maybe_unused]] const float v_inv =
+          kHalf && v_ref > 0.f ? kWeight / v_ref : 0.f;
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
+      for (int nt = 0; nt < 2 * kN; ++nt)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           // m is -inf where no key of the row has existed so far.
@@ -588,99 +652,171 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float p1 = ex2_approx(s[nt][2 * half + 1] - ref);
           l[half] += p0 + p1;
           if constexpr (kHalf)
-            a[nt * 2 + half] = pack_half(p0 * (vs[nt].x * v_inv),
-                                         p1 * (vs[nt].y * v_inv));
+            a[nt / 2][(nt & 1) * 2 + half] = pack_half(
+                p0 * (vs[nt].x * v_inv), p1 * (vs[nt].y * v_inv));
           else
-            a[nt * 2 + half] = pack_bf16(p0, p1);
+            a[nt / 2][(nt & 1) * 2 + half] = pack_bf16(p0, p1);
         }
       // O += P V.
       const int vkey = (lane & 7) + ((lane >> 3) & 1) * 8;
-      if constexpr (!kHalf) {
 #pragma unroll
-        for (int dt = 0; dt < kD / 8; dt += 2) {
-          uint32_t b[4];
-          ldsm4_trans(v_addr + piece_at<S::kPieces>(vkey, dt + lane / 16), b);
-          mma16816<false>(o[dt], a, b[0], b[1]);
-          mma16816<false>(o[dt + 1], a, b[2], b[3]);
-        }
-      } else {
-        // A 16-byte piece of a row is 16 d: column n of the even tile is
-        // d = 2 n, of the odd tile 2 n + 1.
+      for (int u = 0; u < kN; ++u) {
+        if constexpr (!kHalf) {
 #pragma unroll
-        for (int dt = 0; dt < kD / 8; dt += 4) {
-          uint32_t b[4];
-          ldsm4_trans(
-              v_addr + piece_at<S::kPieces>(vkey, dt / 2 + lane / 16), b);
+          for (int dt = 0; dt < kD / 8; dt += 2) {
+            uint32_t b[4];
+            ldsm4_trans(
+                v_addr[u] + piece_at<S::kPieces>(vkey, dt + lane / 16), b);
+            mma16816<false>(o[dt], a[u], b[0], b[1]);
+            mma16816<false>(o[dt + 1], a[u], b[2], b[3]);
+          }
+        } else {
+          // A 16-byte piece of a row is 16 d: column n of the even tile is
+          // d = 2 n, of the odd tile 2 n + 1.
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint32_t lo0, hi0, lo1, hi1;
-            codes_to_half<kStore>(__byte_perm(b[2 * i], 0, 0x3120), &lo0,
-                                  &hi0);
-            codes_to_half<kStore>(__byte_perm(b[2 * i + 1], 0, 0x3120), &lo1,
-                                  &hi1);
-            mma16816<true>(o[dt + 2 * i], a, lo0, lo1);
-            mma16816<true>(o[dt + 2 * i + 1], a, hi0, hi1);
+          for (int dt = 0; dt < kD / 8; dt += 4) {
+            uint32_t b[4];
+            ldsm4_trans(
+                v_addr[u] + piece_at<S::kPieces>(vkey, dt / 2 + lane / 16),
+                b);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t lo0, hi0, lo1, hi1;
+              codes_to_half<kStore>(__byte_perm(b[2 * i], 0, 0x3120), &lo0,
+                                    &hi0);
+              codes_to_half<kStore>(__byte_perm(b[2 * i + 1], 0, 0x3120),
+                                    &lo1, &hi1);
+              mma16816<true>(o[dt + 2 * i], a[u], lo0, lo1);
+              mma16816<true>(o[dt + 2 * i + 1], a[u], hi0, hi1);
+            }
           }
         }
       }
-      stage = stage + 1 == kStages ? 0 : stage + 1;
-    }
+      // The other stages of this step are free once the warp has read them.
+      if constexpr (kN > 1) {
+        __syncwarp();
+#pragma unroll
+        for (int u = 1; u < kN; ++u) load_next();
+      }
+    };
+    int chunk = seg.c0;
+    if constexpr (S::kPair == 2)
+      for (; chunk + 2 <= seg.c1; chunk += 2)
+        step(std::integral_constant<int, 2>{}, chunk);
+    for (; chunk < seg.c1; ++chunk)
+      step(std::integral_constant<int, 1>{}, chunk);
 
-    // ---- join the warps ----
+    // ---- the piece's end ----
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
       l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
     }
     const float unit = kHalf ? v_ref * (1.f / kWeight) : 1.f;
-    const int pitch = min(p.group, kRows);
-    __syncthreads();  // the previous piece's join has been read
+    const bool starts = seg.c0 == 0, ends = seg.c1 == seg.n;
+    const int slot = starts ? 1 : 0;
+    if (!(starts && ends)) {
+      if (slot == 1) {
+        // The run's last piece: the ring is empty, but another lane may still
+        // read it.
+        cp_async_wait<0>();
+        __syncwarp();
+      }
+      if (lane == 0) s_parts[warp][slot] = Part{seg.b, seg.vh, starts, ends};
+    }
+    float* part = part_at(warp, slot);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int r = row_lo + 8 * half;
       if (r >= n_rows) continue;
-      float* dst = join + (warp * pitch + r) * S::kJoinFloats;
-      if (quad == 0) {
-        dst[kD] = m[half];
-        dst[kD + 1] = l[half];
-      }
+      const int64_t at =
+          static_cast<int64_t>(seg.b) * (p.c.kv_heads * p.group) + head0 + r;
+      if (starts && ends) {
+        const float inv = l[half] == 0.f ? 0.f : unit / l[half];
+        __nv_bfloat16* dst = p.out + at * kD;
 #pragma unroll
-      for (int dt = 0; dt < kD / 8; dt += 2) {
-        const float a0 = o[dt][2 * half] * unit;
-        const float a1 = o[dt][2 * half + 1] * unit;
-        const float b0 = o[dt + 1][2 * half] * unit;
-        const float b1 = o[dt + 1][2 * half + 1] * unit;
-        if constexpr (!kHalf) {
-          *reinterpret_cast<float2*>(dst + dt * 8 + quad * 2) =
-              make_float2(a0, a1);
-          *reinterpret_cast<float2*>(dst + dt * 8 + 8 + quad * 2) =
-              make_float2(b0, b1);
-        } else {
-          *reinterpret_cast<float4*>(dst + dt * 8 + quad * 4) =
-              make_float4(a0, b0, a1, b1);
+        for (int dt = 0; dt < kD / 8; dt += 2) {
+          const float a0 = o[dt][2 * half] * inv;
+          const float a1 = o[dt][2 * half + 1] * inv;
+          const float b0 = o[dt + 1][2 * half] * inv;
+          const float b1 = o[dt + 1][2 * half + 1] * inv;
+          if constexpr (!kHalf) {
+            *reinterpret_cast<uint32_t*>(dst + dt * 8 + quad * 2) =
+                pack_bf16(a0, a1);
+            *reinterpret_cast<uint32_t*>(dst + dt * 8 + 8 + quad * 2) =
+                pack_bf16(b0, b1);
+          } else {
+            *reinterpret_cast<uint2*>(dst + dt * 8 + quad * 4) =
+                make_uint2(pack_bf16(a0, b0), pack_bf16(a1, b1));
+          }
+        }
+        if (quad == 0 && p.lse != nullptr)
+          p.lse[at] = (m[half] + log2f(l[half])) * kLn2;
+      } else {
+        float* dst = part + r * S::kJoinFloats;
+        if (quad == 0) {
+          dst[kD] = m[half];
+          dst[kD + 1] = l[half];
+        }
+#pragma unroll
+        for (int dt = 0; dt < kD / 8; dt += 2) {
+          const float a0 = o[dt][2 * half] * unit;
+          const float a1 = o[dt][2 * half + 1] * unit;
+          const float b0 = o[dt + 1][2 * half] * unit;
+          const float b1 = o[dt + 1][2 * half + 1] * unit;
+          if constexpr (!kHalf) {
+            *reinterpret_cast<float2*>(dst + dt * 8 + quad * 2) =
+                make_float2(a0, a1);
+            *reinterpret_cast<float2*>(dst + dt * 8 + 8 + quad * 2) =
+                make_float2(b0, b1);
+          } else {
+            *reinterpret_cast<float4*>(dst + dt * 8 + quad * 4) =
+                make_float4(a0, b0, a1, b1);
+          }
         }
       }
     }
-    __syncthreads();
-    const bool whole = seg.c0 == 0 && seg.c1 == seg.n;
-    // The CTA's first piece if it does not begin its (sequence, head), else
-    // its last: at most these two are parts.
-    const int slot =
-        starts_inside && seg.left == hi - lo ? 0 : 1;
-    float* part =
-        p.partial + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * kRows *
-                        (kD + 2);
+  }
+
+  // ---- add up the CTA's parts, (sequence, head tile) by (sequence, head
+  // tile), in the order of the keys ----
+  __syncthreads();
+  int first = 0;  // part number: 2 * warp + slot
+  while (first < 2 * kWarps) {
+    const Part head = s_parts[first / 2][first % 2];
+    if (head.b < 0) {
+      ++first;
+      continue;
+    }
+    int last = first, scan = first + 1;
+    Part tail = head;
+    for (; scan < 2 * kWarps; ++scan) {
+      const Part x = s_parts[scan / 2][scan % 2];
+      if (x.b < 0) continue;
+      if (x.b != head.b || x.vh != head.vh) break;
+      last = scan;
+      tail = x;
+    }
+    const int kvh = head.vh / p.tiles, tile = head.vh % p.tiles;
+    const int n_rows = min(kRows, p.group - tile * kRows);
+    const bool whole = head.starts && tail.ends;
+    // A part that an earlier CTA began, or one that this CTA begins: at most
+    // one of each goes on elsewhere.
+    float* spill = p.partial +
+                   (static_cast<int64_t>(blockIdx.x) * 2 + head.starts) *
+                       kRows * (kD + 2);
     for (int i = threadIdx.x; i < n_rows * (kD / 2); i += kThreads) {
       const int r = i / (kD / 2), d = (i % (kD / 2)) * 2;
       float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w)
-        top = fmaxf(top, join[(w * pitch + r) * S::kJoinFloats + kD]);
+      for (int w = first; w <= last; ++w)
+        if (s_parts[w / 2][w % 2].b >= 0)
+          top = fmaxf(top,
+                      part_at(w / 2, w % 2)[r * S::kJoinFloats + kD]);
       const float ref = top == -INFINITY ? 0.f : top;
       float x = 0.f, y = 0.f, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float* src = join + (w * pitch + r) * S::kJoinFloats;
+      for (int w = first; w <= last; ++w) {
+        if (s_parts[w / 2][w % 2].b < 0) continue;
+        const float* src = part_at(w / 2, w % 2) + r * S::kJoinFloats;
         const float f = ex2_approx(src[kD] - ref);
         const float2 ow = *reinterpret_cast<const float2*>(src + d);
         x = fmaf(f, ow.x, x);
@@ -689,15 +825,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (whole) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int64_t at = static_cast<int64_t>(seg.b) *
-                               (p.c.kv_heads * p.group) +
-                           head0 + r;
+        const int64_t at =
+            static_cast<int64_t>(head.b) * (p.c.kv_heads * p.group) +
+            kvh * p.group + tile * kRows + r;
         *reinterpret_cast<uint32_t*>(p.out + at * kD + d) =
             pack_bf16(x * inv, y * inv);
         if (d == 0 && p.lse != nullptr)
           p.lse[at] = (top + log2f(sum)) * kLn2;
       } else {
-        float* dst = part + r * (kD + 2);
+        float* dst = spill + r * (kD + 2);
         *reinterpret_cast<float2*>(dst + d) = make_float2(x, y);
         if (d == 0) {
           dst[kD] = top;
@@ -705,101 +841,173 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
+    first = scan;
   }
 }
 
-// Adds up the pieces of the (sequence, head tile)s that several CTAs share,
-// in the order of their keys; writes the rows of empty sequences. One block
-// per (sequence, head tile).
+// Adds up the parts of the (sequence, head tile)s that several CTAs share, in
+// the order of the keys; writes the rows of empty sequences. One block per
+// (sequence, head tile).
 template <int kD>
 __global__ void __launch_bounds__(kJoinThreads)
     decode_join_kernel(const __grid_constant__ DecodeParams p) {
-  __shared__ Prefix<kJoinThreads> prefix;
+  constexpr int kPer = kD / 32;  // elements a lane
+  __shared__ int64_t sums[2][kJoinThreads / 32];
+  __shared__ float tops[kJoinThreads / 32], totals[kJoinThreads / 32];
+  __shared__ float rows[kJoinThreads / 32][kD];
   const int heads = p.c.kv_heads * p.tiles;
   const int b = blockIdx.x / heads, vh = blockIdx.x % heads;
-  int64_t before = 0, all = 0;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  int64_t before = 0, total = 0;
   for (int i = threadIdx.x; i < p.c.n_seqs; i += kJoinThreads) {
     const int n = chunks_of(context(p, i));
-    all += n;
+    total += n;
     if (i < b) before += n;
   }
-  int64_t total, sum_before;
-  block_scan<kJoinThreads>(&prefix, all, &total);
-  block_scan<kJoinThreads>(&prefix, before, &sum_before);
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, s);
+    total += __shfl_xor_sync(0xffffffffu, total, s);
+  }
+  if (lane == 0) {
+    sums[0][warp] = before;
+    sums[1][warp] = total;
+  }
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) {
+    before += sums[0][w];
+    total += sums[1][w];
+  }
   total *= heads;
-  const int n_ctas = active_ctas(p, total);
+  const Split split(p, total);
   const int n = chunks_of(context(p, b));
-  const int64_t first = sum_before * heads + static_cast<int64_t>(vh) * n;
-  const int64_t last = first + n - 1;
+  const int64_t first = before * heads + static_cast<int64_t>(vh) * n;
   const int kvh = vh / p.tiles, tile = vh % p.tiles;
   const int n_rows = min(kRows, p.group - tile * kRows);
   const int64_t at0 = static_cast<int64_t>(b) * (p.c.kv_heads * p.group) +
                       kvh * p.group + tile * kRows;
-  // The CTA of chunk c: the largest i with run_begin(i) <= c.
-  auto cta_of = [&](int64_t c) {
-    int i = static_cast<int>((c * n_ctas) / total);
-    while (i + 1 < n_ctas && run_begin(total, i + 1, n_ctas) <= c) ++i;
-    while (i > 0 && run_begin(total, i, n_ctas) > c) --i;
-    return i;
-  };
+  // CTAs c0 .. c1 hold the head's chunks: c0 begins it (its slot 1), in the
+  // others it goes on (their slot 0).
   int c0 = 0, c1 = -1;
   if (n > 0) {
-    c0 = cta_of(first);
-    c1 = cta_of(last);
-    if (c0 == c1) return;  // one CTA had all of it
+    c0 = split.warp_of(first) / kWarps;
+    c1 = split.warp_of(first + n - 1) / kWarps;
   }
-  for (int i = threadIdx.x; i < n_rows * (kD / 2); i += kJoinThreads) {
-    const int r = i / (kD / 2), d = (i % (kD / 2)) * 2;
-    float top = -INFINITY, sum = 0.f, x = 0.f, y = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      // Slot 0 holds a CTA's first piece if it starts inside its head.
-      const int slot = run_begin(total, c, n_ctas) > first ? 0 : 1;
-      const float* src =
-          p.partial +
-          ((static_cast<int64_t>(c) * 2 + slot) * kRows + r) * (kD + 2);
-      const float m = src[kD];
-      const float2 ow = *reinterpret_cast<const float2*>(src + d);
-      const float next = fmaxf(top, m);
+  // Every block waits, so that this grid ends after the one it follows.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (c0 == c1) return;  // one CTA had all of it
+  // `ways` warps a row, every ways-th part each, then added up.
+  constexpr int kBatch = 4;
+  const int ways = min(kJoinThreads / 32 / n_rows, c1 - c0 + 1);
+  const int r = warp % n_rows, way = warp / n_rows;
+  float top = -INFINITY, sum = 0.f, acc[kPer] = {};
+  if (way < ways) {
+    for (int base = c0 + way; base <= c1; base += ways * kBatch) {
+      float m[kBatch], l[kBatch], x[kBatch][kPer];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int c = base + i * ways;
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) x[i][e] = 0.f;
+        if (c > c1) continue;
+        const float* src =
+            p.partial + ((static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) *
+                             kRows +
+                         r) *
+                            (kD + 2);
+        m[i] = src[kD];
+        l[i] = src[kD + 1];
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2) {
+          const float2 v =
+              *reinterpret_cast<const float2*>(src + lane * kPer + e);
+          x[i][e] = v.x;
+          x[i][e + 1] = v.y;
+        }
+      }
+      float next = top;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) next = fmaxf(next, m[i]);
       const float ref = next == -INFINITY ? 0.f : next;
-      const float f = ex2_approx(top - ref), g = ex2_approx(m - ref);
-      x = fmaf(x, f, ow.x * g);
-      y = fmaf(y, f, ow.y * g);
-      sum = fmaf(sum, f, src[kD + 1] * g);
+      const float f = ex2_approx(top - ref);
       top = next;
+      sum *= f;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] *= f;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float g = ex2_approx(m[i] - ref);
+        sum = fmaf(g, l[i], sum);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) acc[e] = fmaf(g, x[i][e], acc[e]);
+      }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    *reinterpret_cast<uint32_t*>(p.out + (at0 + r) * kD + d) =
-        pack_bf16(x * inv, y * inv);
-    if (d == 0 && p.lse != nullptr)
-      p.lse[at0 + r] = (top + log2f(sum)) * kLn2;
+    if (lane == 0) {
+      tops[warp] = top;
+      totals[warp] = sum;
+    }
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) rows[warp][lane * kPer + e] = acc[e];
   }
+  __syncthreads();
+  if (way != 0) return;
+  float all = -INFINITY;
+  for (int w = 0; w < ways; ++w) all = fmaxf(all, tops[r + w * n_rows]);
+  const float ref = all == -INFINITY ? 0.f : all;
+  sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+  for (int w = 0; w < ways; ++w) {
+    const int at = r + w * n_rows;
+    const float g = ex2_approx(tops[at] - ref);
+    sum = fmaf(g, totals[at], sum);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      acc[e] = fmaf(g, rows[at][lane * kPer + e], acc[e]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint32_t* dst =
+      reinterpret_cast<uint32_t*>(p.out + (at0 + r) * kD + lane * kPer);
+#pragma unroll
+  for (int e = 0; e < kPer / 2; ++e)
+    dst[e] = pack_bf16(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  if (lane == 0 && p.lse != nullptr)
+    p.lse[at0 + r] = (all + log2f(sum)) * kLn2;
 }
 
-int sm_count(int* sms) {
-  int dev = 0;
-  VEDA_CUDA(cudaGetDevice(&dev));
-  VEDA_CUDA(
-      cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
-  return VEDA_OK;
-}
-
-template <int kD, int kStore, int kStages>
+// kPitch: the heads of a tile, at most.
+template <int kD, int kStore, int kStages, int kPitch>
 int launch(const DecodeParams& p, cudaStream_t stream) {
   using S = Shape<kD, kStore>;
-  const int pitch = p.group < kRows ? p.group : kRows;
-  const int smem = kWarps * kStages * S::kStageBytes +
-                   kWarps * pitch * S::kJoinFloats * 4;
-  VEDA_CUDA(cudaFuncSetAttribute(decode_kernel<kD, kStore, kStages>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 smem));
-  decode_kernel<kD, kStore, kStages>
-      <<<p.n_ctas, kThreads, smem, stream>>>(p);
-  int rc = check_launch("decode_kernel");
+  constexpr int kSmem = kWarps * (kStages * S::kStageBytes +
+                                  part_floats<kD, kStore>(kPitch) * 4);
+  static_assert(kSmem <= 226 * 1024, "beside the static part");
+  static std::atomic<uint64_t> allowed{0};
+  int rc = allow_smem(
+      reinterpret_cast<const void*>(decode_kernel<kD, kStore, kStages>),
+      kSmem, &allowed);
   if (rc != VEDA_OK) return rc;
+  decode_kernel<kD, kStore, kStages>
+      <<<p.n_ctas, kThreads, kSmem, stream>>>(p);
+  rc = check_launch("decode_kernel");
+  if (rc != VEDA_OK) return rc;
+  // The join starts while the last CTAs run (griddepcontrol).
   const int64_t blocks =
       static_cast<int64_t>(p.c.n_seqs) * p.c.kv_heads * p.tiles;
-  decode_join_kernel<kD>
-      <<<static_cast<unsigned>(blocks), kJoinThreads, 0, stream>>>(p);
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.blockDim = dim3(kJoinThreads);
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  VEDA_CUDA(cudaLaunchKernelEx(&config, decode_join_kernel<kD>, p));
   return check_launch("decode_join_kernel");
 }
 
@@ -808,13 +1016,13 @@ int launch(const DecodeParams& p, cudaStream_t stream) {
 template <int kD, int kStore>
 int launch_stages(const DecodeParams& p, cudaStream_t stream) {
   if constexpr (kD == 64) {
-    return launch<kD, kStore, kStore == kStoreBf16 ? 5 : 8>(p, stream);
+    return launch<kD, kStore, kStore == kStoreBf16 ? 5 : 8, kRows>(p, stream);
   } else if constexpr (kStore == kStoreBf16) {
-    return p.group <= 8 ? launch<kD, kStore, 3>(p, stream)
-                        : launch<kD, kStore, 2>(p, stream);
+    return p.group <= 8 ? launch<kD, kStore, 3, 8>(p, stream)
+                        : launch<kD, kStore, 2, kRows>(p, stream);
   } else {
-    return p.group <= 8 ? launch<kD, kStore, 5>(p, stream)
-                        : launch<kD, kStore, 4>(p, stream);
+    return p.group <= 8 ? launch<kD, kStore, 5, 8>(p, stream)
+                        : launch<kD, kStore, 4, kRows>(p, stream);
   }
 }
 
@@ -827,7 +1035,7 @@ using namespace veda;
 extern "C" int64_t veda_decode_workspace(int32_t head_dim) {
   if (head_dim != 64 && head_dim != 128) return -1;
   int sms = 0;
-  if (sm_count(&sms) != VEDA_OK) return -1;
+  if (device_sms(&sms) != VEDA_OK) return -1;
   return static_cast<int64_t>(sms) * 2 * kRows * (head_dim + 2) *
          static_cast<int64_t>(sizeof(float));
 }
@@ -866,7 +1074,7 @@ extern "C" int veda_decode(
   const int64_t need = veda_decode_workspace(head_dim);
   VEDA_REQUIRE(need > 0 && workspace_bytes >= need,
                "workspace too small (veda_decode_workspace)");
-  rc = sm_count(&p.n_ctas);
+  rc = device_sms(&p.n_ctas);
   if (rc != VEDA_OK) return rc;
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_sb = q_stride_b;

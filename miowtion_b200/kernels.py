@@ -147,18 +147,26 @@ def aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """t [rows, heads, D] as the kernels read it (16-byte pieces of a row):
     itself, or a contiguous copy where its address or strides do not allow
     that."""
-    if t.data_ptr() % 16 == 0 and t.stride(2) == 1 and all(
-            s >= 0 and s % 8 == 0 for s in t.stride()[:2]):
+    rows, heads, last = t.stride()
+    if last == 1 and not (rows % 8 or heads % 8 or t.data_ptr() % 16):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def on_stream(t: torch.Tensor) -> torch.Tensor:
-    """t, kept alive for the work of the current stream: a pack's tensors
-    may be dropped by their owner while another stream still reads them."""
-    if not torch.cuda.is_current_stream_capturing():
-        t.record_stream(torch.cuda.current_stream(t.device))
-    return t
+# CUDA devices on which the kernels have been found to run.
+_READY: set[int] = set()
+
+
+def require_ready(device: torch.device, op: str) -> None:
+    """Raises NotImplementedError where the kernels cannot run (no
+    fallback)."""
+    if device.type == 'cuda' and device.index in _READY:
+        return
+    reason = unavailable_reason(device)
+    if reason is not None:
+        raise NotImplementedError(
+            f'{op} unavailable on {device}: {reason}; there is no fallback')
+    _READY.add(device.index)
 
 
 def block_sparse_attention_lists(q: torch.Tensor, k: torch.Tensor,
@@ -476,27 +484,35 @@ def _causal_checks(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                    pack: sequences.SequencePack) -> int:
     """Argument checks of the causal attention; returns the heads per key
     head."""
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
+    q_shape, k_shape = q.shape, k.shape
+    if len(q_shape) != 3 or len(k_shape) != 3 or k_shape != v.shape:
         raise ValueError('q, k and v must be [rows, heads, D], k and v of '
                          'one shape')
-    if q.shape[2] not in (64, 128) or k.shape[2] != q.shape[2]:
+    rows, heads, dim = q_shape
+    k_rows, kv_heads, k_dim = k_shape
+    if dim not in (64, 128) or k_dim != dim:
         raise ValueError('q, k and v need one head dim, 64 or 128: '
-                         f'{q.shape[2]} and {k.shape[2]}')
-    heads, kv_heads = q.shape[1], k.shape[1]
+                         f'{dim} and {k_dim}')
     if (kv_heads < 1 or heads % kv_heads
             or not 1 <= heads // kv_heads <= sequences.TILE):
         raise ValueError('the query heads must be 1 to 128 times the key '
                          f'heads: {heads} and {kv_heads}')
-    if q.shape[0] != pack.total_q or k.shape[0] != pack.total_k:
+    if rows != pack.total_q or k_rows != pack.total_k:
         raise ValueError(f'the pack has {pack.total_q} query and '
-                         f'{pack.total_k} key rows, not {q.shape[0]} and '
-                         f'{k.shape[0]}')
-    if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
+                         f'{pack.total_k} key rows, not {rows} and {k_rows}')
+    bf16, device = torch.bfloat16, pack.device
+    if q.dtype != bf16 or k.dtype != bf16 or v.dtype != bf16:
         raise ValueError('q, k and v must be bf16: '
                          f'{q.dtype}, {k.dtype}, {v.dtype}')
-    if any(t.device != pack.device for t in (q, k, v)):
-        raise ValueError(f'q, k and v must be on {pack.device}, as the pack')
+    if q.device != device or k.device != device or v.device != device:
+        raise ValueError(f'q, k and v must be on {device}, as the pack')
     return heads // kv_heads
+
+
+def _rows_args(t: torch.Tensor) -> tuple[int, int, int]:
+    """Address and row and head strides, as the C ABI takes them."""
+    rows, heads, _ = t.stride()
+    return t.data_ptr(), rows, heads
 
 
 def causal_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -505,22 +521,18 @@ def causal_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """(out [rows, heads, D] bf16, lse [rows, heads] fp32 or None) of
     `causal_attention`, without gradients."""
     group = _causal_checks(q, k, v, pack)
-    _require(q, 'causal_attention')
+    require_ready(q.device, 'causal_attention')
     q, k, v = aligned_rows(q), aligned_rows(k), aligned_rows(v)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = (torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-           if return_lse else None)
-    with torch.cuda.device(q.device):
-        items = on_stream(pack.tables(group).forward)
-        _lib.call('veda_causal_fwd', q.data_ptr(), q.stride(0), q.stride(1),
-                  k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                  v.stride(0), v.stride(1), q.shape[0], k.shape[0],
-                  q.shape[1], k.shape[1], q.shape[2], items.data_ptr(),
-                  items.shape[0], out.data_ptr(), out.stride(0),
-                  out.stride(1), _lib.ptr(lse),
-                  lse.stride(0) if lse is not None else 0,
-                  lse.stride(1) if lse is not None else 0, scale,
-                  _lib.stream_ptr(q.device))
+    rows, heads, dim = q.shape
+    k_rows, kv_heads, _ = k.shape
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = (q.new_empty((rows, heads), dtype=torch.float32) if return_lse
+           else None)
+    _lib.call_on(q.device.index, 'veda_causal_fwd', *_rows_args(q),
+                 *_rows_args(k), *_rows_args(v), rows, k_rows, heads,
+                 kv_heads, dim, *pack.tables(group).forward_args,
+                 out.data_ptr(), heads * dim, dim, _lib.ptr(lse), heads, 1,
+                 scale)
     return out, lse
 
 
@@ -532,35 +544,34 @@ def causal_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """(dq, dk, dv) of `causal_attention` (None where not wanted); out and lse
     as the forward returned them."""
     group = _causal_checks(q, k, v, pack)
-    _require(q, 'causal_attention backward')
-    q, k, v, out, dout = (aligned_rows(t) for t in (q, k, v, out, dout))
-
-    def empty(t, wanted):
-        return (torch.empty(t.shape, dtype=t.dtype, device=t.device)
-                if wanted else None)
-
-    dq, dk, dv = empty(q, want_q), empty(k, want_kv), empty(v, want_kv)
-    grads = []
-    for g in (dq, dk, dv):
-        grads += ([g.data_ptr(), g.stride(0), g.stride(1)] if g is not None
-                  else [None, 0, 0])
-    with torch.cuda.device(q.device):
-        tables = pack.tables(group)
-        need = _lib.load().veda_causal_bwd_workspace(k.shape[1],
-                                                     tables.n_tiles)
-        ws = torch.empty(max(need, 16) // 4, dtype=torch.float32,
-                         device=q.device)
-        q_items, k_items = on_stream(tables.query), on_stream(tables.key)
-        _lib.call('veda_causal_bwd', q.data_ptr(), q.stride(0), q.stride(1),
-                  k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                  v.stride(0), v.stride(1), out.data_ptr(), out.stride(0),
-                  out.stride(1), dout.data_ptr(), dout.stride(0),
-                  dout.stride(1), lse.data_ptr(), lse.stride(0),
-                  lse.stride(1), q.shape[0], k.shape[0], q.shape[1],
-                  k.shape[1], q.shape[2], q_items.data_ptr(),
-                  q_items.shape[0], k_items.data_ptr(), k_items.shape[0],
-                  tables.n_tiles, *grads, scale, ws.data_ptr(),
-                  ws.numel() * 4, _lib.stream_ptr(q.device))
+    require_ready(q.device, 'causal_attention backward')
+    if out.shape != q.shape or dout.shape != q.shape or (
+            lse.shape != q.shape[:2]) or lse.dtype != torch.float32:
+        raise ValueError('out and dout must have the shape of q, lse be fp32 '
+                         '[rows, heads]')
+    if out.dtype != q.dtype or dout.dtype != q.dtype:
+        raise ValueError('out and dout must be bf16')
+    if any(t.device != q.device for t in (out, dout, lse)):
+        raise ValueError(f'out, dout and lse must be on {q.device}')
+    q, k, v = aligned_rows(q), aligned_rows(k), aligned_rows(v)
+    out, dout = aligned_rows(out), aligned_rows(dout)
+    rows, heads, dim = q.shape
+    k_rows, kv_heads, _ = k.shape
+    contiguous = torch.contiguous_format
+    dq = torch.empty_like(q, memory_format=contiguous) if want_q else None
+    dk = torch.empty_like(k, memory_format=contiguous) if want_kv else None
+    dv = torch.empty_like(v, memory_format=contiguous) if want_kv else None
+    tables = pack.tables(group)
+    # The workspace of veda_causal_bwd: two floats per row of a query tile.
+    ws = q.new_empty((max(1, 2 * kv_heads * tables.n_tiles * sequences.TILE),),
+                     dtype=torch.float32)
+    _lib.call_on(q.device.index, 'veda_causal_bwd', *_rows_args(q),
+                 *_rows_args(k), *_rows_args(v), *_rows_args(out),
+                 *_rows_args(dout), lse.data_ptr(), *lse.stride(), rows,
+                 k_rows, heads, kv_heads, dim, *tables.gradient_args,
+                 _lib.ptr(dq), heads * dim, dim, _lib.ptr(dk),
+                 kv_heads * dim, dim, _lib.ptr(dv), kv_heads * dim, dim,
+                 scale, ws.data_ptr(), ws.numel() * 4)
     return dq, dk, dv
 
 
@@ -572,11 +583,14 @@ class _CausalAttention(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, out, lse)
         ctx.pack, ctx.scale = pack, scale
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _dlse):
+        if dout is None:
+            return None, None, None, None, None
         q, k, v, out, lse = ctx.saved_tensors
         need = ctx.needs_input_grad
         dq, dk, dv = causal_attention_bwd(q, k, v, out, dout, lse, ctx.pack,
@@ -611,7 +625,8 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         before it that share its key tile.
     """
     scale = softmax_scale(scale, q.shape[-1])
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
+                                    or v.requires_grad):
         out, lse = _CausalAttention.apply(q, k, v, pack, scale)
     else:
         out, lse = causal_attention_fwd(q, k, v, pack, scale, return_lse)

@@ -85,6 +85,14 @@ class PagedCache:
             raise ValueError('pages and scales must be contiguous, 16-byte '
                              'aligned and on one device')
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_pages, self.kv_heads, self.page_size, self.head_dim = (
+            n_pages, kv_heads, page_size, dim)
+        self.device = k.device
+        # The C ABI's arguments that describe the pages.
+        self._pages = (k.data_ptr(), v.data_ptr(), _lib.ptr(k_scale),
+                       _lib.ptr(v_scale), n_pages, page_size, kv_heads, dim,
+                       STORAGE[self.storage][0])
+        self._workspace: int | None = None
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, kv_heads: int, head_dim: int,
@@ -104,61 +112,40 @@ class PagedCache:
         ks, vs = (torch.empty(shape[:3], device=device) for _ in range(2))
         return cls(k, v, ks, vs)
 
-    @property
-    def n_pages(self) -> int:
-        return self.k.shape[0]
+    def _index(self, t: torch.Tensor, name: str, n: int) -> int:
+        """Address of an int32 [n] argument."""
+        if (t.dtype != torch.int32 or t.shape != (n,)
+                or t.device != self.device):
+            raise ValueError(f'{name} must be int32 [{n}] on {self.device}')
+        if n > 1 and t.stride(0) != 1:
+            raise ValueError(f'{name} must be contiguous')
+        return t.data_ptr()
 
-    @property
-    def kv_heads(self) -> int:
-        return self.k.shape[1]
-
-    @property
-    def page_size(self) -> int:
-        return self.k.shape[2]
-
-    @property
-    def head_dim(self) -> int:
-        return self.k.shape[3]
-
-    def _require(self, op: str) -> None:
-        reason = kernels.unavailable_reason(self.k.device)
-        if reason is not None:
-            raise NotImplementedError(
-                f'PagedCache.{op} unavailable on {self.k.device}: {reason}')
-
-    def _index(self, t: torch.Tensor, name: str, shape: tuple) -> None:
-        if (t.dtype != torch.int32 or t.device != self.k.device
-                or t.dim() != len(shape)
-                or any(n is not None and n != m
-                       for n, m in zip(shape, t.shape))):
-            raise ValueError(f'{name} must be int32 {list(shape)} on '
-                             f'{self.k.device}')
-        if t.stride(-1) != 1 and t.shape[-1] > 1:
-            raise ValueError(f'{name} must be contiguous in its last '
-                             'dimension')
-
-    def _table(self, table: torch.Tensor, n: int) -> None:
-        self._index(table, 'table', (n, None))
-        if table.shape[1] < 1:
+    def _view(self, table: torch.Tensor, n: int) -> tuple:
+        """The C ABI's arguments that describe the cache and its table of n
+        sequences."""
+        if (table.dtype != torch.int32 or table.dim() != 2
+                or table.shape[0] != n or table.device != self.device):
+            raise ValueError(f'table must be int32 [{n}, max_pages] on '
+                             f'{self.device}')
+        width = table.shape[1]
+        if width < 1:
             raise ValueError('a table row holds one page at least')
-        if table.shape[1] * self.page_size >= 2 ** 31:
+        if width * self.page_size >= 2 ** 31:
             raise ValueError('a table row addresses fewer than 2^31 rows')
-        if n > 1 and table.stride(0) < table.shape[1]:
+        pitch, step = table.stride()
+        if width > 1 and step != 1:
+            raise ValueError('table must be contiguous in its last dimension')
+        if n == 1:
+            pitch = width
+        elif pitch < width:
             raise ValueError('the rows of the table must not overlap')
+        return (*self._pages, table.data_ptr(), pitch, width, n)
 
     def _pack(self, pack: sequences.SequencePack) -> None:
-        if pack.device != self.k.device:
+        if pack.device != self.device:
             raise ValueError(f'the pack is on {pack.device}, the cache on '
-                             f'{self.k.device}')
-
-    def _view(self, table: torch.Tensor) -> tuple:
-        """The C ABI's arguments that describe the cache and its table."""
-        n, width = table.shape
-        return (self.k.data_ptr(), self.v.data_ptr(), _lib.ptr(self.k_scale),
-                _lib.ptr(self.v_scale), self.n_pages, self.page_size,
-                self.kv_heads, self.head_dim, STORAGE[self.storage][0],
-                table.data_ptr(), table.stride(0) if n > 1 else width, width,
-                n)
+                             f'{self.device}')
 
     def write(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
               starts: torch.Tensor, pack: sequences.SequencePack) -> None:
@@ -172,40 +159,35 @@ class PagedCache:
             starts: [n_sequences] int32, rows already in each context.
             pack: The rows of each sequence (its q_lengths).
         """
+        rows = (pack.total_q, self.kv_heads, self.head_dim)
         for name, t in (('k', k), ('v', v)):
-            if (t.shape != (pack.total_q, self.kv_heads, self.head_dim)
-                    or t.dtype != torch.bfloat16
-                    or t.device != self.k.device):
-                raise ValueError(
-                    f'{name} must be bf16 [{pack.total_q}, {self.kv_heads}, '
-                    f'{self.head_dim}] on {self.k.device}')
-        self._table(table, pack.n_sequences)
-        self._index(starts, 'starts', (pack.n_sequences,))
+            if (t.shape != rows or t.dtype != torch.bfloat16
+                    or t.device != self.device):
+                raise ValueError(f'{name} must be bf16 {list(rows)} on '
+                                 f'{self.device}')
+        view = self._view(table, pack.n_sequences)
+        start_args = self._index(starts, 'starts', pack.n_sequences)
         self._pack(pack)
-        self._require('write')
+        kernels.require_ready(self.device, 'PagedCache.write')
         k, v = kernels.aligned_rows(k), kernels.aligned_rows(v)
-        with torch.cuda.device(self.k.device):
-            pack_offsets = kernels.on_stream(pack.q_offsets)
-            _lib.call('veda_cache_write', *self._view(table), k.data_ptr(),
-                      k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                      v.stride(1), pack.total_q, pack_offsets.data_ptr(),
-                      starts.data_ptr(), _lib.stream_ptr(self.k.device))
+        (k_row, k_head, _), (v_row, v_head, _) = k.stride(), v.stride()
+        _lib.call_on(self.device.index, 'veda_cache_write', *view,
+                     k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
+                     rows[0], pack.offsets()[0].data_ptr(), start_args)
 
     def read(self, table: torch.Tensor, pack: sequences.SequencePack
              ) -> tuple[torch.Tensor, torch.Tensor]:
         """The contexts' rows as bf16 (k, v), [pack.total_k, kv_heads, D]:
         rows 0 .. k_lengths[b] - 1 of each sequence, packed."""
-        self._table(table, pack.n_sequences)
+        view = self._view(table, pack.n_sequences)
         self._pack(pack)
-        self._require('read')
-        shape = (pack.total_k, self.kv_heads, self.head_dim)
-        k, v = (torch.empty(shape, dtype=torch.bfloat16,
-                            device=self.k.device) for _ in range(2))
-        with torch.cuda.device(self.k.device):
-            offsets = kernels.on_stream(pack.k_offsets)
-            _lib.call('veda_cache_read', *self._view(table),
-                      offsets.data_ptr(), pack.total_k, k.data_ptr(),
-                      v.data_ptr(), _lib.stream_ptr(self.k.device))
+        kernels.require_ready(self.device, 'PagedCache.read')
+        k, v = (torch.empty((pack.total_k, self.kv_heads, self.head_dim),
+                            dtype=torch.bfloat16, device=self.device)
+                for _ in range(2))
+        _lib.call_on(self.device.index, 'veda_cache_read', *view,
+                     pack.offsets()[1].data_ptr(), pack.total_k, k.data_ptr(),
+                     v.data_ptr())
         return k, v
 
     def attend(self, q: torch.Tensor, table: torch.Tensor,
@@ -228,29 +210,30 @@ class PagedCache:
             sequence without rows.
         """
         if (q.dim() != 3 or q.shape[2] != self.head_dim
-                or q.dtype != torch.bfloat16 or q.device != self.k.device):
+                or q.dtype != torch.bfloat16 or q.device != self.device):
             raise ValueError(f'q must be bf16 [n_sequences, heads, '
-                             f'{self.head_dim}] on {self.k.device}')
-        n, heads = q.shape[:2]
+                             f'{self.head_dim}] on {self.device}')
+        n, heads, dim = q.shape
         if n < 1 or heads < 1 or heads % self.kv_heads:
             raise ValueError('q needs a sequence, and heads a multiple of '
                              f'{self.kv_heads}')
-        if torch.is_grad_enabled() and q.requires_grad:
+        if q.requires_grad and torch.is_grad_enabled():
             raise ValueError('attention over the cache has no gradient')
-        self._table(table, n)
-        self._index(lengths, 'lengths', (n,))
-        scale = kernels.softmax_scale(scale, self.head_dim)
-        self._require('attend')
+        view = self._view(table, n)
+        length_args = self._index(lengths, 'lengths', n)
+        scale = kernels.softmax_scale(scale, dim)
+        kernels.require_ready(self.device, 'PagedCache.attend')
         q = kernels.aligned_rows(q)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = (torch.empty(n, heads, dtype=torch.float32, device=q.device)
-               if return_lse else None)
-        with torch.cuda.device(self.k.device):
-            need = _lib.load().veda_decode_workspace(self.head_dim)
-            ws = torch.empty(max(need, 16) // 4, dtype=torch.float32,
-                             device=q.device)
-            _lib.call('veda_decode', *self._view(table), lengths.data_ptr(),
-                      q.data_ptr(), q.stride(0), q.stride(1), heads,
-                      out.data_ptr(), _lib.ptr(lse), scale, ws.data_ptr(),
-                      ws.numel() * 4, _lib.stream_ptr(q.device))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        lse = (q.new_empty((n, heads), dtype=torch.float32) if return_lse
+               else None)
+        if self._workspace is None:
+            with torch.cuda.device(self.device):
+                self._workspace = _lib.load().veda_decode_workspace(dim)
+        # Allocated for the call: captured graphs share no workspace.
+        ws = q.new_empty((self._workspace // 4,), dtype=torch.float32)
+        q_row, q_head, _ = q.stride()
+        _lib.call_on(self.device.index, 'veda_decode', *view, length_args,
+                     q.data_ptr(), q_row, q_head, heads, out.data_ptr(),
+                     _lib.ptr(lse), scale, ws.data_ptr(), self._workspace)
         return (out, lse) if return_lse else out

@@ -35,6 +35,10 @@ class WorkTables:
     query: torch.Tensor
     key: torch.Tensor
     n_tiles: int
+    # Address and items of each table, as a launch passes them.
+    forward_args: tuple[int, int]
+    gradient_args: tuple[int, int, int, int, int]
+    stream: int
 
 
 class SequencePack:
@@ -72,27 +76,25 @@ class SequencePack:
         self._k0 = np.concatenate([[0], np.cumsum(self.k_lengths)])
         both = _to_device(np.stack([self._q0, self._k0]), self.device)
         self.q_offsets, self.k_offsets = both[0], both[1]
+        self._stream = _stream(self.device)
+        self.n_sequences = self.q_lengths.size
+        # Every sequence has exactly one query.
+        self.single_tokens = bool((self.q_lengths == 1).all())
+        # No sequence has keys before (or without) its queries.
+        self.whole = bool((self.q_lengths == self.k_lengths).all())
         self._tables: dict[int, WorkTables] = {}
 
-    @property
-    def n_sequences(self) -> int:
-        return self.q_lengths.size
-
-    @property
-    def single_tokens(self) -> bool:
-        """Every sequence has exactly one query."""
-        return bool((self.q_lengths == 1).all())
-
-    @property
-    def whole(self) -> bool:
-        """No sequence has keys before (or without) its queries."""
-        return bool((self.q_lengths == self.k_lengths).all())
+    def offsets(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """(q_offsets, k_offsets) for a launch on the current stream."""
+        _keep(self._stream, self.q_offsets)
+        return self.q_offsets, self.k_offsets
 
     def tables(self, group: int) -> WorkTables:
         """The work tables for `group` query heads per key head, built (and
         copied to the device) on first use; build them before capturing a
         CUDA graph."""
-        if group not in self._tables:
+        tables = self._tables.get(group)
+        if tables is None:
             if (self.device.type == 'cuda'
                     and torch.cuda.is_current_stream_capturing()):
                 raise RuntimeError(
@@ -103,9 +105,31 @@ class SequencePack:
             flat = _to_device(np.concatenate([forward, query, key]),
                               self.device)
             a, b = len(forward), len(forward) + len(query)
-            self._tables[group] = WorkTables(group, flat[:a], flat[a:b],
-                                             flat[b:], n)
-        return self._tables[group]
+            parts = flat[:a], flat[a:b], flat[b:]
+            addresses = [t.data_ptr() if len(t) else 0 for t in parts]
+            tables = WorkTables(
+                group, *parts, n, (addresses[0], a),
+                (addresses[1], b - a, addresses[2], len(key), n),
+                _stream(self.device))
+            self._tables[group] = tables
+        else:
+            _keep(tables.stream, tables.forward)
+        return tables
+
+
+def _stream(device: torch.device) -> int:
+    return (torch.cuda.current_stream(device).cuda_stream
+            if device.type == 'cuda' else 0)
+
+
+def _keep(stream: int, t: torch.Tensor) -> None:
+    """Keeps the memory of a tensor made on `stream` until the work queued on
+    the current stream is done, should its owner drop it before."""
+    if not t.is_cuda or torch._C._cuda_getCurrentRawStream(
+            t.device.index) == stream:
+        return
+    if not torch.cuda.is_current_stream_capturing():
+        t.record_stream(torch.cuda.current_stream(t.device))
 
 
 def _lengths(values: Sequence[int], name: str) -> np.ndarray:
