@@ -14,16 +14,30 @@
 //               grows by more than 2^8, then O is rescaled). P goes back over
 //               S as bf16, in two halves of 64 keys.
 //   warp 8      TMA producer: the two Q tiles of an item, then its K and V
-//               tiles through one ring, V one tile behind K.
-//   warp 9      S = Q K^T of both tiles (owner of the tensor memory).
-//   warp 10     O += P V of both tiles.
-//   warp 11     idle; it completes the third warpgroup, whose registers go to
-//               the softmax warps (setmaxnreg).
-// While one tile's softmax runs the tensor core has the other tile's
-// products. Rows past a sequence's end belong to the next sequence (or to
-// nothing): their scores are set to -inf by selection and the value rows are
-// cleared in shared memory, so what stands there, NaN included, reaches no
-// row of this sequence.
+//               tiles through one ring.
+//   warp 9      issues every product (and owns the tensor memory), in one
+//               order: PV_A(b), QK_A(b + 1), PV_B(b), QK_B(b + 1).
+//   warps 10-11 idle; they complete the third warpgroup, whose registers go
+//               to the softmax warps (setmaxnreg).
+// The tensor core works on one tile while the softmax of the other runs: in
+// this order S_A is ready two products after P_A, and S_B two products later,
+// so the two softmaxes do not run at the same time and wait at the same time.
+// (With an issuer for QK and one for PV, P_A and P_B that became ready
+// together led to PV_A, PV_B, QK_A, QK_B, which keeps them together: 1,050
+// against 1,230 TFLOP/s on a causal sequence of 16,384 tokens, 24/6 heads, D =
+// 128. Measured on it and not kept: a block's first 32 weights computed
+// against the reference so far while the other scores come in, 1,191; a
+// quarter, half of the exponentials on the FMA pipes, 1,210 and 1,117 against
+// 1,247 without.) The blocks of
+// consecutive items form one stream, so the next item's first scores are
+// computed while this item's epilogue runs. One issuer also makes most
+// barriers superfluous: when the scores of block b arrive, everything issued
+// before them has finished, the product of block b - 1 among it; and the warps
+// that write P of an item's first block have read the previous item's O.
+// Rows past a sequence's end belong to the next sequence (or to nothing):
+// their scores are set to -inf by selection and the value rows are cleared in
+// shared memory, so what stands there, NaN included, reaches no row of this
+// sequence.
 //
 // All waits are bounded (common.cuh).
 #include "causal.cuh"
@@ -34,7 +48,7 @@ namespace causal {
 namespace {
 
 constexpr int kWarps = 12;
-constexpr int kProducer = 8, kQk = 9, kPv = 10;
+constexpr int kProducer = 8, kMma = 9;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
@@ -53,11 +67,8 @@ enum Bar {
   kSFull,       // [2] S of the tile's block finished
   kPHalfA = kSFull + 2,   // [2] P of keys 0-63 written (4 warps)
   kPHalfB = kPHalfA + 2,  // [2] P of keys 64-127 written (4 warps)
-  kPvDone = kPHalfB + 2,  // [2] O += P V of the tile's block finished
-  kODone = kPvDone + 2,   // the item's last products finished
-  kOFree,                 // the epilogue has read O (8 warps)
-  kDrainQk,
-  kDrainPv,
+  kODone = kPHalfB + 2,   // [2] the tile's last product of the item finished
+  kDrain = kODone + 2,
   kFull,                  // [kRing]
   kEmpty = kFull + 8,     // [kRing]
   kNumBars = kEmpty + 8
@@ -94,8 +105,8 @@ __device__ __forceinline__ float row_max32(const float* s) {
 }
 
 // exp2(s * scale - m) of 32 scores, as bf16 pairs into r; returns their sum.
-__device__ __forceinline__ float2 weights32(uint32_t* r, const float* s,
-                                            float2 scale2, float2 neg_m2) {
+__device__ __forceinline__ float weights32(uint32_t* r, const float* s,
+                                           float2 scale2, float2 neg_m2) {
   float2 sum_a = make_float2(0.f, 0.f), sum_b = make_float2(0.f, 0.f);
 #pragma unroll
   for (int c = 0; c < 32; c += 4) {
@@ -109,7 +120,8 @@ __device__ __forceinline__ float2 weights32(uint32_t* r, const float* s,
     r[c / 2] = pack_bf16(e0.x, e0.y);
     r[c / 2 + 1] = pack_bf16(e1.x, e1.y);
   }
-  return __fadd2_rn(sum_a, sum_b);
+  sum_a = __fadd2_rn(sum_a, sum_b);
+  return sum_a.x + sum_a.y;
 }
 
 __device__ __forceinline__ void rescale16(uint32_t t_row, float alpha) {
@@ -123,12 +135,26 @@ __device__ __forceinline__ void rescale16(uint32_t t_row, float alpha) {
   tmem_wait_st();
 }
 
-// Position in the ring's sequence of the K and V tiles of block j of an item
-// of n blocks: K0, K1, V0, K2, V1, ..., K(n-1), V(n-2), V(n-1).
-__device__ __forceinline__ int k_place(int j) { return j == 0 ? 0 : 2 * j - 1; }
-__device__ __forceinline__ int v_place(int j, int n) {
-  return j == n - 1 ? 2 * n - 1 : 2 * j + 2;
-}
+// The items of a CTA that have key tiles (every role walks the same ones).
+struct Stream {
+  int t;  // turns taken
+  int h;
+  QueryItem it;
+  // The next item with blocks (kEmpty: any); false at the end.
+  __device__ __forceinline__ bool next(const FwdParams& p, int64_t n_items,
+                                       bool keep_empty) {
+    while (static_cast<int64_t>(t) * gridDim.x < n_items) {
+      const int64_t i = turn(t++);
+      if (i >= n_items) continue;
+      const int entry = static_cast<int>(
+          static_cast<uint32_t>(i) / static_cast<uint32_t>(p.kv_heads));
+      h = static_cast<int>(i) - entry * p.kv_heads;
+      it = load_item<QueryItem>(p.table, entry);
+      if (it.blocks > 0 || keep_empty) return true;
+    }
+    return false;
+  }
+};
 
 template <int kD>
 __global__ void __launch_bounds__(32 * kWarps, 1)
@@ -158,14 +184,13 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   if (tid == 0) {
     for (int b = 0; b < kNumBars; ++b) {
       uint32_t count = 1;
-      if (b >= kPHalfA && b < kPvDone) count = 4;
-      if (b == kOFree) count = 8;
+      if (b >= kPHalfA && b < kODone) count = 4;
       mbar_init(&bars[b], count);
     }
     *abort = 0;
     fence_barrier_init();
   }
-  if (warp == kQk) {
+  if (warp == kMma) {
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
@@ -206,14 +231,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         ++n_ring;
         return true;
       };
-      for (int t = 0; run; ++t) {
-        const int64_t i = turn(t);
-        if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
-        if (i >= n_items) continue;
-        const int h = static_cast<int>(i % p.kv_heads);
-        const QueryItem it =
-            load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads));
-        if (it.blocks == 0) continue;
+      Stream st{0};
+      while (run && st.next(p, n_items, false)) {
         if (q_loads > 0 && !wait_all(&bars[kQEmpty], (q_loads - 1) & 1, abort,
                                      p.status))
           break;
@@ -224,17 +243,15 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
 #pragma unroll
             for (int c = 0; c < kD / 64; ++c)
               tma_load_3d(s_q + g * kTileBytes + c * 16384, &map_q,
-                          &bars[kQFull], c * 64, h * p.group,
-                          it.row + g * p.tokens);
+                          &bars[kQFull], c * 64, st.h * p.group,
+                          st.it.row + g * p.tokens);
         }
         __syncwarp();
         ++q_loads;
-        for (int j = 0; run && j < it.blocks; ++j) {
-          run = load(&map_k, h, it.k_row + j * kTile);
-          if (run && j >= 1)
-            run = load(&map_v, h, it.k_row + (j - 1) * kTile);
+        for (int j = 0; run && j < st.it.blocks; ++j) {
+          run = load(&map_k, st.h, st.it.k_row + j * kTile);
+          if (run) run = load(&map_v, st.h, st.it.k_row + j * kTile);
         }
-        if (run) run = load(&map_v, h, it.k_row + (it.blocks - 1) * kTile);
       }
       if (lane == 0 && *abort) {
         // Let the copies in flight land before the CTA retires.
@@ -246,93 +263,66 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
             mbar_wait(&bars[kFull + k % kRing], (k / kRing) & 1, &never,
                       nullptr);
       }
-    } else if (warp == kQk) {
-      // ---------------- S = Q K^T ----------------
-      constexpr uint32_t idesc = idesc_bf16(128, 128, false, false);
+    } else if (warp == kMma) {
+      // ---------------- the products ----------------
+      constexpr uint32_t idesc_qk = idesc_bf16(128, 128, false, false);
+      constexpr uint32_t idesc_pv = idesc_bf16(128, kD, false, true);
       const uint32_t q_lo = sw128_desc_lo(smem_u32(s_q), 16);
-      const uint32_t r_lo = sw128_desc_lo(smem_u32(s_ring), 16);
-      uint32_t b = 0;
-      int base = 0, items = 0;
+      const uint32_t k_lo = sw128_desc_lo(smem_u32(s_ring), 16);
+      const uint32_t v_lo = sw128_desc_lo(smem_u32(s_ring), 16384);
+      // Block b of the stream has its K tile at place 2b of the ring's
+      // sequence and its V tile at 2b + 1.
+      auto landed = [&](int place) -> bool {
+        return wait_all(&bars[kFull + place % kRing], (place / kRing) & 1,
+                        abort, p.status);
+      };
+      auto issue_qk = [&](int b, int g) {
+        const uint32_t a = q_lo + g * kTileUnits;
+        const uint32_t bk = k_lo + ((2 * b) % kRing) * kTileUnits;
+#pragma unroll
+        for (int kk = 0; kk < C::kSteps; ++kk) {
+          const uint32_t off = (kk >> 2) * (16384 >> 4) + (kk & 3) * 2;
+          umma_ss_warp(tmem + g * 128, a + off, bk + off, idesc_qk,
+                       kk > 0 ? 1u : 0u);
+        }
+        umma_commit_warp(&bars[kSFull + g]);
+      };
+      // K of block b, the j-th of its item's n, is read by both tiles.
+      auto release_k = [&](int b, int j, int n) {
+        umma_commit_warp(&bars[kEmpty + (2 * b) % kRing]);
+        if (j == n - 1) umma_commit_warp(&bars[kQEmpty]);
+      };
+      Stream st{0};
+      bool more = st.next(p, n_items, false);
       bool ok = true;
-      for (int t = 0; ok; ++t) {
-        const int64_t i = turn(t);
-        if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
-        if (i >= n_items) continue;
-        const int n =
-            load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads))
-                .blocks;
-        if (n == 0) continue;
+      int b = 0, items = 0;
+      if (more) {
+        ok = wait_all(&bars[kQFull], 0, abort, p.status) && landed(0);
+        if (ok) {
+          tc_fence_after();
+          issue_qk(0, 0);
+          issue_qk(0, 1);
+          release_k(0, 0, st.it.blocks);
+        }
+      }
+      while (ok && more) {
+        const int n = st.it.blocks, keys = st.it.keys;
+        more = st.next(p, n_items, false);
         for (int j = 0; j < n; ++j, ++b) {
-          const int place = base + k_place(j);
-          const int slot = place % kRing;
-          if (!wait_all(&bars[kFull + slot], (place / kRing) & 1, abort,
-                        p.status) ||
-              (j == 0 &&
-               !wait_all(&bars[kQFull], items & 1, abort, p.status))) {
+          const bool last = j == n - 1;
+          const bool ahead = !last || more;
+          const int slot = (2 * b + 1) % kRing;
+          if (!landed(2 * b + 1)) {
             ok = false;
             break;
           }
-          for (int g = 0; g < 2; ++g) {
-            // S held the P of the tile's previous block until its product.
-            if (b >= 1 && !wait_all(&bars[kPvDone + g], (b - 1) & 1, abort,
-                                    p.status)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const uint32_t a = q_lo + g * kTileUnits;
-            const uint32_t bk = r_lo + slot * kTileUnits;
-#pragma unroll
-            for (int kk = 0; kk < C::kSteps; ++kk) {
-              const uint32_t off = (kk >> 2) * (16384 >> 4) + (kk & 3) * 2;
-              umma_ss_warp(tmem + g * 128, a + off, bk + off, idesc,
-                           kk > 0 ? 1u : 0u);
-            }
-            umma_commit_warp(&bars[kSFull + g]);
-          }
-          if (!ok) break;
-          umma_commit_warp(&bars[kEmpty + slot]);
-          if (j == n - 1) umma_commit_warp(&bars[kQEmpty]);
-        }
-        base += 2 * n;
-        ++items;
-      }
-      if (*abort) {
-        volatile int never = 0;
-        umma_commit_warp(&bars[kDrainQk]);
-        mbar_wait(&bars[kDrainQk], 0, &never, nullptr);
-      }
-    } else if (warp == kPv) {
-      // ---------------- O += P V ----------------
-      constexpr uint32_t idesc = idesc_bf16(128, kD, false, true);
-      const uint32_t v_lo = sw128_desc_lo(smem_u32(s_ring), 16384);
-      uint32_t b = 0;
-      int base = 0, items = 0;
-      bool ok = true;
-      for (int t = 0; ok; ++t) {
-        const int64_t i = turn(t);
-        if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
-        if (i >= n_items) continue;
-        const QueryItem it =
-            load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads));
-        const int n = it.blocks;
-        if (n == 0) continue;
-        for (int j = 0; j < n; ++j, ++b) {
-          const int place = base + v_place(j, n);
-          const int slot = place % kRing;
-          if (!wait_all(&bars[kFull + slot], (place / kRing) & 1, abort,
-                        p.status))
-            ok = false;
-          if (ok && j == 0 && items >= 1 &&
-              !wait_all(&bars[kOFree], (items - 1) & 1, abort, p.status))
-            ok = false;
-          if (!ok) break;
           // Rows behind the sequence's last key take no part: a weight of 0
           // would not keep a NaN out.
-          const int rows = it.keys - j * kTile;
+          const int rows = keys - j * kTile;
           if (rows < kTile)
             clear_rows<kD>(s_ring + slot * kTileBytes, rows, lane);
           const uint32_t bv = v_lo + slot * kTileUnits;
+#pragma unroll
           for (int g = 0; g < 2; ++g) {
             if (!wait_all(&bars[kPHalfA + g], b & 1, abort, p.status)) {
               ok = false;
@@ -342,7 +332,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
               umma_ts_warp(tmem + 256 + g * 128, tmem + g * 128 + kk * 8,
-                           bv + kk * 128, idesc, (kk > 0 || j > 0) ? 1u : 0u);
+                           bv + kk * 128, idesc_pv,
+                           (kk > 0 || j > 0) ? 1u : 0u);
             if (!wait_all(&bars[kPHalfB + g], b & 1, abort, p.status)) {
               ok = false;
               break;
@@ -351,20 +342,32 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
 #pragma unroll
             for (int kk = 4; kk < 8; ++kk)
               umma_ts_warp(tmem + 256 + g * 128, tmem + g * 128 + kk * 8,
-                           bv + kk * 128, idesc, 1u);
-            umma_commit_warp(&bars[kPvDone + g]);
+                           bv + kk * 128, idesc_pv, 1u);
+            if (last) umma_commit_warp(&bars[kODone + g]);
+            if (ahead) {
+              if (g == 0) {
+                if (!landed(2 * b + 2) ||
+                    (last && !wait_all(&bars[kQFull], (items + 1) & 1, abort,
+                                       p.status))) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
+              }
+              issue_qk(b + 1, g);
+            }
           }
           if (!ok) break;
           umma_commit_warp(&bars[kEmpty + slot]);
-          if (j == n - 1) umma_commit_warp(&bars[kODone]);
+          if (ahead)
+            release_k(b + 1, last ? 0 : j + 1, last ? st.it.blocks : n);
         }
-        base += 2 * n;
         ++items;
       }
       if (*abort) {
         volatile int never = 0;
-        umma_commit_warp(&bars[kDrainPv]);
-        mbar_wait(&bars[kDrainPv], 0, &never, nullptr);
+        umma_commit_warp(&bars[kDrain]);
+        mbar_wait(&bars[kDrain], 0, &never, nullptr);
       }
     }
   } else {
@@ -383,13 +386,10 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     uint32_t b = 0;
     int items = 0;
     bool ok = true;
-    for (int t = 0; ok; ++t) {
-      const int64_t i = turn(t);
-      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
-      if (i >= n_items) continue;
-      const int h = static_cast<int>(i % p.kv_heads);
-      const QueryItem it =
-          load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads));
+    Stream st{0};
+    while (ok && st.next(p, n_items, true)) {
+      const int h = st.h;
+      const QueryItem it = st.it;
       const int n = it.blocks;
       // Keys of this row.
       const int seen = max(0, min(it.keys, it.kpos + token + 1));
@@ -403,25 +403,24 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         }
         tc_fence_after();
         uint32_t x[4][32];
+        auto scores = [&](int q) { return reinterpret_cast<float*>(x[q]); };
 #pragma unroll
-        for (int q32 = 0; q32 < 4; ++q32) tmem_ld32(t_s + q32 * 32, x[q32]);
+        for (int q = 0; q < 4; ++q) tmem_ld32(t_s + q * 32, x[q]);
         tmem_wait_ld();
         if (masked) {
 #pragma unroll
-          for (int q32 = 0; q32 < 4; ++q32) {
-            const int k = visible - q32 * 32;
+          for (int q = 0; q < 4; ++q) {
+            const int k = visible - q * 32;
             const uint32_t word =
                 k >= 32 ? ~0u : (k <= 0 ? 0u : (1u << k) - 1u);
-            float* f = reinterpret_cast<float*>(x[q32]);
 #pragma unroll
             for (int c = 0; c < 32; ++c)
-              if (!((word >> c) & 1u)) f[c] = -INFINITY;
+              if (!((word >> c) & 1u)) scores(q)[c] = -INFINITY;
           }
         }
-        float mx = -INFINITY;
+        float mx = row_max32(scores(0));
 #pragma unroll
-        for (int q32 = 0; q32 < 4; ++q32)
-          mx = fmaxf(mx, row_max32(reinterpret_cast<float*>(x[q32])));
+        for (int q = 1; q < 4; ++q) mx = fmaxf(mx, row_max32(scores(q)));
         const float mb = mx * p.scale_log2;
         const bool grow = mb > m_ref + 8.0f;
         if (j == 0) {
@@ -432,13 +431,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
           const float alpha =
               m_ref == -INFINITY ? 0.f : ex2_approx(m_ref - m_new);
           m_ref = m_new;
-          // O holds the previous blocks once their product finished; it is
-          // rescaled before this block's P is released.
-          if (!wait_all(&bars[kPvDone + grp], (b - 1) & 1, abort, p.status)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
+          // The previous blocks' products are in O (they were issued before
+          // this block's scores); this block's waits for P.
 #pragma unroll 1
           for (int q16 = 0; q16 < kD / 16; ++q16)
             rescale16(t_o + q16 * 16, alpha);
@@ -446,24 +440,20 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         }
         const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
         const float2 negm2 = make_float2(neg, neg);
-        float2 sums[4];
+        float sum = 0.f;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int q32 = half * 2 + q;
-            sums[q32] = weights32(x[q32], reinterpret_cast<float*>(x[q32]),
-                                  scale2, negm2);
-            tmem_st16(t_s + q32 * 16, x[q32]);
+        for (int q = 0; q < 4; ++q) {
+          sum += weights32(x[q], scores(q), scale2, negm2);
+          tmem_st16(t_s + q * 16, x[q]);
+          if (q & 1) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+              mbar_arrive(&bars[(q == 1 ? kPHalfA : kPHalfB) + grp]);
           }
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0)
-            mbar_arrive(&bars[(half == 0 ? kPHalfA : kPHalfB) + grp]);
         }
-        l += ((sums[0].x + sums[0].y) + (sums[1].x + sums[1].y)) +
-             ((sums[2].x + sums[2].y) + (sums[3].x + sums[3].y));
+        l += sum;
       }
       if (!ok) break;
       // ---------------- epilogue ----------------
@@ -473,11 +463,12 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       __nv_bfloat16* dst = p.out + out_row * p.out_st + out_head * p.out_sh;
       const float inv_l = l == 0.f ? 0.f : 1.0f / l;
       if (n > 0) {
-        if (!wait_all(&bars[kODone], items & 1, abort, p.status)) {
+        if (!wait_all(&bars[kODone + grp], items & 1, abort, p.status)) {
           ok = false;
           break;
         }
         tc_fence_after();
+        ++items;
       }
 #pragma unroll 1
       for (int c = 0; c < kD / 32; ++c) {
@@ -505,12 +496,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
                           __uint_as_float(o[8 * e + 7]) * inv_l));
         }
       }
-      if (n > 0) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[kOFree]);
-        ++items;
-      }
+      tc_fence_before();  // O is read before P of the next item is released
       if (write && p.lse != nullptr)
         p.lse[out_row * p.lse_st + out_head * p.lse_sh] =
             l == 0.f ? -INFINITY : (m_ref + log2f(l)) * kLn2;
@@ -518,7 +504,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kQk) {
+  if (warp == kMma) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
@@ -566,8 +552,7 @@ extern "C" int veda_causal_fwd(
                "n_heads must be 1 to 128 times kv_heads");
   VEDA_REQUIRE(total_q >= 0 && total_k >= 0 && total_q < (int64_t(1) << 31) &&
                    total_k < (int64_t(1) << 31) && n_items >= 0 &&
-                   n_items * kv_heads < (int64_t(1) << 40) &&
-                   n_items < (int64_t(1) << 31),
+                   n_items * kv_heads < (int64_t(1) << 31) - 65536,
                "bad sizes");
   VEDA_REQUIRE(softmax_scale > 0.f && isfinite(softmax_scale),
                "softmax_scale must be positive and finite");
