@@ -79,6 +79,35 @@ __device__ __forceinline__ void fence_async_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// Writes 16 bf16 (32 bytes, aligned): the rows of a tile are the lanes of a
+// warp, so a store meets 32 lines however narrow it is, and the widest takes
+// the fewest passes through them.
+__device__ __forceinline__ void store32(__nv_bfloat16* dst,
+                                        const uint32_t* w) {
+  asm volatile(
+      "st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst),
+      "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+      "r"(w[6]), "r"(w[7])
+      : "memory");
+}
+
+// TMA: stores a box from shared memory (written by this warp, ordered by
+// fence_async_shared); one lane issues it and later waits until the boxes it
+// stored have been read from shared memory.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map,
+                                             const void* src, int c0, int c1,
+                                             int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, "
+      "%4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
+      "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
 // Clears rows [first, 128) of a 128 x kD bf16 tile (64-column halves of 128
 // bytes a row; the swizzle moves pieces inside a row only). One warp.
 template <int kD>

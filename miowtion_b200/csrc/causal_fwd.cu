@@ -56,15 +56,16 @@ constexpr float kLn2 = 0.69314718055994531f;
 template <int kD>
 struct Fwd {
   static constexpr uint32_t kTileBytes = kTile * kD * 2;
-  static constexpr int kRing = kD == 128 ? 5 : 8;
-  static constexpr int kSmem = (2 + kRing) * kTileBytes + 512 + 1024;
+  static constexpr int kRing = kD == 128 ? 4 : 8;
+  // Q tiles, ring, then 4 KB a softmax warp to stage its output in.
+  static constexpr int kSmem = (2 + kRing) * kTileBytes + 8 * 4096 + 512 + 1024;
   static constexpr int kSteps = kD / 16;  // K-steps of Q K^T
 };
 
 enum Bar {
-  kQFull = 0,   // Q of the item landed
-  kQEmpty,      // the item's last S products finished
-  kSFull,       // [2] S of the tile's block finished
+  kQFull = 0,             // [2] Q of the tile landed
+  kQEmpty = kQFull + 2,   // [2] the tile's last S product finished
+  kSFull = kQEmpty + 2,   // [2] S of the tile's block finished
   kPHalfA = kSFull + 2,   // [2] P of keys 0-63 written (4 warps)
   kPHalfB = kPHalfA + 2,  // [2] P of keys 64-127 written (4 warps)
   kODone = kPHalfB + 2,   // [2] the tile's last product of the item finished
@@ -80,6 +81,7 @@ struct FwdParams {
   int kv_heads;
   int group;
   int tokens;    // of a query tile: 128 / group
+  int warp_boxes;  // a warp's 32 rows are whole tokens: TMA stores them
   __nv_bfloat16* out;
   int64_t out_st, out_sh;
   float* lse;    // or null
@@ -161,6 +163,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     causal_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
                       const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v,
+                      const __grid_constant__ CUtensorMap map_out,
                       const __grid_constant__ FwdParams p) {
   using C = Fwd<kD>;
   constexpr int kRing = C::kRing;
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   uint8_t* s_q = smem;                     // [2] tiles
   uint8_t* s_ring = smem + 2 * kTileBytes;  // [kRing] tiles
   uint64_t* bars =
-      reinterpret_cast<uint64_t*>(smem + (2 + kRing) * kTileBytes);
+      reinterpret_cast<uint64_t*>(smem + (2 + kRing) * kTileBytes + 8 * 4096);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -209,8 +212,9 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         prefetch_tensor_map(&map_k);
         prefetch_tensor_map(&map_v);
       }
-      const uint32_t q_bytes = 2u * p.group * p.tokens * kD * 2;
+      const uint32_t q_bytes = p.group * p.tokens * kD * 2;  // of a tile
       int n_ring = 0, q_loads = 0;
+      int q_issued[2] = {0, 0};
       bool run = true;
       // One K or V tile (rows k_row ..) into the ring's next place.
       auto load = [&](const CUtensorMap* map, int h, int row) -> bool {
@@ -233,31 +237,38 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       };
       Stream st{0};
       while (run && st.next(p, n_items, false)) {
-        if (q_loads > 0 && !wait_all(&bars[kQEmpty], (q_loads - 1) & 1, abort,
-                                     p.status))
-          break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&bars[kQFull], q_bytes);
-#pragma unroll
-          for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int c = 0; c < kD / 64; ++c)
-              tma_load_3d(s_q + g * kTileBytes + c * 16384, &map_q,
-                          &bars[kQFull], c * 64, st.h * p.group,
-                          st.it.row + g * p.tokens);
-        }
-        __syncwarp();
-        ++q_loads;
         for (int j = 0; run && j < st.it.blocks; ++j) {
           run = load(&map_k, st.h, st.it.k_row + j * kTile);
+          // Q behind the first K tile: it has to wait for the last scores of
+          // the item before.
+          for (int g = 0; run && j == 0 && g < 2; ++g) {
+            if (q_loads > 0 && !wait_all(&bars[kQEmpty + g],
+                                         (q_loads - 1) & 1, abort, p.status)) {
+              run = false;
+              break;
+            }
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&bars[kQFull + g], q_bytes);
+#pragma unroll
+              for (int c = 0; c < kD / 64; ++c)
+                tma_load_3d(s_q + g * kTileBytes + c * 16384, &map_q,
+                            &bars[kQFull + g], c * 64, st.h * p.group,
+                            st.it.row + g * p.tokens);
+              q_issued[g] = q_loads + 1;
+            }
+            __syncwarp();
+          }
           if (run) run = load(&map_v, st.h, st.it.k_row + j * kTile);
         }
+        ++q_loads;
       }
       if (lane == 0 && *abort) {
         // Let the copies in flight land before the CTA retires.
         volatile int never = 0;
-        if (q_loads > 0)
-          mbar_wait(&bars[kQFull], (q_loads - 1) & 1, &never, nullptr);
+        for (int g = 0; g < 2; ++g)
+          if (q_issued[g] > 0)
+            mbar_wait(&bars[kQFull + g], (q_issued[g] - 1) & 1, &never,
+                      nullptr);
         for (int k = n_ring - kRing; k < n_ring; ++k)
           if (k >= 0)
             mbar_wait(&bars[kFull + k % kRing], (k / kRing) & 1, &never,
@@ -276,7 +287,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         return wait_all(&bars[kFull + place % kRing], (place / kRing) & 1,
                         abort, p.status);
       };
-      auto issue_qk = [&](int b, int g) {
+      // (last: the item's last block.)
+      auto issue_qk = [&](int b, int g, bool last) {
         const uint32_t a = q_lo + g * kTileUnits;
         const uint32_t bk = k_lo + ((2 * b) % kRing) * kTileUnits;
 #pragma unroll
@@ -286,23 +298,21 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
                        kk > 0 ? 1u : 0u);
         }
         umma_commit_warp(&bars[kSFull + g]);
-      };
-      // K of block b, the j-th of its item's n, is read by both tiles.
-      auto release_k = [&](int b, int j, int n) {
-        umma_commit_warp(&bars[kEmpty + (2 * b) % kRing]);
-        if (j == n - 1) umma_commit_warp(&bars[kQEmpty]);
+        if (last) umma_commit_warp(&bars[kQEmpty + g]);
+        if (g == 1) umma_commit_warp(&bars[kEmpty + (2 * b) % kRing]);
       };
       Stream st{0};
       bool more = st.next(p, n_items, false);
       bool ok = true;
       int b = 0, items = 0;
       if (more) {
-        ok = wait_all(&bars[kQFull], 0, abort, p.status) && landed(0);
-        if (ok) {
-          tc_fence_after();
-          issue_qk(0, 0);
-          issue_qk(0, 1);
-          release_k(0, 0, st.it.blocks);
+        ok = landed(0);
+        for (int g = 0; ok && g < 2; ++g) {
+          ok = wait_all(&bars[kQFull + g], 0, abort, p.status);
+          if (ok) {
+            tc_fence_after();
+            issue_qk(0, g, st.it.blocks == 1);
+          }
         }
       }
       while (ok && more) {
@@ -345,22 +355,18 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
                            bv + kk * 128, idesc_pv, 1u);
             if (last) umma_commit_warp(&bars[kODone + g]);
             if (ahead) {
-              if (g == 0) {
-                if (!landed(2 * b + 2) ||
-                    (last && !wait_all(&bars[kQFull], (items + 1) & 1, abort,
-                                       p.status))) {
-                  ok = false;
-                  break;
-                }
-                tc_fence_after();
+              if ((g == 0 && !landed(2 * b + 2)) ||
+                  (last && !wait_all(&bars[kQFull + g], (items + 1) & 1,
+                                     abort, p.status))) {
+                ok = false;
+                break;
               }
-              issue_qk(b + 1, g);
+              tc_fence_after();
+              issue_qk(b + 1, g, last ? st.it.blocks == 1 : j + 1 == n - 1);
             }
           }
           if (!ok) break;
           umma_commit_warp(&bars[kEmpty + slot]);
-          if (ahead)
-            release_k(b + 1, last ? 0 : j + 1, last ? st.it.blocks : n);
         }
         ++items;
       }
@@ -382,6 +388,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t t_s = tmem + grp * 128 + lane_base;
     const uint32_t t_o = tmem + 256 + grp * 128 + lane_base;
+    uint8_t* s_stage = smem + (2 + kRing) * kTileBytes + warp * 4096;
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     uint32_t b = 0;
     int items = 0;
@@ -470,30 +477,51 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         tc_fence_after();
         ++items;
       }
+      // A warp whose rows all have tokens stages 64 columns at a time and
+      // stores them by TMA; others store from registers, 32 rows at a time.
+      const bool boxed =
+          p.warp_boxes && __all_sync(0xffffffffu, write) && n > 0;
 #pragma unroll 1
-      for (int c = 0; c < kD / 32; ++c) {
-        uint32_t o[32];
-        if (n > 0) {
-          tmem_ld32(t_o + c * 32, o);
-          tmem_wait_ld();
+      for (int c = 0; c < kD / 64; ++c) {
+        if (boxed) {
+          if (lane == 0) bulk_wait_read();
+          __syncwarp();
         }
-        if (l == 0.f) {  // no key
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        for (int c2 = 0; c2 < 2; ++c2) {
+          uint32_t o[32];
+          if (n > 0) {
+            tmem_ld32(t_o + c * 64 + c2 * 32, o);
+            tmem_wait_ld();
+          }
+          if (l == 0.f) {  // no key
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0u;
+          }
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            w[e] = pack_bf16(__uint_as_float(o[2 * e]) * inv_l,
+                             __uint_as_float(o[2 * e + 1]) * inv_l);
+          if (boxed) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(
+                  s_stage + lane * 128 +
+                  (((c2 * 4 + e) ^ (lane & 7)) << 4)) =
+                  make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2],
+                             w[4 * e + 3]);
+          } else if (write) {
+            store32(dst + c * 64 + c2 * 32, w);
+            store32(dst + c * 64 + c2 * 32 + 16, w + 8);
+          }
         }
-        if (write) {
-          uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            d4[e] = make_uint4(
-                pack_bf16(__uint_as_float(o[8 * e]) * inv_l,
-                          __uint_as_float(o[8 * e + 1]) * inv_l),
-                pack_bf16(__uint_as_float(o[8 * e + 2]) * inv_l,
-                          __uint_as_float(o[8 * e + 3]) * inv_l),
-                pack_bf16(__uint_as_float(o[8 * e + 4]) * inv_l,
-                          __uint_as_float(o[8 * e + 5]) * inv_l),
-                pack_bf16(__uint_as_float(o[8 * e + 6]) * inv_l,
-                          __uint_as_float(o[8 * e + 7]) * inv_l));
+        if (boxed) {
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0)
+            tma_store_3d(&map_out, s_stage, c * 64,
+                         static_cast<int>(out_head), static_cast<int>(out_row));
         }
       }
       tc_fence_before();  // O is read before P of the next item is released
@@ -501,6 +529,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         p.lse[out_row * p.lse_st + out_head * p.lse_sh] =
             l == 0.f ? -INFINITY : (m_ref + log2f(l)) * kLn2;
     }
+    if (lane == 0) bulk_wait_read();  // the stores have read the stage
   }
   tc_fence_before();
   __syncthreads();
@@ -512,7 +541,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
 
 template <int kD>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-           const FwdParams& p, cudaStream_t stream) {
+           const CUtensorMap& mo, const FwdParams& p, cudaStream_t stream) {
   int sms = 0;
   int rc = device_sms(&sms);
   if (rc != VEDA_OK) return rc;
@@ -524,7 +553,7 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
   const int64_t items = static_cast<int64_t>(p.entries) * p.kv_heads;
   const int grid = static_cast<int>(items < cap ? items : cap);
   causal_fwd_kernel<kD><<<grid, 32 * kWarps, Fwd<kD>::kSmem, stream>>>(
-      mq, mk, mv, p);
+      mq, mk, mv, mo, p);
   return check_launch("causal_fwd_kernel");
 }
 
@@ -558,16 +587,21 @@ extern "C" int veda_causal_fwd(
                "softmax_scale must be positive and finite");
   if (total_q == 0 || n_items == 0) return VEDA_OK;
   VEDA_REQUIRE(q && out && items, "q, out and items are required");
-  VEDA_REQUIRE(reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
-                   out_stride_t % 8 == 0 && out_stride_h % 8 == 0 &&
+  VEDA_REQUIRE(reinterpret_cast<uintptr_t>(out) % 32 == 0 &&
+                   out_stride_t % 16 == 0 && out_stride_h % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(items) % 16 == 0,
-               "out must be 16-byte aligned with strides multiple of 8, items "
-               "16-byte aligned");
+               "out must be 32-byte aligned with strides multiple of 16, "
+               "items 16-byte aligned");
   const int group = n_heads / kv_heads;
   const int tokens = kTile / group;
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo;
   rc = causal::make_rows_map(&mq, q, total_q, n_heads, head_dim, q_stride_t,
                              q_stride_h, group, tokens, "q");
+  const bool warp_boxes = 32 % group == 0;
+  if (rc == VEDA_OK)
+    rc = causal::make_rows_map(&mo, out, total_q, n_heads, head_dim,
+                               out_stride_t, out_stride_h, group,
+                               warp_boxes ? 32 / group : 1, "out");
   // Without keys no item loads any; the maps then only have to exist.
   if (total_k == 0) {
     mk = mv = mq;
@@ -587,6 +621,7 @@ extern "C" int veda_causal_fwd(
   p.kv_heads = kv_heads;
   p.group = group;
   p.tokens = tokens;
+  p.warp_boxes = warp_boxes;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.out_st = out_stride_t;
   p.out_sh = out_stride_h;
@@ -596,6 +631,6 @@ extern "C" int veda_causal_fwd(
   p.scale_log2 = softmax_scale * causal::kLog2e;
   p.status = device_status_ptr();
   cudaStream_t s = as_stream(stream);
-  return head_dim == 128 ? causal::launch<128>(mq, mk, mv, p, s)
-                         : causal::launch<64>(mq, mk, mv, p, s);
+  return head_dim == 128 ? causal::launch<128>(mq, mk, mv, mo, p, s)
+                         : causal::launch<64>(mq, mk, mv, mo, p, s);
 }
