@@ -91,10 +91,8 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map,
 template <int kN>
 __device__ __forceinline__ void store_row(__nv_bfloat16* dst,
                                           const uint32_t* w) {
-  uint4* d4 = reinterpret_cast<uint4*>(dst);
 #pragma unroll
-  for (int i = 0; i < kN / 8; ++i)
-    d4[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  for (int i = 0; i < kN / 16; ++i) store32(dst + 16 * i, w + 8 * i);
 }
 
 // Reads kN fp32 TMEM columns of this thread's lane, scales them and packs
@@ -115,54 +113,65 @@ __device__ __forceinline__ void tmem_row_bf16(uint32_t taddr, float scale,
 }
 
 // ---------------------------------------------------------------------------
-// prep: one warp per (query tile row, key head).
+// prep: a block per (query tile, key head), kD / 8 lanes a row. Bound by
+// memory (out and dout once): every thread has its rows' loads in flight at
+// once.
 // ---------------------------------------------------------------------------
+constexpr int kPrepThreads = 256;
+
 template <int kD>
-__global__ void causal_bwd_prep_kernel(
-    const int32_t* table, int entries, int kv_heads, int group, int tokens,
-    const __nv_bfloat16* out, int64_t o_st, int64_t o_sh,
-    const __nv_bfloat16* dout, int64_t d_st, int64_t d_sh, const float* lse,
-    int64_t l_st, int64_t l_sh, float* lse2, float* delta, int n_tiles) {
-  constexpr int kPer = kD / 32;  // elements a lane
-  const int64_t w =
-      (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
-  const int lane = threadIdx.x % 32;
-  const int r = static_cast<int>(w % kTile);
-  const int64_t u = w / kTile;
-  if (u >= static_cast<int64_t>(entries) * kv_heads) return;
-  const int h = static_cast<int>(u % kv_heads);
-  const QueryItem it =
-      load_item<QueryItem>(table, static_cast<int>(u / kv_heads));
-  const int token = r / group, head = r % group;
-  const int64_t at =
-      (static_cast<int64_t>(h) * n_tiles + it.tile) * kTile + r;
-  if (token >= it.tokens || token >= tokens) {
-    if (lane == 0) {
-      delta[at] = 0.f;
-      lse2[at] = INFINITY;
+__global__ void __launch_bounds__(kPrepThreads) causal_bwd_prep_kernel(
+    const int32_t* table, int group, int tokens, const __nv_bfloat16* out,
+    int64_t o_st, int64_t o_sh, const __nv_bfloat16* dout, int64_t d_st,
+    int64_t d_sh, const float* lse, int64_t l_st, int64_t l_sh, float* lse2,
+    float* delta, int n_tiles) {
+  constexpr int kLanes = kD / 8;
+  constexpr int kStep = kPrepThreads / kLanes;  // rows at a time
+  constexpr int kRounds = kTile / kStep;
+  const int lane = threadIdx.x % kLanes;
+  const int h = blockIdx.y;
+  const QueryItem it = load_item<QueryItem>(table, blockIdx.x);
+  const int64_t at = (static_cast<int64_t>(h) * n_tiles + it.tile) * kTile;
+  uint4 a[kRounds], b[kRounds];
+  float l[kRounds];
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const int r = i * kStep + threadIdx.x / kLanes;
+    const int token = r / group;
+    a[i] = b[i] = make_uint4(0, 0, 0, 0);
+    l[i] = -INFINITY;
+    if (token < it.tokens && token < tokens) {
+      const int64_t row = static_cast<int64_t>(it.row) + token;
+      const int64_t hq = static_cast<int64_t>(h) * group + r % group;
+      a[i] = *reinterpret_cast<const uint4*>(out + row * o_st + hq * o_sh +
+                                             lane * 8);
+      b[i] = *reinterpret_cast<const uint4*>(dout + row * d_st + hq * d_sh +
+                                             lane * 8);
+      l[i] = lse[row * l_st + hq * l_sh];
     }
-    return;
-  }
-  const int64_t row = static_cast<int64_t>(it.row) + token;
-  const int64_t hq = static_cast<int64_t>(h) * group + head;
-  const __nv_bfloat162* a = reinterpret_cast<const __nv_bfloat162*>(
-      out + row * o_st + hq * o_sh + lane * kPer);
-  const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(
-      dout + row * d_st + hq * d_sh + lane * kPer);
-  float acc = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPer / 2; ++i) {
-    const float2 x = __bfloat1622float2(a[i]);
-    const float2 y = __bfloat1622float2(b[i]);
-    acc = fmaf(x.x, y.x, fmaf(x.y, y.y, acc));
   }
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, s);
-  if (lane == 0) {
-    const float l = lse[row * l_st + hq * l_sh];
-    const bool none = l == -INFINITY;
-    delta[at] = none ? 0.f : acc;
-    lse2[at] = none ? INFINITY : l * kLog2e;
+  for (int i = 0; i < kRounds; ++i) {
+    const uint32_t x[4] = {a[i].x, a[i].y, a[i].z, a[i].w};
+    const uint32_t y[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
+    float acc = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc = fmaf(__uint_as_float(x[e] << 16), __uint_as_float(y[e] << 16),
+                 acc);
+      acc = fmaf(__uint_as_float(x[e] & 0xFFFF0000u),
+                 __uint_as_float(y[e] & 0xFFFF0000u), acc);
+    }
+#pragma unroll
+    for (int s = kLanes / 2; s > 0; s >>= 1)
+      acc += __shfl_xor_sync(0xffffffffu, acc, s);
+    if (lane == 0) {
+      const int r = i * kStep + threadIdx.x / kLanes;
+      // A row without keys or token.
+      const bool none = l[i] == -INFINITY;
+      delta[at + r] = none ? 0.f : acc;
+      lse2[at + r] = none ? INFINITY : l[i] * kLog2e;
+    }
   }
 }
 
@@ -873,11 +882,9 @@ int launch(const Maps& m, const BwdParams& pq, const BwdParams& pk,
   int rc = device_sms(&sms);
   if (rc != VEDA_OK) return rc;
   if (pq.entries > 0) {
-    const int64_t warps =
-        static_cast<int64_t>(pq.entries) * pq.kv_heads * kTile;
     causal_bwd_prep_kernel<kD>
-        <<<static_cast<unsigned>((warps * 32 + 255) / 256), 256, 0, stream>>>(
-            pq.table, pq.entries, pq.kv_heads, pq.group, pq.tokens,
+        <<<dim3(pq.entries, pq.kv_heads), kPrepThreads, 0, stream>>>(
+            pq.table, pq.group, pq.tokens,
             static_cast<const __nv_bfloat16*>(a.out), a.o_st, a.o_sh,
             static_cast<const __nv_bfloat16*>(a.dout), a.d_st, a.d_sh, a.lse,
             a.l_st, a.l_sh, a.lse2, a.delta, pq.n_tiles);
@@ -948,9 +955,10 @@ extern "C" int veda_causal_bwd(
   VEDA_REQUIRE(total_q >= 0 && total_k >= 0 && total_q < (int64_t(1) << 31) &&
                    total_k < (int64_t(1) << 31) && n_q_items >= 0 &&
                    n_k_items >= 0 && n_tiles >= n_q_items &&
-                   n_tiles * kv_heads < (int64_t(1) << 24) &&
-                   n_k_items < (int64_t(1) << 31),
-               "bad sizes (at most 2^24 query tiles times key heads)");
+                   kv_heads <= 65535 &&
+                   n_tiles * kv_heads < (int64_t(1) << 31) - 65536 &&
+                   n_k_items * kv_heads < (int64_t(1) << 31) - 65536,
+               "bad sizes");
   VEDA_REQUIRE(softmax_scale > 0.f && isfinite(softmax_scale),
                "softmax_scale must be positive and finite");
   VEDA_REQUIRE((dk == nullptr) == (dv == nullptr),
@@ -961,17 +969,17 @@ extern "C" int veda_causal_bwd(
                    reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
                "workspace too small or not 16-byte aligned "
                "(veda_causal_bwd_workspace)");
-  auto aligned = [](const void* ptr, int64_t st, int64_t sh) {
-    return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && st % 8 == 0 &&
-           sh % 8 == 0;
+  auto aligned = [](const void* ptr, int64_t st, int64_t sh, int elements) {
+    return reinterpret_cast<uintptr_t>(ptr) % (2 * elements) == 0 &&
+           st % elements == 0 && sh % elements == 0;
   };
-  VEDA_REQUIRE(aligned(out, out_stride_t, out_stride_h) &&
-                   aligned(dout, dout_stride_t, dout_stride_h) &&
-                   aligned(dq, dq_stride_t, dq_stride_h) &&
-                   aligned(dk, dk_stride_t, dk_stride_h) &&
-                   aligned(dv, dv_stride_t, dv_stride_h),
-               "out, dout, dq, dk, dv must be 16-byte aligned with strides "
-               "multiple of 8");
+  VEDA_REQUIRE(aligned(out, out_stride_t, out_stride_h, 8) &&
+                   aligned(dout, dout_stride_t, dout_stride_h, 8) &&
+                   aligned(dq, dq_stride_t, dq_stride_h, 16) &&
+                   aligned(dk, dk_stride_t, dk_stride_h, 16) &&
+                   aligned(dv, dv_stride_t, dv_stride_h, 16),
+               "out and dout must be 16-byte aligned with strides multiple of "
+               "8; dq, dk, dv 32-byte aligned with strides multiple of 16");
   cudaStream_t s = as_stream(stream);
   const int group = n_heads / kv_heads;
   const int tokens = kTile / group;

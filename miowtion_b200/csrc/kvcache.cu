@@ -13,7 +13,13 @@
 // rounded fp32 quotient of 127 x (exact: 8 + 7 bits) and max|x|: an exact
 // half is representable and stays one, and a quotient that is not a half
 // differs from it by more than the quotient's rounding error (bf16 operands),
-// so the codes are those of real arithmetic. A row with a value that is not
+// so the codes are those of real arithmetic. It is computed as the product with
+// the reciprocal of max|x|, corrected once by the exact remainder: a product
+// that is off by a relative e leaves a remainder that brings it to within e^2,
+// which the last rounding takes to the quotient where that is representable.
+// (The
+// kernel is close to bound by its instructions: 55,504 tokens of 8 heads, D =
+// 128, took 131 us with a division for each value.) A row with a value that is not
 // finite gets the scale NaN, and reads back as NaN throughout; an all-zero
 // row has scale 0.
 //
@@ -58,35 +64,55 @@ __device__ __forceinline__ void unpack8(const uint4& w, float* x) {
 // the row.
 template <int kStore, int kGroup>
 __device__ __forceinline__ uint2 encode8(const uint4& w, float* scale) {
-  float x[8];
-  unpack8(w, x);
-  float top = 0.f;
-  // NaN must not vanish in the maximum: it is carried as infinity.
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    top = fmaxf(top, x[i] == x[i] ? fabsf(x[i]) : INFINITY);
+  // max|x|: magnitudes of bf16 order as their bits do, infinity behind the
+  // numbers and NaN behind infinity, so nothing is lost in the maximum.
+  constexpr uint32_t kAbs = 0x7fff7fffu;
+  uint32_t high = __vmaxu2(__vmaxu2(w.x & kAbs, w.y & kAbs),
+                           __vmaxu2(w.z & kAbs, w.w & kAbs));
 #pragma unroll
   for (int s = kGroup / 2; s > 0; s >>= 1)
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    high = __vmaxu2(high, __shfl_xor_sync(0xffffffffu, high, s));
+  high = max(high >> 16, high & 0xffffu);
+  const float top = __uint_as_float(high << 16);
   uint32_t word[2] = {0u, 0u};
-  if (top == INFINITY) {
+  if (high >= 0x7f80u) {
     *scale = __int_as_float(0x7fffffff);
     return make_uint2(0u, 0u);
   }
-  if (top == 0.f) {
+  if (high == 0u) {
     *scale = 0.f;
     return make_uint2(0u, 0u);
   }
+  float x[8];
+  unpack8(w, x);
   if constexpr (kStore == kStoreInt8) {
-    *scale = __fdiv_rn(top, 127.f);
-    // Large rows are brought down by a power of two: 127 x stays finite.
-    const float pre = top > 1.f ? 0x1p-8f : 1.f;
+    // top / 127, corrected the same way (the correctly rounded quotient for
+    // each of the 32,639 finite magnitudes: checked one by one).
+    const float unit = 1.f / 127.f;
+    float sc = top * unit;
+    sc = fmaf(fmaf(-sc, 127.f, top), unit, sc);
+    *scale = sc;
+    // By a power of two 127 x stays finite in large rows, and max|x| normal in
+    // small ones.
+    const float pre = top > 1.f ? 0x1p-8f : 0x1p24f;
     const float den = top * pre, num = 127.f * pre;
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(den));
+    // Adding 1.5 2^23 rounds to an integer (ties to even) and leaves it in
+    // the low bits.
+    uint32_t c[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int c = __float2int_rn(__fdiv_rn(x[i] * num, den));
-      word[i >> 2] |= (static_cast<uint32_t>(c) & 0xffu) << (8 * (i & 3));
+      const float n = x[i] * num;
+      float quot = n * inv;
+      quot = fmaf(fmaf(-quot, den, n), inv, quot);
+      c[i] = __float_as_uint(quot + 12582912.f);
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      word[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040),
+                            __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040),
+                            0x5410);
   } else {
     // top = 1.f 2^x: 448 = 1.75 2^8. Subnormal tops end at the clamp.
     const uint32_t bits = __float_as_uint(top);
@@ -131,49 +157,78 @@ __device__ __forceinline__ uint4 decode8(const uint2& w, float scale) {
                     pack_bf16(x[6] * scale, x[7] * scale));
 }
 
+// Rows of k and v a group of lanes takes at a time. Finding a row's place is a
+// chain of four dependent loads and more: each lane of a warp finds one row's,
+// and the data of all of them is in flight meanwhile (55,504 tokens of 8 heads,
+// D = 128, int8: 79 us against 104 with every lane finding its rows' places).
+constexpr int kBatch = 4;
+
 template <int kStore, int kD>
 __global__ void __launch_bounds__(kThreads)
     cache_write_kernel(CacheView c, const __nv_bfloat16* k, int64_t k_st,
                        int64_t k_sh, const __nv_bfloat16* v, int64_t v_st,
                        int64_t v_sh, const int32_t* offsets,
-                       const int32_t* starts, int64_t n_rows,
+                       const int32_t* starts, int n_rows,
                        unsigned int* status) {
   constexpr int kGroup = kD / 8;
-  const int64_t row =
-      (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kGroup;
+  constexpr int kGroups = kThreads / kGroup;
   const int lane = threadIdx.x % kGroup;
-  // A group past the end repeats the last row's work without storing it: the
-  // shuffles need whole warps.
-  const bool live = row < n_rows;
-  const int64_t r = live ? row : n_rows - 1;
-  const int64_t t = r / c.kv_heads;
-  const int h = static_cast<int>(r % c.kv_heads);
-  const uint4 kw = *reinterpret_cast<const uint4*>(k + t * k_st + h * k_sh +
-                                                   lane * 8);
-  const uint4 vw = *reinterpret_cast<const uint4*>(v + t * v_st + h * v_sh +
-                                                   lane * 8);
-  const int b = find_sequence(offsets, c.n_seqs, t);
-  const int64_t pos = static_cast<int64_t>(starts[b]) + (t - offsets[b]);
-  const int64_t at = cache_row(c, b, h, pos);
-  if (at < 0) {
-    if (live && lane == 0) raise_status(status, VEDA_ERR_INVALID);
-  }
-  const bool store = live && at >= 0;
-  if constexpr (kStore == kStoreBf16) {
-    if (store) {
-      reinterpret_cast<uint4*>(c.k)[at * kGroup + lane] = kw;
-      reinterpret_cast<uint4*>(c.v)[at * kGroup + lane] = vw;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kGroups * kBatch +
+                       threadIdx.x / kGroup;
+  // Lane i * kWide + g finds the place of row i of group g of the warp; the
+  // groups then take theirs from it.
+  constexpr int kWide = 32 / kGroup;  // groups of a warp
+  const int64_t warp_row = row0 - (threadIdx.x % 32) / kGroup;
+  const int wl = threadIdx.x % 32;
+  int my_t = 0, my_h = 0;
+  int64_t my_at = -1;
+  {
+    const int64_t row = warp_row + (wl / kWide % kBatch) * kGroups + wl % kWide;
+    // Past the end: the last row's values, stored nowhere.
+    const int r = row < n_rows ? static_cast<int>(row) : n_rows - 1;
+    my_t = r / c.kv_heads;
+    my_h = r - my_t * c.kv_heads;
+    if (row < n_rows && wl < kWide * kBatch) {
+      const int b = find_sequence(offsets, c.n_seqs, my_t);
+      my_at = cache_row(c, b, my_h,
+                        static_cast<int64_t>(starts[b]) +
+                            (my_t - offsets[b]));
+      if (my_at < 0) raise_status(status, VEDA_ERR_INVALID);
     }
-  } else {
-    float ks, vs;
-    const uint2 kc = encode8<kStore, kGroup>(kw, &ks);
-    const uint2 vc = encode8<kStore, kGroup>(vw, &vs);
-    if (store) {
-      reinterpret_cast<uint2*>(c.k)[at * kGroup + lane] = kc;
-      reinterpret_cast<uint2*>(c.v)[at * kGroup + lane] = vc;
-      if (lane == 0) {
-        c.k_scale[at] = ks;
-        c.v_scale[at] = vs;
+  }
+  uint4 kw[kBatch], vw[kBatch];
+  int64_t at[kBatch];
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    const int from = i * kWide + wl / kGroup;
+    const int t = __shfl_sync(0xffffffffu, my_t, from);
+    const int h = __shfl_sync(0xffffffffu, my_h, from);
+    kw[i] = *reinterpret_cast<const uint4*>(k + t * k_st + h * k_sh +
+                                            lane * 8);
+    vw[i] = *reinterpret_cast<const uint4*>(v + t * v_st + h * v_sh +
+                                            lane * 8);
+  }
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i)
+    at[i] = __shfl_sync(0xffffffffu, my_at, i * kWide + wl / kGroup);
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    if constexpr (kStore == kStoreBf16) {
+      if (at[i] >= 0) {
+        reinterpret_cast<uint4*>(c.k)[at[i] * kGroup + lane] = kw[i];
+        reinterpret_cast<uint4*>(c.v)[at[i] * kGroup + lane] = vw[i];
+      }
+    } else {
+      float ks, vs;
+      const uint2 kc = encode8<kStore, kGroup>(kw[i], &ks);
+      const uint2 vc = encode8<kStore, kGroup>(vw[i], &vs);
+      if (at[i] >= 0) {
+        reinterpret_cast<uint2*>(c.k)[at[i] * kGroup + lane] = kc;
+        reinterpret_cast<uint2*>(c.v)[at[i] * kGroup + lane] = vc;
+        if (lane == 0) {
+          c.k_scale[at[i]] = ks;
+          c.v_scale[at[i]] = vs;
+        }
       }
     }
   }
@@ -189,8 +244,8 @@ __global__ void __launch_bounds__(kThreads)
       (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kGroup;
   const int lane = threadIdx.x % kGroup;
   if (row >= n_rows) return;
-  const int64_t t = row / c.kv_heads;
-  const int h = static_cast<int>(row % c.kv_heads);
+  const int t = static_cast<int>(row) / c.kv_heads;
+  const int h = static_cast<int>(row) - t * c.kv_heads;
   const int b = find_sequence(offsets, c.n_seqs, t);
   const int64_t at = cache_row(c, b, h, t - offsets[b]);
   uint4 kw = make_uint4(0, 0, 0, 0), vw = kw;
@@ -233,10 +288,12 @@ struct WriteLaunch {
   cudaStream_t stream;
   template <int kStore, int kD>
   int operator()() const {
-    const int64_t blocks = (rows * (kD / 8) + kThreads - 1) / kThreads;
+    constexpr int kRows = kThreads / (kD / 8) * kBatch;  // of a block
+    const int64_t blocks = (rows + kRows - 1) / kRows;
     cache_write_kernel<kStore, kD>
         <<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-            c, k, k_st, k_sh, v, v_st, v_sh, offsets, starts, rows, status);
+            c, k, k_st, k_sh, v, v_st, v_sh, offsets, starts,
+            static_cast<int>(rows), status);
     return check_launch("cache_write_kernel");
   }
 };
