@@ -507,17 +507,26 @@ int veda_compensate(const void* o_kept, int64_t ok_stride_n,
  * work items describe the sequences (miowtion_b200/sequences.py builds them;
  * csrc/causal.cuh gives the fields) and must agree with the sizes. */
 
+/* Bytes of workspace veda_causal_fwd needs for n_parts parts (0 for none); -1
+ * for sizes out of range. */
+int64_t veda_causal_fwd_workspace(int32_t kv_heads, int32_t head_dim,
+                                  int64_t n_parts);
+
 /* out [total_q, n_heads, head_dim] bf16, lse (fp32, or NULL): the
  * log-sum-exp of the scaled scores; 0 and -inf for a token without keys.
- * items: n_items forward work items. */
+ * items: n_items forward work items, n_parts of them parts of items that were
+ * cut along the keys, which the n_joins joins put together (joins may be NULL
+ * and the workspace too without parts). */
 int veda_causal_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                     const void* k, int64_t k_stride_t, int64_t k_stride_h,
                     const void* v, int64_t v_stride_t, int64_t v_stride_h,
                     int64_t total_q, int64_t total_k, int32_t n_heads,
                     int32_t kv_heads, int32_t head_dim, const int32_t* items,
-                    int64_t n_items, void* out, int64_t out_stride_t,
+                    int64_t n_items, const int32_t* joins, int64_t n_joins,
+                    int64_t n_parts, void* out, int64_t out_stride_t,
                     int64_t out_stride_h, float* lse, int64_t lse_stride_t,
-                    int64_t lse_stride_h, float softmax_scale, void* stream);
+                    int64_t lse_stride_h, float softmax_scale, void* workspace,
+                    int64_t workspace_bytes, void* stream);
 
 /* Bytes of workspace veda_causal_bwd needs; -1 for sizes out of range. */
 int64_t veda_causal_bwd_workspace(int32_t kv_heads, int64_t n_tiles);

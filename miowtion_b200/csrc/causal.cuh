@@ -23,16 +23,39 @@
 namespace veda {
 namespace causal {
 
-// A run of query tokens of one sequence (forward: two tiles, query gradient:
-// one tile).
-struct alignas(16) QueryItem {
+// Forward: two query tiles of one sequence and the key tiles that the second
+// reaches, or a part of them (sequences.py cuts items along the keys where
+// there are few).
+struct alignas(16) ForwardItem {
   int row;     // packed row of the first token
-  int tokens;  // tokens of the run
+  int tokens;  // tokens of the two tiles
   int k_row;   // packed row of the sequence's first key
   int kpos;    // the first token sees keys 0 .. kpos (negative: none)
   int keys;    // keys of the sequence
-  int blocks;  // key tiles that the run's last token reaches
-  int tile;    // number of the first query tile, over the whole pack
+  int blocks;  // key tiles
+  int first;   // the first of them
+  int part;    // number of the part; -1: the whole
+};
+
+// The parts of a forward item: part .. part + parts - 1 (in the order of the
+// keys).
+struct alignas(16) JoinItem {
+  int row;
+  int tokens;
+  int part;
+  int parts;
+  int pad[4];
+};
+
+// Query gradient: a query tile of one sequence.
+struct alignas(16) QueryItem {
+  int row;     // packed row of the first token
+  int tokens;  // tokens of the tile
+  int k_row;   // packed row of the sequence's first key
+  int kpos;    // the first token sees keys 0 .. kpos (negative: none)
+  int keys;    // keys of the sequence
+  int blocks;  // key tiles that the last token reaches
+  int tile;    // number of the query tile, over the whole pack
   int pad;
 };
 
@@ -79,11 +102,10 @@ __device__ __forceinline__ void fence_async_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// Writes 16 bf16 (32 bytes, aligned): the rows of a tile are the lanes of a
+// Writes 32 bytes (aligned): the rows of a tile are the lanes of a
 // warp, so a store meets 32 lines however narrow it is, and the widest takes
 // the fewest passes through them.
-__device__ __forceinline__ void store32(__nv_bfloat16* dst,
-                                        const uint32_t* w) {
+__device__ __forceinline__ void store32(void* dst, const uint32_t* w) {
   asm volatile(
       "st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst),
       "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),

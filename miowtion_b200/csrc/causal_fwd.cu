@@ -87,6 +87,12 @@ struct FwdParams {
   float* lse;    // or null
   int64_t lse_st, lse_sh;
   float scale_log2;
+  // Parts: [kv_heads][n_parts][2 tiles][128 rows][kD] accumulators, then
+  // [...][128 rows][2] maxima and sums.
+  float* part_o;
+  float2* part_ml;
+  int n_parts;
+  const int32_t* joins;
   unsigned int* status;
 };
 
@@ -141,7 +147,7 @@ __device__ __forceinline__ void rescale16(uint32_t t_row, float alpha) {
 struct Stream {
   int t;  // turns taken
   int h;
-  QueryItem it;
+  ForwardItem it;
   // The next item with blocks (kEmpty: any); false at the end.
   __device__ __forceinline__ bool next(const FwdParams& p, int64_t n_items,
                                        bool keep_empty) {
@@ -151,7 +157,7 @@ struct Stream {
       const int entry = static_cast<int>(
           static_cast<uint32_t>(i) / static_cast<uint32_t>(p.kv_heads));
       h = static_cast<int>(i) - entry * p.kv_heads;
-      it = load_item<QueryItem>(p.table, entry);
+      it = load_item<ForwardItem>(p.table, entry);
       if (it.blocks > 0 || keep_empty) return true;
     }
     return false;
@@ -183,6 +189,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   const int warp = tid / 32;
   const int lane = tid % 32;
   const int64_t n_items = static_cast<int64_t>(p.entries) * p.kv_heads;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (tid == 0) {
     for (int b = 0; b < kNumBars; ++b) {
@@ -238,7 +245,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       Stream st{0};
       while (run && st.next(p, n_items, false)) {
         for (int j = 0; run && j < st.it.blocks; ++j) {
-          run = load(&map_k, st.h, st.it.k_row + j * kTile);
+          const int k_row = st.it.k_row + (st.it.first + j) * kTile;
+          run = load(&map_k, st.h, k_row);
           // Q behind the first K tile: it has to wait for the last scores of
           // the item before.
           for (int g = 0; run && j == 0 && g < 2; ++g) {
@@ -258,7 +266,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
             }
             __syncwarp();
           }
-          if (run) run = load(&map_v, st.h, st.it.k_row + j * kTile);
+          if (run) run = load(&map_v, st.h, k_row);
         }
         ++q_loads;
       }
@@ -316,7 +324,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         }
       }
       while (ok && more) {
-        const int n = st.it.blocks, keys = st.it.keys;
+        const int n = st.it.blocks;
+        const int keys = st.it.keys - st.it.first * kTile;
         more = st.next(p, n_items, false);
         for (int j = 0; j < n; ++j, ++b) {
           const bool last = j == n - 1;
@@ -396,10 +405,11 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     Stream st{0};
     while (ok && st.next(p, n_items, true)) {
       const int h = st.h;
-      const QueryItem it = st.it;
+      const ForwardItem it = st.it;
       const int n = it.blocks;
-      // Keys of this row.
-      const int seen = max(0, min(it.keys, it.kpos + token + 1));
+      // Keys of this row, from the item's first key tile on.
+      const int seen = max(0, min(it.keys, it.kpos + token + 1)) -
+                       it.first * kTile;
       float m_ref = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j, ++b) {
         const int visible = seen - j * kTile;
@@ -477,6 +487,25 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         tc_fence_after();
         ++items;
       }
+      if (it.part >= 0) {
+        // A part leaves its accumulator, maximum and sum to the join.
+        const int64_t at =
+            ((static_cast<int64_t>(h) * p.n_parts + it.part) * 2 + grp) *
+                kTile +
+            row;
+        if (write) p.part_ml[at] = make_float2(m_ref, l);
+#pragma unroll 1
+        for (int c = 0; c < kD / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + c * 32, o);
+          tmem_wait_ld();
+          if (write) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              store32(p.part_o + at * kD + c * 32 + e * 8, o + e * 8);
+          }
+        }
+      } else {
       // A warp whose rows all have tokens stages 64 columns at a time and
       // stores them by TMA; others store from registers, 32 rows at a time.
       const bool boxed =
@@ -524,8 +553,9 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
                          static_cast<int>(out_head), static_cast<int>(out_row));
         }
       }
+      }
       tc_fence_before();  // O is read before P of the next item is released
-      if (write && p.lse != nullptr)
+      if (write && it.part < 0 && p.lse != nullptr)
         p.lse[out_row * p.lse_st + out_head * p.lse_sh] =
             l == 0.f ? -INFINITY : (m_ref + log2f(l)) * kLn2;
     }
@@ -539,9 +569,81 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   }
 }
 
+// Puts the parts of cut items together, in the order of the keys: a block per
+// cut item, key head and 32 of the 256 rows, a warp a row, four parts' loads in
+// flight.
+constexpr int kJoinThreads = 512;
+constexpr int kJoinRows = 32;
+
+template <int kD>
+__global__ void __launch_bounds__(kJoinThreads)
+    causal_join_kernel(const __grid_constant__ FwdParams p) {
+  constexpr int kPer = kD / 32;  // elements a lane
+  constexpr int kBatch = 4;
+  const JoinItem it = load_item<JoinItem>(p.joins, blockIdx.x);
+  const int h = blockIdx.y, lane = threadIdx.x % 32;
+  // The parts are written by the kernel that this one follows.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < kJoinRows / (kJoinThreads / 32); ++i) {
+    const int r = blockIdx.z * kJoinRows + i * (kJoinThreads / 32) +
+                  threadIdx.x / 32;
+    const int grp = r / kTile, row = r % kTile;
+    const int token = grp * p.tokens + row / p.group;
+    if (row >= p.tokens * p.group || token >= it.tokens) continue;
+    const int64_t at0 =
+        ((static_cast<int64_t>(h) * p.n_parts + it.part) * 2 + grp) * kTile +
+        row;
+    float m = -INFINITY, l = 0.f, o[kPer] = {};
+    for (int base = 0; base < it.parts; base += kBatch) {
+      float2 ml[kBatch];
+      float x[kBatch][kPer];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        // (Past the last part: the last one again, with no weight.)
+        const int part = min(base + b, it.parts - 1);
+        const int64_t at = at0 + static_cast<int64_t>(part) * 2 * kTile;
+        ml[b] = p.part_ml[at];
+        const float* src = p.part_o + at * kD + lane * kPer;
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(src + e);
+          x[b][e] = v.x;
+          x[b][e + 1] = v.y;
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        // A part that the row sees nothing of has no weight either (and an
+        // accumulator of zeros).
+        if (base + b >= it.parts || ml[b].x == -INFINITY) continue;
+        const float next = fmaxf(m, ml[b].x);
+        const float f = ex2_approx(m - next), g = ex2_approx(ml[b].x - next);
+        m = next;
+        l = l * f + ml[b].y * g;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) o[e] = o[e] * f + x[b][e] * g;
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t out_row = static_cast<int64_t>(it.row) + token;
+    const int64_t out_head =
+        static_cast<int64_t>(h) * p.group + row % p.group;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(
+        p.out + out_row * p.out_st + out_head * p.out_sh + lane * kPer);
+#pragma unroll
+    for (int e = 0; e < kPer / 2; ++e)
+      dst[e] = pack_bf16(o[2 * e] * inv, o[2 * e + 1] * inv);
+    if (lane == 0 && p.lse != nullptr)
+      p.lse[out_row * p.lse_st + out_head * p.lse_sh] =
+          l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  }
+}
+
 template <int kD>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-           const CUtensorMap& mo, const FwdParams& p, cudaStream_t stream) {
+           const CUtensorMap& mo, const FwdParams& p, int64_t n_joins,
+           cudaStream_t stream) {
   int sms = 0;
   int rc = device_sms(&sms);
   if (rc != VEDA_OK) return rc;
@@ -554,7 +656,21 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
   const int grid = static_cast<int>(items < cap ? items : cap);
   causal_fwd_kernel<kD><<<grid, 32 * kWarps, Fwd<kD>::kSmem, stream>>>(
       mq, mk, mv, mo, p);
-  return check_launch("causal_fwd_kernel");
+  rc = check_launch("causal_fwd_kernel");
+  if (rc != VEDA_OK || n_joins == 0) return rc;
+  // The join starts while the last CTAs run (griddepcontrol).
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(n_joins), p.kv_heads,
+                        2 * kTile / kJoinRows);
+  config.blockDim = dim3(kJoinThreads);
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  VEDA_CUDA(cudaLaunchKernelEx(&config, causal_join_kernel<kD>, p));
+  return check_launch("causal_join_kernel");
 }
 
 }  // namespace
@@ -564,14 +680,24 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
 
 using namespace veda;
 
+extern "C" int64_t veda_causal_fwd_workspace(int32_t kv_heads,
+                                             int32_t head_dim,
+                                             int64_t n_parts) {
+  if (kv_heads < 1 || (head_dim != 64 && head_dim != 128) || n_parts < 0 ||
+      n_parts >= (int64_t(1) << 31))
+    return -1;
+  return static_cast<int64_t>(kv_heads) * n_parts * 2 * kTile *
+         (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+}
+
 extern "C" int veda_causal_fwd(
     const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
     int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
     int64_t v_stride_h, int64_t total_q, int64_t total_k, int32_t n_heads,
     int32_t kv_heads, int32_t head_dim, const int32_t* items, int64_t n_items,
-    void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse,
+    const int32_t* joins, int64_t n_joins, int64_t n_parts, void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse,
     int64_t lse_stride_t, int64_t lse_stride_h, float softmax_scale,
-    void* stream) {
+    void* workspace, int64_t workspace_bytes, void* stream) {
   int rc = require_sm100("veda_causal_fwd");
   if (rc != VEDA_OK) return rc;
   VEDA_REQUIRE(head_dim == 64 || head_dim == 128,
@@ -592,6 +718,18 @@ extern "C" int veda_causal_fwd(
                    reinterpret_cast<uintptr_t>(items) % 16 == 0,
                "out must be 32-byte aligned with strides multiple of 16, "
                "items 16-byte aligned");
+  VEDA_REQUIRE(n_joins >= 0 && n_joins <= n_items && n_parts >= n_joins &&
+                   n_parts <= n_items && kv_heads <= 65535 &&
+                   (n_joins == 0) == (n_parts == 0) &&
+                   (n_joins == 0 || joins != nullptr) &&
+                   reinterpret_cast<uintptr_t>(joins) % 16 == 0,
+               "the joins do not match the parts");
+  const int64_t need = veda_causal_fwd_workspace(kv_heads, head_dim, n_parts);
+  VEDA_REQUIRE(need >= 0 && workspace_bytes >= need &&
+                   (need == 0 || workspace != nullptr) &&
+                   reinterpret_cast<uintptr_t>(workspace) % 32 == 0,
+               "workspace too small or not 32-byte aligned "
+               "(veda_causal_fwd_workspace)");
   const int group = n_heads / kv_heads;
   const int tokens = kTile / group;
   CUtensorMap mq, mk, mv, mo;
@@ -629,8 +767,14 @@ extern "C" int veda_causal_fwd(
   p.lse_st = lse_stride_t;
   p.lse_sh = lse_stride_h;
   p.scale_log2 = softmax_scale * causal::kLog2e;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(
+      p.part_o + static_cast<int64_t>(kv_heads) * n_parts * 2 * kTile *
+                     head_dim);
+  p.n_parts = static_cast<int>(n_parts);
+  p.joins = joins;
   p.status = device_status_ptr();
   cudaStream_t s = as_stream(stream);
-  return head_dim == 128 ? causal::launch<128>(mq, mk, mv, mo, p, s)
-                         : causal::launch<64>(mq, mk, mv, mo, p, s);
+  return head_dim == 128 ? causal::launch<128>(mq, mk, mv, mo, p, n_joins, s)
+                         : causal::launch<64>(mq, mk, mv, mo, p, n_joins, s);
 }

@@ -26,13 +26,19 @@
 // decode_join_kernel. Parts are added in the order of the keys, with no
 // atomics: repeats are bit-identical.
 //
-// int8 and e4m3 codes become fp16 exactly, in registers. A key's scale
-// multiplies its scores; a value row's scale multiplies its weights, relative
-// to the largest scale met so far so that they stay inside fp16. q is brought
-// to [1, 2) per head by a power of two, so it loses nothing in fp16 but
-// elements 2^-14 below the head's largest. Scores, maxima, sums and
-// accumulators are fp32; weights are rounded to the 16-bit type of the
-// products (bf16 pages: bf16), as everywhere in this library.
+// int8 and e4m3 codes become fp16 exactly, in registers. An int8 code is
+// widened to the fp16 number (code + 128) 2^-24 (a subnormal: its bits are the
+// byte), which takes an instruction and a half a pair; the 128 comes out of the
+// scores as 128 sum(q) and out of the values as 128 sum(weights), which one
+// more product with ones gives with the weights as rounded. The order of d
+// inside the first product and of the columns of the second is free, and is
+// the one that the bytes of a word have. A key's scale multiplies its scores; a
+// value row's scale multiplies its weights, relative to the largest scale met
+// so far so that they stay inside fp16. q is brought to [1, 2) per head by a
+// power of two, so it loses nothing in fp16 but elements 2^-14 below the
+// head's largest. Scores, maxima, sums and accumulators are fp32; weights are
+// rounded to the 16-bit type of the products (bf16 pages: bf16), as everywhere
+// in this library.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <math.h>
@@ -45,8 +51,6 @@ namespace veda {
 
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = 32 * kWarps;
 constexpr int kChunk = 16;  // keys
 constexpr int kRows = 16;   // heads of a tile
 constexpr int kJoinThreads = 512;
@@ -65,6 +69,7 @@ struct DecodeParams {
   float* lse;          // [n_seqs, heads] or null
   float* partial;      // [n_ctas][2][kRows][D + 2]
   int n_ctas;
+  int warps;      // of a CTA
   float scale_log2;
   unsigned int* status;
 };
@@ -96,7 +101,7 @@ struct Split {
   int extra;
   int warps;
   __device__ __forceinline__ Split(const DecodeParams& p, int64_t total) {
-    const int all = p.n_ctas * kWarps;
+    const int all = p.n_ctas * p.warps;
     warps = total < all ? static_cast<int>(total) : all;
     size = warps > 0 ? quotient(total, warps) : 0;
     extra = static_cast<int>(total - size * warps);
@@ -140,6 +145,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t* warp_sum, int64_t x,
 // Where this warp's run begins: chunk numbers [*lo, *hi), the sequence of the
 // first and the chunks before that sequence. `ends` holds kThreads numbers.
 // Returns false for a warp without a run. All threads of the block call it.
+template <int kThreads>
 __device__ __forceinline__ bool find_run(const DecodeParams& p, int heads,
                                          int64_t* warp_sum, int64_t* ends,
                                          int64_t* lo, int64_t* hi, int* seq,
@@ -153,7 +159,7 @@ __device__ __forceinline__ bool find_run(const DecodeParams& p, int heads,
   int64_t sum;
   int64_t pre = block_scan<kThreads>(warp_sum, mine, &sum);
   const Split split(p, sum);
-  const int w = blockIdx.x * kWarps + tid / 32;
+  const int w = blockIdx.x * (kThreads / 32) + tid / 32;
   const bool run = w < split.warps;
   *lo = run ? split.begin(w) : 0;
   *hi = run ? split.begin(w + 1) : 0;
@@ -222,6 +228,14 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src,
                "l"(src), "r"(take ? 16 : 0)
                : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src)
+               : "memory");
+}
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src,
                                           bool take) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst),
@@ -251,6 +265,15 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t* r) {
       : "memory");
 }
 
+__device__ __forceinline__ float2 lds64(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 // c[4] += A (16 x 16) . B (16 x 8), bf16 or fp16 in, fp32 accumulate.
 template <bool kHalf>
 __device__ __forceinline__ void mma16816(float* c, const uint32_t* a,
@@ -269,28 +292,35 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a,
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Four codes (bytes 0 .. 3) as two fp16 pairs, exactly.
+// Four codes (bytes 0 .. 3 of a word) as two fp16 pairs, exactly: bytes 0 and
+// 2, and bytes 1 and 3. int8: as (code + 128) 2^-24.
 template <int kStore>
-__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t* lo,
-                                              uint32_t* hi) {
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t* even,
+                                              uint32_t* odd) {
   if constexpr (kStore == kStoreInt8) {
-    // 0x6400 | u is the fp16 number 1024 + u; u = code + 128.
-    w ^= 0x80808080u;
-    const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
-    uint32_t a = __byte_perm(w, 0x64646464u, 0x4140);
-    uint32_t b = __byte_perm(w, 0x64646464u, 0x4342);
-    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), bias);
-    const __half2 y = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
-    *lo = *reinterpret_cast<const uint32_t*>(&x);
-    *hi = *reinterpret_cast<const uint32_t*>(&y);
+    *even = (w ^ 0x00800080u) & 0x00ff00ffu;
+    *odd = __byte_perm(w, 0, 0x4341) ^ 0x00800080u;
   } else {
+    w = __byte_perm(w, 0, 0x3120);
     const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2(
         static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
     const __half2_raw y = __nv_cvt_fp8x2_to_halfraw2(
         static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
-    *lo = static_cast<uint32_t>(x.x) | (static_cast<uint32_t>(x.y) << 16);
-    *hi = static_cast<uint32_t>(y.x) | (static_cast<uint32_t>(y.y) << 16);
+    *even = static_cast<uint32_t>(x.x) | (static_cast<uint32_t>(x.y) << 16);
+    *odd = static_cast<uint32_t>(y.x) | (static_cast<uint32_t>(y.y) << 16);
   }
+}
+
+// Bytes 0, 1 and bytes 2, 3 of a word of e4m3 codes (the K operand; no
+// regrouping).
+__device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t* lo,
+                                           uint32_t* hi) {
+  const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2(
+      static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
+  const __half2_raw y = __nv_cvt_fp8x2_to_halfraw2(
+      static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
+  *lo = static_cast<uint32_t>(x.x) | (static_cast<uint32_t>(x.y) << 16);
+  *hi = static_cast<uint32_t>(y.x) | (static_cast<uint32_t>(y.y) << 16);
 }
 
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
@@ -301,13 +331,18 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 template <int kD, int kStore>
 struct Shape {
   static constexpr bool kHalf = kStore != kStoreBf16;
+  // Warps of a CTA (one a SM). Twelve warps of one chunk a step and eight of
+  // two take the same time with int8 pages (64 x 8,192 rows, 8 heads, D = 128:
+  // 211 and 213 us), twelve less with e4m3 (235 and 253): converting codes is
+  // what bounds both, at 80 and 72 % of the copy rate (bf16 pages: 100 %).
+  static constexpr int kWarps = kHalf && kD == 128 ? 12 : 8;
   static constexpr int kRowBytes = kHalf ? kD : 2 * kD;
   static constexpr int kTileBytes = kChunk * kRowBytes;  // k or v of a chunk
   // k, v, and (8-bit) 16 k scales and 16 v scales.
   static constexpr int kStageBytes = 2 * kTileBytes + (kHalf ? 128 : 0);
   static constexpr int kPieces = kRowBytes / 16;  // 16-byte pieces of a row
   // Chunks a step: two share the maxima and the loop's overhead.
-  static constexpr int kPair = kHalf ? 2 : 1;
+  static constexpr int kPair = kHalf && kWarps == 8 ? 2 : 1;
   static constexpr int kJoinFloats = kD + 4;      // a row of the join buffer
 };
 
@@ -337,18 +372,21 @@ __host__ __device__ constexpr int part_floats(int pitch) {
 }
 
 template <int kD, int kStore, int kStages>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
     decode_kernel(const __grid_constant__ DecodeParams p) {
   using S = Shape<kD, kStore>;
   constexpr bool kHalf = S::kHalf;
+  constexpr int kWarps = S::kWarps;
+  constexpr int kThreads = 32 * kWarps;
   constexpr int kSteps = kD / 16;
   constexpr int kRingBytes = kStages * S::kStageBytes;
   static_assert(kRingBytes >= kRows * S::kJoinFloats * 4,
                 "a last part fits the ring");
   static_assert(kWarps * kRingBytes >= kThreads * 8, "find_run's numbers fit");
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t s_sums[kWarps];
   __shared__ Part s_parts[kWarps][2];
+  __shared__ int s_list[2 * kWarps], s_open[2 * kWarps + 1], s_groups;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int quad = lane % 4, row_lo = lane / 4;  // fragment coordinates
   const int pitch = min(p.group, kRows);
@@ -375,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int64_t lo, hi, before = 0;
   Pieces seg;
   seg.left = 0;
-  if (find_run(p, heads, s_sums, reinterpret_cast<int64_t*>(smem), &lo, &hi,
+  if (find_run<kThreads>(p, heads, s_sums, reinterpret_cast<int64_t*>(smem), &lo, &hi,
                &seg.b, &before)) {
     seg.length = context(p, seg.b);
     seg.n = chunks_of(seg.length);
@@ -406,6 +444,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   if (ld.valid()) look_up();
   int ld_stage = 0;
+  // This lane's 16-byte pieces of a tile are 512 bytes apart; where pieces move
+  // with the row, every other one lies at the other side of bit 6.
+  const uint32_t ring_at = smem_u32(ring);
+  const uint32_t put = piece_at<S::kPieces>(lane / S::kPieces,
+                                            lane % S::kPieces);
+  auto put_at = [&](int i) -> uint32_t {
+    const int r = i * (32 / S::kPieces);  // the rows' step
+    if constexpr (S::kPieces >= 8)
+      return (put ^ ((r & 7) * 16)) + i * 512;
+    else
+      return (put ^ (((r >> 1) & 3) * 16)) + i * 512;
+  };
   auto load_next = [&]() {
     if (ld.valid()) {
       const int key0 = ld_chunk * kChunk;
@@ -419,21 +469,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                  << p.c.page_shift) +
                 (key0 & ((1 << p.c.page_shift) - 1)))
              : 0;
-      const uint32_t dst = smem_u32(ring + ld_stage * S::kStageBytes);
+      const uint32_t dst = ring_at + ld_stage * S::kStageBytes;
       const uint8_t* ksrc = p.c.k + row0 * S::kRowBytes + lane * 16;
       const uint8_t* vsrc = p.c.v + row0 * S::kRowBytes + lane * 16;
+      const float* scales = nullptr;
+      if constexpr (kHalf)
+        scales = (lane < 16 ? p.c.k_scale : p.c.v_scale) + row0 + lane % 16;
+      if (live >= kChunk) {
 #pragma unroll
-      for (int i = 0; i < kChunk * S::kPieces / 32; ++i) {
-        const int piece = i * 32 + lane;
-        const int r = piece / S::kPieces, c = piece % S::kPieces;
-        const uint32_t off = piece_at<S::kPieces>(r, c);
-        cp_async16(dst + off, ksrc + i * 512, r < live);
-        cp_async16(dst + S::kTileBytes + off, vsrc + i * 512, r < live);
-      }
-      if constexpr (kHalf) {
-        const int r = lane % 16;
-        const float* src = (lane < 16 ? p.c.k_scale : p.c.v_scale) + row0 + r;
-        cp_async4(dst + 2 * S::kTileBytes + lane * 4, src, r < live);
+        for (int i = 0; i < kChunk * S::kPieces / 32; ++i) {
+          cp_async16(dst + put_at(i), ksrc + i * 512);
+          cp_async16(dst + S::kTileBytes + put_at(i), vsrc + i * 512);
+        }
+        if constexpr (kHalf)
+          cp_async4(dst + 2 * S::kTileBytes + lane * 4, scales);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kChunk * S::kPieces / 32; ++i) {
+          const int r = (i * 32 + lane) / S::kPieces;
+          cp_async16(dst + put_at(i), ksrc + i * 512, r < live);
+          cp_async16(dst + S::kTileBytes + put_at(i), vsrc + i * 512,
+                     r < live);
+        }
+        if constexpr (kHalf)
+          cp_async4(dst + 2 * S::kTileBytes + lane * 4, scales,
+                    lane % 16 < live);
       }
       ++ld_chunk;
       look_up();
@@ -452,6 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- q fragments of the piece's heads ----
     uint32_t qf[kSteps][4];
     float row_scale[2] = {p.scale_log2, p.scale_log2};
+    [[maybe_unused]] float row_bias[2] = {0.f, 0.f};  // int8: the 128s'
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int r = row_lo + 8 * half;
@@ -467,7 +528,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         // The products' depth index runs over d in the order that a thread's
-        // four consecutive code bytes give.
+        // four consecutive code bytes give: int8 takes bytes 0, 2 and 1, 3
+        // together, e4m3 bytes 0, 1 and 2, 3.
         float x[kSteps][4];
         float top = 0.f;
 #pragma unroll
@@ -492,35 +554,63 @@ __global__ void __launch_bounds__(kThreads, 1)
         row_scale[half] =
             p.scale_log2 *
             __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        if constexpr (kStore == kStoreInt8) {
+          float sum = 0.f;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          qf[s][half] = pack_half(x[s][0] * inv, x[s][1] * inv);
-          qf[s][half + 2] = pack_half(x[s][2] * inv, x[s][3] * inv);
+          for (int s = 0; s < kSteps; ++s) {
+            qf[s][half] = pack_half(x[s][0] * inv, x[s][2] * inv);
+            qf[s][half + 2] = pack_half(x[s][1] * inv, x[s][3] * inv);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t w = qf[s][half + 2 * i];
+              const float2 f =
+                  __half22float2(*reinterpret_cast<const __half2*>(&w));
+              sum += f.x + f.y;
+            }
+          }
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          row_bias[half] = -128.f * sum * row_scale[half];
+          row_scale[half] *= 0x1p24f;
+        } else {
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            qf[s][half] = pack_half(x[s][0] * inv, x[s][1] * inv);
+            qf[s][half + 2] = pack_half(x[s][2] * inv, x[s][3] * inv);
+          }
         }
       }
     }
 
     // ---- the piece's chunks, kPair a step ----
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    // m: the rows' references (-inf before the first key), m_ref: the same or
+    // 0; v_ref, v_inv: the values' reference and kWeight over it.
+    float m[2] = {-INFINITY, -INFINITY}, m_ref[2] = {0.f, 0.f};
+    float l[2] = {0.f, 0.f};
     float v_ref = 0.f;
+    [[maybe_unused]] float v_inv = 0.f;
     float o[kD / 8][4];
+    [[maybe_unused]] float ones[4] = {0.f, 0.f, 0.f, 0.f};  // int8: weights
 #pragma unroll
     for (int i = 0; i < kD / 8; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    // This lane's rows of the tiles that ldmatrix reads: in k, 16-byte pieces
+    // lane / 8 + 0 .. 3 of key lane % 8; in v, piece lane / 16 of key lane %
+    // 16. Further pieces differ in bits that only the exclusive or meets.
+    const uint32_t k_get = piece_at<S::kPieces>(lane & 7, lane / 8);
+    const uint32_t v_get =
+        piece_at<S::kPieces>((lane & 7) + ((lane >> 3) & 1) * 8, lane / 16);
+    constexpr uint32_t kEight = 8 * S::kRowBytes;  // eight keys on
     // kN chunks (1 or kPair) from `chunk` on.
     auto step = [&](auto count, int chunk) {
       constexpr int kN = decltype(count)::value;
       cp_async_wait<kStages - 1 - kN>();
       __syncwarp();
-      uint32_t k_addr[kN], v_addr[kN];
-      const float* scales[kN];
+      uint32_t base[kN];
 #pragma unroll
       for (int u = 0; u < kN; ++u) {
-        const uint8_t* st = ring + stage * S::kStageBytes;
-        k_addr[u] = smem_u32(st);
-        v_addr[u] = k_addr[u] + S::kTileBytes;
-        scales[u] = reinterpret_cast<const float*>(st + 2 * S::kTileBytes);
+        base[u] = ring_at + stage * S::kStageBytes;
         stage = stage + 1 == kStages ? 0 : stage + 1;
       }
       // The chunks have landed, and the whole warp has read the stages before
@@ -531,28 +621,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       float s[2 * kN][4] = {};
 #pragma unroll
       for (int nt = 0; nt < 2 * kN; ++nt) {
-        const int key = (nt & 1) * 8 + (lane & 7);
-        if constexpr (!kHalf) {
+        const uint32_t at = base[nt / 2] + k_get;
 #pragma unroll
-          for (int st2 = 0; st2 < kSteps; st2 += 2) {
-            uint32_t b[4];
-            ldsm4(k_addr[nt / 2] +
-                      piece_at<S::kPieces>(key, st2 * 2 + lane / 8),
-                  b);
-            mma16816<false>(s[nt], qf[st2], b[0], b[1]);
-            mma16816<false>(s[nt], qf[st2 + 1], b[2], b[3]);
-          }
-        } else {
-#pragma unroll
-          for (int st4 = 0; st4 < kSteps; st4 += 4) {
-            uint32_t b[4];
-            ldsm4(k_addr[nt / 2] + piece_at<S::kPieces>(key, st4 + lane / 8),
-                  b);
+        for (int pc = 0; pc < S::kPieces; pc += 4) {
+          uint32_t b[4];
+          ldsm4((at ^ (pc * 16)) + (nt & 1) * kEight, b);
+          if constexpr (!kHalf) {
+            mma16816<false>(s[nt], qf[pc / 2], b[0], b[1]);
+            mma16816<false>(s[nt], qf[pc / 2 + 1], b[2], b[3]);
+          } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint32_t b0, b1;
-              codes_to_half<kStore>(b[i], &b0, &b1);
-              mma16816<true>(s[nt], qf[st4 + i], b0, b1);
+              if constexpr (kStore == kStoreInt8)
+                codes_to_half<kStore>(b[i], &b0, &b1);
+              else
+                e4m3_pairs(b[i], &b0, &b1);
+              mma16816<true>(s[nt], qf[pc + i], b0, b1);
             }
           }
         }
@@ -560,19 +645,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       // Columns of this thread: keys 2 quad + {0, 1} of each tile of 8.
       const int live = seg.length - chunk * kChunk;
       float top[2] = {-INFINITY, -INFINITY};
+      [[maybe_unused]] float v_top = 0.f;
+      [[maybe_unused]] float2 vs[2 * kN];
 #pragma unroll
       for (int nt = 0; nt < 2 * kN; ++nt) {
-        float k0 = 1.f, k1 = 1.f;
+        float2 ks = make_float2(1.f, 1.f);
         if constexpr (kHalf) {
-          const float2 ks = *reinterpret_cast<const float2*>(
-              scales[nt / 2] + (nt & 1) * 8 + quad * 2);
-          k0 = ks.x;
-          k1 = ks.y;
+          const uint32_t at = base[nt / 2] + 2 * S::kTileBytes +
+                              (nt & 1) * 32 + quad * 8;
+          ks = lds64(at);
+          vs[nt] = lds64(at + 64);
+          v_top = fmaxf(v_top, fmaxf(vs[nt].x, vs[nt].y));
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          s[nt][2 * half] *= row_scale[half] * k0;
-          s[nt][2 * half + 1] *= row_scale[half] * k1;
+          float& a = s[nt][2 * half];
+          float& b = s[nt][2 * half + 1];
+          if constexpr (kStore == kStoreInt8) {
+            a = fmaf(a, row_scale[half], row_bias[half]) * ks.x;
+            b = fmaf(b, row_scale[half], row_bias[half]) * ks.y;
+          } else if constexpr (kHalf) {
+            a *= row_scale[half] * ks.x;
+            b *= row_scale[half] * ks.y;
+          } else {
+            a *= row_scale[half];
+            b *= row_scale[half];
+          }
         }
         if (live < kN * kChunk) {
           const int key = nt * 8 + quad * 2;
@@ -587,46 +685,37 @@ __global__ void __launch_bounds__(kThreads, 1)
           top[half] = fmaxf(top[half],
                             fmaxf(s[nt][2 * half], s[nt][2 * half + 1]));
       }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        top[half] =
-            fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
-        top[half] =
-            fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
-      }
       // The references move only when they must: a maximum by more than 2^8,
-      // the values' scale by more than 2. fp16 weights carry a factor 2^6
-      // (kWeight) and stay below 2^15; those down to 2^-20 of the references
-      // keep all of fp16's bits.
-      float v_top = 0.f;
-      [[maybe_unused]] float2 vs[2 * kN];
-      if constexpr (kHalf) {
-#pragma unroll
-        for (int nt = 0; nt < 2 * kN; ++nt) {
-          vs[nt] = *reinterpret_cast<const float2*>(
-              scales[nt / 2] + 16 + (nt & 1) * 8 + quad * 2);
-          v_top = fmaxf(v_top, fmaxf(vs[nt].x, vs[nt].y));
-        }
-        v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, 1));
-        v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, 2));
-      }
+      // the values' scale by more than 2. (A row's maximum is taken over its
+      // four threads only then.) fp16 weights carry a factor 2^6 (kWeight)
+      // and stay below 2^15; those down to 2^-20 of the references keep all of
+      // fp16's bits.
       const bool grow = top[0] > m[0] + 8.f || top[1] > m[1] + 8.f ||
                         (kHalf && v_top > 2.f * v_ref);
       if (__any_sync(0xffffffffu, grow)) {
         float f[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const float next = fmaxf(m[half], top[half]);
+          float x = top[half];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          const float next = fmaxf(m[half], x);
           f[half] = m[half] == -INFINITY ? 0.f : ex2_approx(m[half] - next);
           m[half] = next;
+          // m is -inf where no key of the row has existed so far.
+          m_ref[half] = next == -INFINITY ? 0.f : next;
           l[half] *= f[half];
         }
         if constexpr (kHalf) {
+          float x = v_top;
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
           // (Held above 2^-100: its inverse exists.)
           const float next =
-              v_top > 0.f ? fmaxf(fmaxf(v_ref, v_top), 0x1p-100f) : v_ref;
+              x > 0.f ? fmaxf(fmaxf(v_ref, x), 0x1p-100f) : v_ref;
           const float g = v_ref > 0.f ? v_ref / next : 0.f;
           v_ref = next;
+          v_inv = next > 0.f ? kWeight / next : 0.f;
           f[0] *= g;
           f[1] *= g;
         }
@@ -637,19 +726,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           o[i][2] *= f[1];
           o[i][3] *= f[1];
         }
+        if constexpr (kStore == kStoreInt8) {
+          ones[0] *= f[0];
+          ones[2] *= f[1];
+        }
       }
       // Weights, as the A operand of the second product.
       uint32_t a[kN][4];
-      [[maybe_unused]] const float v_inv =
-          kHalf && v_ref > 0.f ? kWeight / v_ref : 0.f;
 #pragma unroll
       for (int nt = 0; nt < 2 * kN; ++nt)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          // m is -inf where no key of the row has existed so far.
-          const float ref = m[half] == -INFINITY ? 0.f : m[half];
-          const float p0 = ex2_approx(s[nt][2 * half] - ref);
-          const float p1 = ex2_approx(s[nt][2 * half + 1] - ref);
+          const float p0 = ex2_approx(s[nt][2 * half] - m_ref[half]);
+          const float p1 = ex2_approx(s[nt][2 * half + 1] - m_ref[half]);
           l[half] += p0 + p1;
           if constexpr (kHalf)
             a[nt / 2][(nt & 1) * 2 + half] = pack_half(
@@ -658,39 +747,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             a[nt / 2][(nt & 1) * 2 + half] = pack_bf16(p0, p1);
         }
       // O += P V.
-      const int vkey = (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
       for (int u = 0; u < kN; ++u) {
-        if constexpr (!kHalf) {
+        const uint32_t at = base[u] + S::kTileBytes + v_get;
 #pragma unroll
-          for (int dt = 0; dt < kD / 8; dt += 2) {
-            uint32_t b[4];
-            ldsm4_trans(
-                v_addr[u] + piece_at<S::kPieces>(vkey, dt + lane / 16), b);
-            mma16816<false>(o[dt], a[u], b[0], b[1]);
-            mma16816<false>(o[dt + 1], a[u], b[2], b[3]);
-          }
-        } else {
-          // A 16-byte piece of a row is 16 d: column n of the even tile is
-          // d = 2 n, of the odd tile 2 n + 1.
-#pragma unroll
-          for (int dt = 0; dt < kD / 8; dt += 4) {
-            uint32_t b[4];
-            ldsm4_trans(
-                v_addr[u] + piece_at<S::kPieces>(vkey, dt / 2 + lane / 16),
-                b);
+        for (int pc = 0; pc < S::kPieces; pc += 2) {
+          uint32_t b[4];
+          ldsm4_trans(at ^ (pc * 16), b);
+          if constexpr (!kHalf) {
+            mma16816<false>(o[pc], a[u], b[0], b[1]);
+            mma16816<false>(o[pc + 1], a[u], b[2], b[3]);
+          } else {
+            // A 16-byte piece of a row is 16 d: column n of the even tile is
+            // d = 2 n, of the odd tile 2 n + 1.
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              uint32_t lo0, hi0, lo1, hi1;
-              codes_to_half<kStore>(__byte_perm(b[2 * i], 0, 0x3120), &lo0,
-                                    &hi0);
-              codes_to_half<kStore>(__byte_perm(b[2 * i + 1], 0, 0x3120),
-                                    &lo1, &hi1);
-              mma16816<true>(o[dt + 2 * i], a[u], lo0, lo1);
-              mma16816<true>(o[dt + 2 * i + 1], a[u], hi0, hi1);
+              uint32_t even0, odd0, even1, odd1;
+              codes_to_half<kStore>(b[2 * i], &even0, &odd0);
+              codes_to_half<kStore>(b[2 * i + 1], &even1, &odd1);
+              mma16816<true>(o[2 * (pc + i)], a[u], even0, even1);
+              mma16816<true>(o[2 * (pc + i) + 1], a[u], odd0, odd1);
             }
           }
         }
+        if constexpr (kStore == kStoreInt8)
+          mma16816<true>(ones, a[u], 0x3C003C00u, 0x3C003C00u);
       }
       // The other stages of this step are free once the warp has read them.
       if constexpr (kN > 1) {
@@ -713,6 +794,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
     }
     const float unit = kHalf ? v_ref * (1.f / kWeight) : 1.f;
+    if constexpr (kStore == kStoreInt8) {
+      // (ones' columns are all alike.)
+#pragma unroll
+      for (int i = 0; i < kD / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[i][e] = fmaf(o[i][e], 0x1p24f, -128.f * ones[e & 2]);
+    }
     const bool starts = seg.c0 == 0, ends = seg.c1 == seg.n;
     const int slot = starts ? 1 : 0;
     if (!(starts && ends)) {
@@ -778,126 +867,151 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
-  // ---- add up the CTA's parts, (sequence, head tile) by (sequence, head
-  // tile), in the order of the keys ----
+  // ---- add up the CTA's parts in the order of the keys ----
+  // Warp 0 lists the parts that there are (part number 2 * warp + slot) and
+  // where each (sequence, head tile)'s begin in the list.
   __syncthreads();
-  int first = 0;  // part number: 2 * warp + slot
-  while (first < 2 * kWarps) {
-    const Part head = s_parts[first / 2][first % 2];
-    if (head.b < 0) {
-      ++first;
-      continue;
+  if (warp == 0) {
+    Part x = Part{-1, 0, 0, 0};
+    if (lane < 2 * kWarps) x = s_parts[lane / 2][lane % 2];
+    const unsigned there = __ballot_sync(0xffffffffu, x.b >= 0);
+    const unsigned below = there & ((1u << lane) - 1);
+    const int prev = below != 0 ? 31 - __clz(below) : lane;
+    const int pb = __shfl_sync(0xffffffffu, x.b, prev);
+    const int pv = __shfl_sync(0xffffffffu, x.vh, prev);
+    const bool opens =
+        x.b >= 0 && (below == 0 || pb != x.b || pv != x.vh);
+    const unsigned open = __ballot_sync(0xffffffffu, opens);
+    if (x.b >= 0) s_list[__popc(below)] = lane;
+    if (opens)
+      s_open[__popc(open & ((1u << lane) - 1))] = __popc(below);
+    if (lane == 0) {
+      s_open[__popc(open)] = __popc(there);
+      s_groups = __popc(open);
     }
-    int last = first, scan = first + 1;
-    Part tail = head;
-    for (; scan < 2 * kWarps; ++scan) {
-      const Part x = s_parts[scan / 2][scan % 2];
-      if (x.b < 0) continue;
-      if (x.b != head.b || x.vh != head.vh) break;
-      last = scan;
-      tail = x;
-    }
+  }
+  __syncthreads();
+  const int per_group = pitch * (kD / 2);
+  for (int i = threadIdx.x; i < s_groups * per_group; i += kThreads) {
+    const int g = i / per_group, r = i % per_group / (kD / 2);
+    const int d = i % (kD / 2) * 2;
+    const int first = s_open[g], end = s_open[g + 1];
+    const int f0 = s_list[first], f1 = s_list[end - 1];
+    const Part head = s_parts[f0 / 2][f0 % 2];
     const int kvh = head.vh / p.tiles, tile = head.vh % p.tiles;
-    const int n_rows = min(kRows, p.group - tile * kRows);
-    const bool whole = head.starts && tail.ends;
-    // A part that an earlier CTA began, or one that this CTA begins: at most
-    // one of each goes on elsewhere.
-    float* spill = p.partial +
-                   (static_cast<int64_t>(blockIdx.x) * 2 + head.starts) *
-                       kRows * (kD + 2);
-    for (int i = threadIdx.x; i < n_rows * (kD / 2); i += kThreads) {
-      const int r = i / (kD / 2), d = (i % (kD / 2)) * 2;
-      float top = -INFINITY;
-      for (int w = first; w <= last; ++w)
-        if (s_parts[w / 2][w % 2].b >= 0)
-          top = fmaxf(top,
-                      part_at(w / 2, w % 2)[r * S::kJoinFloats + kD]);
-      const float ref = top == -INFINITY ? 0.f : top;
-      float x = 0.f, y = 0.f, sum = 0.f;
-      for (int w = first; w <= last; ++w) {
-        if (s_parts[w / 2][w % 2].b < 0) continue;
-        const float* src = part_at(w / 2, w % 2) + r * S::kJoinFloats;
-        const float f = ex2_approx(src[kD] - ref);
-        const float2 ow = *reinterpret_cast<const float2*>(src + d);
-        x = fmaf(f, ow.x, x);
-        y = fmaf(f, ow.y, y);
-        sum = fmaf(f, src[kD + 1], sum);
-      }
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int64_t at =
-            static_cast<int64_t>(head.b) * (p.c.kv_heads * p.group) +
-            kvh * p.group + tile * kRows + r;
-        *reinterpret_cast<uint32_t*>(p.out + at * kD + d) =
-            pack_bf16(x * inv, y * inv);
-        if (d == 0 && p.lse != nullptr)
-          p.lse[at] = (top + log2f(sum)) * kLn2;
-      } else {
-        float* dst = spill + r * (kD + 2);
-        *reinterpret_cast<float2*>(dst + d) = make_float2(x, y);
-        if (d == 0) {
-          dst[kD] = top;
-          dst[kD + 1] = sum;
-        }
+    if (r >= min(kRows, p.group - tile * kRows)) continue;
+    float top = -INFINITY;
+    for (int w = first; w < end; ++w) {
+      const int at = s_list[w];
+      top = fmaxf(top, part_at(at / 2, at % 2)[r * S::kJoinFloats + kD]);
+    }
+    const float ref = top == -INFINITY ? 0.f : top;
+    float x = 0.f, y = 0.f, sum = 0.f;
+#pragma unroll 4
+    for (int w = first; w < end; ++w) {
+      const int at = s_list[w];
+      const float* src = part_at(at / 2, at % 2) + r * S::kJoinFloats;
+      const float f = ex2_approx(src[kD] - ref);
+      const float2 ow = *reinterpret_cast<const float2*>(src + d);
+      x = fmaf(f, ow.x, x);
+      y = fmaf(f, ow.y, y);
+      sum = fmaf(f, src[kD + 1], sum);
+    }
+    if (head.starts && s_parts[f1 / 2][f1 % 2].ends) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int64_t at =
+          static_cast<int64_t>(head.b) * (p.c.kv_heads * p.group) +
+          kvh * p.group + tile * kRows + r;
+      *reinterpret_cast<uint32_t*>(p.out + at * kD + d) =
+          pack_bf16(x * inv, y * inv);
+      if (d == 0 && p.lse != nullptr)
+        p.lse[at] = (top + log2f(sum)) * kLn2;
+    } else {
+      // One that an earlier CTA began (slot 0), or one that this CTA begins
+      // (slot 1): at most one of each goes on elsewhere.
+      float* dst = p.partial +
+                   ((static_cast<int64_t>(blockIdx.x) * 2 + head.starts) *
+                        kRows +
+                    r) *
+                       (kD + 2);
+      *reinterpret_cast<float2*>(dst + d) = make_float2(x, y);
+      if (d == 0) {
+        dst[kD] = top;
+        dst[kD + 1] = sum;
       }
     }
-    first = scan;
   }
 }
 
 // Adds up the parts of the (sequence, head tile)s that several CTAs share, in
-// the order of the keys; writes the rows of empty sequences. One block per
-// (sequence, head tile).
+// the order of the keys, and writes the rows of empty sequences. Block i takes
+// the head tile, if there is one, that goes on from CTA i (where it begins) to
+// CTA i + 1.
 template <int kD>
 __global__ void __launch_bounds__(kJoinThreads)
     decode_join_kernel(const __grid_constant__ DecodeParams p) {
   constexpr int kPer = kD / 32;  // elements a lane
-  __shared__ int64_t sums[2][kJoinThreads / 32];
+  __shared__ int64_t sums[kJoinThreads / 32];
   __shared__ float tops[kJoinThreads / 32], totals[kJoinThreads / 32];
   __shared__ float rows[kJoinThreads / 32][kD];
+  __shared__ int s_seq;
+  __shared__ int64_t s_before;
   const int heads = p.c.kv_heads * p.tiles;
-  const int b = blockIdx.x / heads, vh = blockIdx.x % heads;
+  const int all_heads = p.c.kv_heads * p.group;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  int64_t before = 0, total = 0;
-  for (int i = threadIdx.x; i < p.c.n_seqs; i += kJoinThreads) {
-    const int n = chunks_of(context(p, i));
-    total += n;
-    if (i < b) before += n;
+  int64_t total = 0;
+  for (int i = threadIdx.x; i < p.c.n_seqs; i += kJoinThreads)
+    total += chunks_of(context(p, i));
+  {
+    int64_t sum;
+    block_scan<kJoinThreads>(sums, total * heads, &sum);
+    total = sum;
   }
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, s);
-    total += __shfl_xor_sync(0xffffffffu, total, s);
-  }
-  if (lane == 0) {
-    sums[0][warp] = before;
-    sums[1][warp] = total;
+  const Split split(p, total);
+  // The first chunk of CTA i + 1, and the sequence it lies in.
+  const int next_warp = (static_cast<int>(blockIdx.x) + 1) * p.warps;
+  const int64_t at = next_warp < split.warps ? split.begin(next_warp) : total;
+  if (threadIdx.x == 0) s_seq = -1;
+  int64_t base = 0;
+  for (int b0 = 0; b0 < p.c.n_seqs; b0 += kJoinThreads) {
+    const int b = b0 + threadIdx.x;
+    const int64_t n =
+        b < p.c.n_seqs ? chunks_of(context(p, b)) * static_cast<int64_t>(heads)
+                       : int64_t(0);
+    int64_t sum;
+    const int64_t pre = base + block_scan<kJoinThreads>(sums, n, &sum);
+    if (pre <= at && at < pre + n) {
+      s_seq = b;
+      s_before = pre;
+    }
+    base += sum;
   }
   __syncthreads();
-  before = total = 0;
-#pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) {
-    before += sums[0][w];
-    total += sums[1][w];
-  }
-  total *= heads;
-  const Split split(p, total);
-  const int n = chunks_of(context(p, b));
-  const int64_t first = before * heads + static_cast<int64_t>(vh) * n;
-  const int kvh = vh / p.tiles, tile = vh % p.tiles;
-  const int n_rows = min(kRows, p.group - tile * kRows);
-  const int64_t at0 = static_cast<int64_t>(b) * (p.c.kv_heads * p.group) +
-                      kvh * p.group + tile * kRows;
-  // CTAs c0 .. c1 hold the head's chunks: c0 begins it (its slot 1), in the
-  // others it goes on (their slot 0).
-  int c0 = 0, c1 = -1;
-  if (n > 0) {
-    c0 = split.warp_of(first) / kWarps;
-    c1 = split.warp_of(first + n - 1) / kWarps;
-  }
   // Every block waits, so that this grid ends after the one it follows.
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (c0 == c1) return;  // one CTA had all of it
+  // Rows of empty sequences, a sequence a block at a time.
+  for (int b = blockIdx.x; b < p.c.n_seqs; b += gridDim.x) {
+    if (context(p, b) > 0) continue;
+    const int64_t first = static_cast<int64_t>(b) * all_heads;
+    for (int i = threadIdx.x; i < all_heads * (kD / 2); i += kJoinThreads)
+      reinterpret_cast<uint32_t*>(p.out + first * kD)[i] = 0u;
+    if (p.lse != nullptr)
+      for (int i = threadIdx.x; i < all_heads; i += kJoinThreads)
+        p.lse[first + i] = -INFINITY;
+  }
+  const int b = s_seq;
+  if (b < 0) return;  // CTA i + 1 has no chunks
+  const int n = chunks_of(context(p, b));
+  const int vh = static_cast<int>(quotient(at - s_before, n));
+  const int64_t first = s_before + static_cast<int64_t>(vh) * n;
+  const int c0 = split.warp_of(first) / p.warps;
+  const int c1 = split.warp_of(first + n - 1) / p.warps;
+  // It begins at CTA i + 1 itself, or began before CTA i.
+  if (c0 != static_cast<int>(blockIdx.x)) return;
+  const int kvh = vh / p.tiles, tile = vh % p.tiles;
+  const int n_rows = min(kRows, p.group - tile * kRows);
+  const int64_t at0 = static_cast<int64_t>(b) * all_heads + kvh * p.group +
+                      tile * kRows;
   // `ways` warps a row, every ways-th part each, then added up.
   constexpr int kBatch = 4;
   const int ways = min(kJoinThreads / 32 / n_rows, c1 - c0 + 1);
@@ -981,25 +1095,24 @@ __global__ void __launch_bounds__(kJoinThreads)
 
 // kPitch: the heads of a tile, at most.
 template <int kD, int kStore, int kStages, int kPitch>
-int launch(const DecodeParams& p, cudaStream_t stream) {
+int launch(DecodeParams p, cudaStream_t stream) {
   using S = Shape<kD, kStore>;
-  constexpr int kSmem = kWarps * (kStages * S::kStageBytes +
-                                  part_floats<kD, kStore>(kPitch) * 4);
+  constexpr int kSmem = S::kWarps * (kStages * S::kStageBytes +
+                                     part_floats<kD, kStore>(kPitch) * 4);
   static_assert(kSmem <= 226 * 1024, "beside the static part");
+  p.warps = S::kWarps;
   static std::atomic<uint64_t> allowed{0};
   int rc = allow_smem(
       reinterpret_cast<const void*>(decode_kernel<kD, kStore, kStages>),
       kSmem, &allowed);
   if (rc != VEDA_OK) return rc;
   decode_kernel<kD, kStore, kStages>
-      <<<p.n_ctas, kThreads, kSmem, stream>>>(p);
+      <<<p.n_ctas, 32 * S::kWarps, kSmem, stream>>>(p);
   rc = check_launch("decode_kernel");
   if (rc != VEDA_OK) return rc;
   // The join starts while the last CTAs run (griddepcontrol).
-  const int64_t blocks =
-      static_cast<int64_t>(p.c.n_seqs) * p.c.kv_heads * p.tiles;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.gridDim = dim3(static_cast<unsigned>(p.n_ctas));
   config.blockDim = dim3(kJoinThreads);
   config.stream = stream;
   cudaLaunchAttribute attr{};
@@ -1021,8 +1134,8 @@ int launch_stages(const DecodeParams& p, cudaStream_t stream) {
     return p.group <= 8 ? launch<kD, kStore, 3, 8>(p, stream)
                         : launch<kD, kStore, 2, kRows>(p, stream);
   } else {
-    return p.group <= 8 ? launch<kD, kStore, 5, 8>(p, stream)
-                        : launch<kD, kStore, 4, kRows>(p, stream);
+    return p.group <= 8 ? launch<kD, kStore, 3, 8>(p, stream)
+                        : launch<kD, kStore, 2, kRows>(p, stream);
   }
 }
 

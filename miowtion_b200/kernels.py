@@ -528,11 +528,18 @@ def causal_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = (q.new_empty((rows, heads), dtype=torch.float32) if return_lse
            else None)
+    tables = pack.tables(group, kv_heads)
+    ws = None
+    if tables.n_parts:
+        # The workspace of veda_causal_fwd: fp32 rows of two query tiles, with
+        # their maximum and sum, for every part.
+        ws = q.new_empty((kv_heads * tables.n_parts * 2 * sequences.TILE *
+                          (dim + 2),), dtype=torch.float32)
     _lib.call_on(q.device.index, 'veda_causal_fwd', *_rows_args(q),
                  *_rows_args(k), *_rows_args(v), rows, k_rows, heads,
-                 kv_heads, dim, *pack.tables(group).forward_args,
-                 out.data_ptr(), heads * dim, dim, _lib.ptr(lse), heads, 1,
-                 scale)
+                 kv_heads, dim, *tables.forward_args, out.data_ptr(),
+                 heads * dim, dim, _lib.ptr(lse), heads, 1, scale,
+                 _lib.ptr(ws), ws.numel() * 4 if ws is not None else 0)
     return out, lse
 
 
@@ -561,7 +568,7 @@ def causal_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     dq = torch.empty_like(q, memory_format=contiguous) if want_q else None
     dk = torch.empty_like(k, memory_format=contiguous) if want_kv else None
     dv = torch.empty_like(v, memory_format=contiguous) if want_kv else None
-    tables = pack.tables(group)
+    tables = pack.tables(group, kv_heads)
     # The workspace of veda_causal_bwd: two floats per row of a query tile.
     ws = q.new_empty((max(1, 2 * kv_heads * tables.n_tiles * sequences.TILE),),
                      dtype=torch.float32)

@@ -26,17 +26,19 @@ ITEM_FIELDS = 8
 
 @dataclasses.dataclass(frozen=True)
 class WorkTables:
-    """Work items of one group size: forward (pairs of query tiles), query
-    gradient (query tiles) and key gradient (key tiles), each [n, 8] int32 on
-    the device, longest first; `n_tiles` query tiles in all."""
+    """Work items of one group size and number of key heads: forward (pairs
+    of query tiles, or parts of them), joins (of the parts), query gradient
+    (query tiles) and key gradient (key tiles), each [n, 8] int32 on the
+    device, longest first; `n_tiles` query tiles and `n_parts` parts in all."""
 
-    group: int
     forward: torch.Tensor
+    joins: torch.Tensor
     query: torch.Tensor
     key: torch.Tensor
     n_tiles: int
+    n_parts: int
     # Address and items of each table, as a launch passes them.
-    forward_args: tuple[int, int]
+    forward_args: tuple[int, int, int, int, int]
     gradient_args: tuple[int, int, int, int, int]
     stream: int
 
@@ -82,36 +84,41 @@ class SequencePack:
         self.single_tokens = bool((self.q_lengths == 1).all())
         # No sequence has keys before (or without) its queries.
         self.whole = bool((self.q_lengths == self.k_lengths).all())
-        self._tables: dict[int, WorkTables] = {}
+        self._tables: dict[tuple[int, int], WorkTables] = {}
 
     def offsets(self) -> tuple[torch.Tensor, torch.Tensor]:
         """(q_offsets, k_offsets) for a launch on the current stream."""
         _keep(self._stream, self.q_offsets)
         return self.q_offsets, self.k_offsets
 
-    def tables(self, group: int) -> WorkTables:
-        """The work tables for `group` query heads per key head, built (and
-        copied to the device) on first use; build them before capturing a
-        CUDA graph."""
-        tables = self._tables.get(group)
+    def tables(self, group: int, kv_heads: int) -> WorkTables:
+        """The work tables for `kv_heads` key heads of `group` query heads
+        each, built (and copied to the device) on first use; build them
+        before capturing a CUDA graph."""
+        tables = self._tables.get((group, kv_heads))
         if tables is None:
-            if (self.device.type == 'cuda'
-                    and torch.cuda.is_current_stream_capturing()):
-                raise RuntimeError(
-                    'the work tables of this pack do not exist yet: call '
-                    f'tables({group}) or run once before the capture')
-            forward, query, key, n = work_items(
-                self.q_lengths, self.k_lengths, group)
-            flat = _to_device(np.concatenate([forward, query, key]),
-                              self.device)
-            a, b = len(forward), len(forward) + len(query)
-            parts = flat[:a], flat[a:b], flat[b:]
-            addresses = [t.data_ptr() if len(t) else 0 for t in parts]
+            sms = 148
+            if self.device.type == 'cuda':
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError(
+                        'the work tables of this pack do not exist yet: call '
+                        f'tables({group}, {kv_heads}) or run once before the '
+                        'capture')
+                sms = torch.cuda.get_device_properties(
+                    self.device).multi_processor_count
+            whole, query, key, n = work_items(self.q_lengths, self.k_lengths,
+                                              group)
+            forward, joins, n_parts = split_items(whole, kv_heads, sms)
+            parts = forward, joins, query, key
+            flat = _to_device(np.concatenate(parts), self.device)
+            parts = flat.split([len(t) for t in parts])
+            at = [t.data_ptr() if len(t) else 0 for t in parts]
             tables = WorkTables(
-                group, *parts, n, (addresses[0], a),
-                (addresses[1], b - a, addresses[2], len(key), n),
+                *parts, n, n_parts,
+                (at[0], len(forward), at[1], len(joins), n_parts),
+                (at[2], len(query), at[3], len(key), n),
                 _stream(self.device))
-            self._tables[group] = tables
+            self._tables[group, kv_heads] = tables
         else:
             _keep(tables.stream, tables.forward)
         return tables
@@ -200,3 +207,73 @@ def work_items(q_lengths: np.ndarray, k_lengths: np.ndarray, group: int
                     tile_base[seq]], axis=1)
     key = key[np.argsort(-blocks, kind='stable')]
     return query_items(2), query_items(1), key, int(tiles.sum())
+
+
+# What an item costs beside its key tiles, in key tiles: its loads and its
+# epilogue; for a part, which leaves fp32 rows for a second kernel; and that
+# kernel.
+ITEM_COST, PART_COST, JOIN_COST = 2.0, 3.0, 3.0
+# No part is shorter (a row of it is written and read again in fp32).
+SHORTEST_PART = 4
+
+
+def split_items(whole: np.ndarray, kv_heads: int, sms: int
+                ) -> tuple[np.ndarray, np.ndarray, int]:
+    """Forward items, possibly cut along the keys: (items, joins, parts).
+
+    With few items (a chunk behind a long context) whole ones leave
+    processors idle or give some of them one item more than others. Items
+    longer than a limit are cut into equal parts, and the limit is the one (or
+    none) for which the busiest processor's estimated cost is least, dealt
+    back and forth as the kernel does. With many items nothing is gained and
+    nothing tried."""
+    items = whole.copy()
+    items[:, 6], items[:, 7] = 0, -1  # first key tile, part
+    none = np.zeros((0, ITEM_FIELDS), np.int64)
+    blocks = whole[:, 5]
+    total = int(blocks.sum()) * kv_heads
+    longest = int(blocks.max(initial=0))
+    if (longest < 2 * SHORTEST_PART
+            or (len(whole) * kv_heads >= 8 * sms
+                and 2 * longest * sms <= total)):
+        return items, none, 0
+
+    def pieces(limit: int) -> np.ndarray:
+        return np.maximum(1, -(-blocks // limit))
+
+    def busiest(count: np.ndarray) -> float:
+        cost = np.where(count > 1, blocks / count + PART_COST,
+                        blocks + ITEM_COST)
+        cost = np.sort(np.repeat(cost, count * kv_heads))[::-1]
+        rounds = -(-cost.size // sms)
+        dealt = np.zeros(rounds * sms)
+        dealt[:cost.size] = cost
+        dealt = dealt.reshape(rounds, sms)
+        dealt[1::2] = dealt[1::2, ::-1]
+        return dealt.sum(0).max() + (JOIN_COST if (count > 1).any() else 0)
+
+    best, best_cost = None, busiest(np.ones_like(blocks))
+    for ways in (2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 148):
+        limit = -(-longest // ways)
+        if limit < SHORTEST_PART:
+            break
+        count = pieces(limit)
+        cost = busiest(count)
+        if cost < best_cost:
+            best, best_cost = count, cost
+    if best is None:
+        return items, none, 0
+    src, i = _expand(best)
+    out = items[src]
+    n = best[src]
+    first = blocks[src] * i // n
+    out[:, 5] = blocks[src] * (i + 1) // n - first
+    out[:, 6] = first
+    cut = n > 1
+    out[cut, 7] = np.arange(int(cut.sum()))
+    owners = np.nonzero(best > 1)[0]
+    joins = np.zeros((owners.size, ITEM_FIELDS), np.int64)
+    joins[:, 0], joins[:, 1] = whole[owners, 0], whole[owners, 1]
+    joins[:, 2] = np.cumsum(best[owners]) - best[owners]
+    joins[:, 3] = best[owners]
+    return out[np.argsort(-out[:, 5], kind='stable')], joins, int(cut.sum())

@@ -127,6 +127,20 @@ def test_forward_of_more_items_than_processors(dim):
     check_forward(pack, q, k, v, out, lse)
 
 
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('q_lengths, k_lengths, heads, kv_heads', [
+    ([70, 5], [6000, 3001], 8, 2), ([1], [20000], 14, 2),
+    ([33, 300, 9], [4000, 300, 0], 6, 2)])
+def test_forward_of_items_cut_along_the_keys(q_lengths, k_lengths, heads,
+                                             kv_heads, dim):
+    pack, q, k, v = problem(q_lengths, k_lengths, heads, kv_heads, dim)
+    assert pack.tables(heads // kv_heads, kv_heads).n_parts > 0
+    out, lse = kernels.causal_attention(q, k, v, pack, return_lse=True)
+    check_forward(pack, q, k, v, out, lse)
+    dout = rows(pack.total_q, heads, dim, 9)
+    check_gradients(pack, q, k, v, dout, gradients(pack, q, k, v, dout))
+
+
 def test_forward_of_scores_that_grow_along_the_keys():
     # Maxima rise from tile to tile, so the accumulator is rescaled, and a
     # scale of its own.

@@ -83,6 +83,36 @@ def test_work_items_cover_every_visible_pair_once(group, q, k):
     assert tiles <= set(range(n_tiles))
 
 
+@pytest.mark.parametrize('q, k, group, kv_heads, sms', [
+    ([64] * 3, [9000, 8000, 300], 4, 2, 148), ([1], [100000], 8, 1, 148),
+    ([1000, 40], [1000, 40], 1, 8, 148), ([500], [7000], 7, 2, 16),
+    ([64, 64], [1, 1], 4, 2, 148)])
+def test_split_items_are_the_whole_ones(q, k, group, kv_heads, sms):
+    whole, _, _, _ = sequences.work_items(np.array(q), np.array(k), group)
+    items, joins, n_parts = sequences.split_items(whole, kv_heads, sms)
+    assert (np.diff(items[:, 5]) <= 0).all()
+    parts = {}
+    for it in items:
+        parts.setdefault((it[0], it[1]), []).append(tuple(it[5:]))
+    join_of = {(j[0], j[1]): (j[2], j[3]) for j in joins}
+    assert len(parts) == len(whole)
+    for it in whole:
+        own = sorted(parts[it[0], it[1]], key=lambda x: x[1])
+        at = 0
+        for blocks, first, _ in own:
+            assert first == at
+            at += blocks
+        assert at == it[5]
+        if len(own) == 1:
+            assert own[0][2] == -1 and (it[0], it[1]) not in join_of
+        else:
+            assert min(b for b, _, _ in own) >= 2
+            start, count = join_of[it[0], it[1]]
+            assert [x[2] for x in own] == list(range(start, start + count))
+    numbers = [it[7] for it in items if it[7] >= 0]
+    assert sorted(numbers) == list(range(n_parts))
+
+
 def test_group_is_bounded():
     for group in (0, 129):
         with pytest.raises(ValueError, match='share'):
