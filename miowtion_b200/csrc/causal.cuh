@@ -143,6 +143,80 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int first,
   __syncwarp();
 }
 
+// A run of MMAs issued by one elected lane of a converged warp. One election
+// and one conversion of the operands' addresses for the whole run: issued one
+// by one (umma_ss_warp) an MMA costs the issuing warp some 70 cycles, more
+// than a product of 64 columns takes.
+//
+// D[tmem] (+)= A . B over kSteps steps of 16 along the depth, A and B K-major
+// tiles of 64-column halves (16 KB apart). Descriptors as low halves.
+#define VEDA_SS_STEP(N, OFF)                                            \
+  "add.u32 al, %1, " OFF "; add.u32 bl, %2, " OFF ";"                   \
+  "mov.b64 da, {al, %5}; mov.b64 db, {bl, %5};"                         \
+  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, " N ";"
+template <int kSteps>
+__device__ __forceinline__ void umma_ss_run(uint32_t d_tmem, uint32_t a_lo,
+                                            uint32_t b_lo, uint32_t idesc) {
+  static_assert(kSteps == 4 || kSteps == 8, "64 or 128 columns");
+  if constexpr (kSteps == 8)
+    asm volatile(
+        "{ .reg .pred z, o, e; .reg .b64 da, db; .reg .b32 rx, al, bl;"
+        "elect.sync rx|e, 0xFFFFFFFF; setp.ne.b32 z, %4, 0; "
+        "setp.eq.b32 o, %4, 0;"
+        VEDA_SS_STEP("z", "0") VEDA_SS_STEP("o", "2") VEDA_SS_STEP("o", "4")
+        VEDA_SS_STEP("o", "6") VEDA_SS_STEP("o", "1024")
+        VEDA_SS_STEP("o", "1026") VEDA_SS_STEP("o", "1028")
+        VEDA_SS_STEP("o", "1030") "}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(0u), "r"(kSw128DescHi)
+        : "memory");
+  else
+    asm volatile(
+        "{ .reg .pred z, o, e; .reg .b64 da, db; .reg .b32 rx, al, bl;"
+        "elect.sync rx|e, 0xFFFFFFFF; setp.ne.b32 z, %4, 0; "
+        "setp.eq.b32 o, %4, 0;"
+        VEDA_SS_STEP("z", "0") VEDA_SS_STEP("o", "2") VEDA_SS_STEP("o", "4")
+        VEDA_SS_STEP("o", "6") "}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(0u), "r"(kSw128DescHi)
+        : "memory");
+}
+#undef VEDA_SS_STEP
+
+// D[tmem] (+)= A[tmem] . B over 64 of the depth: A's steps at columns 0, 8,
+// 16, 24 (kGap: 0, 8, 32, 40) from a_tmem, B MN-major, 2 KB a step. The first
+// step overwrites D unless `accumulate`.
+#define VEDA_TS_STEP(N, COL, OFF)                                       \
+  "add.u32 al, %1, " COL "; add.u32 bl, %2, " OFF ";"                   \
+  "mov.b64 db, {bl, %5};"                                               \
+  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [al], db, %3, " N ";"
+template <bool kGap>
+__device__ __forceinline__ void umma_ts_run(uint32_t d_tmem, uint32_t a_tmem,
+                                            uint32_t b_lo, uint32_t idesc,
+                                            uint32_t accumulate) {
+  if constexpr (kGap)
+    asm volatile(
+        "{ .reg .pred z, o, e; .reg .b64 db; .reg .b32 rx, al, bl;"
+        "elect.sync rx|e, 0xFFFFFFFF; setp.ne.b32 z, %4, 0; "
+        "setp.ne.b32 o, %5, 0;"
+        VEDA_TS_STEP("z", "0", "0") VEDA_TS_STEP("o", "8", "128")
+        VEDA_TS_STEP("o", "32", "256") VEDA_TS_STEP("o", "40", "384")
+        "}" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate),
+        "r"(kSw128DescHi)
+        : "memory");
+  else
+    asm volatile(
+        "{ .reg .pred z, o, e; .reg .b64 db; .reg .b32 rx, al, bl;"
+        "elect.sync rx|e, 0xFFFFFFFF; setp.ne.b32 z, %4, 0; "
+        "setp.ne.b32 o, %5, 0;"
+        VEDA_TS_STEP("z", "0", "0") VEDA_TS_STEP("o", "8", "128")
+        VEDA_TS_STEP("o", "16", "256") VEDA_TS_STEP("o", "24", "384")
+        "}" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate),
+        "r"(kSw128DescHi)
+        : "memory");
+}
+#undef VEDA_TS_STEP
+
 // 3D bf16 tensor map over rows x heads x kD with a (64, heads_box, rows_box)
 // box and 128-byte swizzle.
 int make_rows_map(CUtensorMap* map, const void* base, int64_t rows,

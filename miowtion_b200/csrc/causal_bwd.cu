@@ -18,10 +18,18 @@
 //   dkdv    a key tile an item, the query tiles that see it: S^T = K Q^T and
 //           dP^T = V dO^T, P^T and dS^T written back over them, dV += P^T dO
 //           and dK += dS^T Q.
-// Each block's 128 columns run as two halves of 64, so that the tensor core
-// has one half's products while the compute warps work on the other. One CTA
-// per SM, 8 compute warps (warp w: TMEM lanes 32(w%4).., 32 of a half's
-// columns), a TMA producer warp and a converged MMA warp.
+// One CTA per SM, 8 compute warps, a TMA producer warp and a converged MMA warp.
+// Tensor memory decides how the two kernels overlap their products with the
+// elementwise work. dq has one accumulator, so there is room for two S buffers
+// beside dP: while the compute warps turn block b into dS, the tensor core has
+// dP of b + 1 (as soon as dP of b is in registers), dQ of b - 1 and S of b + 1,
+// all 128 columns wide. dk/dv has two accumulators and no room: a block's 128
+// columns run as two halves of 64, and the tensor core has one half's products
+// while the compute warps work on the other. (dq in halves as well: 904 against
+// 874 us for the whole backward of 8,192 tokens, 16/4 heads, D = 128, where a
+// product 64 columns wide reads 6 KB of shared memory for 32 cycles' work, 48
+// cycles' worth; 736 against 740 us at D = 64. 16 compute warps, a group per
+// half, in both kernels: 2 % faster at D = 128, 8 % slower at D = 64.)
 //
 // Rows behind a sequence's end are cleared in shared memory where they are
 // the depth of a product (keys in dq, queries in dkdv); elsewhere they are
@@ -50,8 +58,13 @@ struct Bwd {
   static constexpr uint32_t kTileUnits = kTileBytes >> 4;
   static constexpr int kSteps = kD / 16;
   static constexpr int kStages = kD == 128 ? 2 : 4;  // pairs of tiles
+  // dk/dv: two resident tiles, the stages and their (L, D) vectors.
   static constexpr int kSmem = (2 + 2 * kStages) * kTileBytes +
                                kStages * 1024 + 512 + 1024;
+  // dq: Q and dO, rings of K and V.
+  static constexpr int kKRing = 3, kVRing = 2;
+  static constexpr int kDqSmem =
+      (2 + kKRing + kVRing) * kTileBytes + 512 + 1024;
 };
 
 struct BwdParams {
@@ -176,20 +189,69 @@ __global__ void __launch_bounds__(kPrepThreads) causal_bwd_prep_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// dq. TMEM, per half h: S [128h, 128h+64) (dS over its columns 0-15 and
-// 32-47), dP [128h+64, 128h+128); dQ [256, 256 + kD).
+// dq. TMEM: S of block b in [128 (b % 2), ..) (then dS, bf16, over columns 0-31
+// and 64-95 of it), dP [256, 384), dQ [384, 384 + kD). Blocks are numbered
+// through the CTA's items.
 // ---------------------------------------------------------------------------
 enum DqBar {
-  kQFull = 0,                 // Q and dO of the item landed
-  kQEmpty,                    // the item's last S and dP finished
-  kSdFull,                    // [2 halves] S and dP of the block's half
-  kDsFull = kSdFull + 2,      // [2 halves] dS written (8 warps)
-  kDqDone = kDsFull + 2,      // the item's last dQ product finished
+  kQFull = 0,                 // Q of the item landed
+  kQEmpty,                    // the item's last S finished
+  kDoFull,                    // dO of the item landed
+  kDoEmpty,                   // the item's last dP finished
+  kSFull,                     // [2] S of the block (by its parity)
+  kDpFull = kSFull + 2,       // dP of the block
+  kDpFree,                    // dP is in registers (8 warps)
+  kDsFull,                    // dS written (8 warps)
+  kDqDone,                    // the item's last dQ product finished
   kDqFree,                    // the epilogue has read dQ (8 warps)
   kDqDrain,
-  kKvFull,                    // [kStages] K and V of the block landed
-  kKvEmpty = kKvFull + 4,     // [kStages] the block's products finished
-  kDqNumBars = kKvEmpty + 4
+  kKFull,                     // [kKRing]
+  kKEmpty = kKFull + 3,       // [kKRing]
+  kVFull = kKEmpty + 3,       // [kVRing]
+  kVEmpty = kVFull + 2,       // [kVRing]
+  kDqNumBars = kVEmpty + 2
+};
+
+// The query items of a CTA that have key tiles (all with keep_empty).
+struct QueryStream {
+  int t;  // turns taken
+  int h;
+  QueryItem it;
+  __device__ __forceinline__ bool next(const BwdParams& p, int n_items,
+                                       bool keep_empty) {
+    while (static_cast<int64_t>(t) * gridDim.x < n_items) {
+      const int64_t i = turn(t++);
+      if (i >= n_items) continue;
+      const int entry = static_cast<int>(i) / p.kv_heads;
+      h = static_cast<int>(i) - entry * p.kv_heads;
+      it = load_item<QueryItem>(p.table, entry);
+      if (it.blocks > 0 || keep_empty) return true;
+    }
+    return false;
+  }
+};
+
+// A position in the stream of blocks: block j of the current item.
+struct BlockCursor {
+  QueryStream st;
+  int b, j, items;
+  bool valid;
+  __device__ __forceinline__ void init(const BwdParams& p, int n_items) {
+    st.t = 0;
+    b = j = items = 0;
+    valid = st.next(p, n_items, false);
+  }
+  __device__ __forceinline__ bool first() const { return j == 0; }
+  __device__ __forceinline__ bool last() const {
+    return j == st.it.blocks - 1;
+  }
+  __device__ __forceinline__ void next(const BwdParams& p, int n_items) {
+    ++b;
+    if (++j < st.it.blocks) return;
+    j = 0;
+    ++items;
+    valid = st.next(p, n_items, false);
+  }
 };
 
 template <int kD>
@@ -200,27 +262,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                      const __grid_constant__ CUtensorMap map_v,
                      const __grid_constant__ BwdParams p) {
   using C = Bwd<kD>;
-  constexpr int kStages = C::kStages;
   constexpr uint32_t kTileBytes = C::kTileBytes;
+  constexpr int kKRing = C::kKRing, kVRing = C::kVRing;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_q = smem;
   uint8_t* s_do = smem + kTileBytes;
-  uint8_t* s_kv = smem + 2 * kTileBytes;  // [kStages] x (K, V)
-  uint64_t* bars =
-      reinterpret_cast<uint64_t*>(smem + (2 + 2 * kStages) * kTileBytes);
+  uint8_t* s_k = smem + 2 * kTileBytes;  // [kKRing]
+  uint8_t* s_v = s_k + kKRing * kTileBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + kVRing * kTileBytes);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kDqNumBars);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int tid = threadIdx.x;
   const int warp = tid / 32;
   const int lane = tid % 32;
-  const int64_t n_items = static_cast<int64_t>(p.entries) * p.kv_heads;
+  const int n_items = p.entries * p.kv_heads;
   if (tid == 0) {
     for (int b = 0; b < kDqNumBars; ++b)
       mbar_init(&bars[b],
-                (b == kDsFull || b == kDsFull + 1 || b == kDqFree) ? 8 : 1);
+                (b == kDpFree || b == kDsFull || b == kDqFree) ? 8 : 1);
     *abort = 0;
     fence_barrier_init();
   }
@@ -240,165 +302,149 @@ __global__ void __launch_bounds__(kThreads, 1)
       prefetch_tensor_map(&map_k);
       prefetch_tensor_map(&map_v);
     }
-    const uint32_t q_bytes = 2u * p.group * p.tokens * kD * 2;
-    int q_loads = 0, kv_loads = 0;
-    bool run = true;
-    for (int t = 0; run; ++t) {
-      const int64_t i = turn(t);
-      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
-      if (i >= n_items) continue;
-      const int h = static_cast<int>(i % p.kv_heads);
-      const QueryItem it =
-          load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads));
-      if (it.blocks == 0) continue;
-      if (q_loads > 0 &&
-          !wait_all(&bars[kQEmpty], (q_loads - 1) & 1, abort, p.status))
-        break;
+    const uint32_t q_bytes = p.group * p.tokens * kD * 2;
+    int q_loads = 0, do_loads = 0, k_loads = 0, v_loads = 0;
+    // Waits for place n of a ring, then loads a tile into it.
+    auto ring_load = [&](int& n, int ring, int full, int empty, uint8_t* base,
+                         const CUtensorMap* map, int h, int row) -> bool {
+      const int slot = n % ring;
+      if (n >= ring && !wait_all(&bars[empty + slot], ((n / ring) - 1) & 1,
+                                 abort, p.status))
+        return false;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&bars[kQFull], q_bytes);
-        load_tile<kD>(s_q, &map_q, &bars[kQFull], h * p.group, it.row);
-        load_tile<kD>(s_do, &map_do, &bars[kQFull], h * p.group, it.row);
+        mbar_arrive_expect_tx(&bars[full + slot], kTileBytes);
+        load_tile<kD>(base + slot * kTileBytes, map, &bars[full + slot], h,
+                      row);
       }
       __syncwarp();
-      ++q_loads;
-      for (int j = 0; j < it.blocks; ++j) {
-        const int stage = kv_loads % kStages;
-        if (kv_loads >= kStages &&
-            !wait_all(&bars[kKvEmpty + stage],
-                      ((kv_loads / kStages) - 1) & 1, abort, p.status)) {
-          run = false;
-          break;
-        }
-        if (lane == 0) {
-          uint8_t* dst = s_kv + stage * 2 * kTileBytes;
-          mbar_arrive_expect_tx(&bars[kKvFull + stage], 2 * kTileBytes);
-          load_tile<kD>(dst, &map_k, &bars[kKvFull + stage], h,
-                        it.k_row + j * kTile);
-          load_tile<kD>(dst + kTileBytes, &map_v, &bars[kKvFull + stage], h,
-                        it.k_row + j * kTile);
-        }
-        __syncwarp();
-        ++kv_loads;
+      ++n;
+      return true;
+    };
+    auto item_load = [&](int& n, int full, int empty, uint8_t* dst,
+                         const CUtensorMap* map, int h, int row) -> bool {
+      if (n > 0 && !wait_all(&bars[empty], (n - 1) & 1, abort, p.status))
+        return false;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bars[full], q_bytes);
+        load_tile<kD>(dst, map, &bars[full], h, row);
+      }
+      __syncwarp();
+      ++n;
+      return true;
+    };
+    QueryStream st{0};
+    bool run = true;
+    while (run && st.next(p, n_items, false)) {
+      for (int j = 0; run && j < st.it.blocks; ++j) {
+        const int row = st.it.k_row + j * kTile;
+        run = ring_load(k_loads, kKRing, kKFull, kKEmpty, s_k, &map_k, st.h,
+                        row);
+        if (run && j == 0)
+          run = item_load(q_loads, kQFull, kQEmpty, s_q, &map_q,
+                          st.h * p.group, st.it.row);
+        if (run)
+          run = ring_load(v_loads, kVRing, kVFull, kVEmpty, s_v, &map_v, st.h,
+                          row);
+        if (run && j == 0)
+          run = item_load(do_loads, kDoFull, kDoEmpty, s_do, &map_do,
+                          st.h * p.group, st.it.row);
       }
     }
     if (lane == 0 && *abort) {
+      // Let the copies in flight land before the CTA retires.
       volatile int never = 0;
       if (q_loads > 0)
         mbar_wait(&bars[kQFull], (q_loads - 1) & 1, &never, nullptr);
-      for (int b = kv_loads - kStages; b < kv_loads; ++b)
-        if (b >= 0)
-          mbar_wait(&bars[kKvFull + b % kStages], (b / kStages) & 1, &never,
+      if (do_loads > 0)
+        mbar_wait(&bars[kDoFull], (do_loads - 1) & 1, &never, nullptr);
+      for (int n = k_loads - kKRing; n < k_loads; ++n)
+        if (n >= 0)
+          mbar_wait(&bars[kKFull + n % kKRing], (n / kKRing) & 1, &never,
+                    nullptr);
+      for (int n = v_loads - kVRing; n < v_loads; ++n)
+        if (n >= 0)
+          mbar_wait(&bars[kVFull + n % kVRing], (n / kVRing) & 1, &never,
                     nullptr);
     }
   } else if (warp == kMma) {
-    // Per block j, halves a (keys 0-63) and b (64-127):
-    //   S_a, dP_a, S_b, dP_b of block 0 of the item, then for each j
-    //   dQ += half a of j; S_a, dP_a of j + 1;
-    //   dQ += half b of j; S_b, dP_b of j + 1.
-    constexpr uint32_t idesc_sd = idesc_bf16(128, 64, false, false);
+    constexpr uint32_t idesc_sd = idesc_bf16(128, 128, false, false);
     constexpr uint32_t idesc_acc = idesc_bf16(128, kD, false, true);
     const uint32_t q_lo = sw128_desc_lo(smem_u32(s_q), 16);
     const uint32_t do_lo = sw128_desc_lo(smem_u32(s_do), 16);
-    const uint32_t kv_lo = sw128_desc_lo(smem_u32(s_kv), 16);
-    const uint32_t kvmn_lo = sw128_desc_lo(smem_u32(s_kv), 16384);
-    const uint32_t t_dq = tmem + 256;
-    auto issue_sd = [&](int stage, int h) {
-      const uint32_t k_lo =
-          kv_lo + stage * 2 * C::kTileUnits + h * (8192 >> 4);
-      const uint32_t v_lo = k_lo + C::kTileUnits;
-      const uint32_t t_s = tmem + h * 128, t_dp = t_s + 64;
-#pragma unroll
-      for (int kk = 0; kk < C::kSteps; ++kk) {
-        const uint32_t off = (kk >> 2) * (16384 >> 4) + (kk & 3) * 2;
-        umma_ss_warp(t_s, q_lo + off, k_lo + off, idesc_sd, kk > 0);
-      }
-#pragma unroll
-      for (int kk = 0; kk < C::kSteps; ++kk) {
-        const uint32_t off = (kk >> 2) * (16384 >> 4) + (kk & 3) * 2;
-        umma_ss_warp(t_dp, do_lo + off, v_lo + off, idesc_sd, kk > 0);
-      }
-      umma_commit_warp(&bars[kSdFull + h]);
+    const uint32_t k_lo = sw128_desc_lo(smem_u32(s_k), 16);
+    const uint32_t v_lo = sw128_desc_lo(smem_u32(s_v), 16);
+    const uint32_t kmn_lo = sw128_desc_lo(smem_u32(s_k), 16384);
+    bool ok = true;
+    auto wait = [&](int bar, int phase) -> bool {
+      if (ok && !wait_all(&bars[bar], phase & 1, abort, p.status)) ok = false;
+      return ok;
     };
-    // dQ += dS K over half h's 64 keys (dS of keys 16kk' .. lies in columns
-    // 32(kk'/2) + 8(kk'%2) of the half's S).
-    auto issue_dq = [&](int stage, int h, bool first) {
-      const uint32_t kmn = kvmn_lo + stage * 2 * C::kTileUnits;
-      const uint32_t t_a = tmem + h * 128;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        umma_ts_warp(t_dq, t_a + (kk >> 1) * 32 + (kk & 1) * 8,
-                     kmn + (4 * h + kk) * 128, idesc_acc,
-                     (kk > 0 || h > 0 || !first) ? 1u : 0u);
+    // S of the block at `c` (waits for its Q and K).
+    auto issue_s = [&](const BlockCursor& c) {
+      const int slot = c.b % kKRing;
+      if (c.first()) wait(kQFull, c.items);
+      if (!wait(kKFull + slot, c.b / kKRing)) return;
+      // Key rows behind the sequence are the depth of dQ's product.
+      const int rows = c.st.it.keys - c.j * kTile;
+      if (rows < kTile) clear_rows<kD>(s_k + slot * kTileBytes, rows, lane);
+      tc_fence_after();
+      const uint32_t bk = k_lo + slot * C::kTileUnits;
+      umma_ss_run<C::kSteps>(tmem + (c.b & 1) * 128, q_lo, bk, idesc_sd);
+      umma_commit_warp(&bars[kSFull + (c.b & 1)]);
+      if (c.last()) umma_commit_warp(&bars[kQEmpty]);
     };
-    int blk = 0, items = 0;
-    bool run = true;
-    for (int t = 0; run; ++t) {
-      const int64_t i = turn(t);
-      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
-      if (i >= n_items) continue;
-      const QueryItem it =
-          load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads));
-      const int n = it.blocks;
-      if (n == 0) continue;
-      // K and V of block j of the item have landed, and the key rows behind
-      // the sequence are clear (they are the depth of dQ's product).
-      auto block_ready = [&](int j) -> bool {
-        const int b = blk + j;
-        if (!wait_all(&bars[kKvFull + b % kStages], (b / kStages) & 1, abort,
-                      p.status))
-          return false;
-        if (it.keys - j * kTile < kTile)
-          clear_rows<kD>(s_kv + (b % kStages) * 2 * kTileBytes,
-                         it.keys - j * kTile, lane);
-        tc_fence_after();
-        return true;
-      };
-      if (!wait_all(&bars[kQFull], items & 1, abort, p.status) ||
-          !block_ready(0))
-        break;
-      issue_sd(blk % kStages, 0);
-      issue_sd(blk % kStages, 1);
-      if (n == 1) umma_commit_warp(&bars[kQEmpty]);
-      for (int j = 0; j < n; ++j) {
-        const int b = blk + j;
-        const int stage = b % kStages;
-        const int next = (b + 1) % kStages;
-        const bool first = j == 0, last = j == n - 1;
-        // The item's first dQ overwrites dQ: the epilogue must have read it.
-        if (first && items > 0 &&
-            !wait_all(&bars[kDqFree], (items - 1) & 1, abort, p.status)) {
-          run = false;
-          break;
-        }
-        if (!wait_all(&bars[kDsFull + 0], b & 1, abort, p.status)) {
-          run = false;
-          break;
-        }
-        tc_fence_after();
-        issue_dq(stage, 0, first);
-        if (!last) {
-          if (!block_ready(j + 1)) {
-            run = false;
-            break;
-          }
-          issue_sd(next, 0);
-        }
-        if (!wait_all(&bars[kDsFull + 1], b & 1, abort, p.status)) {
-          run = false;
-          break;
-        }
-        tc_fence_after();
-        issue_dq(stage, 1, first);
-        umma_commit_warp(&bars[kKvEmpty + stage]);
-        if (!last) {
-          issue_sd(next, 1);
-          if (j + 1 == n - 1) umma_commit_warp(&bars[kQEmpty]);
-        } else {
-          umma_commit_warp(&bars[kDqDone]);
-        }
+    auto issue_dp = [&](const BlockCursor& c) {
+      const int slot = c.b % kVRing;
+      if (c.first()) wait(kDoFull, c.items);
+      if (!wait(kVFull + slot, c.b / kVRing)) return;
+      tc_fence_after();
+      const uint32_t bv = v_lo + slot * C::kTileUnits;
+      umma_ss_run<C::kSteps>(tmem + 256, do_lo, bv, idesc_sd);
+      umma_commit_warp(&bars[kDpFull]);
+      umma_commit_warp(&bars[kVEmpty + slot]);
+      if (c.last()) umma_commit_warp(&bars[kDoEmpty]);
+    };
+    // Three places in the stream: dQ of block b, dP of b + 1, S of b + 2.
+    BlockCursor at, at_dp, at_s;
+    at.init(p, n_items);
+    at_dp = at_s = at;
+    if (at_s.valid) {
+      issue_s(at_s);
+      at_s.next(p, n_items);
+    }
+    if (ok && at_dp.valid) {
+      issue_dp(at_dp);
+      at_dp.next(p, n_items);
+    }
+    if (ok && at_s.valid) {
+      issue_s(at_s);
+      at_s.next(p, n_items);
+    }
+    while (ok && at.valid) {
+      if (!wait(kDpFree, at.b)) break;
+      tc_fence_after();
+      if (at_dp.valid) {
+        issue_dp(at_dp);
+        if (!ok) break;
+        at_dp.next(p, n_items);
       }
-      blk += n;
-      ++items;
+      // The item's first dQ overwrites dQ: the epilogue must have read it.
+      if (at.first() && at.items > 0 && !wait(kDqFree, at.items - 1)) break;
+      if (!wait(kDsFull, at.b)) break;
+      tc_fence_after();
+      const int slot = at.b % kKRing;
+      const uint32_t bk = kmn_lo + slot * C::kTileUnits;
+      const uint32_t ds = tmem + (at.b & 1) * 128;
+      umma_ts_run<false>(tmem + 384, ds, bk, idesc_acc, !at.first());
+      umma_ts_run<false>(tmem + 384, ds + 64, bk + 512, idesc_acc, 1);
+      umma_commit_warp(&bars[kKEmpty + slot]);
+      if (at.last()) umma_commit_warp(&bars[kDqDone]);
+      if (at_s.valid) {
+        issue_s(at_s);
+        if (!ok) break;
+        at_s.next(p, n_items);
+      }
+      at.next(p, n_items);
     }
     if (*abort) {
       volatile int never = 0;
@@ -407,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------- compute warps 0-7 ----------------
-    const int wq = warp / 4;  // keys 32 wq .. 32 wq + 31 of each half
+    const int half = warp / 4;  // keys 64 half .. of each block
     const int quarter = warp % 4;
     const int row = quarter * 32 + lane;
     const int token = row / p.group;
@@ -416,46 +462,48 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     int blk = 0, items = 0;
     bool ok = true;
-    for (int t = 0; ok; ++t) {
-      const int64_t i = turn(t);
-      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
-      if (i >= n_items) continue;
-      const int h = static_cast<int>(i % p.kv_heads);
-      const QueryItem it =
-          load_item<QueryItem>(p.table, static_cast<int>(i / p.kv_heads));
-      const int n = it.blocks;
-      const bool write = row_used && token < it.tokens;
+    QueryStream st{0};
+    while (ok && st.next(p, n_items, true)) {
+      const int n = st.it.blocks;
+      const bool write = row_used && token < st.it.tokens;
       __nv_bfloat16* dst =
-          p.grad + (static_cast<int64_t>(it.row) + token) * p.grad_st +
-          (static_cast<int64_t>(h) * p.group + head) * p.grad_sh +
-          wq * (kD / 2);
+          p.grad + (static_cast<int64_t>(st.it.row) + token) * p.grad_st +
+          (static_cast<int64_t>(st.h) * p.group + head) * p.grad_sh +
+          half * (kD / 2);
       if (n == 0) {
         uint32_t z[kD / 4] = {0};
         if (write) store_row<kD / 2>(dst, z);
         continue;
       }
       const int64_t at =
-          (static_cast<int64_t>(h) * p.n_tiles + it.tile) * kTile + row;
+          (static_cast<int64_t>(st.h) * p.n_tiles + st.it.tile) * kTile + row;
       const float l2 = p.lse2[at];
       const float dlt = p.delta[at];
-      const int seen = max(0, min(it.keys, it.kpos + token + 1));
-      for (int j = 0; j < n && ok; ++j, ++blk) {
-        const int visible = seen - j * kTile;
-        const bool masked = __any_sync(0xffffffffu, visible < kTile);
+      const int seen = max(0, min(st.it.keys, st.it.kpos + token + 1));
+      for (int j = 0; j < n; ++j, ++blk) {
+        const int visible = seen - j * kTile - half * 64;
+        const bool masked = __any_sync(0xffffffffu, visible < 64);
+        const uint32_t t_s = tmem + (blk & 1) * 128 + half * 64 + lane_base;
+        const uint32_t t_dp = tmem + 256 + half * 64 + lane_base;
+        if (!wait_all(&bars[kSFull + (blk & 1)], (blk >> 1) & 1, abort,
+                      p.status) ||
+            !wait_all(&bars[kDpFull], blk & 1, abort, p.status)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t dp[2][32], s[32], w[2][16];
+        tmem_ld32(t_dp, dp[0]);
+        tmem_ld32(t_dp + 32, dp[1]);
+        tmem_ld32(t_s, s);
+        tmem_wait_ld();
+        arrive_warp(&bars[kDpFree]);
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          if (!wait_all(&bars[kSdFull + hh], blk & 1, abort, p.status)) {
-            ok = false;
-            break;
+        for (int q = 0; q < 2; ++q) {
+          if (q == 1) {
+            tmem_ld32(t_s + 32, s);
+            tmem_wait_ld();
           }
-          tc_fence_after();
-          const int key0 = hh * 64 + wq * 32;  // key column of the block
-          const uint32_t t_s = tmem + hh * 128 + wq * 32 + lane_base;
-          uint32_t s[32], dp[32];
-          tmem_ld32(t_s, s);
-          tmem_ld32(t_s + 64, dp);
-          tmem_wait_ld();
-          uint32_t w[16];
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             float d2[2];
@@ -464,24 +512,25 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int cc = 2 * c + e;
               const float pr = ex2_approx(
                   fmaf(__uint_as_float(s[cc]), p.scale_log2, -l2));
-              d2[e] = pr * (__uint_as_float(dp[cc]) - dlt);
-              if (masked && key0 + cc >= visible) d2[e] = 0.f;
+              d2[e] = pr * (__uint_as_float(dp[q][cc]) - dlt);
+              if (masked && q * 32 + cc >= visible) d2[e] = 0.f;
             }
-            w[c] = pack_bf16(d2[0], d2[1]);
+            w[q][c] = pack_bf16(d2[0], d2[1]);
           }
-          // dS of these 32 keys over the first 16 of this warp's own 32
-          // columns of S.
-          tmem_st16(t_s, w);
-          tmem_wait_st();
-          arrive_warp(&bars[kDsFull + hh]);
         }
+        // dS of these 64 keys over the first 32 of this warp's own 64 columns
+        // of S (all of them are in registers).
+        tmem_st16(t_s, w[0]);
+        tmem_st16(t_s + 16, w[1]);
+        tmem_wait_st();
+        arrive_warp(&bars[kDsFull]);
       }
       if (!ok) break;
       if (!wait_all(&bars[kDqDone], items & 1, abort, p.status)) break;
       ++items;
       tc_fence_after();
       uint32_t w[kD / 4];
-      tmem_row_bf16<kD / 2>(tmem + 256 + wq * (kD / 2) + lane_base, p.scale,
+      tmem_row_bf16<kD / 2>(tmem + 384 + half * (kD / 2) + lane_base, p.scale,
                             w);
       arrive_warp(&bars[kDqFree]);
       if (write) store_row<kD / 2>(dst, w);
@@ -643,16 +692,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           qd_lo + stage * 2 * C::kTileUnits + h * (8192 >> 4);
       const uint32_t do_lo = q_lo + C::kTileUnits;
       const uint32_t t_s = tmem + h * 128, t_dp = t_s + 64;
-#pragma unroll
-      for (int kk = 0; kk < C::kSteps; ++kk) {
-        const uint32_t off = (kk >> 2) * (16384 >> 4) + (kk & 3) * 2;
-        umma_ss_warp(t_s, k_lo + off, q_lo + off, idesc_st, kk > 0);
-      }
-#pragma unroll
-      for (int kk = 0; kk < C::kSteps; ++kk) {
-        const uint32_t off = (kk >> 2) * (16384 >> 4) + (kk & 3) * 2;
-        umma_ss_warp(t_dp, v_lo + off, do_lo + off, idesc_st, kk > 0);
-      }
+      umma_ss_run<C::kSteps>(t_s, k_lo, q_lo, idesc_st);
+      umma_ss_run<C::kSteps>(t_dp, v_lo, do_lo, idesc_st);
       umma_commit_warp(&bars[kStFull + h]);
     };
     // dV += P^T dO and dK += dS^T Q over half h's 64 query rows.
@@ -660,16 +701,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t qmn = qdmn_lo + stage * 2 * C::kTileUnits;
       const uint32_t domn = qmn + C::kTileUnits;
       const uint32_t t_p = tmem + h * 128, t_ds = t_p + 64;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        umma_ts_warp(t_dv, t_p + (kk >> 1) * 32 + (kk & 1) * 8,
-                     domn + (4 * h + kk) * 128, idesc_acc,
-                     (kk > 0 || h > 0 || !first) ? 1u : 0u);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        umma_ts_warp(t_dk, t_ds + (kk >> 1) * 32 + (kk & 1) * 8,
-                     qmn + (4 * h + kk) * 128, idesc_acc,
-                     (kk > 0 || h > 0 || !first) ? 1u : 0u);
+      const uint32_t more = (h > 0 || !first) ? 1u : 0u;
+      umma_ts_run<true>(t_dv, t_p, domn + h * 512, idesc_acc, more);
+      umma_ts_run<true>(t_dk, t_ds, qmn + h * 512, idesc_acc, more);
     };
     int blk = 0, items = 0;
     bool run = true;
@@ -895,10 +929,10 @@ int launch(const Maps& m, const BwdParams& pq, const BwdParams& pk,
   if (want_q && q_items > 0) {
     static std::atomic<uint64_t> allowed{0};
     rc = allow_smem(reinterpret_cast<const void*>(causal_dq_kernel<kD>),
-                    C::kSmem, &allowed);
+                    C::kDqSmem, &allowed);
     if (rc != VEDA_OK) return rc;
     const int grid = static_cast<int>(q_items < sms ? q_items : sms);
-    causal_dq_kernel<kD><<<grid, kThreads, C::kSmem, stream>>>(
+    causal_dq_kernel<kD><<<grid, kThreads, C::kDqSmem, stream>>>(
         m.q, m.dout, m.k, m.v, pq);
     rc = check_launch("causal_dq_kernel");
     if (rc != VEDA_OK) return rc;

@@ -299,12 +299,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       auto issue_qk = [&](int b, int g, bool last) {
         const uint32_t a = q_lo + g * kTileUnits;
         const uint32_t bk = k_lo + ((2 * b) % kRing) * kTileUnits;
-#pragma unroll
-        for (int kk = 0; kk < C::kSteps; ++kk) {
-          const uint32_t off = (kk >> 2) * (16384 >> 4) + (kk & 3) * 2;
-          umma_ss_warp(tmem + g * 128, a + off, bk + off, idesc_qk,
-                       kk > 0 ? 1u : 0u);
-        }
+        umma_ss_run<C::kSteps>(tmem + g * 128, a, bk, idesc_qk);
         umma_commit_warp(&bars[kSFull + g]);
         if (last) umma_commit_warp(&bars[kQEmpty + g]);
         if (g == 1) umma_commit_warp(&bars[kEmpty + (2 * b) % kRing]);
@@ -348,20 +343,15 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
               break;
             }
             tc_fence_after();
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_ts_warp(tmem + 256 + g * 128, tmem + g * 128 + kk * 8,
-                           bv + kk * 128, idesc_pv,
-                           (kk > 0 || j > 0) ? 1u : 0u);
+            umma_ts_run<false>(tmem + 256 + g * 128, tmem + g * 128, bv,
+                               idesc_pv, j > 0);
             if (!wait_all(&bars[kPHalfB + g], b & 1, abort, p.status)) {
               ok = false;
               break;
             }
             tc_fence_after();
-#pragma unroll
-            for (int kk = 4; kk < 8; ++kk)
-              umma_ts_warp(tmem + 256 + g * 128, tmem + g * 128 + kk * 8,
-                           bv + kk * 128, idesc_pv, 1u);
+            umma_ts_run<false>(tmem + 256 + g * 128, tmem + g * 128 + 32,
+                               bv + 512, idesc_pv, 1);
             if (last) umma_commit_warp(&bars[kODone + g]);
             if (ahead) {
               if ((g == 0 && !landed(2 * b + 2)) ||
