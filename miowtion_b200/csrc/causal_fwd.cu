@@ -6,8 +6,10 @@
 //
 // A persistent kernel, one CTA per SM, on tcgen05. A CTA holds two query
 // tiles A and B of one key head (causal.cuh: 128 rows of tokens x heads) and
-// streams the key and value tiles of 128 keys once for both. Tensor memory:
-//     S_A [0,128)  S_B [128,256)  O_A [256,384)  O_B [384,512) columns
+// streams the key and value tiles of 128 keys once for both. Tensor memory
+// (512 columns) holds an accumulator O for each tile and two (D = 128) or three
+// (D = 64) buffers of 128 columns for scores, taken in turn by A(0), B(0), A(1),
+// B(1), ...
 //   warps 0-7   softmax and epilogue: warps 4g .. 4g + 3 own tile g, a query
 //               row a thread over all 128 keys, with the running maximum and
 //               sum of an online softmax (the maximum moves only when it
@@ -16,7 +18,12 @@
 //   warp 8      TMA producer: the two Q tiles of an item, then its K and V
 //               tiles through one ring.
 //   warp 9      issues every product (and owns the tensor memory), in one
-//               order: PV_A(b), QK_A(b + 1), PV_B(b), QK_B(b + 1).
+//               order: PV_A(b), QK_A(b + 1), PV_B(b), QK_B(b + 1) with two
+//               buffers (the scores take the place of the weights that the
+//               product before them read); with three, QK_B(b + 1) follows
+//               PV_A(b) and QK_A(b + 2) follows PV_B(b), so that a tile's next
+//               scores wait for nothing of its own (644 -> 711 TFLOP/s on
+//               16,384 tokens, 24/6 heads).
 //   warps 10-11 idle; they complete the third warpgroup, whose registers go
 //               to the softmax warps (setmaxnreg).
 // The tensor core works on one tile while the softmax of the other runs: in
@@ -30,10 +37,10 @@
 // quarter, half of the exponentials on the FMA pipes, 1,210 and 1,117 against
 // 1,247 without.) The blocks of
 // consecutive items form one stream, so the next item's first scores are
-// computed while this item's epilogue runs. One issuer also makes most
-// barriers superfluous: when the scores of block b arrive, everything issued
-// before them has finished, the product of block b - 1 among it; and the warps
-// that write P of an item's first block have read the previous item's O.
+// computed while this item's epilogue runs. One issuer also makes barriers
+// superfluous: the warps that write P of an item's first block have read the
+// previous item's O, and with two buffers the scores of block b arrive after
+// the product of block b - 1.
 // Rows past a sequence's end belong to the next sequence (or to nothing):
 // their scores are set to -inf by selection and the value rows are cleared in
 // shared memory, so what stands there, NaN included, reaches no row of this
@@ -57,6 +64,12 @@ template <int kD>
 struct Fwd {
   static constexpr uint32_t kTileBytes = kTile * kD * 2;
   static constexpr int kRing = kD == 128 ? 4 : 8;
+  // S buffers, taken in turn by A(0), B(0), A(1), B(1), ..., and the columns of
+  // O_A and O_B behind them.
+  static constexpr int kSBufs = kD == 128 ? 2 : 3;
+  static constexpr uint32_t kO = kSBufs * 128;
+  // With three the scores run a block ahead: V behind the next block's K.
+  static constexpr bool kAhead = kSBufs == 3;
   // Q tiles, ring, then 4 KB a softmax warp to stage its output in.
   static constexpr int kSmem = (2 + kRing) * kTileBytes + 8 * 4096 + 512 + 1024;
   static constexpr int kSteps = kD / 16;  // K-steps of Q K^T
@@ -65,11 +78,12 @@ struct Fwd {
 enum Bar {
   kQFull = 0,             // [2] Q of the tile landed
   kQEmpty = kQFull + 2,   // [2] the tile's last S product finished
-  kSFull = kQEmpty + 2,   // [2] S of the tile's block finished
-  kPHalfA = kSFull + 2,   // [2] P of keys 0-63 written (4 warps)
+  kSFull = kQEmpty + 2,   // [kSBufs] the scores in the buffer are finished
+  kPHalfA = kSFull + 3,   // [2] P of keys 0-63 written (4 warps)
   kPHalfB = kPHalfA + 2,  // [2] P of keys 64-127 written (4 warps)
   kODone = kPHalfB + 2,   // [2] the tile's last product of the item finished
-  kDrain = kODone + 2,
+  kPvDone = kODone + 2,   // [2] the tile's product of the block (3 buffers)
+  kDrain = kPvDone + 2,
   kFull,                  // [kRing]
   kEmpty = kFull + 8,     // [kRing]
   kNumBars = kEmpty + 8
@@ -164,6 +178,29 @@ struct Stream {
   }
 };
 
+// A place in the stream of blocks of a CTA's items: block j of the current
+// item, block b of the stream.
+struct Cursor {
+  Stream st;
+  int b, j, items;
+  bool valid;
+  __device__ __forceinline__ void init(const FwdParams& p, int64_t n_items) {
+    st.t = 0;
+    b = j = items = 0;
+    valid = st.next(p, n_items, false);
+  }
+  __device__ __forceinline__ bool last() const {
+    return j == st.it.blocks - 1;
+  }
+  __device__ __forceinline__ void next(const FwdParams& p, int64_t n_items) {
+    ++b;
+    if (++j < st.it.blocks) return;
+    j = 0;
+    ++items;
+    valid = st.next(p, n_items, false);
+  }
+};
+
 template <int kD>
 __global__ void __launch_bounds__(32 * kWarps, 1)
     causal_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
@@ -220,7 +257,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         prefetch_tensor_map(&map_v);
       }
       const uint32_t q_bytes = p.group * p.tokens * kD * 2;  // of a tile
-      int n_ring = 0, q_loads = 0;
+      int n_ring = 0;
       int q_issued[2] = {0, 0};
       bool run = true;
       // One K or V tile (rows k_row ..) into the ring's next place.
@@ -242,34 +279,43 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         ++n_ring;
         return true;
       };
-      Stream st{0};
-      while (run && st.next(p, n_items, false)) {
-        for (int j = 0; run && j < st.it.blocks; ++j) {
-          const int k_row = st.it.k_row + (st.it.first + j) * kTile;
-          run = load(&map_k, st.h, k_row);
-          // Q behind the first K tile: it has to wait for the last scores of
-          // the item before.
-          for (int g = 0; run && j == 0 && g < 2; ++g) {
-            if (q_loads > 0 && !wait_all(&bars[kQEmpty + g],
-                                         (q_loads - 1) & 1, abort, p.status)) {
-              run = false;
-              break;
-            }
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&bars[kQFull + g], q_bytes);
-#pragma unroll
-              for (int c = 0; c < kD / 64; ++c)
-                tma_load_3d(s_q + g * kTileBytes + c * 16384, &map_q,
-                            &bars[kQFull + g], c * 64, st.h * p.group,
-                            st.it.row + g * p.tokens);
-              q_issued[g] = q_loads + 1;
-            }
-            __syncwarp();
+      // K0, V0, K1, V1, ..., or K0, K1, V0, K2, V1, ... (kAhead).
+      Cursor c;
+      c.init(p, n_items);
+      [[maybe_unused]] int v_row = 0, v_head = 0;
+      while (run && c.valid) {
+        const int row = c.st.it.k_row + (c.st.it.first + c.j) * kTile;
+        const int h = c.st.h;
+        run = load(&map_k, h, row);
+        // Q behind the item's first K tile: it has to wait for the last scores
+        // of the item before.
+        for (int g = 0; run && c.j == 0 && g < 2; ++g) {
+          if (c.items > 0 && !wait_all(&bars[kQEmpty + g], (c.items - 1) & 1,
+                                       abort, p.status)) {
+            run = false;
+            break;
           }
-          if (run) run = load(&map_v, st.h, k_row);
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bars[kQFull + g], q_bytes);
+#pragma unroll
+            for (int x = 0; x < kD / 64; ++x)
+              tma_load_3d(s_q + g * kTileBytes + x * 16384, &map_q,
+                          &bars[kQFull + g], x * 64, h * p.group,
+                          c.st.it.row + g * p.tokens);
+            q_issued[g] = c.items + 1;
+          }
+          __syncwarp();
         }
-        ++q_loads;
+        if constexpr (C::kAhead) {
+          if (run && c.b > 0) run = load(&map_v, v_head, v_row);
+          v_row = row;
+          v_head = h;
+        } else {
+          if (run) run = load(&map_v, h, row);
+        }
+        c.next(p, n_items);
       }
+      if (C::kAhead && run && c.b > 0) run = load(&map_v, v_head, v_row);
       if (lane == 0 && *abort) {
         // Let the copies in flight land before the CTA retires.
         volatile int never = 0;
@@ -289,85 +335,155 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       const uint32_t q_lo = sw128_desc_lo(smem_u32(s_q), 16);
       const uint32_t k_lo = sw128_desc_lo(smem_u32(s_ring), 16);
       const uint32_t v_lo = sw128_desc_lo(smem_u32(s_ring), 16384);
-      // Block b of the stream has its K tile at place 2b of the ring's
-      // sequence and its V tile at 2b + 1.
+      // K of block b lies at place 2b of the ring's sequence and V at 2b + 1;
+      // with kAhead K at 2b - 1 (0 of the first) and V at 2b + 2 (2b + 1 of
+      // the last).
       auto landed = [&](int place) -> bool {
         return wait_all(&bars[kFull + place % kRing], (place / kRing) & 1,
                         abort, p.status);
       };
-      // (last: the item's last block.)
-      auto issue_qk = [&](int b, int g, bool last) {
-        const uint32_t a = q_lo + g * kTileUnits;
-        const uint32_t bk = k_lo + ((2 * b) % kRing) * kTileUnits;
-        umma_ss_run<C::kSteps>(tmem + g * 128, a, bk, idesc_qk);
-        umma_commit_warp(&bars[kSFull + g]);
-        if (last) umma_commit_warp(&bars[kQEmpty + g]);
-        if (g == 1) umma_commit_warp(&bars[kEmpty + (2 * b) % kRing]);
-      };
-      Stream st{0};
-      bool more = st.next(p, n_items, false);
       bool ok = true;
-      int b = 0, items = 0;
-      if (more) {
-        ok = landed(0);
-        for (int g = 0; ok && g < 2; ++g) {
-          ok = wait_all(&bars[kQFull + g], 0, abort, p.status);
-          if (ok) {
-            tc_fence_after();
-            issue_qk(0, g, st.it.blocks == 1);
+      if constexpr (C::kAhead) {
+        // Scores of tile `qg` of the block at `qk`, then on to the next.
+        Cursor pv;
+        pv.init(p, n_items);
+        Cursor qk = pv;
+        int qg = 0;
+        auto issue_qk = [&]() {
+          if (!ok || !qk.valid) return;
+          const int place =
+              2 * qk.b - (qk.b > 0 ? 1 : 0);
+          if (qg == 0) ok = landed(place);
+          if (ok && qk.j == 0)
+            ok = wait_all(&bars[kQFull + qg], qk.items & 1, abort, p.status);
+          if (!ok) return;
+          tc_fence_after();
+          const int buf = (2 * qk.b + qg) % C::kSBufs;
+          umma_ss_run<C::kSteps>(tmem + buf * 128, q_lo + qg * kTileUnits,
+                                 k_lo + (place % kRing) * kTileUnits, idesc_qk);
+          umma_commit_warp(&bars[kSFull + buf]);
+          if (qk.last()) umma_commit_warp(&bars[kQEmpty + qg]);
+          if (qg == 1) {
+            umma_commit_warp(&bars[kEmpty + place % kRing]);
+            qk.next(p, n_items);
           }
-        }
-      }
-      while (ok && more) {
-        const int n = st.it.blocks;
-        const int keys = st.it.keys - st.it.first * kTile;
-        more = st.next(p, n_items, false);
-        for (int j = 0; j < n; ++j, ++b) {
-          const bool last = j == n - 1;
-          const bool ahead = !last || more;
-          const int slot = (2 * b + 1) % kRing;
-          if (!landed(2 * b + 1)) {
+          qg ^= 1;
+        };
+#pragma unroll
+        for (int i = 0; i < C::kSBufs; ++i) issue_qk();
+        while (ok && pv.valid) {
+          // (The scores are ahead of the products: is this the last block?)
+          const bool end = !qk.valid && qk.b == pv.b + 1;
+          const int place = 2 * pv.b + (end ? 1 : 2);
+          const int slot = place % kRing;
+          if (!landed(place)) {
             ok = false;
             break;
           }
           // Rows behind the sequence's last key take no part: a weight of 0
           // would not keep a NaN out.
-          const int rows = keys - j * kTile;
+          const int rows = pv.st.it.keys - (pv.st.it.first + pv.j) * kTile;
           if (rows < kTile)
             clear_rows<kD>(s_ring + slot * kTileBytes, rows, lane);
           const uint32_t bv = v_lo + slot * kTileUnits;
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
-            if (!wait_all(&bars[kPHalfA + g], b & 1, abort, p.status)) {
+            const uint32_t t_p = tmem + (2 * pv.b + g) % C::kSBufs * 128;
+            const uint32_t t_o = tmem + C::kO + g * kD;
+            if (!wait_all(&bars[kPHalfA + g], pv.b & 1, abort, p.status)) {
               ok = false;
               break;
             }
             tc_fence_after();
-            umma_ts_run<false>(tmem + 256 + g * 128, tmem + g * 128, bv,
-                               idesc_pv, j > 0);
-            if (!wait_all(&bars[kPHalfB + g], b & 1, abort, p.status)) {
+            umma_ts_run<false>(t_o, t_p, bv, idesc_pv, pv.j > 0);
+            if (!wait_all(&bars[kPHalfB + g], pv.b & 1, abort, p.status)) {
               ok = false;
               break;
             }
             tc_fence_after();
-            umma_ts_run<false>(tmem + 256 + g * 128, tmem + g * 128 + 32,
-                               bv + 512, idesc_pv, 1);
-            if (last) umma_commit_warp(&bars[kODone + g]);
-            if (ahead) {
-              if ((g == 0 && !landed(2 * b + 2)) ||
-                  (last && !wait_all(&bars[kQFull + g], (items + 1) & 1,
-                                     abort, p.status))) {
+            umma_ts_run<false>(t_o, t_p + 32, bv + 512, idesc_pv, 1);
+            if (pv.last()) umma_commit_warp(&bars[kODone + g]);
+            umma_commit_warp(&bars[kPvDone + g]);
+            issue_qk();
+          }
+          if (!ok) break;
+          umma_commit_warp(&bars[kEmpty + slot]);
+          pv.next(p, n_items);
+        }
+      } else {
+        // (last: the item's last block.)
+        auto issue_qk = [&](int b, int g, bool last) {
+          const uint32_t a = q_lo + g * kTileUnits;
+          const uint32_t bk = k_lo + ((2 * b) % kRing) * kTileUnits;
+          umma_ss_run<C::kSteps>(tmem + g * 128, a, bk, idesc_qk);
+          umma_commit_warp(&bars[kSFull + g]);
+          if (last) umma_commit_warp(&bars[kQEmpty + g]);
+          if (g == 1) umma_commit_warp(&bars[kEmpty + (2 * b) % kRing]);
+        };
+        Stream st{0};
+        bool more = st.next(p, n_items, false);
+        int b = 0, items = 0;
+        if (more) {
+          ok = landed(0);
+          for (int g = 0; ok && g < 2; ++g) {
+            ok = wait_all(&bars[kQFull + g], 0, abort, p.status);
+            if (ok) {
+              tc_fence_after();
+              issue_qk(0, g, st.it.blocks == 1);
+            }
+          }
+        }
+        while (ok && more) {
+          const int n = st.it.blocks;
+          const int keys = st.it.keys - st.it.first * kTile;
+          more = st.next(p, n_items, false);
+          for (int j = 0; j < n; ++j, ++b) {
+            const bool last = j == n - 1;
+            const bool ahead = !last || more;
+            const int slot = (2 * b + 1) % kRing;
+            if (!landed(2 * b + 1)) {
+              ok = false;
+              break;
+            }
+            // Rows behind the sequence's last key take no part: a weight of 0
+            // would not keep a NaN out.
+            const int rows = keys - j * kTile;
+            if (rows < kTile)
+              clear_rows<kD>(s_ring + slot * kTileBytes, rows, lane);
+            const uint32_t bv = v_lo + slot * kTileUnits;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              if (!wait_all(&bars[kPHalfA + g], b & 1, abort, p.status)) {
                 ok = false;
                 break;
               }
               tc_fence_after();
-              issue_qk(b + 1, g, last ? st.it.blocks == 1 : j + 1 == n - 1);
+              umma_ts_run<false>(tmem + C::kO + g * kD, tmem + g * 128, bv,
+                                 idesc_pv, j > 0);
+              if (!wait_all(&bars[kPHalfB + g], b & 1, abort, p.status)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              umma_ts_run<false>(tmem + C::kO + g * kD, tmem + g * 128 + 32,
+                                 bv + 512, idesc_pv, 1);
+              if (last) umma_commit_warp(&bars[kODone + g]);
+              if (ahead) {
+                if ((g == 0 && !landed(2 * b + 2)) ||
+                    (last && !wait_all(&bars[kQFull + g], (items + 1) & 1,
+                                       abort, p.status))) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
+                issue_qk(b + 1, g, last ? st.it.blocks == 1 : j + 1 == n - 1);
+              }
             }
+            if (!ok) break;
+            umma_commit_warp(&bars[kEmpty + slot]);
           }
-          if (!ok) break;
-          umma_commit_warp(&bars[kEmpty + slot]);
+          ++items;
         }
-        ++items;
       }
       if (*abort) {
         volatile int never = 0;
@@ -385,8 +501,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     const int head = row % p.group;
     const bool row_used = row < p.tokens * p.group;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t t_s = tmem + grp * 128 + lane_base;
-    const uint32_t t_o = tmem + 256 + grp * 128 + lane_base;
+    const uint32_t t_o = tmem + C::kO + grp * kD + lane_base;
     uint8_t* s_stage = smem + (2 + kRing) * kTileBytes + warp * 4096;
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     uint32_t b = 0;
@@ -404,7 +519,11 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       for (int j = 0; j < n; ++j, ++b) {
         const int visible = seen - j * kTile;
         const bool masked = __any_sync(0xffffffffu, visible < kTile);
-        if (!wait_all(&bars[kSFull + grp], b & 1, abort, p.status)) {
+        const uint32_t turn_s = 2 * b + grp;  // of the S buffers
+        const uint32_t t_s =
+            tmem + turn_s % C::kSBufs * 128 + lane_base;
+        if (!wait_all(&bars[kSFull + turn_s % C::kSBufs],
+                      (turn_s / C::kSBufs) & 1, abort, p.status)) {
           ok = false;
           break;
         }
@@ -438,8 +557,16 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
           const float alpha =
               m_ref == -INFINITY ? 0.f : ex2_approx(m_ref - m_new);
           m_ref = m_new;
-          // The previous blocks' products are in O (they were issued before
-          // this block's scores); this block's waits for P.
+          // The previous blocks' products are in O: with two buffers they
+          // were issued before this block's scores. This block's waits for P.
+          if constexpr (C::kSBufs == 3) {
+            if (!wait_all(&bars[kPvDone + grp], (b - 1) & 1, abort,
+                          p.status)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+          }
 #pragma unroll 1
           for (int q16 = 0; q16 < kD / 16; ++q16)
             rescale16(t_o + q16 * 16, alpha);

@@ -585,25 +585,26 @@ def causal_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 class _CausalAttention(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, q, k, v, pack, scale):
+    def forward(ctx, q, k, v, pack, scale, return_lse):
         out, lse = causal_attention_fwd(q, k, v, pack, scale)
         ctx.save_for_backward(q, k, v, out, lse)
         ctx.pack, ctx.scale = pack, scale
+        if not return_lse:
+            return out
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, dout, _dlse):
+    def backward(ctx, dout, *_):
         if dout is None:
-            return None, None, None, None, None
+            return None, None, None, None, None, None
         q, k, v, out, lse = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dq, dk, dv = causal_attention_bwd(q, k, v, out, dout, lse, ctx.pack,
-                                          ctx.scale, need[0],
-                                          need[1] or need[2])
-        return dq, dk, dv, None, None
+        return (*causal_attention_bwd(q, k, v, out, dout, lse, ctx.pack,
+                                      ctx.scale, need[0], need[1] or need[2]),
+                None, None, None)
 
 
 def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -634,7 +635,6 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     scale = softmax_scale(scale, q.shape[-1])
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
                                     or v.requires_grad):
-        out, lse = _CausalAttention.apply(q, k, v, pack, scale)
-    else:
-        out, lse = causal_attention_fwd(q, k, v, pack, scale, return_lse)
+        return _CausalAttention.apply(q, k, v, pack, scale, return_lse)
+    out, lse = causal_attention_fwd(q, k, v, pack, scale, return_lse)
     return (out, lse) if return_lse else out
