@@ -206,11 +206,16 @@ def device_status(reset: bool = True) -> int:
 def raise_on_device_status() -> None:
     """Reads and clears the device status word; raises RuntimeError when a
     kernel's bounded wait expired since the last read (the kernel returned
-    early, so its outputs are not to be trusted)."""
+    early, so its outputs are not to be trusted) or a paged cache was
+    addressed where it has nothing."""
     status = device_status(reset=True)
     if status == VEDA_ERR_TIMEOUT:
         raise RuntimeError('a Veda kernel wait timed out on the device; its '
                            'outputs are incomplete')
+    if status == VEDA_ERR_INVALID:
+        raise RuntimeError('a Veda kernel met a place in a paged cache that '
+                           'does not exist (a page number, position or '
+                           'length out of range) and left it out')
     if status != 0:
         raise RuntimeError(f'device status word holds {status}')
 

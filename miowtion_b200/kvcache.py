@@ -84,13 +84,12 @@ class PagedCache:
                or t.data_ptr() % 16 for t in tensors):
             raise ValueError('pages and scales must be contiguous, 16-byte '
                              'aligned and on one device')
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._tensors = k, v, k_scale, v_scale
         self.n_pages, self.kv_heads, self.page_size, self.head_dim = (
             n_pages, kv_heads, page_size, dim)
         self.device = k.device
         # The C ABI's arguments that describe the pages.
-        self._pages = (k.data_ptr(), v.data_ptr(), _lib.ptr(k_scale),
-                       _lib.ptr(v_scale), n_pages, page_size, kv_heads, dim,
+        self._shape = (n_pages, page_size, kv_heads, dim,
                        STORAGE[self.storage][0])
         self._workspace: int | None = None
 
@@ -111,6 +110,23 @@ class PagedCache:
             return cls(k, v)
         ks, vs = (torch.empty(shape[:3], device=device) for _ in range(2))
         return cls(k, v, ks, vs)
+
+    # The pages are fixed for the life of the cache (their contents are not).
+    @property
+    def k(self) -> torch.Tensor:
+        return self._tensors[0]
+
+    @property
+    def v(self) -> torch.Tensor:
+        return self._tensors[1]
+
+    @property
+    def k_scale(self) -> torch.Tensor | None:
+        return self._tensors[2]
+
+    @property
+    def v_scale(self) -> torch.Tensor | None:
+        return self._tensors[3]
 
     def _index(self, t: torch.Tensor, name: str, n: int) -> int:
         """Address of an int32 [n] argument."""
@@ -140,7 +156,10 @@ class PagedCache:
             pitch = width
         elif pitch < width:
             raise ValueError('the rows of the table must not overlap')
-        return (*self._pages, table.data_ptr(), pitch, width, n)
+        k, v, k_scale, v_scale = self._tensors
+        return (k.data_ptr(), v.data_ptr(), _lib.ptr(k_scale),
+                _lib.ptr(v_scale), *self._shape, table.data_ptr(), pitch,
+                width, n)
 
     def _pack(self, pack: sequences.SequencePack) -> None:
         if pack.device != self.device:

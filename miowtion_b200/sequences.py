@@ -51,6 +51,9 @@ class SequencePack:
     tokens of its keys: query i sees keys j <= i + k_length - q_length. With
     fewer keys than queries the first rows see none. Any length may be zero.
 
+    A captured CUDA graph reads the pack's tensors: keep the pack for as long
+    as the graph is replayed.
+
     Args:
         q_lengths: Query rows of each sequence (host integers).
         k_lengths: Key rows of each sequence; None for q_lengths.
@@ -153,6 +156,7 @@ def _lengths(values: Sequence[int], name: str) -> np.ndarray:
         raise ValueError(f'{name} must not be negative')
     if (out >= 2 ** 31).any():
         raise ValueError(f'{name} must be below 2^31')
+    out.setflags(write=False)  # offsets and tables are made from them
     return out
 
 

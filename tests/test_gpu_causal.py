@@ -279,7 +279,13 @@ def test_gradients_of_shared_broadcast_and_single_inputs():
     out = kernels.causal_attention(q, k1.expand(130, 2, 64), leaf, pack)
     out.backward(dout)
     assert torch.equal(leaf.grad, full[2])
-    # A gradient without strides of its own (that of a sum).
+    # Gradients without strides of their own (that of a sum; one row's).
+    row = rows(1, 1, 64, 8)
+    leaves = [t.clone().requires_grad_(True) for t in (q, v, v)]
+    got = torch.autograd.grad(kernels.causal_attention(*leaves, pack), leaves,
+                              row.expand(130, 4, 64))
+    want = gradients(pack, q, v, v, row.expand(130, 4, 64).contiguous())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
     leaves = [t.clone().requires_grad_(True) for t in (q, v, v)]
     ones = torch.ones_like(dout)
     got = torch.autograd.grad(kernels.causal_attention(*leaves, pack).sum(),

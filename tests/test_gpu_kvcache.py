@@ -362,6 +362,31 @@ def test_places_that_do_not_exist_are_reported_and_touch_nothing(storage):
         assert _lib.device_status(reset=True) == _lib.VEDA_ERR_INVALID
 
 
+@pytest.mark.parametrize('storage', STORAGES)
+def test_a_wider_table_and_shared_pages(storage):
+    # A slice of a wider table, and two sequences that read one prefix page.
+    contexts, size, dim = [40, 33], 16, 64
+    cache, table, _, k, v = filled(storage, contexts, size, 2, dim, 37)
+    wide = torch.full((2, 9), -1, dtype=torch.int32, device=DEV)
+    wide[:, :3] = table
+    wide[1, 0] = wide[0, 0]
+    k, v = k.clone(), v.clone()
+    for t in (k, v):
+        t[40:56] = t[:16]
+    got, _ = cache.read(wide[:, :3], sequences.SequencePack(contexts,
+                                                            device=DEV))
+    assert torch.equal(got, held(k, storage).bfloat16())
+    q = rows(2, 4, dim, 5)
+    check_attend(cache, wide[:, :3], q, k, v, contexts, storage)
+    check_attend(cache, wide, q, k, v, contexts, storage)
+
+
+def test_many_heads_share_a_key_head():
+    contexts = [70, 9]
+    cache, table, _, k, v = filled('int8', contexts, 16, 1, 128, 41)
+    check_attend(cache, table, rows(2, 130, 128, 6), k, v, contexts, 'int8')
+
+
 def test_no_rows_and_other_streams():
     cache, table, pack, k, v = filled('int8', [30, 5], 16, 2, 64, 29)
     none = sequences.SequencePack([0, 0], device=DEV)

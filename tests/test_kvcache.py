@@ -37,6 +37,8 @@ def test_pack_properties():
     assert p.q_offsets.tolist() == [0, 3, 3, 8]
     assert p.k_offsets.tolist() == [0, 4, 11, 16]
     assert not p.whole and not p.single_tokens
+    with pytest.raises(ValueError):
+        p.q_lengths[0] = 5
     assert pack([1, 1], [5, 1]).single_tokens and pack([2, 0]).whole
 
 
@@ -173,6 +175,12 @@ def test_cache_calls_refuse_wrong_arguments():
         c.read(table[:1], p)
 
 
+def test_the_pages_of_a_cache_are_fixed():
+    c = cache()
+    with pytest.raises(AttributeError):
+        c.k = c.v
+
+
 def test_cache_calls_refuse_to_fall_back():
     c = cache('bf16')
     p = pack([1])
@@ -183,3 +191,25 @@ def test_cache_calls_refuse_to_fall_back():
                  lambda: c.read(table, p), lambda: c.attend(k, table, one)):
         with pytest.raises(NotImplementedError, match='unavailable'):
             call()
+
+
+def test_causal_attention_refuses():
+    from miowtion_b200 import kernels
+    p = pack([3, 2])
+    q = torch.zeros(5, 4, 64, dtype=torch.bfloat16)
+    k = torch.zeros(5, 2, 64, dtype=torch.bfloat16)
+    for args, match in [
+            ((q, k, k[:4], p), 'one shape'), ((q[0], k, k, p), 'rows, heads'),
+            ((q[:, :, :32], k[:, :, :32], k[:, :, :32], p), 'head dim'),
+            ((q, k[:, :, :32], k[:, :, :32], p), 'head dim'),
+            ((q[:, :3], k, k, p), 'key heads'),
+            ((q[:4], k, k, p), 'rows, not'), ((q, k[:4], k[:4], p), 'rows, not'),
+            ((q.half(), k, k, p), 'bf16'), ((q, k, k, p, -1.0), 'scale'),
+            ((q, k, k, p, float('inf')), 'scale')]:
+        with pytest.raises(ValueError, match=match):
+            kernels.causal_attention(*args)
+    wide = torch.zeros(5, 130, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match='1 to 128'):
+        kernels.causal_attention(wide, k[:, :1], k[:, :1], p)
+    with pytest.raises(NotImplementedError, match='unavailable'):
+        kernels.causal_attention(q, k, k, p)
