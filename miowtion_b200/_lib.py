@@ -232,8 +232,11 @@ def call_on(index: int, name: str, *args) -> None:
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
             call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+        return
+    rc = getattr(_LIB or load(), name)(
+        *args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != VEDA_OK:
+        check(rc, name)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

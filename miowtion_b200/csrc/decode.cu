@@ -23,8 +23,10 @@
 // (sequence, head) that lies inside the run is written out; the run's first
 // and last may be parts, which the CTA adds up in shared memory at its end and,
 // where they go on in another CTA, leaves in the workspace for
-// decode_join_kernel. Parts are added in the order of the keys, with no
-// atomics: repeats are bit-identical.
+// decode_join_kernel, which starts while the last CTAs run. (The last CTA to
+// arrive doing that, by a counter, took the smallest calls longer, 18 against
+// 14 us on the device, and no less on the host.) Parts are added in the order of
+// the keys, with no atomics: repeats are bit-identical.
 //
 // int8 and e4m3 codes become fp16 exactly, in registers. An int8 code is
 // widened to the fp16 number (code + 128) 2^-24 (a subnormal: its bits are the

@@ -400,3 +400,21 @@ def test_no_rows_and_other_streams():
         got = cache.read(table, sequences.SequencePack([30, 5], device=DEV))
     side.synchronize()
     assert torch.equal(got[0], held(k, 'int8').bfloat16())
+
+
+def test_calls_on_two_streams():
+    contexts = [3000, 0, 500]
+    cache, table, _, k, v = filled('e4m3', contexts, 64, 2, 128, 43)
+    q = rows(3, 8, 128, 7)
+    lengths = torch.tensor(contexts, dtype=torch.int32, device=DEV)
+    want = cache.attend(q, table, lengths)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for s, out in zip(streams, outs):
+            with torch.cuda.stream(s):
+                out.append(cache.attend(q, table, lengths))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for out in outs for o in out)
