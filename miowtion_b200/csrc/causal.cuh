@@ -96,6 +96,14 @@ __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity,
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status));
 }
 
+// 2^x of a pair, free to be scheduled among other work.
+__device__ __forceinline__ float2 exp2_pair(float2 x) {
+  float2 y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(x.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(x.y));
+  return y;
+}
+
 // Orders this thread's shared memory accesses before later accesses of the
 // asynchronous proxy (TMA, tcgen05).
 __device__ __forceinline__ void fence_async_shared() {

@@ -9,9 +9,9 @@
 // product's depth: no atomics, no second pass, and repeats are bit-identical.
 //
 // Three launches:
-//   prep    D and L * log2(e) of each query row into the workspace, in tile
+//   prep    -D and -L * log2(e) of each query row into the workspace, in tile
 //           order [kv_heads][tiles][128], a row without keys or token as
-//           L = inf, D = 0;
+//           -L = -inf, D = 0;
 //   dq      a query tile an item, its key tiles one after the other: S and dP
 //           (SS products), dS written back over S in tensor memory as bf16,
 //           dQ += dS K (TS product);
@@ -74,8 +74,8 @@ struct BwdParams {
   int group;
   int tokens;           // of a query tile
   int n_tiles;          // query tiles of the pack
-  const float* lse2;    // [kv_heads][n_tiles][128]
-  const float* delta;   // [kv_heads][n_tiles][128]
+  const float* neg_l;   // [kv_heads][n_tiles][128], -L log2(e)
+  const float* neg_d;   // [kv_heads][n_tiles][128], -D
   __nv_bfloat16* grad;  // dq or dk
   int64_t grad_st, grad_sh;
   __nv_bfloat16* grad2;  // dv
@@ -98,6 +98,10 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map,
 #pragma unroll
   for (int c = 0; c < kD / 64; ++c)
     tma_load_3d(dst + c * 16384, map, bar, c * 64, h, row);
+}
+
+__device__ __forceinline__ float2 pair_of(const uint32_t* x, int i) {
+  return make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
 }
 
 // Writes kN bf16 columns of a row (kN / 2 words).
@@ -136,8 +140,8 @@ template <int kD>
 __global__ void __launch_bounds__(kPrepThreads) causal_bwd_prep_kernel(
     const int32_t* table, int group, int tokens, const __nv_bfloat16* out,
     int64_t o_st, int64_t o_sh, const __nv_bfloat16* dout, int64_t d_st,
-    int64_t d_sh, const float* lse, int64_t l_st, int64_t l_sh, float* lse2,
-    float* delta, int n_tiles) {
+    int64_t d_sh, const float* lse, int64_t l_st, int64_t l_sh, float* neg_l,
+    float* neg_d, int n_tiles) {
   constexpr int kLanes = kD / 8;
   constexpr int kStep = kPrepThreads / kLanes;  // rows at a time
   constexpr int kRounds = kTile / kStep;
@@ -182,8 +186,8 @@ __global__ void __launch_bounds__(kPrepThreads) causal_bwd_prep_kernel(
       const int r = i * kStep + threadIdx.x / kLanes;
       // A row without keys or token.
       const bool none = l[i] == -INFINITY;
-      delta[at + r] = none ? 0.f : acc;
-      lse2[at + r] = none ? INFINITY : l[i] * kLog2e;
+      neg_d[at + r] = none ? 0.f : -acc;
+      neg_l[at + r] = none ? -INFINITY : -(l[i] * kLog2e);
     }
   }
 }
@@ -454,6 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---------------- compute warps 0-7 ----------------
     const int half = warp / 4;  // keys 64 half .. of each block
+    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     const int quarter = warp % 4;
     const int row = quarter * 32 + lane;
     const int token = row / p.group;
@@ -477,8 +482,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const int64_t at =
           (static_cast<int64_t>(st.h) * p.n_tiles + st.it.tile) * kTile + row;
-      const float l2 = p.lse2[at];
-      const float dlt = p.delta[at];
+      const float2 nl = make_float2(p.neg_l[at], p.neg_l[at]);
+      const float2 nd = make_float2(p.neg_d[at], p.neg_d[at]);
       const int seen = max(0, min(st.it.keys, st.it.kpos + token + 1));
       for (int j = 0; j < n; ++j, ++blk) {
         const int visible = seen - j * kTile - half * 64;
@@ -506,16 +511,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
-            float d2[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int cc = 2 * c + e;
-              const float pr = ex2_approx(
-                  fmaf(__uint_as_float(s[cc]), p.scale_log2, -l2));
-              d2[e] = pr * (__uint_as_float(dp[q][cc]) - dlt);
-              if (masked && q * 32 + cc >= visible) d2[e] = 0.f;
+            const float2 pr = exp2_pair(
+                __ffma2_rn(pair_of(s, c), scale2, nl));
+            float2 ds = __fmul2_rn(pr, __fadd2_rn(pair_of(dp[q], c), nd));
+            if (masked) {
+              if (q * 32 + 2 * c >= visible) ds.x = 0.f;
+              if (q * 32 + 2 * c + 1 >= visible) ds.y = 0.f;
             }
-            w[q][c] = pack_bf16(d2[0], d2[1]);
+            w[q][c] = pack_bf16(ds.x, ds.y);
           }
         }
         // dS of these 64 keys over the first 32 of this warp's own 64 columns
@@ -659,8 +662,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_expect_tx(bar, qd_bytes);
           load_tile<kD>(dst, &map_q, bar, h * p.group, q_row);
           load_tile<kD>(dst + kTileBytes, &map_do, bar, h * p.group, q_row);
-          bulk_load(s_vec + stage * 256, p.lse2 + base, 512, bar);
-          bulk_load(s_vec + stage * 256 + 128, p.delta + base, 512, bar);
+          bulk_load(s_vec + stage * 256, p.neg_l + base, 512, bar);
+          bulk_load(s_vec + stage * 256 + 128, p.neg_d + base, 512, bar);
         }
         __syncwarp();
         ++qd_loads;
@@ -788,6 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---------------- compute warps 0-7 ----------------
     const int wq = warp / 4;  // query rows 32 wq .. of each half
+    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     const int quarter = warp % 4;
     const int row = quarter * 32 + lane;  // key row of the tile
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
@@ -816,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         continue;
       }
       for (int j = 0; j < n && ok; ++j, ++blk) {
-        const float* vl = s_vec + (blk % kStages) * 256;  // L log2(e), then D
+        const float* vl = s_vec + (blk % kStages) * 256;  // -L log2(e), then -D
         // First query row of the block that sees this key.
         const int64_t from =
             (static_cast<int64_t>(it.shift) + row -
@@ -840,28 +844,28 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_wait_ld();
           uint32_t wp[16], wd[16];
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const float4 l4 = *reinterpret_cast<const float4*>(vl + q0 + 4 * c);
+          for (int c = 0; c < 16; c += 2) {
+            const float4 l4 = *reinterpret_cast<const float4*>(vl + q0 + 2 * c);
             const float4 d4 =
-                *reinterpret_cast<const float4*>(vl + 128 + q0 + 4 * c);
-            const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
-            const float dv[4] = {d4.x, d4.y, d4.z, d4.w};
-            float pr[4], ds[4];
+                *reinterpret_cast<const float4*>(vl + 128 + q0 + 2 * c);
+            const float2 nl[2] = {make_float2(l4.x, l4.y),
+                                  make_float2(l4.z, l4.w)};
+            const float2 nd[2] = {make_float2(d4.x, d4.y),
+                                  make_float2(d4.z, d4.w)};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int cc = 4 * c + e;
-              pr[e] = ex2_approx(
-                  fmaf(__uint_as_float(s[cc]), p.scale_log2, -lv[e]));
-              ds[e] = pr[e] * (__uint_as_float(dp[cc]) - dv[e]);
-              if (masked && q0 + cc < cmin) {
-                pr[e] = 0.f;
-                ds[e] = 0.f;
+            for (int e = 0; e < 2; ++e) {
+              float2 pr =
+                  exp2_pair(__ffma2_rn(pair_of(s, c + e), scale2, nl[e]));
+              float2 ds =
+                  __fmul2_rn(pr, __fadd2_rn(pair_of(dp, c + e), nd[e]));
+              if (masked) {
+                const int col = q0 + 2 * (c + e);
+                if (col < cmin) pr.x = ds.x = 0.f;
+                if (col + 1 < cmin) pr.y = ds.y = 0.f;
               }
+              wp[c + e] = pack_bf16(pr.x, pr.y);
+              wd[c + e] = pack_bf16(ds.x, ds.y);
             }
-            wp[2 * c] = pack_bf16(pr[0], pr[1]);
-            wp[2 * c + 1] = pack_bf16(pr[2], pr[3]);
-            wd[2 * c] = pack_bf16(ds[0], ds[1]);
-            wd[2 * c + 1] = pack_bf16(ds[2], ds[3]);
           }
           // P^T and dS^T of these 32 queries over the first 16 of this
           // warp's own 32 columns of S^T and dP^T.
@@ -905,7 +909,7 @@ struct PrepArgs {
   int64_t d_st, d_sh;
   const float* lse;
   int64_t l_st, l_sh;
-  float *lse2, *delta;
+  float *neg_l, *neg_d;
 };
 
 template <int kD>
@@ -921,7 +925,7 @@ int launch(const Maps& m, const BwdParams& pq, const BwdParams& pk,
             pq.table, pq.group, pq.tokens,
             static_cast<const __nv_bfloat16*>(a.out), a.o_st, a.o_sh,
             static_cast<const __nv_bfloat16*>(a.dout), a.d_st, a.d_sh, a.lse,
-            a.l_st, a.l_sh, a.lse2, a.delta, pq.n_tiles);
+            a.l_st, a.l_sh, a.neg_l, a.neg_d, pq.n_tiles);
     rc = check_launch("causal_bwd_prep_kernel");
     if (rc != VEDA_OK) return rc;
   }
@@ -1047,10 +1051,10 @@ extern "C" int veda_causal_bwd(
   p.group = group;
   p.tokens = tokens;
   p.n_tiles = static_cast<int>(n_tiles);
-  float* lse2 = static_cast<float*>(workspace);
-  float* delta = lse2 + static_cast<int64_t>(kv_heads) * n_tiles * kTile;
-  p.lse2 = lse2;
-  p.delta = delta;
+  float* neg_l = static_cast<float*>(workspace);
+  float* neg_d = neg_l + static_cast<int64_t>(kv_heads) * n_tiles * kTile;
+  p.neg_l = neg_l;
+  p.neg_d = neg_d;
   p.scale = softmax_scale;
   p.scale_log2 = softmax_scale * causal::kLog2e;
   p.status = device_status_ptr();
@@ -1070,7 +1074,7 @@ extern "C" int veda_causal_bwd(
   pk.grad2_sh = dv_stride_h;
   const causal::PrepArgs a{out,           out_stride_t, out_stride_h, dout,
                            dout_stride_t, dout_stride_h, lse,
-                           lse_stride_t,  lse_stride_h,  lse2, delta};
+                           lse_stride_t,  lse_stride_h,  neg_l, neg_d};
   return head_dim == 128
              ? causal::launch<128>(m, pq, pk, a, dq != nullptr, dk != nullptr,
                                    s)
