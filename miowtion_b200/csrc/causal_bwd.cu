@@ -41,6 +41,8 @@
 // (common.cuh).
 #include "causal.cuh"
 
+#include <type_traits>
+
 namespace veda {
 namespace causal {
 
@@ -509,17 +511,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld32(t_s + 32, s);
             tmem_wait_ld();
           }
+          // (On the diagonal apart: a selection costs as much as the rest.)
+          auto weigh = [&](auto diagonal) {
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const float2 pr = exp2_pair(
-                __ffma2_rn(pair_of(s, c), scale2, nl));
-            float2 ds = __fmul2_rn(pr, __fadd2_rn(pair_of(dp[q], c), nd));
-            if (masked) {
-              if (q * 32 + 2 * c >= visible) ds.x = 0.f;
-              if (q * 32 + 2 * c + 1 >= visible) ds.y = 0.f;
+            for (int c = 0; c < 16; ++c) {
+              const float2 pr =
+                  exp2_pair(__ffma2_rn(pair_of(s, c), scale2, nl));
+              float2 ds = __fmul2_rn(pr, __fadd2_rn(pair_of(dp[q], c), nd));
+              if (decltype(diagonal)::value) {
+                if (q * 32 + 2 * c >= visible) ds.x = 0.f;
+                if (q * 32 + 2 * c + 1 >= visible) ds.y = 0.f;
+              }
+              w[q][c] = pack_bf16(ds.x, ds.y);
             }
-            w[q][c] = pack_bf16(ds.x, ds.y);
-          }
+          };
+          if (masked)
+            weigh(std::true_type{});
+          else
+            weigh(std::false_type{});
         }
         // dS of these 64 keys over the first 32 of this warp's own 64 columns
         // of S (all of them are in registers).
@@ -827,7 +836,8 @@ __global__ void __launch_bounds__(kThreads, 1)
              static_cast<int64_t>(it.first + j) * p.tokens) *
             p.group;
         const bool masked = __any_sync(0xffffffffu, from > 0);
-        const int cmin = static_cast<int>(from < 0 ? 0 : min(from, (int64_t)kTile));
+        const int cmin = static_cast<int>(
+            from < 0 ? 0 : (from < kTile ? from : kTile));
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           if (!wait_all(&bars[kStFull + hh], blk & 1, abort, p.status)) {
@@ -843,30 +853,37 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld32(t_dp, dp);
           tmem_wait_ld();
           uint32_t wp[16], wd[16];
+          auto weigh = [&](auto diagonal) {
 #pragma unroll
-          for (int c = 0; c < 16; c += 2) {
-            const float4 l4 = *reinterpret_cast<const float4*>(vl + q0 + 2 * c);
-            const float4 d4 =
-                *reinterpret_cast<const float4*>(vl + 128 + q0 + 2 * c);
-            const float2 nl[2] = {make_float2(l4.x, l4.y),
-                                  make_float2(l4.z, l4.w)};
-            const float2 nd[2] = {make_float2(d4.x, d4.y),
-                                  make_float2(d4.z, d4.w)};
+            for (int c = 0; c < 16; c += 2) {
+              const float4 l4 =
+                  *reinterpret_cast<const float4*>(vl + q0 + 2 * c);
+              const float4 d4 =
+                  *reinterpret_cast<const float4*>(vl + 128 + q0 + 2 * c);
+              const float2 nl[2] = {make_float2(l4.x, l4.y),
+                                    make_float2(l4.z, l4.w)};
+              const float2 nd[2] = {make_float2(d4.x, d4.y),
+                                    make_float2(d4.z, d4.w)};
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float2 pr =
-                  exp2_pair(__ffma2_rn(pair_of(s, c + e), scale2, nl[e]));
-              float2 ds =
-                  __fmul2_rn(pr, __fadd2_rn(pair_of(dp, c + e), nd[e]));
-              if (masked) {
-                const int col = q0 + 2 * (c + e);
-                if (col < cmin) pr.x = ds.x = 0.f;
-                if (col + 1 < cmin) pr.y = ds.y = 0.f;
+              for (int e = 0; e < 2; ++e) {
+                float2 pr =
+                    exp2_pair(__ffma2_rn(pair_of(s, c + e), scale2, nl[e]));
+                float2 ds =
+                    __fmul2_rn(pr, __fadd2_rn(pair_of(dp, c + e), nd[e]));
+                if (decltype(diagonal)::value) {
+                  const int col = q0 + 2 * (c + e);
+                  if (col < cmin) pr.x = ds.x = 0.f;
+                  if (col + 1 < cmin) pr.y = ds.y = 0.f;
+                }
+                wp[c + e] = pack_bf16(pr.x, pr.y);
+                wd[c + e] = pack_bf16(ds.x, ds.y);
               }
-              wp[c + e] = pack_bf16(pr.x, pr.y);
-              wd[c + e] = pack_bf16(ds.x, ds.y);
             }
-          }
+          };
+          if (masked)
+            weigh(std::true_type{});
+          else
+            weigh(std::false_type{});
           // P^T and dS^T of these 32 queries over the first 16 of this
           // warp's own 32 columns of S^T and dP^T.
           tmem_st16(t_s, wp);
