@@ -18,18 +18,35 @@
 //   dkdv    a key tile an item, the query tiles that see it: S^T = K Q^T and
 //           dP^T = V dO^T, P^T and dS^T written back over them, dV += P^T dO
 //           and dK += dS^T Q.
-// One CTA per SM, 8 compute warps, a TMA producer warp and a converged MMA warp.
-// Tensor memory decides how the two kernels overlap their products with the
-// elementwise work. dq has one accumulator, so there is room for two S buffers
+// One CTA per SM, 8 compute warps, a TMA producer warp and a converged MMA
+// warp. Tensor memory decides how the two kernels overlap their products with
+// the elementwise work. dq has one accumulator, so there is room for two S buffers
 // beside dP: while the compute warps turn block b into dS, the tensor core has
 // dP of b + 1 (as soon as dP of b is in registers), dQ of b - 1 and S of b + 1,
 // all 128 columns wide. dk/dv has two accumulators and no room: a block's 128
 // columns run as two halves of 64, and the tensor core has one half's products
-// while the compute warps work on the other. (dq in halves as well: 904 against
-// 874 us for the whole backward of 8,192 tokens, 16/4 heads, D = 128, where a
-// product 64 columns wide reads 6 KB of shared memory for 32 cycles' work, 48
-// cycles' worth; 736 against 740 us at D = 64. 16 compute warps, a group per
-// half, in both kernels: 2 % faster at D = 128, 8 % slower at D = 64.)
+// while the compute warps work on the other.
+//
+// Bound by the tensor core's products at D = 128 (busy 57 % of dq, 64 % of
+// dkdv; a product 64 columns wide reads 6 KB of shared memory for 32 cycles'
+// work, 48 cycles' worth) and by the elementwise work at D = 64. The whole
+// backward of 8,192 tokens, 16/4 heads, by step, at D = 128 and 64:
+//     dq in halves too, S alone ahead            904 and 736 us
+//     dq 128 columns wide                        874 and 743
+//     elementwise work on pairs (f32x2), L and D
+//     negated so that it is one fma and one add  840 and 709
+//     the diagonal's selections in a copy of the
+//     loop of their own                          802 and 615
+// which is 857 and 557 TFLOP/s of the 10 D operations a pair that a backward
+// pass is counted with, and 1,200 and 780 of the 14 D that these kernels do.
+// 16 compute warps in dkdv, a group of eight a half: 797 and 664 us; not kept.
+//
+// P and dS are rounded to bf16 for their products, which costs the gradients
+// as much again as the rounding of the results: dQ and dK are 2.5e-3 off (in
+// the 2-norm, relative) where results that are only rounded are 1.7e-3 off;
+// 0.6 to 0.9e-3 of it are D's, which is computed from out as rounded. Two bf16
+// numbers for a dS would be two more products of seven, and the rest of out
+// another tensor kept for every layer's backward.
 //
 // Rows behind a sequence's end are cleared in shared memory where they are
 // the depth of a product (keys in dq, queries in dkdv); elsewhere they are
@@ -1014,7 +1031,8 @@ extern "C" int veda_causal_bwd(
                    n_tiles * kv_heads < (int64_t(1) << 31) - 65536 &&
                    n_k_items * kv_heads < (int64_t(1) << 31) - 65536,
                "bad sizes");
-  VEDA_REQUIRE(softmax_scale > 0.f && isfinite(softmax_scale),
+  VEDA_REQUIRE(softmax_scale > 0.f &&
+                   isfinite(softmax_scale * causal::kLog2e),
                "softmax_scale must be positive and finite");
   VEDA_REQUIRE((dk == nullptr) == (dv == nullptr),
                "dk and dv are computed together");

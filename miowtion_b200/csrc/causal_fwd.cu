@@ -812,7 +812,8 @@ extern "C" int veda_causal_fwd(
     int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
     int64_t v_stride_h, int64_t total_q, int64_t total_k, int32_t n_heads,
     int32_t kv_heads, int32_t head_dim, const int32_t* items, int64_t n_items,
-    const int32_t* joins, int64_t n_joins, int64_t n_parts, void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse,
+    const int32_t* joins, int64_t n_joins, int64_t n_parts, void* out,
+    int64_t out_stride_t, int64_t out_stride_h, float* lse,
     int64_t lse_stride_t, int64_t lse_stride_h, float softmax_scale,
     void* workspace, int64_t workspace_bytes, void* stream) {
   int rc = require_sm100("veda_causal_fwd");
@@ -826,7 +827,8 @@ extern "C" int veda_causal_fwd(
                    total_k < (int64_t(1) << 31) && n_items >= 0 &&
                    n_items * kv_heads < (int64_t(1) << 31) - 65536,
                "bad sizes");
-  VEDA_REQUIRE(softmax_scale > 0.f && isfinite(softmax_scale),
+  VEDA_REQUIRE(softmax_scale > 0.f &&
+                   isfinite(softmax_scale * causal::kLog2e),
                "softmax_scale must be positive and finite");
   if (total_q == 0 || n_items == 0) return VEDA_OK;
   VEDA_REQUIRE(q && out && items, "q, out and items are required");

@@ -1178,7 +1178,7 @@ extern "C" int veda_decode(
   VEDA_REQUIRE(n_heads >= 1 && n_heads % kv_heads == 0,
                "n_heads must be a multiple of kv_heads");
   VEDA_REQUIRE(n_seqs * n_heads < (int64_t(1) << 31), "too many rows");
-  VEDA_REQUIRE(softmax_scale > 0.f && isfinite(softmax_scale),
+  VEDA_REQUIRE(softmax_scale > 0.f && isfinite(softmax_scale * kLog2e),
                "softmax_scale must be positive and finite");
   VEDA_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
                    q_stride_b % 8 == 0 && q_stride_h % 8 == 0 &&

@@ -14,14 +14,14 @@
 // half is representable and stays one, and a quotient that is not a half
 // differs from it by more than the quotient's rounding error (bf16 operands),
 // so the codes are those of real arithmetic. It is computed as the product with
-// the reciprocal of max|x|, corrected once by the exact remainder: a product
-// that is off by a relative e leaves a remainder that brings it to within e^2,
-// which the last rounding takes to the quotient where that is representable.
-// (The
-// kernel is close to bound by its instructions: 55,504 tokens of 8 heads, D =
-// 128, took 131 us with a division for each value.) A row with a value that is not
-// finite gets the scale NaN, and reads back as NaN throughout; an all-zero
-// row has scale 0.
+// the reciprocal of max|x|, corrected once by the exact remainder (Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000 processor",
+// 1990): a product that is off by a relative e leaves a remainder that brings
+// it to within e^2, which the last rounding takes to the quotient where that is
+// representable. (The kernel is close to bound by its instructions: 55,504
+// tokens of 8 heads, D = 128, took 131 us with a division for each value.) A
+// row with a value that is not finite gets the scale NaN, and reads back as
+// NaN throughout; an all-zero row has scale 0.
 //
 // Both kernels are bound by memory: a group of D / 8 lanes holds a row of k
 // and the row of v at the same place, 16 bytes of bf16 a lane each, and the

@@ -138,8 +138,9 @@ def softmax_scale(scale: float | None, dim: int) -> float:
     if scale is None:
         return dim ** -0.5
     scale = float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError(f'scale must be positive and finite: {scale}')
+    # In fp32, times log2(e) too.
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:
+        raise ValueError(f'scale must be positive and finite in fp32: {scale}')
     return scale
 
 
@@ -629,8 +630,14 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     Returns:
         out [total_q, heads, D] bf16 (and lse); 0 and -inf for rows without
         keys. Rows of one sequence never reach another, whatever they hold;
-        inside a sequence a value row that is not finite may reach queries
-        before it that share its key tile.
+        inside a sequence a row that is not finite may reach rows that it
+        does not see (a value the queries before it, a gradient of the output
+        the keys behind it) inside a tile of 128 keys.
+
+    A forward and backward pass may be captured into a CUDA graph once the
+    same pass has run on the capturing stream. As with every operator of
+    autograd, no graph of the same leaves that another stream recorded may be
+    alive then: its accumulation nodes would wait for that stream.
     """
     scale = softmax_scale(scale, q.shape[-1])
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad

@@ -213,3 +213,10 @@ def test_causal_attention_refuses():
         kernels.causal_attention(wide, k[:, :1], k[:, :1], p)
     with pytest.raises(NotImplementedError, match='unavailable'):
         kernels.causal_attention(q, k, k, p)
+
+
+@pytest.mark.parametrize('scale', [0.0, 1e-40, 1e38, 1e300, float('nan')])
+def test_scales_that_fp32_does_not_hold_are_refused(scale):
+    from miowtion_b200 import kernels
+    with pytest.raises(ValueError, match='positive and finite'):
+        kernels.softmax_scale(scale, 64)
