@@ -31,6 +31,8 @@
 
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 namespace veda {
 
 namespace {
@@ -51,28 +53,40 @@ __device__ __forceinline__ int find_sequence(const int32_t* offsets, int n,
   return lo;
 }
 
-__device__ __forceinline__ void unpack8(const uint4& w, float* x) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(u[i] << 16);
-    x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-  }
+// Two bf16 as floats.
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16),
+                     __uint_as_float(w & 0xFFFF0000u));
 }
 
-// Codes of a lane's 8 values of a row and the row's scale. kGroup lanes hold
-// the row.
-template <int kStore, int kGroup>
-__device__ __forceinline__ uint2 encode8(const uint4& w, float* scale) {
-  // max|x|: magnitudes of bf16 order as their bits do, infinity behind the
-  // numbers and NaN behind infinity, so nothing is lost in the maximum.
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// The larger of the eight magnitudes of a lane, as bf16 bits. Magnitudes of
+// bf16 order as their bits do, infinity behind the numbers and NaN behind
+// infinity, so nothing is lost in the maximum.
+__device__ __forceinline__ uint32_t top8(const uint4& w) {
   constexpr uint32_t kAbs = 0x7fff7fffu;
-  uint32_t high = __vmaxu2(__vmaxu2(w.x & kAbs, w.y & kAbs),
-                           __vmaxu2(w.z & kAbs, w.w & kAbs));
+  const uint32_t high = __vmaxu2(__vmaxu2(w.x & kAbs, w.y & kAbs),
+                                 __vmaxu2(w.z & kAbs, w.w & kAbs));
+  return max(high >> 16, high & 0xffffu);
+}
+
+// max|x| of a row of k (low half) and of the row of v at its place (high
+// half), which kGroup lanes hold.
+template <int kGroup>
+__device__ __forceinline__ uint32_t row_tops(const uint4& k, const uint4& v) {
+  uint32_t high = top8(k) | (top8(v) << 16);
 #pragma unroll
   for (int s = kGroup / 2; s > 0; s >>= 1)
     high = __vmaxu2(high, __shfl_xor_sync(0xffffffffu, high, s));
-  high = max(high >> 16, high & 0xffffu);
+  return high;
+}
+
+// Codes of a lane's 8 values of a row whose largest magnitude has the bits
+// `high`, and the row's scale.
+template <int kStore>
+__device__ __forceinline__ uint2 encode8(const uint4& w, uint32_t high,
+                                         float* scale) {
   const float top = __uint_as_float(high << 16);
   uint32_t word[2] = {0u, 0u};
   if (high >= 0x7f80u) {
@@ -83,8 +97,7 @@ __device__ __forceinline__ uint2 encode8(const uint4& w, float* scale) {
     *scale = 0.f;
     return make_uint2(0u, 0u);
   }
-  float x[8];
-  unpack8(w, x);
+  const float2 x[4] = {unpack2(w.x), unpack2(w.y), unpack2(w.z), unpack2(w.w)};
   if constexpr (kStore == kStoreInt8) {
     // top / 127, corrected the same way (the correctly rounded quotient for
     // each of the 32,639 finite magnitudes: checked one by one).
@@ -102,11 +115,13 @@ __device__ __forceinline__ uint2 encode8(const uint4& w, float* scale) {
     // the low bits.
     uint32_t c[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float n = x[i] * num;
-      float quot = n * inv;
-      quot = fmaf(fmaf(-quot, den, n), inv, quot);
-      c[i] = __float_as_uint(quot + 12582912.f);
+    for (int i = 0; i < 4; ++i) {
+      const float2 n = __fmul2_rn(x[i], both(num));
+      float2 quot = __fmul2_rn(n, both(inv));
+      quot = __ffma2_rn(__ffma2_rn(quot, both(-den), n), both(inv), quot);
+      quot = __fadd2_rn(quot, both(12582912.f));
+      c[2 * i] = __float_as_uint(quot.x);
+      c[2 * i + 1] = __float_as_uint(quot.y);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -124,8 +139,7 @@ __device__ __forceinline__ uint2 encode8(const uint4& w, float* scale) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const __nv_fp8x2_storage_t c = __nv_cvt_float2_to_fp8x2(
-          make_float2(x[2 * i] * inv, x[2 * i + 1] * inv), __NV_SATFINITE,
-          __NV_E4M3);
+          __fmul2_rn(x[i], both(inv)), __NV_SATFINITE, __NV_E4M3);
       word[i >> 1] |= static_cast<uint32_t>(c) << (16 * (i & 1));
     }
   }
@@ -135,26 +149,29 @@ __device__ __forceinline__ uint2 encode8(const uint4& w, float* scale) {
 // Eight codes times their scale, rounded once to bf16.
 template <int kStore>
 __device__ __forceinline__ uint4 decode8(const uint2& w, float scale) {
-  float x[8];
   const uint32_t u[2] = {w.x, w.y};
+  uint32_t out[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t pair = (u[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+    float2 x;
     if constexpr (kStore == kStoreInt8) {
-      x[2 * i] = static_cast<float>(static_cast<int8_t>(pair & 0xffu));
-      x[2 * i + 1] = static_cast<float>(static_cast<int8_t>(pair >> 8));
+      // 2^23 + (code + 128), less 2^23 + 128.
+      const uint32_t biased = u[i >> 1] ^ 0x80808080u;
+      x.x = __uint_as_float(
+          __byte_perm(biased, 0x4B000000u, 0x7540 | 2 * (i & 1)));
+      x.y = __uint_as_float(
+          __byte_perm(biased, 0x4B000000u, 0x7541 | 2 * (i & 1)));
+      x = __fadd2_rn(x, both(-8388736.f));
     } else {
+      const uint32_t pair = u[i >> 1] >> (16 * (i & 1));
       const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
-          static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3);
-      const float2 f = __half22float2(__half2(h));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
+          static_cast<__nv_fp8x2_storage_t>(pair & 0xffffu), __NV_E4M3);
+      x = __half22float2(__half2(h));
     }
+    x = __fmul2_rn(x, both(scale));
+    out[i] = pack_bf16(x.x, x.y);
   }
-  return make_uint4(pack_bf16(x[0] * scale, x[1] * scale),
-                    pack_bf16(x[2] * scale, x[3] * scale),
-                    pack_bf16(x[4] * scale, x[5] * scale),
-                    pack_bf16(x[6] * scale, x[7] * scale));
+  return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
 // Rows of k and v a group of lanes takes at a time. Finding a row's place is a
@@ -220,8 +237,9 @@ __global__ void __launch_bounds__(kThreads)
       }
     } else {
       float ks, vs;
-      const uint2 kc = encode8<kStore, kGroup>(kw[i], &ks);
-      const uint2 vc = encode8<kStore, kGroup>(vw[i], &vs);
+      const uint32_t tops = row_tops<kGroup>(kw[i], vw[i]);
+      const uint2 kc = encode8<kStore>(kw[i], tops & 0xffffu, &ks);
+      const uint2 vc = encode8<kStore>(vw[i], tops >> 16, &vs);
       if (at[i] >= 0) {
         reinterpret_cast<uint2*>(c.k)[at[i] * kGroup + lane] = kc;
         reinterpret_cast<uint2*>(c.v)[at[i] * kGroup + lane] = vc;
@@ -240,29 +258,61 @@ __global__ void __launch_bounds__(kThreads)
                       __nv_bfloat16* k, __nv_bfloat16* v,
                       unsigned int* status) {
   constexpr int kGroup = kD / 8;
-  const int64_t row =
-      (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kGroup;
-  const int lane = threadIdx.x % kGroup;
-  if (row >= n_rows) return;
-  const int t = static_cast<int>(row) / c.kv_heads;
-  const int h = static_cast<int>(row) - t * c.kv_heads;
-  const int b = find_sequence(offsets, c.n_seqs, t);
-  const int64_t at = cache_row(c, b, h, t - offsets[b]);
-  uint4 kw = make_uint4(0, 0, 0, 0), vw = kw;
-  if (at < 0) {
-    if (lane == 0) raise_status(status, VEDA_ERR_INVALID);
-  } else if constexpr (kStore == kStoreBf16) {
-    kw = reinterpret_cast<const uint4*>(c.k)[at * kGroup + lane];
-    vw = reinterpret_cast<const uint4*>(c.v)[at * kGroup + lane];
-  } else {
-    const uint2 kc = reinterpret_cast<const uint2*>(c.k)[at * kGroup + lane];
-    const uint2 vc = reinterpret_cast<const uint2*>(c.v)[at * kGroup + lane];
-    kw = decode8<kStore>(kc, c.k_scale[at]);
-    vw = decode8<kStore>(vc, c.v_scale[at]);
+  constexpr int kGroups = kThreads / kGroup;
+  constexpr int kWide = 32 / kGroup;
+  const int lane = threadIdx.x % kGroup, wl = threadIdx.x % 32;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kGroups * kBatch +
+                       threadIdx.x / kGroup;
+  // As in the other kernel, a lane a row.
+  int64_t my_at = -1;
+  {
+    const int64_t row = row0 - wl / kGroup +
+                        (wl / kWide % kBatch) * kGroups + wl % kWide;
+    if (row < n_rows && wl < kWide * kBatch) {
+      const int t = static_cast<int>(row) / c.kv_heads;
+      const int h = static_cast<int>(row) - t * c.kv_heads;
+      const int b = find_sequence(offsets, c.n_seqs, t);
+      my_at = cache_row(c, b, h, t - offsets[b]);
+      if (my_at < 0) raise_status(status, VEDA_ERR_INVALID);
+    }
   }
-  // Packed outputs [rows, kv_heads, D]: row-major in (token, head).
-  reinterpret_cast<uint4*>(k)[row * kGroup + lane] = kw;
-  reinterpret_cast<uint4*>(v)[row * kGroup + lane] = vw;
+  // Rows that are nowhere read as zeros (and load the cache's first row: with
+  // a branch around the loads the compiler puts a row's conversion behind its
+  // load, inside the branch, and the rows wait for one another).
+  using Word = typename std::conditional<kStore == kStoreBf16, uint4,
+                                         uint2>::type;
+  Word kw[kBatch], vw[kBatch];
+  float ks[kBatch], vs[kBatch];
+  bool there[kBatch];
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    int64_t at = __shfl_sync(0xffffffffu, my_at, i * kWide + wl / kGroup);
+    there[i] = at >= 0;
+    if (at < 0) at = 0;
+    kw[i] = reinterpret_cast<const Word*>(c.k)[at * kGroup + lane];
+    vw[i] = reinterpret_cast<const Word*>(c.v)[at * kGroup + lane];
+    if constexpr (kStore != kStoreBf16) {
+      ks[i] = c.k_scale[at];
+      vs[i] = c.v_scale[at];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    // Packed outputs [rows, kv_heads, D]: row-major in (token, head).
+    const int64_t row = row0 + i * kGroups;
+    if (row >= n_rows) continue;
+    uint4 ko, vo;
+    if constexpr (kStore == kStoreBf16) {
+      ko = kw[i];
+      vo = vw[i];
+    } else {
+      ko = decode8<kStore>(kw[i], ks[i]);
+      vo = decode8<kStore>(vw[i], vs[i]);
+    }
+    if (!there[i]) ko = vo = make_uint4(0, 0, 0, 0);
+    reinterpret_cast<uint4*>(k)[row * kGroup + lane] = ko;
+    reinterpret_cast<uint4*>(v)[row * kGroup + lane] = vo;
+  }
 }
 
 // Calls fn.template operator()<kStore, kD>() for the runtime pair.
@@ -307,7 +357,8 @@ struct ReadLaunch {
   cudaStream_t stream;
   template <int kStore, int kD>
   int operator()() const {
-    const int64_t blocks = (rows * (kD / 8) + kThreads - 1) / kThreads;
+    constexpr int kRows = kThreads / (kD / 8) * kBatch;  // of a block
+    const int64_t blocks = (rows + kRows - 1) / kRows;
     cache_read_kernel<kStore, kD>
         <<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
             c, offsets, rows, k, v, status);
