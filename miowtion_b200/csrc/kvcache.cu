@@ -19,8 +19,8 @@
 // 1990): a product that is off by a relative e leaves a remainder that brings
 // it to within e^2, which the last rounding takes to the quotient where that is
 // representable. (With a division for each value 55,504 tokens of 8 heads, D =
-// 128, took 131 us.) A row with a value that is not finite gets the scale NaN, and reads back as
-// NaN throughout; an all-zero row has scale 0.
+// 128, took 131 us.) A row with a value that is not finite gets the scale NaN,
+// and reads back as NaN throughout; an all-zero row has scale 0.
 //
 // Both kernels are bound by memory: a group of D / 8 lanes holds a row of k
 // and the row of v at the same place, 16 bytes of bf16 a lane each, and the
