@@ -514,6 +514,8 @@ int64_t veda_causal_fwd_workspace(int32_t kv_heads, int32_t head_dim,
 
 /* out [total_q, n_heads, head_dim] bf16, lse (fp32, or NULL): the
  * log-sum-exp of the scaled scores; 0 and -inf for a token without keys.
+ * out_low (int8, contiguous, out's shape, or NULL): the bits of out behind
+ * bf16's, for the backward.
  * items: n_items forward work items, n_parts of them parts of items that were
  * cut along the keys, which the n_joins joins put together (joins may be NULL
  * and the workspace too without parts). */
@@ -524,24 +526,29 @@ int veda_causal_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                     int32_t kv_heads, int32_t head_dim, const int32_t* items,
                     int64_t n_items, const int32_t* joins, int64_t n_joins,
                     int64_t n_parts, void* out, int64_t out_stride_t,
-                    int64_t out_stride_h, float* lse, int64_t lse_stride_t,
-                    int64_t lse_stride_h, float softmax_scale, void* workspace,
+                    int64_t out_stride_h, void* out_low, float* lse,
+                    int64_t lse_stride_t, int64_t lse_stride_h,
+                    float softmax_scale, void* workspace,
                     int64_t workspace_bytes, void* stream);
 
 /* Bytes of workspace veda_causal_bwd needs; -1 for sizes out of range. */
 int64_t veda_causal_bwd_workspace(int32_t kv_heads, int64_t n_tiles);
 
 /* Gradients of sum(out * dout): dq of q's shape, dk and dv of k's, bf16. dq
- * may be NULL, dk and dv together too. out and lse are the forward's;
+ * may be NULL, dk and dv together too. out, out_low and lse are the
+ * forward's (out_low may be NULL: the row sums of out * dout then come from
+ * out as rounded, which costs the gradients accuracy where few keys hold the
+ * weight);
  * q_items and k_items the query tile and key tile work items, n_tiles the
  * query tiles of the pack. Deterministic. */
 int veda_causal_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                     const void* k, int64_t k_stride_t, int64_t k_stride_h,
                     const void* v, int64_t v_stride_t, int64_t v_stride_h,
                     const void* out, int64_t out_stride_t,
-                    int64_t out_stride_h, const void* dout,
-                    int64_t dout_stride_t, int64_t dout_stride_h,
-                    const float* lse, int64_t lse_stride_t,
+                    int64_t out_stride_h, const void* out_low,
+                    const void* dout, int64_t dout_stride_t,
+                    int64_t dout_stride_h, const float* lse,
+                    int64_t lse_stride_t,
                     int64_t lse_stride_h, int64_t total_q, int64_t total_k,
                     int32_t n_heads, int32_t kv_heads, int32_t head_dim,
                     const int32_t* q_items, int64_t n_q_items,

@@ -131,11 +131,12 @@ SIGNATURES = {
     'veda_causal_fwd': (c_i32, [c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64,
                                 c_ptr, c_i64, c_i64, c_i64, c_i64, c_i32,
                                 c_i32, c_i32, c_ptr, c_i64, c_ptr, c_i64,
-                                c_i64, c_ptr, c_i64, c_i64, c_ptr, c_i64,
-                                c_i64, c_f32, c_ptr, c_i64, c_ptr]),
+                                c_i64, c_ptr, c_i64, c_i64, c_ptr, c_ptr,
+                                c_i64, c_i64, c_f32, c_ptr, c_i64, c_ptr]),
     'veda_causal_fwd_workspace': (c_i64, [c_i32, c_i32, c_i64]),
     'veda_causal_bwd_workspace': (c_i64, [c_i32, c_i64]),
-    'veda_causal_bwd': (c_i32, [c_ptr, c_i64, c_i64] * 5 +
+    'veda_causal_bwd': (c_i32, [c_ptr, c_i64, c_i64] * 4 +
+                        [c_ptr, c_ptr, c_i64, c_i64] +
                         [c_ptr, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32,
                          c_i32, c_ptr, c_i64, c_ptr, c_i64, c_i64] +
                         [c_ptr, c_i64, c_i64] * 3 +

@@ -121,6 +121,28 @@ __device__ __forceinline__ void store32(void* dst, const uint32_t* w) {
       : "memory");
 }
 
+// An fp32 number keeps, beside its rounding to bf16, the eight bits behind
+// bf16's: value = the float whose bits are (bf16 bits << 16) + (low << 8), low
+// in [-128, 127], to 2^-17 of it. (The bits of a float's magnitude are in the
+// order of the numbers, so the sum carries into the exponent where it has to.)
+//
+// The low bits of two numbers whose bf16 pair is w: in bits 0-7 and 16-23.
+__device__ __forceinline__ uint32_t low_bits(float a, float b, uint32_t w) {
+  const int x = (__float_as_int(a) - static_cast<int>(w << 16) + 128) >> 8;
+  const int y =
+      (__float_as_int(b) - static_cast<int>(w & 0xFFFF0000u) + 128) >> 8;
+  return __byte_perm(max(-128, min(127, x)), max(-128, min(127, y)), 0x5410);
+}
+
+// The float of bf16 bits (in the high half of `high`) and byte kByte of low
+// bits.
+template <int kByte>
+__device__ __forceinline__ float with_low(uint32_t high, uint32_t low) {
+  const int sign_extended = static_cast<int>(low << (24 - 8 * kByte)) >> 16;
+  return __uint_as_float((high & 0xFFFF0000u) +
+                         (static_cast<uint32_t>(sign_extended) & ~0xffu));
+}
+
 // TMA: stores a box from shared memory (written by this warp, ordered by
 // fence_async_shared); one lane issues it and later waits until the boxes it
 // stored have been read from shared memory.

@@ -42,11 +42,13 @@
 // 16 compute warps in dkdv, a group of eight a half: 797 and 664 us; not kept.
 //
 // P and dS are rounded to bf16 for their products, which costs the gradients
-// as much again as the rounding of the results: dQ and dK are 2.5e-3 off (in
-// the 2-norm, relative) where results that are only rounded are 1.7e-3 off;
-// 0.6 to 0.9e-3 of it are D's, which is computed from out as rounded. Two bf16
-// numbers for a dS would be two more products of seven, and the rest of out
-// another tensor kept for every layer's backward.
+// as much again as the rounding of the results: dQ and dK are 2.4e-3 off (in
+// the 2-norm, relative) where results that are only rounded are 1.7e-3 off.
+// (Two bf16 numbers for a dS would be two more products of seven.) D's error
+// is the same for all keys of a row and meets a sum that cancels, most of all
+// where few keys hold the weight: from out as rounded to bf16 it made that
+// 2.5 to 3.2e-3, and 8e-3 for weights peaked on a key, so the forward also
+// leaves the eight bits behind (causal.cuh), a byte an element.
 //
 // Rows behind a sequence's end are cleared in shared memory where they are
 // the depth of a product (keys in dq, queries in dkdv); elsewhere they are
@@ -158,7 +160,8 @@ constexpr int kPrepThreads = 256;
 template <int kD>
 __global__ void __launch_bounds__(kPrepThreads) causal_bwd_prep_kernel(
     const int32_t* table, int group, int tokens, const __nv_bfloat16* out,
-    int64_t o_st, int64_t o_sh, const __nv_bfloat16* dout, int64_t d_st,
+    int64_t o_st, int64_t o_sh, const int8_t* low, const __nv_bfloat16* dout,
+    int64_t d_st,
     int64_t d_sh, const float* lse, int64_t l_st, int64_t l_sh, float* neg_l,
     float* neg_d, int n_tiles) {
   constexpr int kLanes = kD / 8;
@@ -169,12 +172,14 @@ __global__ void __launch_bounds__(kPrepThreads) causal_bwd_prep_kernel(
   const QueryItem it = load_item<QueryItem>(table, blockIdx.x);
   const int64_t at = (static_cast<int64_t>(h) * n_tiles + it.tile) * kTile;
   uint4 a[kRounds], b[kRounds];
+  uint2 c[kRounds];
   float l[kRounds];
 #pragma unroll
   for (int i = 0; i < kRounds; ++i) {
     const int r = i * kStep + threadIdx.x / kLanes;
     const int token = r / group;
     a[i] = b[i] = make_uint4(0, 0, 0, 0);
+    c[i] = make_uint2(0, 0);
     l[i] = -INFINITY;
     if (token < it.tokens && token < tokens) {
       const int64_t row = static_cast<int64_t>(it.row) + token;
@@ -184,6 +189,9 @@ __global__ void __launch_bounds__(kPrepThreads) causal_bwd_prep_kernel(
       b[i] = *reinterpret_cast<const uint4*>(dout + row * d_st + hq * d_sh +
                                              lane * 8);
       l[i] = lse[row * l_st + hq * l_sh];
+      if (low != nullptr)
+        c[i] = *reinterpret_cast<const uint2*>(
+            low + (row * gridDim.y * group + hq) * kD + lane * 8);
     }
   }
 #pragma unroll
@@ -193,10 +201,11 @@ __global__ void __launch_bounds__(kPrepThreads) causal_bwd_prep_kernel(
     float acc = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      acc = fmaf(__uint_as_float(x[e] << 16), __uint_as_float(y[e] << 16),
+      const uint32_t z = (e < 2 ? c[i].x : c[i].y) >> (16 * (e & 1));
+      acc = fmaf(with_low<0>(x[e] << 16, z), __uint_as_float(y[e] << 16),
                  acc);
-      acc = fmaf(__uint_as_float(x[e] & 0xFFFF0000u),
-                 __uint_as_float(y[e] & 0xFFFF0000u), acc);
+      acc = fmaf(with_low<1>(x[e], z), __uint_as_float(y[e] & 0xFFFF0000u),
+                 acc);
     }
 #pragma unroll
     for (int s = kLanes / 2; s > 0; s >>= 1)
@@ -939,6 +948,7 @@ struct Maps {
 struct PrepArgs {
   const void* out;
   int64_t o_st, o_sh;
+  const void* low;
   const void* dout;
   int64_t d_st, d_sh;
   const float* lse;
@@ -958,6 +968,7 @@ int launch(const Maps& m, const BwdParams& pq, const BwdParams& pk,
         <<<dim3(pq.entries, pq.kv_heads), kPrepThreads, 0, stream>>>(
             pq.table, pq.group, pq.tokens,
             static_cast<const __nv_bfloat16*>(a.out), a.o_st, a.o_sh,
+            static_cast<const int8_t*>(a.low),
             static_cast<const __nv_bfloat16*>(a.dout), a.d_st, a.d_sh, a.lse,
             a.l_st, a.l_sh, a.neg_l, a.neg_d, pq.n_tiles);
     rc = check_launch("causal_bwd_prep_kernel");
@@ -1008,7 +1019,8 @@ extern "C" int veda_causal_bwd(
     const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
     int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
     int64_t v_stride_h, const void* out, int64_t out_stride_t,
-    int64_t out_stride_h, const void* dout, int64_t dout_stride_t,
+    int64_t out_stride_h, const void* out_low, const void* dout,
+    int64_t dout_stride_t,
     int64_t dout_stride_h, const float* lse, int64_t lse_stride_t,
     int64_t lse_stride_h, int64_t total_q, int64_t total_k, int32_t n_heads,
     int32_t kv_heads, int32_t head_dim, const int32_t* q_items,
@@ -1047,12 +1059,13 @@ extern "C" int veda_causal_bwd(
            st % elements == 0 && sh % elements == 0;
   };
   VEDA_REQUIRE(aligned(out, out_stride_t, out_stride_h, 8) &&
+                   reinterpret_cast<uintptr_t>(out_low) % 8 == 0 &&
                    aligned(dout, dout_stride_t, dout_stride_h, 8) &&
                    aligned(dq, dq_stride_t, dq_stride_h, 16) &&
                    aligned(dk, dk_stride_t, dk_stride_h, 16) &&
                    aligned(dv, dv_stride_t, dv_stride_h, 16),
                "out and dout must be 16-byte aligned with strides multiple of "
-               "8; dq, dk, dv 32-byte aligned with strides multiple of 16");
+               "8, out_low 8-byte aligned; dq, dk, dv 32-byte aligned with strides multiple of 16");
   cudaStream_t s = as_stream(stream);
   const int group = n_heads / kv_heads;
   const int tokens = kTile / group;
@@ -1107,9 +1120,10 @@ extern "C" int veda_causal_bwd(
   pk.grad2 = static_cast<__nv_bfloat16*>(dv);
   pk.grad2_st = dv_stride_t;
   pk.grad2_sh = dv_stride_h;
-  const causal::PrepArgs a{out,           out_stride_t, out_stride_h, dout,
-                           dout_stride_t, dout_stride_h, lse,
-                           lse_stride_t,  lse_stride_h,  neg_l, neg_d};
+  const causal::PrepArgs a{out,     out_stride_t,  out_stride_h,
+                           out_low, dout,          dout_stride_t,
+                           dout_stride_h, lse,     lse_stride_t,
+                           lse_stride_h,  neg_l,   neg_d};
   return head_dim == 128
              ? causal::launch<128>(m, pq, pk, a, dq != nullptr, dk != nullptr,
                                    s)

@@ -98,6 +98,7 @@ struct FwdParams {
   int warp_boxes;  // a warp's 32 rows are whole tokens: TMA stores them
   __nv_bfloat16* out;
   int64_t out_st, out_sh;
+  int8_t* low;   // [tokens][heads][kD], out's low bits, or null
   float* lse;    // or null
   int64_t lse_st, lse_sh;
   float scale_log2;
@@ -661,6 +662,23 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
             store32(dst + c * 64 + c2 * 32, w);
             store32(dst + c * 64 + c2 * 32 + 16, w + 8);
           }
+          if (p.low != nullptr && write) {
+            uint32_t low[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              uint32_t two[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                two[i] = low_bits(__uint_as_float(o[4 * e + 2 * i]) * inv_l,
+                                  __uint_as_float(o[4 * e + 2 * i + 1]) *
+                                      inv_l,
+                                  w[2 * e + i]);
+              low[e] = __byte_perm(two[0], two[1], 0x6420);
+            }
+            store32(p.low + (out_row * p.kv_heads * p.group + out_head) * kD +
+                        c * 64 + c2 * 32,
+                    low);
+          }
         }
         if (boxed) {
           fence_async_shared();
@@ -748,9 +766,18 @@ __global__ void __launch_bounds__(kJoinThreads)
         static_cast<int64_t>(h) * p.group + row % p.group;
     uint32_t* dst = reinterpret_cast<uint32_t*>(
         p.out + out_row * p.out_st + out_head * p.out_sh + lane * kPer);
+    int8_t* low = p.low == nullptr
+                      ? nullptr
+                      : p.low + (out_row * p.kv_heads * p.group + out_head) *
+                                    kD + lane * kPer;
 #pragma unroll
-    for (int e = 0; e < kPer / 2; ++e)
-      dst[e] = pack_bf16(o[2 * e] * inv, o[2 * e + 1] * inv);
+    for (int e = 0; e < kPer / 2; ++e) {
+      const float a = o[2 * e] * inv, b = o[2 * e + 1] * inv;
+      dst[e] = pack_bf16(a, b);
+      if (low != nullptr)
+        reinterpret_cast<uint16_t*>(low)[e] = static_cast<uint16_t>(
+            __byte_perm(low_bits(a, b, dst[e]), 0, 0x4420));
+    }
     if (lane == 0 && p.lse != nullptr)
       p.lse[out_row * p.lse_st + out_head * p.lse_sh] =
           l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
@@ -813,7 +840,7 @@ extern "C" int veda_causal_fwd(
     int64_t v_stride_h, int64_t total_q, int64_t total_k, int32_t n_heads,
     int32_t kv_heads, int32_t head_dim, const int32_t* items, int64_t n_items,
     const int32_t* joins, int64_t n_joins, int64_t n_parts, void* out,
-    int64_t out_stride_t, int64_t out_stride_h, float* lse,
+    int64_t out_stride_t, int64_t out_stride_h, void* out_low, float* lse,
     int64_t lse_stride_t, int64_t lse_stride_h, float softmax_scale,
     void* workspace, int64_t workspace_bytes, void* stream) {
   int rc = require_sm100("veda_causal_fwd");
@@ -834,9 +861,10 @@ extern "C" int veda_causal_fwd(
   VEDA_REQUIRE(q && out && items, "q, out and items are required");
   VEDA_REQUIRE(reinterpret_cast<uintptr_t>(out) % 32 == 0 &&
                    out_stride_t % 16 == 0 && out_stride_h % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(out_low) % 32 == 0 &&
                    reinterpret_cast<uintptr_t>(items) % 16 == 0,
                "out must be 32-byte aligned with strides multiple of 16, "
-               "items 16-byte aligned");
+               "out_low 32-byte aligned, items 16-byte aligned");
   VEDA_REQUIRE(n_joins >= 0 && n_joins <= n_items && n_parts >= n_joins &&
                    n_parts <= n_items && kv_heads <= 65535 &&
                    (n_joins == 0) == (n_parts == 0) &&
@@ -882,6 +910,7 @@ extern "C" int veda_causal_fwd(
   p.out = static_cast<__nv_bfloat16*>(out);
   p.out_st = out_stride_t;
   p.out_sh = out_stride_h;
+  p.low = static_cast<int8_t*>(out_low);
   p.lse = lse;
   p.lse_st = lse_stride_t;
   p.lse_sh = lse_stride_h;

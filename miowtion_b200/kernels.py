@@ -518,9 +518,10 @@ def _rows_args(t: torch.Tensor) -> tuple[int, int, int]:
 
 def causal_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                          pack: sequences.SequencePack, scale: float,
-                         return_lse: bool = True):
+                         return_lse: bool = True, return_low: bool = False):
     """(out [rows, heads, D] bf16, lse [rows, heads] fp32 or None) of
-    `causal_attention`, without gradients."""
+    `causal_attention`, without gradients; with `return_low` also the int8
+    bits of out behind bf16's, for the backward."""
     group = _causal_checks(q, k, v, pack)
     require_ready(q.device, 'causal_attention')
     q, k, v = aligned_rows(q), aligned_rows(k), aligned_rows(v)
@@ -529,6 +530,7 @@ def causal_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = (q.new_empty((rows, heads), dtype=torch.float32) if return_lse
            else None)
+    low = torch.empty_like(out, dtype=torch.int8) if return_low else None
     tables = pack.tables(group, kv_heads)
     ws = None
     if tables.n_parts:
@@ -539,18 +541,21 @@ def causal_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _lib.call_on(q.device.index, 'veda_causal_fwd', *_rows_args(q),
                  *_rows_args(k), *_rows_args(v), rows, k_rows, heads,
                  kv_heads, dim, *tables.forward_args, out.data_ptr(),
-                 heads * dim, dim, _lib.ptr(lse), heads, 1, scale,
-                 _lib.ptr(ws), ws.numel() * 4 if ws is not None else 0)
-    return out, lse
+                 heads * dim, dim, _lib.ptr(low), _lib.ptr(lse), heads, 1,
+                 scale, _lib.ptr(ws), ws.numel() * 4 if ws is not None else 0)
+    return (out, lse, low) if return_low else (out, lse)
 
 
 def causal_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                          out: torch.Tensor, dout: torch.Tensor,
                          lse: torch.Tensor, pack: sequences.SequencePack,
                          scale: float, want_q: bool = True,
-                         want_kv: bool = True):
-    """(dq, dk, dv) of `causal_attention` (None where not wanted); out and lse
-    as the forward returned them."""
+                         want_kv: bool = True,
+                         low: torch.Tensor | None = None):
+    """(dq, dk, dv) of `causal_attention` (None where not wanted); out, lse
+    and low as the forward returned them. Without low the row sums of out *
+    dout come from out as rounded to bf16, and the gradients lose accuracy
+    where few keys hold the weight."""
     group = _causal_checks(q, k, v, pack)
     require_ready(q.device, 'causal_attention backward')
     if out.shape != q.shape or dout.shape != q.shape or (
@@ -559,6 +564,11 @@ def causal_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                          '[rows, heads]')
     if out.dtype != q.dtype or dout.dtype != q.dtype:
         raise ValueError('out and dout must be bf16')
+    if low is not None and (low.shape != q.shape or low.dtype != torch.int8
+                            or not low.is_contiguous()
+                            or low.device != q.device):
+        raise ValueError('low must be contiguous int8 of the shape of q, on '
+                         f'{q.device}')
     if any(t.device != q.device for t in (out, dout, lse)):
         raise ValueError(f'out, dout and lse must be on {q.device}')
     q, k, v = aligned_rows(q), aligned_rows(k), aligned_rows(v)
@@ -575,9 +585,9 @@ def causal_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                      dtype=torch.float32)
     _lib.call_on(q.device.index, 'veda_causal_bwd', *_rows_args(q),
                  *_rows_args(k), *_rows_args(v), *_rows_args(out),
-                 *_rows_args(dout), lse.data_ptr(), *lse.stride(), rows,
-                 k_rows, heads, kv_heads, dim, *tables.gradient_args,
-                 _lib.ptr(dq), heads * dim, dim, _lib.ptr(dk),
+                 _lib.ptr(low), *_rows_args(dout), lse.data_ptr(),
+                 *lse.stride(), rows, k_rows, heads, kv_heads, dim,
+                 *tables.gradient_args, _lib.ptr(dq), heads * dim, dim, _lib.ptr(dk),
                  kv_heads * dim, dim, _lib.ptr(dv), kv_heads * dim, dim,
                  scale, ws.data_ptr(), ws.numel() * 4)
     return dq, dk, dv
@@ -587,8 +597,9 @@ class _CausalAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, pack, scale, return_lse):
-        out, lse = causal_attention_fwd(q, k, v, pack, scale)
-        ctx.save_for_backward(q, k, v, out, lse)
+        out, lse, low = causal_attention_fwd(q, k, v, pack, scale,
+                                             return_low=True)
+        ctx.save_for_backward(q, k, v, out, lse, low)
         ctx.pack, ctx.scale = pack, scale
         if not return_lse:
             return out
@@ -601,10 +612,11 @@ class _CausalAttention(torch.autograd.Function):
     def backward(ctx, dout, *_):
         if dout is None:
             return None, None, None, None, None, None
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, lse, low = ctx.saved_tensors
         need = ctx.needs_input_grad
         return (*causal_attention_bwd(q, k, v, out, dout, lse, ctx.pack,
-                                      ctx.scale, need[0], need[1] or need[2]),
+                                      ctx.scale, need[0], need[1] or need[2],
+                                      low),
                 None, None, None)
 
 
@@ -625,7 +637,9 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             scaled scores (no gradient flows through it).
 
     q, k and v receive gradients (once differentiable), those of a key head
-    summed over its query heads; repeats are bit-identical.
+    summed over its query heads; repeats are bit-identical. For them the call
+    keeps q, k, v, out, the log-sum-exp and one more byte for each element of
+    out (the bits behind bf16's).
 
     Returns:
         out [total_q, heads, D] bf16 (and lse); 0 and -inf for rows without

@@ -266,6 +266,73 @@ def test_gradients_agree_with_differences():
         assert abs(got - slope) <= 2.0 ** -8 * size, (n, got, slope)
 
 
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('q_lengths, k_lengths, heads, kv_heads', [
+    ([300, 1, 70], None, 4, 2), ([70, 5], [6000, 3001], 8, 2),
+    ([40, 200], [90, 30], 3, 1)])
+def test_out_and_its_low_bits(q_lengths, k_lengths, heads, kv_heads, dim):
+    """out is the rounding of the number that it and its low bits make, which
+    is therefore within half a bf16 step of it, and no output depends on
+    whether the low bits are asked for."""
+    pack, q, k, v = problem(q_lengths, k_lengths, heads, kv_heads, dim)
+    out, lse, low = kernels.causal_attention_fwd(q, k, v, pack, dim ** -0.5,
+                                                 return_low=True)
+    again, _ = kernels.causal_attention_fwd(q, k, v, pack, dim ** -0.5)
+    assert torch.equal(out, again)
+    bits = (out.view(torch.int16).int() << 16) + (low.int() << 8)
+    full = bits.view(torch.float32)
+    off = (full - out.float()).abs()
+    assert (off <= 2.0 ** -8 * out.float().abs()).all()
+    seen = out != 0
+    assert low[~seen].eq(0).all()
+    # Rounding errors are spread evenly over [-128, 128): 255 in 256 are not
+    # zero, and the mean of n is within 5 * 74 / sqrt(n) of it. (Rows of one
+    # key are exact: a tenth of them and more is left out of account.)
+    assert low[seen].ne(0).float().mean() > 0.9
+    mean = float(low[seen].float().mean())
+    assert abs(mean) < 5 * 74 / int(seen.sum()) ** 0.5 + 0.5
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('q_lengths, k_lengths, heads, kv_heads', [
+    ([300, 1, 70], None, 4, 2), ([70, 5], [6000, 3001], 8, 2),
+    ([40, 200], [90, 30], 3, 1)])
+def test_gradients_of_peaked_weights(q_lengths, k_lengths, heads, kv_heads,
+                                     dim):
+    """Where a key holds nearly all of a row's weight, dP and D cancel, and the
+    rounding of out to bf16 is the largest error of dQ and dK (D's: 2^-8 |out
+    dout| against a sum that is a fraction of it). The low bits take it away:
+    with them the gradients are nearer to the definition's than without."""
+    scale = 4 * dim ** -0.5
+    pack, q, k, v = problem(q_lengths, k_lengths, heads, kv_heads, dim)
+    dout = rows(pack.total_q, heads, dim, 9)
+    grads = gradients(pack, q, k, v, dout, scale)
+    check_gradients(pack, q, k, v, dout, grads, scale)
+    out, lse, low = kernels.causal_attention_fwd(q, k, v, pack, scale,
+                                                 return_low=True)
+    exact = [torch.zeros_like(t, dtype=torch.float64) for t in (q, k, v)]
+    for at, keys, h, hk, sees in each_head(pack, q, k):
+        qb, kb, vb = q[at, h].double(), k[keys, hk].double(), v[
+            keys, hk].double()
+        if 0 in (qb.shape[0], kb.shape[0]):
+            continue
+        g = dout[at, h].double()
+        p, _ = softmax64(qb, kb, sees, scale)
+        ds = p * (g @ vb.T - (g * (p @ vb)).sum(-1, keepdim=True))
+        exact[0][at, h] += scale * ds @ kb
+        exact[1][keys, hk] += scale * ds.T @ qb
+        exact[2][keys, hk] += p.T @ g
+    rounded = kernels.causal_attention_bwd(q, k, v, out, dout, lse, pack,
+                                           scale)
+
+    def off(got):
+        return [float((a.double() - b).norm() / b.norm())
+                for a, b in zip(got, exact)]
+    with_low, without = off(grads), off(rounded)
+    assert with_low[0] < without[0] and with_low[1] < without[1]
+    assert with_low[2] == without[2]
+
+
 def test_gradients_of_shared_broadcast_and_single_inputs():
     pack, q, _, _ = problem([90, 40], None, 4, 2, 64)
     dout = rows(130, 4, 64, 9)

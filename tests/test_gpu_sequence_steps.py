@@ -128,11 +128,11 @@ def test_training_step_through_the_attention_function():
     q = rows(291, 4, 64, 1).requires_grad_(True)
     k, v = (rows(291, 2, 64, s).requires_grad_(True) for s in (2, 3))
     fn(q, k, v, 0).float().square().mean().backward()
-    out, lse = kernels.causal_attention(q.detach(), k.detach(), v.detach(),
-                                        pack, 0.2, return_lse=True)
+    out, lse, low = kernels.causal_attention_fwd(
+        q.detach(), k.detach(), v.detach(), pack, 0.2, return_low=True)
     dout = (out.float() * 2 / out.numel()).to(torch.bfloat16)
     want = kernels.causal_attention_bwd(q.detach(), k.detach(), v.detach(),
-                                        out, dout, lse, pack, 0.2)
+                                        out, dout, lse, pack, 0.2, low=low)
     assert all(torch.equal(t.grad, w) for t, w in zip((q, k, v), want))
 
 
