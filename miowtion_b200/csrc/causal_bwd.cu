@@ -152,8 +152,9 @@ __device__ __forceinline__ void tmem_row_bf16(uint32_t taddr, float scale,
 
 // ---------------------------------------------------------------------------
 // prep: a block per (query tile, key head), kD / 8 lanes a row. Bound by
-// memory (out and dout once): every thread has its rows' loads in flight at
-// once.
+// memory (out, its low bits and dout once): every thread has four rows' loads
+// in flight (all eight of D = 128: 122 registers, 19 us against 17 for 8,192
+// tokens of 16 heads).
 // ---------------------------------------------------------------------------
 constexpr int kPrepThreads = 256;
 
@@ -167,55 +168,59 @@ __global__ void __launch_bounds__(kPrepThreads) causal_bwd_prep_kernel(
   constexpr int kLanes = kD / 8;
   constexpr int kStep = kPrepThreads / kLanes;  // rows at a time
   constexpr int kRounds = kTile / kStep;
+  constexpr int kBatch = 4;  // rounds whose loads are in flight together
   const int lane = threadIdx.x % kLanes;
   const int h = blockIdx.y;
   const QueryItem it = load_item<QueryItem>(table, blockIdx.x);
   const int64_t at = (static_cast<int64_t>(h) * n_tiles + it.tile) * kTile;
-  uint4 a[kRounds], b[kRounds];
-  uint2 c[kRounds];
-  float l[kRounds];
+#pragma unroll 1
+  for (int first = 0; first < kRounds; first += kBatch) {
+    uint4 a[kBatch], b[kBatch];
+    uint2 c[kBatch];
+    float l[kBatch];
 #pragma unroll
-  for (int i = 0; i < kRounds; ++i) {
-    const int r = i * kStep + threadIdx.x / kLanes;
-    const int token = r / group;
-    a[i] = b[i] = make_uint4(0, 0, 0, 0);
-    c[i] = make_uint2(0, 0);
-    l[i] = -INFINITY;
-    if (token < it.tokens && token < tokens) {
-      const int64_t row = static_cast<int64_t>(it.row) + token;
-      const int64_t hq = static_cast<int64_t>(h) * group + r % group;
-      a[i] = *reinterpret_cast<const uint4*>(out + row * o_st + hq * o_sh +
-                                             lane * 8);
-      b[i] = *reinterpret_cast<const uint4*>(dout + row * d_st + hq * d_sh +
-                                             lane * 8);
-      l[i] = lse[row * l_st + hq * l_sh];
-      if (low != nullptr)
-        c[i] = *reinterpret_cast<const uint2*>(
-            low + (row * gridDim.y * group + hq) * kD + lane * 8);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kRounds; ++i) {
-    const uint32_t x[4] = {a[i].x, a[i].y, a[i].z, a[i].w};
-    const uint32_t y[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
-    float acc = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t z = (e < 2 ? c[i].x : c[i].y) >> (16 * (e & 1));
-      acc = fmaf(with_low<0>(x[e] << 16, z), __uint_as_float(y[e] << 16),
-                 acc);
-      acc = fmaf(with_low<1>(x[e], z), __uint_as_float(y[e] & 0xFFFF0000u),
-                 acc);
+    for (int i = 0; i < kBatch; ++i) {
+      const int r = (first + i) * kStep + threadIdx.x / kLanes;
+      const int token = r / group;
+      a[i] = b[i] = make_uint4(0, 0, 0, 0);
+      c[i] = make_uint2(0, 0);
+      l[i] = -INFINITY;
+      if (token < it.tokens && token < tokens) {
+        const int64_t row = static_cast<int64_t>(it.row) + token;
+        const int64_t hq = static_cast<int64_t>(h) * group + r % group;
+        a[i] = *reinterpret_cast<const uint4*>(out + row * o_st + hq * o_sh +
+                                               lane * 8);
+        b[i] = *reinterpret_cast<const uint4*>(dout + row * d_st + hq * d_sh +
+                                               lane * 8);
+        l[i] = lse[row * l_st + hq * l_sh];
+        if (low != nullptr)
+          c[i] = *reinterpret_cast<const uint2*>(
+              low + (row * gridDim.y * group + hq) * kD + lane * 8);
+      }
     }
 #pragma unroll
-    for (int s = kLanes / 2; s > 0; s >>= 1)
-      acc += __shfl_xor_sync(0xffffffffu, acc, s);
-    if (lane == 0) {
-      const int r = i * kStep + threadIdx.x / kLanes;
-      // A row without keys or token.
-      const bool none = l[i] == -INFINITY;
-      neg_d[at + r] = none ? 0.f : -acc;
-      neg_l[at + r] = none ? -INFINITY : -(l[i] * kLog2e);
+    for (int i = 0; i < kBatch; ++i) {
+      const uint32_t x[4] = {a[i].x, a[i].y, a[i].z, a[i].w};
+      const uint32_t y[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
+      float acc = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t z = (e < 2 ? c[i].x : c[i].y) >> (16 * (e & 1));
+        acc = fmaf(with_low<0>(x[e] << 16, z), __uint_as_float(y[e] << 16),
+                   acc);
+        acc = fmaf(with_low<1>(x[e], z), __uint_as_float(y[e] & 0xFFFF0000u),
+                   acc);
+      }
+#pragma unroll
+      for (int s = kLanes / 2; s > 0; s >>= 1)
+        acc += __shfl_xor_sync(0xffffffffu, acc, s);
+      if (lane == 0) {
+        const int r = (first + i) * kStep + threadIdx.x / kLanes;
+        // A row without keys or token.
+        const bool none = l[i] == -INFINITY;
+        neg_d[at + r] = none ? 0.f : -acc;
+        neg_l[at + r] = none ? -INFINITY : -(l[i] * kLog2e);
+      }
     }
   }
 }
