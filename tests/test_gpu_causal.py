@@ -410,3 +410,40 @@ def test_forward_repeats_and_replays():
     with pytest.raises(RuntimeError, match='before the capture'):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             kernels.causal_attention(q, k, v, fresh)
+
+
+def test_backward_refuses_what_the_forward_did_not_return():
+    pack, q, k, v = problem([40, 30], None, 4, 2, 64)
+    out, lse, low = kernels.causal_attention_fwd(q, k, v, pack, 0.1,
+                                                 return_low=True)
+    for o, l, b, match in [(out[:69], lse, low, 'shape of q'),
+                           (out, lse[:69], low, 'shape of q'),
+                           (out, lse.double(), low, 'fp32'),
+                           (out.float(), lse, low, 'bf16'),
+                           (out, lse, low[:69], 'low'),
+                           (out, lse, low.short(), 'low'),
+                           (out, lse, low.transpose(0, 1).contiguous()
+                            .transpose(0, 1), 'low'),
+                           (out, lse, low.cpu(), 'low')]:
+        with pytest.raises(ValueError, match=match):
+            kernels.causal_attention_bwd(q, k, v, o, out, l, pack, 0.1, low=b)
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+def test_low_bits_of_values_at_the_ends_of_the_type(dim):
+    """One key a row: out is the value row, exactly, whatever its size, and
+    NaN and infinity stay what they are."""
+    pack, q, k, v = problem([1, 1, 1, 1], None, 2, 1, dim)
+    v[0] = torch.finfo(torch.bfloat16).max
+    v[1] = -2.0 ** -126
+    v[2, 0, :8] = float('inf')
+    v[3, 0, 5] = float('nan')
+    out, _, low = kernels.causal_attention_fwd(q, k, v, pack, 0.1,
+                                               return_low=True)
+    for h in range(2):
+        assert torch.equal(out[:3, h], v[:3, 0])
+        assert out[3, h, 5].isnan() and not out[3, h, 6].isnan()
+    full = ((out.view(torch.int16).int() << 16) + (low.int() << 8)).view(
+        torch.float32)
+    assert torch.equal(full[:3], out[:3].float())
+    assert full[3, :, 5].isnan().all()
