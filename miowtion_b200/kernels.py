@@ -556,7 +556,7 @@ def causal_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     and low as the forward returned them. Without low the row sums of out *
     dout come from out as rounded to bf16, and the gradients lose accuracy
     where few keys hold the weight."""
-    group = _causal_checks(q, k, v, pack)
+    _causal_checks(q, k, v, pack)
     require_ready(q.device, 'causal_attention backward')
     if out.shape != q.shape or dout.shape != q.shape or (
             lse.shape != q.shape[:2]) or lse.dtype != torch.float32:
@@ -571,10 +571,17 @@ def causal_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                          f'{q.device}')
     if any(t.device != q.device for t in (out, dout, lse)):
         raise ValueError(f'out, dout and lse must be on {q.device}')
+    return _causal_bwd(q, k, v, out, dout, lse, low, pack, scale, want_q,
+                       want_kv)
+
+
+def _causal_bwd(q, k, v, out, dout, lse, low, pack, scale, want_q, want_kv):
+    """`causal_attention_bwd` of checked arguments."""
     q, k, v = aligned_rows(q), aligned_rows(k), aligned_rows(v)
     out, dout = aligned_rows(out), aligned_rows(dout)
     rows, heads, dim = q.shape
     k_rows, kv_heads, _ = k.shape
+    group = heads // kv_heads
     contiguous = torch.contiguous_format
     dq = torch.empty_like(q, memory_format=contiguous) if want_q else None
     dk = torch.empty_like(k, memory_format=contiguous) if want_kv else None
@@ -587,9 +594,9 @@ def causal_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                  *_rows_args(k), *_rows_args(v), *_rows_args(out),
                  _lib.ptr(low), *_rows_args(dout), lse.data_ptr(),
                  *lse.stride(), rows, k_rows, heads, kv_heads, dim,
-                 *tables.gradient_args, _lib.ptr(dq), heads * dim, dim, _lib.ptr(dk),
-                 kv_heads * dim, dim, _lib.ptr(dv), kv_heads * dim, dim,
-                 scale, ws.data_ptr(), ws.numel() * 4)
+                 *tables.gradient_args, _lib.ptr(dq), heads * dim, dim,
+                 _lib.ptr(dk), kv_heads * dim, dim, _lib.ptr(dv),
+                 kv_heads * dim, dim, scale, ws.data_ptr(), ws.numel() * 4)
     return dq, dk, dv
 
 
@@ -614,9 +621,9 @@ class _CausalAttention(torch.autograd.Function):
             return None, None, None, None, None, None
         q, k, v, out, lse, low = ctx.saved_tensors
         need = ctx.needs_input_grad
-        return (*causal_attention_bwd(q, k, v, out, dout, lse, ctx.pack,
-                                      ctx.scale, need[0], need[1] or need[2],
-                                      low),
+        # The forward checked its arguments, autograd checks dout.
+        return (*_causal_bwd(q, k, v, out, dout, lse, low, ctx.pack, ctx.scale,
+                             need[0], need[1] or need[2]),
                 None, None, None)
 
 
