@@ -540,7 +540,10 @@ int64_t veda_causal_bwd_workspace(int32_t kv_heads, int64_t n_tiles);
  * out as rounded, which costs the gradients accuracy where few keys hold the
  * weight);
  * q_items and k_items the query tile and key tile work items, n_tiles the
- * query tiles of the pack. Deterministic. */
+ * query tiles of the pack. k_order (or NULL) deals the key tile items, key
+ * heads included (item i is entry i / kv_heads of head i % kv_heads), to
+ * k_ctas CTAs: [k_turns][k_ctas], each item once, -1 behind a CTA's last.
+ * Deterministic. */
 int veda_causal_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                     const void* k, int64_t k_stride_t, int64_t k_stride_h,
                     const void* v, int64_t v_stride_t, int64_t v_stride_h,
@@ -553,6 +556,7 @@ int veda_causal_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                     int32_t n_heads, int32_t kv_heads, int32_t head_dim,
                     const int32_t* q_items, int64_t n_q_items,
                     const int32_t* k_items, int64_t n_k_items,
+                    const int32_t* k_order, int32_t k_ctas, int32_t k_turns,
                     int64_t n_tiles, void* dq, int64_t dq_stride_t,
                     int64_t dq_stride_h, void* dk, int64_t dk_stride_t,
                     int64_t dk_stride_h, void* dv, int64_t dv_stride_t,

@@ -138,7 +138,8 @@ SIGNATURES = {
     'veda_causal_bwd': (c_i32, [c_ptr, c_i64, c_i64] * 4 +
                         [c_ptr, c_ptr, c_i64, c_i64] +
                         [c_ptr, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32,
-                         c_i32, c_ptr, c_i64, c_ptr, c_i64, c_i64] +
+                         c_i32, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i32,
+                         c_i32, c_i64] +
                         [c_ptr, c_i64, c_i64] * 3 +
                         [c_f32, c_ptr, c_i64, c_ptr]),
     'veda_cache_write': (c_i32, _CACHE + [c_ptr, c_i64, c_i64, c_ptr, c_i64,

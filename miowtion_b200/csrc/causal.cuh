@@ -13,7 +13,8 @@
 // Work items (eight int32 each) are built on the host from the lengths,
 // longest first, without the key heads: item i of a kernel is table entry
 // i / kv_heads of key head i % kv_heads. CTA c takes items c, 2G - 1 - c,
-// 2G + c, ... of G CTAs (back and forth), which pairs long with short.
+// 2G + c, ... of G CTAs (back and forth), which pairs long with short; the key
+// gradient's items may come dealt (sequences.py, deal_items).
 #pragma once
 
 #include <math.h>

@@ -103,8 +103,22 @@ struct BwdParams {
   int64_t grad2_st, grad2_sh;
   float scale;
   float scale_log2;
+  // dk/dv: item of each turn of each CTA, [turns][gridDim.x], -1 behind a
+  // CTA's last; null: back and forth.
+  const int32_t* order;
+  int turns;
   unsigned int* status;
 };
+
+// Item number of a CTA's n-th turn; negative behind its last.
+__device__ __forceinline__ int64_t key_turn(const BwdParams& p, int n,
+                                            int64_t n_items) {
+  if (p.order != nullptr)
+    return n < p.turns ? __ldg(p.order + static_cast<int64_t>(n) * gridDim.x +
+                               blockIdx.x)
+                       : -1;
+  return static_cast<int64_t>(n) * gridDim.x < n_items ? turn(n) : -1;
+}
 
 __device__ __forceinline__ void arrive_warp(uint64_t* bar) {
   tc_fence_before();
@@ -667,8 +681,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int kt_loads = 0, qd_loads = 0;
     bool run = true;
     for (int t = 0; run; ++t) {
-      const int64_t i = turn(t);
-      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
+      const int64_t i = key_turn(p, t, n_items);
+      if (i < 0) break;
       if (i >= n_items) continue;
       const int h = static_cast<int>(i % p.kv_heads);
       const KeyItem it =
@@ -751,8 +765,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int blk = 0, items = 0;
     bool run = true;
     for (int t = 0; run; ++t) {
-      const int64_t i = turn(t);
-      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
+      const int64_t i = key_turn(p, t, n_items);
+      if (i < 0) break;
       if (i >= n_items) continue;
       const KeyItem it =
           load_item<KeyItem>(p.table, static_cast<int>(i / p.kv_heads));
@@ -838,8 +852,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int blk = 0, items = 0;
     bool ok = true;
     for (int t = 0; ok; ++t) {
-      const int64_t i = turn(t);
-      if (static_cast<int64_t>(t) * gridDim.x >= n_items) break;
+      const int64_t i = key_turn(p, t, n_items);
+      if (i < 0) break;
       if (i >= n_items) continue;
       const int h = static_cast<int>(i % p.kv_heads);
       const KeyItem it =
@@ -962,7 +976,7 @@ struct PrepArgs {
 };
 
 template <int kD>
-int launch(const Maps& m, const BwdParams& pq, const BwdParams& pk,
+int launch(const Maps& m, const BwdParams& pq, const BwdParams& pk, int k_ctas,
            const PrepArgs& a, bool want_q, bool want_k, cudaStream_t stream) {
   using C = Bwd<kD>;
   int sms = 0;
@@ -997,7 +1011,9 @@ int launch(const Maps& m, const BwdParams& pq, const BwdParams& pk,
     rc = allow_smem(reinterpret_cast<const void*>(causal_dkdv_kernel<kD>),
                     C::kSmem, &allowed);
     if (rc != VEDA_OK) return rc;
-    const int grid = static_cast<int>(k_items < sms ? k_items : sms);
+    const int grid = pk.order != nullptr
+                         ? k_ctas
+                         : static_cast<int>(k_items < sms ? k_items : sms);
     causal_dkdv_kernel<kD><<<grid, kThreads, C::kSmem, stream>>>(
         m.q, m.dout, m.k, m.v, pk);
     return check_launch("causal_dkdv_kernel");
@@ -1030,7 +1046,8 @@ extern "C" int veda_causal_bwd(
     int64_t lse_stride_h, int64_t total_q, int64_t total_k, int32_t n_heads,
     int32_t kv_heads, int32_t head_dim, const int32_t* q_items,
     int64_t n_q_items, const int32_t* k_items, int64_t n_k_items,
-    int64_t n_tiles, void* dq, int64_t dq_stride_t, int64_t dq_stride_h,
+    const int32_t* k_order, int32_t k_ctas, int32_t k_turns, int64_t n_tiles,
+    void* dq, int64_t dq_stride_t, int64_t dq_stride_h,
     void* dk, int64_t dk_stride_t, int64_t dk_stride_h, void* dv,
     int64_t dv_stride_t, int64_t dv_stride_h, float softmax_scale,
     void* workspace, int64_t workspace_bytes, void* stream) {
@@ -1078,6 +1095,8 @@ extern "C" int veda_causal_bwd(
                "q, out, dout, lse and q_items are required");
   VEDA_REQUIRE(n_k_items == 0 || (k && v && k_items),
                "k, v and k_items are required");
+  VEDA_REQUIRE(k_order == nullptr || (k_ctas >= 1 && k_turns >= 1),
+               "k_order needs its CTAs and turns");
   causal::Maps m;
   if (total_q > 0) {
     rc = causal::make_rows_map(&m.q, q, total_q, n_heads, head_dim,
@@ -1119,6 +1138,8 @@ extern "C" int veda_causal_bwd(
   pq.grad_sh = dq_stride_h;
   pk.table = k_items;
   pk.entries = static_cast<int>(n_k_items);
+  pk.order = k_order;
+  pk.turns = k_turns;
   pk.grad = static_cast<__nv_bfloat16*>(dk);
   pk.grad_st = dk_stride_t;
   pk.grad_sh = dk_stride_h;
@@ -1130,8 +1151,8 @@ extern "C" int veda_causal_bwd(
                            dout_stride_h, lse,     lse_stride_t,
                            lse_stride_h,  neg_l,   neg_d};
   return head_dim == 128
-             ? causal::launch<128>(m, pq, pk, a, dq != nullptr, dk != nullptr,
-                                   s)
-             : causal::launch<64>(m, pq, pk, a, dq != nullptr, dk != nullptr,
-                                  s);
+             ? causal::launch<128>(m, pq, pk, k_ctas, a, dq != nullptr,
+                                   dk != nullptr, s)
+             : causal::launch<64>(m, pq, pk, k_ctas, a, dq != nullptr,
+                                  dk != nullptr, s);
 }

@@ -220,3 +220,26 @@ def test_scales_that_fp32_does_not_hold_are_refused(scale):
     from miowtion_b200 import kernels
     with pytest.raises(ValueError, match='positive and finite'):
         kernels.softmax_scale(scale, 64)
+
+
+@pytest.mark.parametrize('lengths, kv_heads, sms', [
+    ([8192, 5000, 1000], 4, 148), ([700, 9, 0, 130], 3, 7), ([1], 1, 4),
+    ([500] * 40, 2, 148), ([300, 200], 1, 5), ([4096], 2, 5)])
+def test_deal_takes_every_key_item_once(lengths, kv_heads, sms):
+    lengths = np.array(lengths, np.int64)
+    _, _, key, _ = sequences.work_items(lengths, lengths, 4)
+    blocks = key[:, 6]
+    turns = sequences.deal_items(blocks, kv_heads, sms)
+    items = len(key) * kv_heads
+    if not sms < items <= sequences.MOST_TURNS * sms:
+        assert turns.shape == (0, sms)
+        return
+    assert turns.shape[1] == sms
+    assert sorted(turns[turns >= 0]) == list(range(items))
+    # A processor's turns end once.
+    assert ((turns[1:] < 0) | (turns[:-1] >= 0)).all()
+    cost = np.append(np.repeat(blocks + sequences.ITEM_COST, kv_heads), 0.0)
+    load = cost[turns].sum(0)
+    # Each item went to the processor that had least, which then had the mean
+    # at most.
+    assert load.max() <= cost.sum() / sms + cost.max()
