@@ -252,8 +252,11 @@ enum DqBar {
   kSFull,                     // [2] S of the block (by its parity)
   kDpFull = kSFull + 2,       // dP of the block
   kDpFree,                    // dP is in registers (8 warps)
-  kDsFull,                    // dS written (8 warps)
-  kDqDone,                    // the item's last dQ product finished
+  // dS written (8 warps), [2] by the block's parity: dP of the next block is
+  // on its way before the product that waits here, so its dS may be written
+  // too, and one barrier could be two phases on.
+  kDsFull,
+  kDqDone = kDsFull + 2,      // the item's last dQ product finished
   kDqFree,                    // the epilogue has read dQ (8 warps)
   kDqDrain,
   kKFull,                     // [kKRing]
@@ -333,7 +336,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int b = 0; b < kDqNumBars; ++b)
       mbar_init(&bars[b],
-                (b == kDpFree || b == kDsFull || b == kDqFree) ? 8 : 1);
+                (b == kDpFree || b == kDsFull || b == kDsFull + 1 ||
+                 b == kDqFree)
+                    ? 8
+                    : 1);
     *abort = 0;
     fence_barrier_init();
   }
@@ -481,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // The item's first dQ overwrites dQ: the epilogue must have read it.
       if (at.first() && at.items > 0 && !wait(kDqFree, at.items - 1)) break;
-      if (!wait(kDsFull, at.b)) break;
+      if (!wait(kDsFull + (at.b & 1), at.b >> 1)) break;
       tc_fence_after();
       const int slot = at.b % kKRing;
       const uint32_t bk = kmn_lo + slot * C::kTileUnits;
@@ -580,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st16(t_s, w[0]);
         tmem_st16(t_s + 16, w[1]);
         tmem_wait_st();
-        arrive_warp(&bars[kDsFull]);
+        arrive_warp(&bars[kDsFull + (blk & 1)]);
       }
       if (!ok) break;
       if (!wait_all(&bars[kDqDone], items & 1, abort, p.status)) break;

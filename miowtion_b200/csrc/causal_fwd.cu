@@ -79,9 +79,13 @@ enum Bar {
   kQFull = 0,             // [2] Q of the tile landed
   kQEmpty = kQFull + 2,   // [2] the tile's last S product finished
   kSFull = kQEmpty + 2,   // [kSBufs] the scores in the buffer are finished
-  kPHalfA = kSFull + 3,   // [2] P of keys 0-63 written (4 warps)
-  kPHalfB = kPHalfA + 2,  // [2] P of keys 64-127 written (4 warps)
-  kODone = kPHalfB + 2,   // [2] the tile's last product of the item finished
+  // P of keys 0-63 and of keys 64-127 written (4 warps), [block % 2][2]: with
+  // three buffers a tile's scores come a block ahead of its product, so its P
+  // may too, and one barrier could be two phases on, which a wait by parity
+  // takes for none.
+  kPHalfA = kSFull + 3,
+  kPHalfB = kPHalfA + 4,
+  kODone = kPHalfB + 4,   // [2] the tile's last product of the item finished
   kPvDone = kODone + 2,   // [2] the tile's product of the block (3 buffers)
   kDrain = kPvDone + 2,
   kFull,                  // [kRing]
@@ -391,13 +395,16 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
           for (int g = 0; g < 2; ++g) {
             const uint32_t t_p = tmem + (2 * pv.b + g) % C::kSBufs * 128;
             const uint32_t t_o = tmem + C::kO + g * kD;
-            if (!wait_all(&bars[kPHalfA + g], pv.b & 1, abort, p.status)) {
+            const int p_bar = 2 * (pv.b & 1) + g;
+            if (!wait_all(&bars[kPHalfA + p_bar], (pv.b >> 1) & 1, abort,
+                          p.status)) {
               ok = false;
               break;
             }
             tc_fence_after();
             umma_ts_run<false>(t_o, t_p, bv, idesc_pv, pv.j > 0);
-            if (!wait_all(&bars[kPHalfB + g], pv.b & 1, abort, p.status)) {
+            if (!wait_all(&bars[kPHalfB + p_bar], (pv.b >> 1) & 1, abort,
+                          p.status)) {
               ok = false;
               break;
             }
@@ -454,14 +461,17 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
             const uint32_t bv = v_lo + slot * kTileUnits;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-              if (!wait_all(&bars[kPHalfA + g], b & 1, abort, p.status)) {
+              const int p_bar = 2 * (b & 1) + g;
+              if (!wait_all(&bars[kPHalfA + p_bar], (b >> 1) & 1, abort,
+                            p.status)) {
                 ok = false;
                 break;
               }
               tc_fence_after();
               umma_ts_run<false>(tmem + C::kO + g * kD, tmem + g * 128, bv,
                                  idesc_pv, j > 0);
-              if (!wait_all(&bars[kPHalfB + g], b & 1, abort, p.status)) {
+              if (!wait_all(&bars[kPHalfB + p_bar], (b >> 1) & 1, abort,
+                            p.status)) {
                 ok = false;
                 break;
               }
@@ -585,7 +595,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0)
-              mbar_arrive(&bars[(q == 1 ? kPHalfA : kPHalfB) + grp]);
+              mbar_arrive(&bars[(q == 1 ? kPHalfA : kPHalfB) + 2 * (b & 1) +
+                                grp]);
           }
         }
         l += sum;

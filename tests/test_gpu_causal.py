@@ -447,3 +447,22 @@ def test_low_bits_of_values_at_the_ends_of_the_type(dim):
         torch.float32)
     assert torch.equal(full[:3], out[:3].float())
     assert full[3, :, 5].isnan().all()
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+def test_many_short_items_repeat(dim):
+    """Items of one block or two: every block loads an item's table entry, so
+    the roles of a kernel run at their most uneven."""
+    lengths = [1 + (37 * i) % 260 for i in range(900)]
+    pack, q, k, v = problem(lengths, None, 8, 4, dim)
+    dout = rows(pack.total_q, 8, dim, 9)
+    out, lse, low = kernels.causal_attention_fwd(q, k, v, pack, 0.1,
+                                                 return_low=True)
+    grads = kernels.causal_attention_bwd(q, k, v, out, dout, lse, pack, 0.1,
+                                         low=low)
+    for _ in range(40):
+        again = kernels.causal_attention_fwd(q, k, v, pack, 0.1)
+        assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+        again = kernels.causal_attention_bwd(q, k, v, out, dout, lse, pack,
+                                             0.1, low=low)
+        assert all(torch.equal(a, b) for a, b in zip(again, grads))
