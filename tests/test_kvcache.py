@@ -240,6 +240,5 @@ def test_deal_takes_every_key_item_once(lengths, kv_heads, sms):
     assert ((turns[1:] < 0) | (turns[:-1] >= 0)).all()
     cost = np.append(np.repeat(blocks + sequences.ITEM_COST, kv_heads), 0.0)
     load = cost[turns].sum(0)
-    # Each item went to the processor that had least, which then had the mean
-    # at most.
-    assert load.max() <= cost.sum() / sms + cost.max()
+    # Each item went to one of the half that had least: twice the mean at most.
+    assert load.max() <= 2 * cost.sum() / sms + cost.max()
