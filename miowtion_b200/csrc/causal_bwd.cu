@@ -20,8 +20,8 @@
 //           and dK += dS^T Q.
 // One CTA per SM, 8 compute warps, a TMA producer warp and a converged MMA
 // warp. Tensor memory decides how the two kernels overlap their products with
-// the elementwise work. dq has one accumulator, so there is room for two S buffers
-// beside dP: while the compute warps turn block b into dS, the tensor core has
+// the elementwise work. dq has one accumulator, so there is room for two S
+// buffers beside dP: while the compute warps turn block b into dS, the tensor core has
 // dP of b + 1 (as soon as dP of b is in registers), dQ of b - 1 and S of b + 1,
 // all 128 columns wide. dk/dv has two accumulators and no room: a block's 128
 // columns run as two halves of 64, and the tensor core has one half's products
@@ -36,10 +36,11 @@
 //     elementwise work on pairs (f32x2), L and D
 //     negated so that it is one fma and one add  840 and 709
 //     the diagonal's selections in a copy of the
-//     loop of their own                          802 and 615
-// which is 857 and 557 TFLOP/s of the 10 D operations a pair that a backward
-// pass is counted with, and 1,200 and 780 of the 14 D that these kernels do.
-// 16 compute warps in dkdv, a group of eight a half: 797 and 664 us; not kept.
+//     loop of their own                          800 and 615-635
+// which is 860 and 550 TFLOP/s of the 10 D operations a pair that a backward
+// pass is counted with, and 1,200 and 770 of the 14 D that these kernels do.
+// 16 compute warps in dkdv, a group of eight a half: 797 against 801 us at D =
+// 128, 664 against 617 at D = 64; not kept.
 //
 // P and dS are rounded to bf16 for their products, which costs the gradients
 // as much again as the rounding of the results: dQ and dK are 2.4e-3 off (in
@@ -889,6 +890,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool masked = __any_sync(0xffffffffu, from > 0);
         const int cmin = static_cast<int>(
             from < 0 ? 0 : (from < kTile ? from : kTile));
+        // The copy engine wrote L and D: who reads them sees their barrier
+        // (which the products, behind it, have long passed).
+        if (!wait_all(&bars[kQdFull + blk % kStages], (blk / kStages) & 1,
+                      abort, p.status)) {
+          ok = false;
+          break;
+        }
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           if (!wait_all(&bars[kStFull + hh], blk & 1, abort, p.status)) {
@@ -1093,7 +1101,8 @@ extern "C" int veda_causal_bwd(
                    aligned(dk, dk_stride_t, dk_stride_h, 16) &&
                    aligned(dv, dv_stride_t, dv_stride_h, 16),
                "out and dout must be 16-byte aligned with strides multiple of "
-               "8, out_low 8-byte aligned; dq, dk, dv 32-byte aligned with strides multiple of 16");
+               "8, out_low 8-byte aligned; dq, dk, dv 32-byte aligned with "
+               "strides multiple of 16");
   cudaStream_t s = as_stream(stream);
   const int group = n_heads / kv_heads;
   const int tokens = kTile / group;

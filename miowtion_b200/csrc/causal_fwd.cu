@@ -8,8 +8,8 @@
 // tiles A and B of one key head (causal.cuh: 128 rows of tokens x heads) and
 // streams the key and value tiles of 128 keys once for both. Tensor memory
 // (512 columns) holds an accumulator O for each tile and two (D = 128) or three
-// (D = 64) buffers of 128 columns for scores, taken in turn by A(0), B(0), A(1),
-// B(1), ...
+// (D = 64) buffers of 128 columns for scores, taken in turn by A(0), B(0),
+// A(1), B(1), ...
 //   warps 0-7   softmax and epilogue: warps 4g .. 4g + 3 own tile g, a query
 //               row a thread over all 128 keys, with the running maximum and
 //               sum of an online softmax (the maximum moves only when it
@@ -22,7 +22,7 @@
 //               buffers (the scores take the place of the weights that the
 //               product before them read); with three, QK_B(b + 1) follows
 //               PV_A(b) and QK_A(b + 2) follows PV_B(b), so that a tile's next
-//               scores wait for nothing of its own (644 -> 711 TFLOP/s on
+//               scores wait for nothing of its own (644 -> 695-710 TFLOP/s on
 //               16,384 tokens, 24/6 heads).
 //   warps 10-11 idle; they complete the third warpgroup, whose registers go
 //               to the softmax warps (setmaxnreg).
@@ -31,13 +31,13 @@
 // so the two softmaxes do not run at the same time and wait at the same time.
 // (With an issuer for QK and one for PV, P_A and P_B that became ready
 // together led to PV_A, PV_B, QK_A, QK_B, which keeps them together: 1,050
-// against 1,230 TFLOP/s on a causal sequence of 16,384 tokens, 24/6 heads, D =
-// 128. Measured on it and not kept: a block's first 32 weights computed
-// against the reference so far while the other scores come in, 1,191; a
-// quarter, half of the exponentials on the FMA pipes, 1,210 and 1,117 against
-// 1,247 without.) The blocks of
-// consecutive items form one stream, so the next item's first scores are
-// computed while this item's epilogue runs. One issuer also makes barriers
+// against 1,250-1,300 TFLOP/s on a causal sequence of 16,384 tokens, 24/6
+// heads, D = 128. Measured on it and not kept: a block's first 32 weights
+// computed against the reference so far while the other scores come in, 1,191;
+// an eighth, a quarter, half of the exponentials as polynomials, 1,223, 1,177
+// to 1,210 and 1,117 against 1,245; at D = 64 678 and 658 against 708.) The
+// blocks of consecutive items form one stream, so the next item's first scores
+// are computed while this item's epilogue runs. One issuer also makes barriers
 // superfluous: the warps that write P of an item's first block have read the
 // previous item's O, and with two buffers the scores of block b arrive after
 // the product of block b - 1.
