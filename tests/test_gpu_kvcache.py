@@ -418,3 +418,32 @@ def test_calls_on_two_streams():
                 out.append(cache.attend(q, table, lengths))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for out in outs for o in out)
+
+
+@pytest.mark.parametrize('storage', STORAGES)
+@pytest.mark.parametrize('dim', [64, 128])
+def test_sums_over_long_runs_of_keys_do_not_drift(storage, dim):
+    """Many contexts (here of shared pages) make a warp's run of keys long, and
+    equal weights make the result small beside the values: the mean of n
+    values, whose sums may lose fp32's bits only of what they add up."""
+    n, rows_, heads = 512, 32768, 2
+    gen = torch.Generator().manual_seed(61)
+    # Integers with the same largest magnitude in every row: every weight times
+    # its scale is the same power of two, and no weight is rounded.
+    v = torch.randint(-14, 15, (rows_, heads, dim), generator=gen).float() * 8
+    v[:, :, 3] = 127
+    v = v.bfloat16().to(DEV)
+    k = rows(rows_, heads, dim, 62)
+    cache = kvcache.PagedCache.empty(rows_ // 256, 256, heads, dim, storage,
+                                     DEV)
+    table = torch.arange(rows_ // 256, dtype=torch.int32, device=DEV)
+    start = torch.zeros(1, dtype=torch.int32, device=DEV)
+    pack = sequences.SequencePack([rows_], device=DEV)
+    cache.write(k, v, table[None], start, pack)
+    q = torch.zeros(n, 4, dim, dtype=torch.bfloat16, device=DEV)
+    out = cache.attend(q, table.repeat(n, 1),
+                       torch.full((n,), rows_, dtype=torch.int32, device=DEV))
+    want = held(v, storage).mean(0).repeat_interleave(2, 0)
+    size = held(v, storage).abs().mean(0).repeat_interleave(2, 0)
+    bound = 2.0 ** -8 * want.abs() + 2.0 ** -14 * size
+    assert ((out.double() - want).abs() <= bound).all()
