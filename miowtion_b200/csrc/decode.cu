@@ -403,6 +403,7 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
   static_assert(kRingBytes >= kRows * S::kJoinFloats * 4,
                 "a last part fits the ring");
   static_assert(kWarps * kRingBytes >= kThreads * 8, "find_run's numbers fit");
+  static_assert(kStages <= 32, "a bit a stage");
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t s_sums[kWarps];
   __shared__ Part s_parts[kWarps][2];
@@ -464,6 +465,10 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
   };
   if (ld.valid()) look_up();
   int ld_stage = 0;
+  // Stages of the ring whose chunk lies in a page that does not exist (a bit
+  // each): its keys are absent, which only the scores' mask can tell from rows
+  // of zeros.
+  unsigned absent = 0;
   // This lane's 16-byte pieces of a tile are 512 bytes apart; where pieces move
   // with the row, every other one lies at the other side of bit 6.
   const uint32_t ring_at = smem_u32(ring);
@@ -481,7 +486,9 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
       const int key0 = ld_chunk * kChunk;
       const bool ok = next_page >= 0 && next_page < p.c.n_pages;
       if (!ok && lane == 0) raise_status(p.status, VEDA_ERR_INVALID);
-      // Keys of the chunk that exist; those of a bad page count as absent.
+      absent = (absent & ~(1u << ld_stage)) |
+               (static_cast<unsigned>(!ok) << ld_stage);
+      // Rows of the chunk to load; the others become zeros.
       const int live = ok ? ld.length - key0 : 0;
       const int64_t row0 =
           ok ? (((static_cast<int64_t>(next_page) * p.c.kv_heads +
@@ -627,9 +634,15 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
       cp_async_wait<kStages - 1 - kN>();
       __syncwarp();
       uint32_t base[kN];
+      int live[kN];  // keys of each chunk that exist (16 and more: all)
+      bool whole = true;
 #pragma unroll
       for (int u = 0; u < kN; ++u) {
         base[u] = ring_at + stage * S::kStageBytes;
+        live[u] = (absent >> stage) & 1u
+                      ? 0
+                      : seg.length - (chunk + u) * kChunk;
+        whole &= live[u] >= kChunk;
         stage = stage + 1 == kStages ? 0 : stage + 1;
       }
       // The chunks have landed, and the whole warp has read the stages before
@@ -662,7 +675,6 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
         }
       }
       // Columns of this thread: keys 2 quad + {0, 1} of each tile of 8.
-      const int live = seg.length - chunk * kChunk;
       float top[2] = {-INFINITY, -INFINITY};
       [[maybe_unused]] float v_top = 0.f;
       [[maybe_unused]] float2 vs[2 * kN];
@@ -691,12 +703,12 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
             b *= row_scale[half];
           }
         }
-        if (live < kN * kChunk) {
-          const int key = nt * 8 + quad * 2;
+        if (!whole) {
+          const int key = (nt & 1) * 8 + quad * 2;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            if (key >= live) s[nt][2 * half] = -INFINITY;
-            if (key + 1 >= live) s[nt][2 * half + 1] = -INFINITY;
+            if (key >= live[nt / 2]) s[nt][2 * half] = -INFINITY;
+            if (key + 1 >= live[nt / 2]) s[nt][2 * half + 1] = -INFINITY;
           }
         }
 #pragma unroll

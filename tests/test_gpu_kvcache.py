@@ -447,3 +447,57 @@ def test_sums_over_long_runs_of_keys_do_not_drift(storage, dim):
     size = held(v, storage).abs().mean(0).repeat_interleave(2, 0)
     bound = 2.0 ** -8 * want.abs() + 2.0 ** -14 * size
     assert ((out.double() - want).abs() <= bound).all()
+
+
+def defined(q, k, v, scale, w):
+    """(out, lse) of one sequence's query [heads, D] over the rows k, v
+    [n, kv_heads, D] (fp64, as held), and their bounds (see above)."""
+    group = q.shape[0] // k.shape[1]
+    k, v = (x.repeat_interleave(group, 1) for x in (k, v))
+    q = q.double()
+    s = torch.einsum('hd,jhd->hj', q, k) * scale
+    lse = torch.logsumexp(s, -1)
+    p = torch.exp(s - lse[:, None])
+    want = torch.einsum('hj,jhd->hd', p, v)
+    size = torch.einsum('hd,jhd->hj', q.abs(), k.abs()).amax(-1) * scale
+    off = 2.0 ** -24 * (q.shape[1] + 8) * size
+    bound = ((w + 2.0 ** -14 + 2 * off)[:, None] *
+             torch.einsum('hj,jhd->hd', p, v.abs()) +
+             2.0 ** -8 * want.abs() + 1e-30)
+    return want, bound, lse, off + 2.0 ** -20 * (1 + lse.abs())
+
+
+@pytest.mark.parametrize('storage', STORAGES)
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('heads', [2, 40])
+def test_keys_of_pages_that_do_not_exist_are_absent(storage, dim, heads):
+    """The attention is that over the other keys, whichever page of a context
+    is missing; without any it is that of a context without rows."""
+    size = 16
+    contexts = [20, 40, 70, 33, 3000, 3000]
+    missing = [{1}, {0}, {1, 2}, {0, 1, 2}, set(range(1, 188, 3)),
+               set(range(188))]
+    cache, table, _, k, v = filled(storage, contexts, size, 2, dim, 47)
+    bad = [-1, cache.n_pages, 2 ** 31 - 1]
+    for b, pages in enumerate(missing):
+        for i, page in enumerate(pages):
+            table[b, page] = bad[(b + i) % 3]
+    q = rows(len(contexts), heads, dim, 48)
+    lengths = torch.tensor(contexts, dtype=torch.int32, device=DEV)
+    out, lse = cache.attend(q, table, lengths, return_lse=True)
+    assert _lib.device_status(reset=True) == _lib.VEDA_ERR_INVALID
+    k, v = held(k, storage), held(v, storage)
+    w = 2.0 ** -8 if storage == 'bf16' else 2.0 ** -11
+    at = 0
+    for b, c in enumerate(contexts):
+        keep = torch.tensor([j // size not in missing[b] for j in range(c)],
+                            device=DEV)
+        kb, vb = k[at:at + c][keep], v[at:at + c][keep]
+        at += c
+        if not keep.any():
+            assert (out[b] == 0).all() and (lse[b] == -math.inf).all()
+            continue
+        want, bound, want_lse, lse_bound = defined(q[b], kb, vb, dim ** -0.5,
+                                                   w)
+        assert ((out[b].double() - want).abs() <= bound).all(), b
+        assert ((lse[b].double() - want_lse).abs() <= lse_bound).all(), b
