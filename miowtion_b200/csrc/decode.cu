@@ -39,9 +39,12 @@
 // taken as 1024 + (code + 128), less 1152, an instruction more a pair (64 x
 // 8,192 rows, 8 heads, D = 128: 222 us against 215). The order of d
 // inside the first product and of the columns of the second is free, and is
-// the one that the bytes of a word have. A key's scale multiplies its scores; a
-// value row's scale multiplies its weights, relative to the largest scale met
-// so far so that they stay inside fp16. q is brought to [1, 2) per head by a
+// the one that the bytes of a word have. A key's scale multiplies its scores. A
+// value row's scale multiplies its weights, and these products are taken
+// relative to the largest of the head so far, so that they stay inside fp16 and
+// what a row adds to the result, not its size, decides which bits it keeps
+// (relative to the largest scale, a large row that nothing attends to cost all
+// others theirs; 2 % of the time). q is brought to [1, 2) per head by a
 // power of two, so it loses nothing in fp16 but elements 2^-14 below the
 // head's largest. Scores, maxima, sums and accumulators are fp32; weights are
 // rounded to the 16-bit type of the products (bf16 pages: bf16), as everywhere
@@ -611,11 +614,12 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
 
     // ---- the piece's chunks, kPair a step ----
     // m: the rows' references (-inf before the first key), m_ref: the same or
-    // 0; v_ref, v_inv: the values' reference and kWeight over it.
+    // 0. 8-bit pages: c_ref, the reference of weight times value scale (0
+    // before the first key), and c_inv, kWeight over it; o is held in units of
+    // c_ref / kWeight.
     float m[2] = {-INFINITY, -INFINITY}, m_ref[2] = {0.f, 0.f};
     float l[2] = {0.f, 0.f};
-    float v_ref = 0.f;
-    [[maybe_unused]] float v_inv = 0.f;
+    [[maybe_unused]] float c_ref[2] = {0.f, 0.f}, c_inv[2] = {0.f, 0.f};
     float o[kD / 8][4];
 #pragma unroll
     for (int i = 0; i < kD / 8; ++i)
@@ -686,7 +690,7 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
                               (nt & 1) * 32 + quad * 8;
           ks = lds64(at);
           vs[nt] = lds64(at + 64);
-          v_top = fmaxf(v_top, fmaxf(vs[nt].x, vs[nt].y));
+          v_top = fmaxf(v_top, fmaxf(fabsf(vs[nt].x), fabsf(vs[nt].y)));
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -716,13 +720,21 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
           top[half] = fmaxf(top[half],
                             fmaxf(s[nt][2 * half], s[nt][2 * half + 1]));
       }
-      // The references move only when they must: a maximum by more than 2^8,
-      // the values' scale by more than 2. (A row's maximum is taken over its
-      // four threads only then.) fp16 weights carry a factor 2^6 (kWeight)
-      // and stay below 2^15; those down to 2^-20 of the references keep all of
-      // fp16's bits.
-      const bool grow = top[0] > m[0] + 8.f || top[1] > m[1] + 8.f ||
-                        (kHalf && v_top > 2.f * v_ref);
+      // The references move only when they must. That of the weights: when a
+      // score is more than 2^8 above it (bf16), or above it at all (8-bit,
+      // where it is put 2^8 above the maximum, so that a weight times any value
+      // scale is finite). That of weights times scales: when one may be more
+      // than 2^9 above it, so that the fp16 weights, with a factor 2^6
+      // (kWeight), stay below 2^15; those down to 2^-20 of it keep all of
+      // fp16's bits. (Maxima over a row's four threads, and of the products
+      // themselves, are taken only then.)
+      constexpr float kAbove = kHalf ? 8.f : 0.f;
+      constexpr float kSlack = 8.f - kAbove;
+      bool grow = top[0] > m[0] + kSlack || top[1] > m[1] + kSlack;
+      if constexpr (kHalf)
+        grow = grow ||
+               ex2_approx(top[0] - m_ref[0]) * v_top > 512.f * c_ref[0] ||
+               ex2_approx(top[1] - m_ref[1]) * v_top > 512.f * c_ref[1];
       if (__any_sync(0xffffffffu, grow)) {
         float f[2];
 #pragma unroll
@@ -730,25 +742,35 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
           float x = top[half];
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          const float next = fmaxf(m[half], x);
-          f[half] = m[half] == -INFINITY ? 0.f : ex2_approx(m[half] - next);
-          m[half] = next;
-          // m is -inf where no key of the row has existed so far.
-          m_ref[half] = next == -INFINITY ? 0.f : next;
-          l[half] *= f[half];
-        }
-        if constexpr (kHalf) {
-          float x = v_top;
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          // (Held above 2^-100: its inverse exists.)
-          const float next =
-              x > 0.f ? fmaxf(fmaxf(v_ref, x), 0x1p-100f) : v_ref;
-          const float g = v_ref > 0.f ? v_ref / next : 0.f;
-          v_ref = next;
-          v_inv = next > 0.f ? kWeight / next : 0.f;
-          f[0] *= g;
-          f[1] *= g;
+          if (kHalf && !(x > m[half])) {
+            f[half] = 1.f;
+          } else {
+            const float next = fmaxf(m[half], x + kAbove);
+            f[half] = m[half] == -INFINITY ? 0.f : ex2_approx(m[half] - next);
+            m[half] = next;
+            // m is -inf where no key of the row has existed so far.
+            m_ref[half] = next == -INFINITY ? 0.f : next;
+            l[half] *= f[half];
+          }
+          if constexpr (kHalf) {
+            // What o holds keeps its unit, which shrinks with the weights, and
+            // goes over to the new one.
+            float c = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < 2 * kN; ++nt)
+              c = fmaxf(c, fmaxf(ex2_approx(s[nt][2 * half] - m_ref[half]) *
+                                     fabsf(vs[nt].x),
+                                 ex2_approx(s[nt][2 * half + 1] -
+                                            m_ref[half]) *
+                                     fabsf(vs[nt].y)));
+            c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, 1));
+            c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, 2));
+            const float held = c_ref[half] * f[half];
+            // (Above 2^-100: its inverse exists.)
+            c_ref[half] = fmaxf(fmaxf(held, c), 0x1p-100f);
+            c_inv[half] = kWeight / c_ref[half];
+            f[half] = held / c_ref[half];
+          }
         }
 #pragma unroll
         for (int i = 0; i < kD / 8; ++i) {
@@ -768,8 +790,9 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
           const float p1 = ex2_approx(s[nt][2 * half + 1] - m_ref[half]);
           l[half] += p0 + p1;
           if constexpr (kHalf)
-            a[nt / 2][(nt & 1) * 2 + half] = pack_half(
-                p0 * (vs[nt].x * v_inv), p1 * (vs[nt].y * v_inv));
+            a[nt / 2][(nt & 1) * 2 + half] =
+                pack_half(p0 * vs[nt].x * c_inv[half],
+                          p1 * vs[nt].y * c_inv[half]);
           else
             a[nt / 2][(nt & 1) * 2 + half] = pack_bf16(p0, p1);
         }
@@ -818,7 +841,8 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
       l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
       l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
     }
-    const float unit = kHalf ? v_ref * (1.f / kWeight) : 1.f;
+    const float unit[2] = {kHalf ? c_ref[0] * (1.f / kWeight) : 1.f,
+                           kHalf ? c_ref[1] * (1.f / kWeight) : 1.f};
     const bool starts = seg.c0 == 0, ends = seg.c1 == seg.n;
     const int slot = starts ? 1 : 0;
     if (!(starts && ends)) {
@@ -838,7 +862,7 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
       const int64_t at =
           static_cast<int64_t>(seg.b) * (p.c.kv_heads * p.group) + head0 + r;
       if (starts && ends) {
-        const float inv = l[half] == 0.f ? 0.f : unit / l[half];
+        const float inv = l[half] == 0.f ? 0.f : unit[half] / l[half];
         __nv_bfloat16* dst = p.out + at * kD;
 #pragma unroll
         for (int dt = 0; dt < kD / 8; dt += 2) {
@@ -866,10 +890,10 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
         }
 #pragma unroll
         for (int dt = 0; dt < kD / 8; dt += 2) {
-          const float a0 = o[dt][2 * half] * unit;
-          const float a1 = o[dt][2 * half + 1] * unit;
-          const float b0 = o[dt + 1][2 * half] * unit;
-          const float b1 = o[dt + 1][2 * half + 1] * unit;
+          const float a0 = o[dt][2 * half] * unit[half];
+          const float a1 = o[dt][2 * half + 1] * unit[half];
+          const float b0 = o[dt + 1][2 * half] * unit[half];
+          const float b1 = o[dt + 1][2 * half + 1] * unit[half];
           if constexpr (!kHalf) {
             *reinterpret_cast<float2*>(dst + dt * 8 + quad * 2) =
                 make_float2(a0, a1);

@@ -501,3 +501,41 @@ def test_keys_of_pages_that_do_not_exist_are_absent(storage, dim, heads):
                                                    w)
         assert ((out[b].double() - want).abs() <= bound).all(), b
         assert ((lse[b].double() - want_lse).abs() <= lse_bound).all(), b
+
+
+@pytest.mark.parametrize('storage', STORAGES)
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('place', [0, 5, 150, 2999])
+@pytest.mark.parametrize('power', [20, 30, 60])
+def test_a_large_value_row_without_weight_costs_no_bits(storage, dim, place,
+                                                        power):
+    """A value row that nothing attends to may be any number of times larger
+    than those that are attended to."""
+    contexts, heads = [3000, 40], 3
+    cache, table, pack, k, v = filled(storage, contexts, 64, heads, dim, 51)
+    q = rows(2, heads, dim, 52)
+    # Its score is about -16 |q|^2 scale: -128 at least.
+    k[place], v[place] = -16 * q[0], v[place] * 2.0 ** power
+    starts = torch.zeros(2, dtype=torch.int32, device=DEV)
+    cache.write(k, v, table, starts, pack)
+    check_attend(cache, table, q, k, v, contexts, storage)
+
+
+@pytest.mark.parametrize('storage', STORAGES)
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('place', [0, 77])
+def test_a_row_with_all_the_weight_may_hold_the_smallest_values(storage, dim,
+                                                                place):
+    """A key that takes nearly all the weight and has values of 2^-40 leaves
+    the others' their bits: weights of e^-20 and values of 1."""
+    contexts, heads = [400], 2
+    cache, table, pack, k, v = filled(storage, contexts, 16, heads, dim, 53)
+    q = rows(1, heads, dim, 54)
+    scale = dim ** -0.5
+    top = q[0].double().square().sum(-1, keepdim=True) * scale
+    k = (k * 0.05).bfloat16()
+    k[place] = (q[0].double() * (20 / top)).bfloat16()
+    v[place] = (v[place] * 2.0 ** -40).bfloat16()
+    starts = torch.zeros(1, dtype=torch.int32, device=DEV)
+    cache.write(k, v, table, starts, pack)
+    check_attend(cache, table, q, k, v, contexts, storage)
