@@ -577,9 +577,10 @@ int veda_causal_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h,
 
 /* Stores packed rows k, v [n_tokens, kv_heads, head_dim] bf16: row
  * offsets[b] + i (i < offsets[b + 1] - offsets[b]) becomes row starts[b] + i
- * of sequence b. int8: scale max|x| / 127; e4m3: scale 2^e, e the smallest
- * integer >= -120 with max|x| <= 448 * 2^e; codes rounded to nearest, ties to
- * even; a row with a non-finite value gets the scale NaN. */
+ * of sequence b; rows before offsets[0] or from offsets[n_seqs] on belong to
+ * none and are stored nowhere. int8: scale max|x| / 127; e4m3: scale 2^e, e
+ * the smallest integer >= -120 with max|x| <= 448 * 2^e; codes rounded to
+ * nearest, ties to even; a row with a non-finite value gets the scale NaN. */
 int veda_cache_write(void* k_pages, void* v_pages, float* k_scale,
                      float* v_scale, int64_t n_pages, int32_t page_size,
                      int32_t kv_heads, int32_t head_dim, int32_t storage,
@@ -592,7 +593,8 @@ int veda_cache_write(void* k_pages, void* v_pages, float* k_scale,
 
 /* Reads contexts back as packed bf16 rows [n_tokens, kv_heads, head_dim]:
  * row offsets[b] + j receives row j of sequence b (code * scale, rounded
- * once; zeros for a place that does not exist). */
+ * once; zeros for a place that does not exist); rows that belong to no
+ * sequence are left as they were. */
 int veda_cache_read(const void* k_pages, const void* v_pages,
                     const float* k_scale, const float* v_scale,
                     int64_t n_pages, int32_t page_size, int32_t kv_heads,

@@ -38,7 +38,8 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// The sequence that packed row t belongs to: offsets[b] <= t < offsets[b+1].
+// The sequence that packed row t belongs to: offsets[b] <= t < offsets[b+1];
+// some sequence for a row outside all of them.
 __device__ __forceinline__ int find_sequence(const int32_t* offsets, int n,
                                              int64_t t) {
   int lo = 0, hi = n - 1;
@@ -211,10 +212,13 @@ __global__ void __launch_bounds__(kThreads)
     my_h = r - my_t * c.kv_heads;
     if (row < n_rows && wl < kWide * kBatch) {
       const int b = find_sequence(offsets, c.n_seqs, my_t);
-      my_at = cache_row(c, b, my_h,
-                        static_cast<int64_t>(starts[b]) +
-                            (my_t - offsets[b]));
-      if (my_at < 0) raise_status(status, VEDA_ERR_INVALID);
+      const int first = offsets[b];
+      // (A row before the first sequence or behind the last is stored nowhere.)
+      if (my_t >= first && my_t < offsets[b + 1]) {
+        my_at = cache_row(c, b, my_h,
+                          static_cast<int64_t>(starts[b]) + (my_t - first));
+        if (my_at < 0) raise_status(status, VEDA_ERR_INVALID);
+      }
     }
   }
   uint4 kw[kBatch], vw[kBatch];
@@ -267,8 +271,10 @@ __global__ void __launch_bounds__(kThreads)
   const int lane = threadIdx.x % kGroup, wl = threadIdx.x % 32;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kGroups * kBatch +
                        threadIdx.x / kGroup;
-  // As in the other kernel, a lane a row.
-  int64_t my_at = -1;
+  // As in the other kernel, a lane a row. (kNoRow: a row before the first
+  // sequence or behind the last, which is not written.)
+  constexpr int64_t kNoRow = -2;
+  int64_t my_at = kNoRow;
   {
     const int64_t row = row0 - wl / kGroup +
                         (wl / kWide % kBatch) * kGroups + wl % kWide;
@@ -276,8 +282,11 @@ __global__ void __launch_bounds__(kThreads)
       const int t = static_cast<int>(row) / c.kv_heads;
       const int h = static_cast<int>(row) - t * c.kv_heads;
       const int b = find_sequence(offsets, c.n_seqs, t);
-      my_at = cache_row(c, b, h, t - offsets[b]);
-      if (my_at < 0) raise_status(status, VEDA_ERR_INVALID);
+      const int first = offsets[b];
+      if (t >= first && t < offsets[b + 1]) {
+        my_at = cache_row(c, b, h, t - first);
+        if (my_at < 0) raise_status(status, VEDA_ERR_INVALID);
+      }
     }
   }
   // Rows that are nowhere read as zeros (and load the cache's first row: with
@@ -287,11 +296,12 @@ __global__ void __launch_bounds__(kThreads)
                                          uint2>::type;
   Word kw[kBatch], vw[kBatch];
   float ks[kBatch], vs[kBatch];
-  bool there[kBatch];
+  bool there[kBatch], taken[kBatch];
 #pragma unroll
   for (int i = 0; i < kBatch; ++i) {
     int64_t at = __shfl_sync(0xffffffffu, my_at, i * kWide + wl / kGroup);
     there[i] = at >= 0;
+    taken[i] = at != kNoRow;
     if (at < 0) at = 0;
     kw[i] = reinterpret_cast<const Word*>(c.k)[at * kGroup + lane];
     vw[i] = reinterpret_cast<const Word*>(c.v)[at * kGroup + lane];
@@ -304,7 +314,7 @@ __global__ void __launch_bounds__(kThreads)
   for (int i = 0; i < kBatch; ++i) {
     // Packed outputs [rows, kv_heads, D]: row-major in (token, head).
     const int64_t row = row0 + i * kGroups;
-    if (row >= n_rows) continue;
+    if (!taken[i]) continue;
     uint4 ko, vo;
     if constexpr (kStore == kStoreBf16) {
       ko = kw[i];

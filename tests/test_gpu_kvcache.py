@@ -539,3 +539,35 @@ def test_a_row_with_all_the_weight_may_hold_the_smallest_values(storage, dim,
     starts = torch.zeros(1, dtype=torch.int32, device=DEV)
     cache.write(k, v, table, starts, pack)
     check_attend(cache, table, q, k, v, contexts, storage)
+
+
+def pages_of(cache):
+    return [t.clone().view(torch.uint8) for t in
+            (cache.k, cache.v, cache.k_scale, cache.v_scale) if t is not None]
+
+
+@pytest.mark.parametrize('storage', STORAGES)
+def test_rows_of_no_sequence_are_left_as_they_are(storage):
+    """Offsets on the device that begin behind the first row or end before the
+    last (a padded batch): the rows outside are neither stored nor read."""
+    size, heads, dim = 16, 2, 64
+    cache, table, pack, k, v = filled(storage, [40, 48], size, heads, dim, 57)
+    starts = torch.tensor([3, 30], dtype=torch.int32, device=DEV)
+    new_k, new_v = rows(20, heads, dim, 58), rows(20, heads, dim, 59)
+    offsets = torch.tensor([4, 9, 15], dtype=torch.int32, device=DEV)
+    exact = sequences.SequencePack([5, 6], device=DEV)
+    cache.write(new_k[4:15], new_v[4:15], table, starts, exact)
+    want = pages_of(cache)
+    cache.write(k, v, table, torch.zeros_like(starts), pack)
+    padded = sequences.SequencePack([10, 10], device=DEV)
+    padded.q_offsets.copy_(offsets)
+    cache.write(new_k, new_v, table, starts, padded)
+    assert all(torch.equal(a, b) for a, b in zip(want, pages_of(cache)))
+    got = [torch.full((20, heads, dim), 7.0, dtype=torch.bfloat16, device=DEV)
+           for _ in range(2)]
+    short = cache.read(table, exact)
+    _lib.call_on(0, 'veda_cache_read', *cache._view(table, 2),
+                 offsets.data_ptr(), 20, *(t.data_ptr() for t in got))
+    for t, inside in zip(got, short):
+        assert torch.equal(t[4:15], inside)
+        assert (t[:4] == 7).all() and (t[15:] == 7).all()
