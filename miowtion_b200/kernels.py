@@ -18,6 +18,7 @@ import math
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from miowtion_b200 import _lib
 from miowtion_b200 import mask as veda_mask
@@ -152,6 +153,16 @@ def aligned_rows(t: torch.Tensor) -> torch.Tensor:
     if last == 1 and not (rows % 8 or heads % 8 or t.data_ptr() % 16):
         return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def refuse_tangents(op: str, *tensors: torch.Tensor) -> None:
+    """Raises ValueError where a tensor carries a forward-mode tangent: a
+    kernel reads values only, and its output would be without one."""
+    # pylint: disable=protected-access
+    if forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():
+        return
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f'{op} has no forward-mode derivative')
 
 
 # CUDA devices on which the kernels have been found to run.
@@ -464,6 +475,7 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         NotImplementedError: Off B200 (no fallback).
         ValueError: If gradients are required for a subset of query tiles.
     """
+    refuse_tangents('block_sparse_attention', q, k, v)
     _require(q, 'block_sparse_attention')
     needs_grad = torch.is_grad_enabled() and any(
         t.requires_grad for t in (q, k, v))
@@ -643,7 +655,7 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         return_lse: Also return the [total_q, heads] fp32 log-sum-exp of the
             scaled scores (no gradient flows through it).
 
-    q, k and v receive gradients (once differentiable), those of a key head
+    q, k and v receive gradients (in reverse mode, once), those of a key head
     summed over its query heads; repeats are bit-identical. For them the call
     keeps q, k, v, out, the log-sum-exp and one more byte for each element of
     out (the bits behind bf16's).
@@ -660,6 +672,7 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     autograd, no graph of the same leaves that another stream recorded may be
     alive then: its accumulation nodes would wait for that stream.
     """
+    refuse_tangents('causal_attention', q, k, v)
     scale = softmax_scale(scale, q.shape[-1])
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
                                     or v.requires_grad):

@@ -184,6 +184,7 @@ class PagedCache:
                     or t.device != self.device):
                 raise ValueError(f'{name} must be bf16 {list(rows)} on '
                                  f'{self.device}')
+        kernels.refuse_tangents('PagedCache.write', k, v)
         view = self._view(table, pack.n_sequences)
         start_args = self._index(starts, 'starts', pack.n_sequences)
         self._pack(pack)
@@ -238,6 +239,7 @@ class PagedCache:
                              f'{self.kv_heads}')
         if q.requires_grad and torch.is_grad_enabled():
             raise ValueError('attention over the cache has no gradient')
+        kernels.refuse_tangents('PagedCache.attend', q)
         view = self._view(table, n)
         length_args = self._index(lengths, 'lengths', n)
         scale = kernels.softmax_scale(scale, dim)

@@ -242,3 +242,40 @@ def test_deal_takes_every_key_item_once(lengths, kv_heads, sms):
     load = cost[turns].sum(0)
     # Each item went to one of the half that had least: twice the mean at most.
     assert load.max() <= 2 * cost.sum() / sms + cost.max()
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor has no requires_grad, and a kernel would read its values
+    and drop its tangent."""
+    from torch.autograd import forward_ad
+
+    from miowtion_b200 import kernels
+    p = pack([3, 2])
+    q = torch.zeros(5, 4, 64, dtype=torch.bfloat16)
+    k = torch.zeros(5, 2, 64, dtype=torch.bfloat16)
+    c = cache('bf16')
+    table = torch.zeros(2, 1, dtype=torch.int32)
+    two = torch.zeros(2, dtype=torch.int32)
+    rows = torch.zeros(128, 2, 128, dtype=torch.bfloat16)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        calls = [lambda: kernels.causal_attention(dual(q), k, k, p),
+                 lambda: kernels.causal_attention(q, dual(k), k, p),
+                 lambda: kernels.causal_attention(q, k, dual(k), p),
+                 lambda: c.write(dual(k), k, table, two, p),
+                 lambda: c.write(k, dual(k), table, two, p),
+                 lambda: c.attend(dual(q[:2]), table, two),
+                 lambda: kernels.block_sparse_attention(
+                     rows, rows, dual(rows), None, None)]
+        for call in calls:
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad):
+                    with pytest.raises(ValueError, match='forward-mode'):
+                        call()
+        # Without tangents, or where they are switched off, as ever.
+        with pytest.raises(NotImplementedError, match='unavailable'):
+            kernels.causal_attention(q, k, k, p)
+        with torch.inference_mode():
+            with pytest.raises(NotImplementedError, match='unavailable'):
+                kernels.causal_attention(dual(q), k, k, p)
