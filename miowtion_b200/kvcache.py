@@ -173,7 +173,7 @@ class PagedCache:
 
         Args:
             k, v: [pack.total_q, kv_heads, D] bf16, contiguous in D (their
-                other strides multiples of 8 elements).
+                other strides multiples of 8 elements), without gradients.
             table: [n_sequences, max_pages] int32 page numbers.
             starts: [n_sequences] int32, rows already in each context.
             pack: The rows of each sequence (its q_lengths).
@@ -184,6 +184,9 @@ class PagedCache:
                     or t.device != self.device):
                 raise ValueError(f'{name} must be bf16 {list(rows)} on '
                                  f'{self.device}')
+        if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+            raise ValueError('rows of the cache carry no gradient: write them '
+                             'under torch.no_grad() or detached')
         kernels.refuse_tangents('PagedCache.write', k, v)
         view = self._view(table, pack.n_sequences)
         start_args = self._index(starts, 'starts', pack.n_sequences)

@@ -279,3 +279,17 @@ def test_forward_mode_derivatives_are_refused():
         with torch.inference_mode():
             with pytest.raises(NotImplementedError, match='unavailable'):
                 kernels.causal_attention(dual(q), k, k, p)
+
+
+def test_a_write_refuses_rows_whose_gradient_it_would_lose():
+    c = cache('bf16')
+    k = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    leaf = k.clone().requires_grad_()
+    table = torch.zeros(2, 1, dtype=torch.int32)
+    two = torch.zeros(2, dtype=torch.int32)
+    for args in ((leaf, k), (k, leaf), (leaf * 2, k)):
+        with pytest.raises(ValueError, match='no gradient'):
+            c.write(*args, table, two, pack([1, 1]))
+        with torch.no_grad():
+            with pytest.raises(NotImplementedError, match='unavailable'):
+                c.write(*args, table, two, pack([1, 1]))
