@@ -505,7 +505,8 @@ int veda_compensate(const void* o_kept, int64_t ok_stride_n,
  * h reads key head h / (n_heads / kv_heads). Sequences own consecutive rows;
  * token i of a sequence of n queries and c keys sees keys j <= i + c - n. The
  * work items describe the sequences (miowtion_b200/sequences.py builds them;
- * csrc/causal.cuh gives the fields) and must agree with the sizes. */
+ * csrc/causal.cuh gives the fields), must agree with the sizes and lie at
+ * 16-byte boundaries (k_order at a 4-byte one). */
 
 /* Bytes of workspace veda_causal_fwd needs for n_parts parts (0 for none); -1
  * for sizes out of range. */

@@ -1065,8 +1065,6 @@ extern "C" int veda_causal_bwd(
     void* dk, int64_t dk_stride_t, int64_t dk_stride_h, void* dv,
     int64_t dv_stride_t, int64_t dv_stride_h, float softmax_scale,
     void* workspace, int64_t workspace_bytes, void* stream) {
-  int rc = require_sm100("veda_causal_bwd");
-  if (rc != VEDA_OK) return rc;
   VEDA_REQUIRE(head_dim == 64 || head_dim == 128,
                "head_dim must be 64 or 128");
   VEDA_REQUIRE(kv_heads >= 1 && n_heads >= 1 && n_heads % kv_heads == 0 &&
@@ -1103,6 +1101,12 @@ extern "C" int veda_causal_bwd(
                "out and dout must be 16-byte aligned with strides multiple of "
                "8, out_low 8-byte aligned; dq, dk, dv 32-byte aligned with "
                "strides multiple of 16");
+  VEDA_REQUIRE(reinterpret_cast<uintptr_t>(q_items) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(k_items) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(k_order) % 4 == 0 &&
+                   reinterpret_cast<uintptr_t>(lse) % 4 == 0,
+               "q_items and k_items must be 16-byte aligned, k_order and lse "
+               "4-byte aligned");
   cudaStream_t s = as_stream(stream);
   const int group = n_heads / kv_heads;
   const int tokens = kTile / group;
@@ -1112,6 +1116,8 @@ extern "C" int veda_causal_bwd(
                "k, v and k_items are required");
   VEDA_REQUIRE(k_order == nullptr || (k_ctas >= 1 && k_turns >= 1),
                "k_order needs its CTAs and turns");
+  int rc = require_sm100("veda_causal_bwd");
+  if (rc != VEDA_OK) return rc;
   causal::Maps m;
   if (total_q > 0) {
     rc = causal::make_rows_map(&m.q, q, total_q, n_heads, head_dim,

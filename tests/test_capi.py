@@ -66,3 +66,19 @@ def test_sm_reserve_is_validated_on_the_host(lib):
     with pytest.raises(ValueError, match='reserve'):
         _lib.call('veda_set_sm_reserve', 1000)
     _lib.call('veda_set_sm_reserve', 0)
+
+
+def test_causal_backward_refuses_tables_off_their_boundaries(lib):
+    """Entries are read 16 bytes at a time; a table at another address is
+    refused before any launch (and before the device is looked at)."""
+    def call(q_items=0, k_items=0, k_order=0, lse=0):
+        rows = (256, 128, 64)  # address, row and head strides
+        return lib.veda_causal_bwd(
+            *rows * 4, 256, *rows, lse or 256, 2, 1, 5, 5, 2, 1, 64,
+            q_items or 256, 1, k_items or 256, 1, k_order or 256, 148, 1, 1,
+            *(512, 128, 64), *(512, 64, 64), *(512, 64, 64), 0.125, 512,
+            1 << 20, None)
+    for bad in (dict(q_items=260), dict(q_items=264), dict(k_items=260),
+                dict(k_items=272 + 8), dict(k_order=257), dict(lse=258)):
+        assert call(**bad) == _lib.VEDA_ERR_INVALID, bad
+        assert '16-byte aligned, k_order' in _lib.last_error()
