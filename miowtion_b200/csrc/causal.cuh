@@ -124,7 +124,8 @@ __device__ __forceinline__ void store32(void* dst, const uint32_t* w) {
 
 // An fp32 number keeps, beside its rounding to bf16, the eight bits behind
 // bf16's: value = the float whose bits are (bf16 bits << 16) + (low << 8), low
-// in [-128, 127], to 2^-17 of it. (The bits of a float's magnitude are in the
+// in [-128, 127], to 2^-16 of it, or to 2^-15 where 128 is held at 127 (a
+// number that lies half way between two of bf16, or nearly). (The bits of a float's magnitude are in the
 // order of the numbers, so the sum carries into the exponent where it has to.)
 //
 // The low bits of two numbers whose bf16 pair is w: in bits 0-7 and 16-23.

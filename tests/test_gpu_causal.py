@@ -466,3 +466,86 @@ def test_many_short_items_repeat(dim):
         again = kernels.causal_attention_bwd(q, k, v, out, dout, lse, pack,
                                              0.1, low=low)
         assert all(torch.equal(a, b) for a, b in zip(again, grads))
+
+
+def equal_keys(lengths, heads, kv_heads, dim, seed=21):
+    """A pack whose sequences repeat one key row, so that a row's weights are
+    equal and none is rounded (all are 1 before the division by their sum)."""
+    pack, q, k, v = problem(lengths, None, heads, kv_heads, dim, seed)
+    first = 0
+    for n in lengths:
+        k[first:first + n] = k[first:first + 1].clone()
+        first += n
+    return pack, q, k, v
+
+
+# At most 64 keys a row: four products of 16 keys, whose 17 terms each may be
+# off by 2^-23 of the sum, 4 * 17 * 2^-23 < 2^-16; the weights' 2^-22 and the
+# division are inside it.
+SHORT = [64, 33, 50, 1, 17]
+SHORT_SUM = 2.0 ** -16
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('heads, kv_heads', [(8, 2), (3, 3)])
+def test_low_bits_hold_seven_bits_more_than_out(heads, kv_heads, dim):
+    """A unit of the low bits is 2^-15 of the number at most, and they are
+    half a unit off, a whole one where 128 is held at 127."""
+    pack, q, k, v = equal_keys(SHORT, heads, kv_heads, dim)
+    v = v.abs()  # no sum cancels
+    out, _, low = kernels.causal_attention_fwd(q, k, v, pack, dim ** -0.5,
+                                               return_low=True)
+    full = ((out.view(torch.int16).int() << 16) + (low.int() << 8)).view(
+        torch.float32)
+    for at, keys, h, hk, sees in each_head(pack, q, k):
+        p = sees.double() / sees.sum(-1, keepdim=True)
+        want = p @ v[keys, hk].double()
+        err = (full[at, h].double() - want).abs()
+        assert (err <= (2.0 ** -15 + SHORT_SUM) * want).all()
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('heads, kv_heads', [(8, 2), (3, 3)])
+def test_row_sums_of_the_backward_take_the_low_bits(heads, kv_heads, dim):
+    """Value rows that differ by a fiftieth: dP and D nearly cancel, and D may
+    be off by what out and its low bits are (2^-15 and the sums' 2^-16, of
+    sum |do out|), not by the 2^-8 of out alone. dP and D are sums of D
+    products, off by (D + 8) 2^-24 each."""
+    scale = dim ** -0.5
+    pack, q, k, v = equal_keys(SHORT, heads, kv_heads, dim)
+    base = rows(1, kv_heads, dim, 31)
+    base = torch.where(base < 0, base - 1, base + 1).float()
+    v = (base * (1 + 0.02 * v.float())).bfloat16()
+    dout = rows(pack.total_q, heads, dim, 9)
+    out, lse, low = kernels.causal_attention_fwd(q, k, v, pack, scale,
+                                                 return_low=True)
+    want = [torch.zeros(t.shape, dtype=torch.float64, device=DEV)
+            for t in (q, k)]
+    bound = [torch.zeros_like(t) for t in want]
+    u, sums = 2.0 ** -8, 2 * (dim + 8) * 2.0 ** -24
+    for at, keys, h, hk, sees in each_head(pack, q, k):
+        qb, kb, vb = q[at, h].double(), k[keys, hk].double(), v[
+            keys, hk].double()
+        g = dout[at, h].double()
+        p = sees.double() / sees.sum(-1, keepdim=True)
+        o = p @ vb
+        size = (qb.abs() @ kb.abs().T).amax(-1, keepdim=True) * scale
+        e = 2 * 2.0 ** -24 * (dim + 8) * size + 2.0 ** -14
+        ds = p * (g @ vb.T - (g * o).sum(-1, keepdim=True))
+        off = (u + e) * ds.abs() + p * (
+            (2.0 ** -15 + SHORT_SUM + sums) *
+            (g * o).abs().sum(-1, keepdim=True) +
+            sums * (g.abs() @ vb.abs().T)) * (1 + u)
+        want[0][at, h] += scale * ds @ kb
+        want[1][keys, hk] += scale * ds.T @ qb
+        bound[0][at, h] += scale * off @ kb.abs()
+        bound[1][keys, hk] += scale * off.T @ qb.abs()
+
+    def holds(low):
+        got = kernels.causal_attention_bwd(q, k, v, out, dout, lse, pack,
+                                           scale, low=low)
+        return [bool(((a.double() - w).abs() <= b + u * w.abs() + 1e-30).all())
+                for a, w, b in zip(got, want, bound)]
+    assert holds(low) == [True, True]
+    # The bound tells the two apart.
+    assert holds(None)[0] is False
