@@ -663,9 +663,11 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     Returns:
         out [total_q, heads, D] bf16 (and lse); 0 and -inf for rows without
         keys. Rows of one sequence never reach another, whatever they hold;
-        inside a sequence a row that is not finite may reach rows that it
-        does not see (a value the queries before it, a gradient of the output
-        the keys behind it) inside a tile of 128 keys.
+        inside a sequence a row that is not finite may also reach rows that
+        do not see it (0 times infinity in a product): a key or value the
+        queries up to 2 * (128 // group) + 126 tokens before it, a query or a
+        gradient of the output the keys as far behind it, `group` being the
+        query heads of a key head.
 
     A forward and backward pass may be captured into a CUDA graph once the
     same pass has run on the capturing stream. As with every operator of

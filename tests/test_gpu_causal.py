@@ -549,3 +549,40 @@ def test_row_sums_of_the_backward_take_the_low_bits(heads, kv_heads, dim):
     assert holds(low) == [True, True]
     # The bound tells the two apart.
     assert holds(None)[0] is False
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('heads, kv_heads', [(2, 2), (6, 2), (8, 1)])
+@pytest.mark.parametrize('q_lengths, k_lengths', [
+    ([1000, 50], None), ([700], [1100])])
+def test_how_far_rows_that_are_not_finite_reach(q_lengths, k_lengths, heads,
+                                                kv_heads, dim):
+    """Rows that do not see a row that is not finite, and are further away
+    than 2 (128 // group) + 126 tokens, are what they are without it."""
+    reach = 2 * (128 // (heads // kv_heads)) + 126
+    pack, q, k, v = problem(q_lengths, k_lengths, heads, kv_heads, dim)
+    dout = rows(pack.total_q, heads, dim, 9)
+    before = int(pack.k_lengths[0] - pack.q_lengths[0])
+    want = kernels.causal_attention(q, k, v, pack)
+    want_grads = gradients(pack, q, k, v, dout)
+    # A key and its value: the queries before it.
+    for key in (before + 384, before + 511, before + 640):
+        k_bad, v_bad = k.clone(), v.clone()
+        k_bad[key], v_bad[key] = math.inf, math.nan
+        out = kernels.causal_attention(q, k_bad, v_bad, pack)
+        dq, _, _ = gradients(pack, q, k_bad, v_bad, dout)
+        far = key - reach - before  # the first query that it may reach
+        assert torch.equal(out[:far], want[:far])
+        assert torch.equal(dq[:far], want_grads[0][:far])
+        assert out[key - before:q_lengths[0]].isnan().all()
+        assert torch.equal(out[q_lengths[0]:], want[q_lengths[0]:])
+    # A query and its output's gradient: the keys behind it.
+    for query in (0, 127, 256):
+        q_bad, dout_bad = q.clone(), dout.clone()
+        q_bad[query], dout_bad[query] = math.nan, math.inf
+        dq, dk, dv = gradients(pack, q_bad, k, v, dout_bad)
+        far = before + query + reach + 1
+        for got, ref in ((dk, want_grads[1]), (dv, want_grads[2])):
+            assert torch.equal(got[far:], ref[far:])
+        other = torch.arange(pack.total_q, device=DEV) != query
+        assert torch.equal(dq[other], want_grads[0][other])
