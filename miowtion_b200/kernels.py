@@ -494,9 +494,8 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
 
 def _causal_checks(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
-                   pack: sequences.SequencePack) -> int:
-    """Argument checks of the causal attention; returns the heads per key
-    head."""
+                   pack: sequences.SequencePack) -> None:
+    """Argument checks of the causal attention."""
     q_shape, k_shape = q.shape, k.shape
     if len(q_shape) != 3 or len(k_shape) != 3 or k_shape != v.shape:
         raise ValueError('q, k and v must be [rows, heads, D], k and v of '
@@ -519,7 +518,6 @@ def _causal_checks(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                          f'{q.dtype}, {k.dtype}, {v.dtype}')
     if q.device != device or k.device != device or v.device != device:
         raise ValueError(f'q, k and v must be on {device}, as the pack')
-    return heads // kv_heads
 
 
 def _rows_args(t: torch.Tensor) -> tuple[int, int, int]:
@@ -534,11 +532,17 @@ def causal_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """(out [rows, heads, D] bf16, lse [rows, heads] fp32 or None) of
     `causal_attention`, without gradients; with `return_low` also the int8
     bits of out behind bf16's, for the backward."""
-    group = _causal_checks(q, k, v, pack)
+    _causal_checks(q, k, v, pack)
+    return _causal_fwd(q, k, v, pack, scale, return_lse, return_low)
+
+
+def _causal_fwd(q, k, v, pack, scale, return_lse=True, return_low=False):
+    """`causal_attention_fwd` of checked arguments."""
     require_ready(q.device, 'causal_attention')
     q, k, v = aligned_rows(q), aligned_rows(k), aligned_rows(v)
     rows, heads, dim = q.shape
     k_rows, kv_heads, _ = k.shape
+    group = heads // kv_heads
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = (q.new_empty((rows, heads), dtype=torch.float32) if return_lse
            else None)
@@ -616,8 +620,7 @@ class _CausalAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, pack, scale, return_lse):
-        out, lse, low = causal_attention_fwd(q, k, v, pack, scale,
-                                             return_low=True)
+        out, lse, low = _causal_fwd(q, k, v, pack, scale, return_low=True)
         ctx.save_for_backward(q, k, v, out, lse, low)
         ctx.pack, ctx.scale = pack, scale
         if not return_lse:
@@ -633,7 +636,7 @@ class _CausalAttention(torch.autograd.Function):
             return None, None, None, None, None, None
         q, k, v, out, lse, low = ctx.saved_tensors
         need = ctx.needs_input_grad
-        # The forward checked its arguments, autograd checks dout.
+        # q, k and v are checked before the forward, dout by autograd.
         return (*_causal_bwd(q, k, v, out, dout, lse, low, ctx.pack, ctx.scale,
                              need[0], need[1] or need[2]),
                 None, None, None)
@@ -674,10 +677,11 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     autograd, no graph of the same leaves that another stream recorded may be
     alive then: its accumulation nodes would wait for that stream.
     """
+    _causal_checks(q, k, v, pack)
     refuse_tangents('causal_attention', q, k, v)
-    scale = softmax_scale(scale, q.shape[-1])
+    scale = softmax_scale(scale, q.shape[2])
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
                                     or v.requires_grad):
         return _CausalAttention.apply(q, k, v, pack, scale, return_lse)
-    out, lse = causal_attention_fwd(q, k, v, pack, scale, return_lse)
+    out, lse = _causal_fwd(q, k, v, pack, scale, return_lse)
     return (out, lse) if return_lse else out

@@ -293,3 +293,11 @@ def test_a_write_refuses_rows_whose_gradient_it_would_lose():
         with torch.no_grad():
             with pytest.raises(NotImplementedError, match='unavailable'):
                 c.write(*args, table, two, pack([1, 1]))
+
+
+@pytest.mark.parametrize('shape', [(), (64,), (5, 64), (5, 4, 0), (1, 5, 4, 64)])
+def test_causal_attention_refuses_other_ranks_and_empty_heads(shape):
+    from miowtion_b200 import kernels
+    q = torch.zeros(shape, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match='rows, heads|head dim'):
+        kernels.causal_attention(q, q, q, pack([3, 2]))
