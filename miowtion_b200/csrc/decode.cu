@@ -1165,15 +1165,20 @@ int launch(DecodeParams p, cudaStream_t stream) {
   return check_launch("decode_join_kernel");
 }
 
-// The ring is as deep as shared memory allows beside the join buffer, whose
-// rows are the group's heads (16 at most).
+// Depth of the ring, beside the buffer of parts, whose rows are the group's
+// heads (16 at most). D = 64 and 8-bit pages: as deep as shared memory allows,
+// which at D = 128 are three stages with parts of 8 rows and two with parts of
+// 16. The buffer is therefore cut to the group where that gives the third stage
+// (64 x 8,192 rows, 8 key heads, D = 128; three stages against two: int8 232 us
+// against 239-246 for groups of 8 and the same for 4, e4m3 240 against 244 for
+// 4). bf16 pages at D = 128 need two (321 us against 329 with three for
+// groups of 4, 328 and 334 for 8; 128 x 300 rows 43 and 42).
 template <int kD, int kStore>
 int launch_stages(const DecodeParams& p, cudaStream_t stream) {
   if constexpr (kD == 64) {
     return launch<kD, kStore, kStore == kStoreBf16 ? 5 : 8, kRows>(p, stream);
   } else if constexpr (kStore == kStoreBf16) {
-    return p.group <= 8 ? launch<kD, kStore, 3, 8>(p, stream)
-                        : launch<kD, kStore, 2, kRows>(p, stream);
+    return launch<kD, kStore, 2, kRows>(p, stream);
   } else {
     return p.group <= 8 ? launch<kD, kStore, 3, 8>(p, stream)
                         : launch<kD, kStore, 2, kRows>(p, stream);
