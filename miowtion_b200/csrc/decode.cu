@@ -18,15 +18,16 @@
 // of the grid takes the i-th of W equal runs of the numbers, whatever the
 // lengths: the split needs the lengths on the device only. A warp streams its
 // run through a ring of its own with cp.async (rows past the length are
-// filled with zeros, not read), two chunks a step, with its own running
-// maximum, sum and accumulator, and never waits for another warp. A
+// filled with zeros, not read), a chunk a step (two with 8-bit pages at D =
+// 64), with its own running maximum, sum and accumulator, and never waits for
+// another warp. A
 // (sequence, head) that lies inside the run is written out; the run's first
 // and last may be parts, which the CTA adds up in shared memory at its end and,
 // where they go on in another CTA, leaves in the workspace for
 // decode_join_kernel, which starts while the last CTAs run. (The last CTA to
 // arrive doing that, by a counter, took the smallest calls longer, 18 against
-// 14 us on the device, and no less on the host.) Parts are added in the order of
-// the keys, with no atomics: repeats are bit-identical.
+// 14 us on the device, and no less on the host.) Parts are added in the order
+// of the keys, with no atomics: repeats are bit-identical.
 //
 // int8 and e4m3 codes become fp16 exactly, in registers. In the scores an int8
 // code is the fp16 number (code + 128) 2^-24 (a subnormal: its bits are the
@@ -354,10 +355,11 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 template <int kD, int kStore>
 struct Shape {
   static constexpr bool kHalf = kStore != kStoreBf16;
-  // Warps of a CTA (one a SM). Twelve warps of one chunk a step and eight of
-  // two take the same time with int8 pages (64 x 8,192 rows, 8 heads, D = 128:
-  // 211 and 213 us), twelve less with e4m3 (235 and 253): converting codes is
-  // what bounds both, at 80 and 72 % of the copy rate (bf16 pages: 100 %).
+  // Warps of a CTA (one a SM). Twelve warps of one chunk a step take less time
+  // than eight of two with 8-bit pages at D = 128 (64 x 8,192 rows, 8 key
+  // heads, groups of 4: int8 225 and 231 us, e4m3 240 and 258): converting
+  // codes is what bounds both, at 76 and 71 % of the copy rate (bf16 pages:
+  // 100 %).
   static constexpr int kWarps = kHalf && kD == 128 ? 12 : 8;
   static constexpr int kRowBytes = kHalf ? kD : 2 * kD;
   static constexpr int kTileBytes = kChunk * kRowBytes;  // k or v of a chunk
@@ -437,8 +439,8 @@ __global__ void __launch_bounds__(32 * Shape<kD, kStore>::kWarps, 1)
   int64_t lo, hi, before = 0;
   Pieces seg;
   seg.left = 0;
-  if (find_run<kThreads>(p, heads, s_sums, reinterpret_cast<int64_t*>(smem), &lo, &hi,
-               &seg.b, &before)) {
+  if (find_run<kThreads>(p, heads, s_sums, reinterpret_cast<int64_t*>(smem),
+                         &lo, &hi, &seg.b, &before)) {
     seg.length = context(p, seg.b);
     seg.n = chunks_of(seg.length);
     seg.heads = heads;
