@@ -611,9 +611,10 @@ int64_t veda_decode_workspace(int32_t head_dim);
 /* Attention of one query per sequence, q [n_seqs, n_heads, head_dim] bf16,
  * over rows 0 .. lengths[b] - 1 of its context; head h reads kv head
  * h / (n_heads / kv_heads). out [n_seqs, n_heads, head_dim] bf16 contiguous,
- * lse [n_seqs, n_heads] fp32 or NULL; 0 and -inf without rows. A length
- * outside [0, max_pages * page_size] is held inside it and sets
- * VEDA_ERR_INVALID in the device status word. */
+ * lse [n_seqs, n_heads] fp32 or NULL; 0 and -inf without rows. Rows in a page
+ * that the cache does not have are absent. They, and a length outside [0,
+ * max_pages * page_size], which is held inside it, set VEDA_ERR_INVALID in the
+ * device status word. */
 int veda_decode(const void* k_pages, const void* v_pages,
                 const float* k_scale, const float* v_scale, int64_t n_pages,
                 int32_t page_size, int32_t kv_heads, int32_t head_dim,

@@ -718,11 +718,12 @@ class CachedAttention:
     the rows of k and v in the layer's cache and attends over the contexts.
 
     A step's rows are `pack`: q_lengths new rows per sequence, k_lengths rows
-    in all once they are stored. A prompt (no earlier rows) attends to k and v
-    as they came; a chunk behind earlier rows to its contexts as the cache
-    holds them; single tokens straight over the pages. With int8 or e4m3
-    pages the first therefore sees unquantised rows, the others quantised
-    ones.
+    in all once they are stored. The whole step takes one way: a single token
+    for every sequence attends straight over the pages; prompts, if no
+    sequence has earlier rows, to k and v as they came; any other step to the
+    contexts as the cache holds them. With int8 or e4m3 pages a prompt
+    therefore sees unquantised rows in a step of prompts and quantised ones in
+    a step with a chunk in it.
 
     Args:
         caches: One `kvcache.PagedCache` per layer.

@@ -19,18 +19,22 @@
 //           dP^T = V dO^T, P^T and dS^T written back over them, dV += P^T dO
 //           and dK += dS^T Q.
 // One CTA per SM, 8 compute warps, a TMA producer warp and a converged MMA
-// warp. Tensor memory decides how the two kernels overlap their products with
-// the elementwise work. dq has one accumulator, so there is room for two S
-// buffers beside dP: while the compute warps turn block b into dS, the tensor core has
-// dP of b + 1 (as soon as dP of b is in registers), dQ of b - 1 and S of b + 1,
-// all 128 columns wide. dk/dv has two accumulators and no room: a block's 128
-// columns run as two halves of 64, and the tensor core has one half's products
-// while the compute warps work on the other.
+// warp. Tensor memory at D = 128 decides how the two kernels overlap their
+// products with the elementwise work. dq has one accumulator, so there is room
+// for two S buffers beside dP: while the compute warps turn block b into dS,
+// the tensor core has dP of b + 1 (as soon as dP of b is in registers), dQ of
+// b - 1 and S of b + 1, all 128 columns wide. dk/dv has two accumulators of D
+// columns and, at D = 128, no room: a block's 128 columns run as two halves of
+// 64, and the tensor core has one half's products while the compute warps work
+// on the other. D = 64 runs the same layout, though it leaves 128 columns
+// unused; products 128 wide have not been measured there.
 //
-// Bound by the tensor core's products at D = 128 (busy 57 % of dq, 64 % of
-// dkdv; a product 64 columns wide reads 6 KB of shared memory for 32 cycles'
-// work, 48 cycles' worth) and by the elementwise work at D = 64. The whole
-// backward of 8,192 tokens, 16/4 heads, by step, at D = 128 and 64:
+// No unit is full. At D = 128 the tensor core is busy 58 % of dq and 57 % of
+// dkdv, whose products are 64 columns wide (such a product reads 6 KB of shared
+// memory, 48 cycles' worth, for 32 cycles' work: the data path is at 72 %); at
+// D = 64 37 and 35 %, the special function unit 50 and 35 %. The rest is
+// products and elementwise work waiting for each other. The whole backward of
+// 8,192 tokens, 16/4 heads, by step, at D = 128 and 64:
 //     dq in halves too, S alone ahead            904 and 736 us
 //     dq 128 columns wide                        874 and 743
 //     elementwise work on pairs (f32x2), L and D
@@ -47,9 +51,10 @@
 // the 2-norm, relative) where results that are only rounded are 1.7e-3 off.
 // (Two bf16 numbers for a dS would be two more products of seven.) D's error
 // is the same for all keys of a row and meets a sum that cancels, most of all
-// where few keys hold the weight: from out as rounded to bf16 it made that
-// 2.5 to 3.2e-3, and 8e-3 for weights peaked on a key, so the forward also
-// leaves the eight bits behind (causal.cuh), a byte an element.
+// where few keys hold the weight: from out as rounded to bf16 it made dQ
+// 2.6e-3 off, and 3.9e-3 and 6.0e-3 with scores 4 and 16 times as large (300, 1
+// and 70 tokens of N(0, 1), 4/2 heads, D = 128), so the forward also leaves the
+// eight bits behind (causal.cuh), a byte an element: 2.4, 2.7 and 3.1e-3.
 //
 // Rows behind a sequence's end are cleared in shared memory where they are
 // the depth of a product (keys in dq, queries in dkdv); elsewhere they are

@@ -48,8 +48,9 @@ class PagedCache:
 
     int8 rows: scale max|x| / 127, codes rounded to nearest (ties to even).
     float8_e4m3fn rows: scale 2^e with the smallest e >= -120 for which
-    max|x| <= 448 * 2^e. A row with a value that is not finite is stored as
-    NaN; an all-zero row has scale 0.
+    max|x| <= 448 * 2^e (a value from 1.9375 * 2^127 on rounds to 2^128 and
+    reads back as infinity). A row with a value that is not finite is stored
+    as NaN; an all-zero row has scale 0.
     """
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor,
